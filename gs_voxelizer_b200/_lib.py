@@ -26,6 +26,17 @@ _SZ = ctypes.c_size_t
 _I3 = ctypes.c_int32 * 3
 _F3 = ctypes.c_float * 3
 
+
+
+class CeOptions(ctypes.Structure):
+    """gsv_ce_options of include/gsvox.h."""
+    _fields_ = [("ignore_index", _I64), ("label_smoothing", ctypes.c_float),
+                ("softcap", ctypes.c_float), ("z_loss", ctypes.c_float),
+                ("reduction", _I32)]
+
+
+_OPT = ctypes.POINTER(CeOptions)
+
 # name -> (restype, argtypes); kept in declaration order of include/gsvox.h
 SIGNATURES = {
     "gsv_last_error": (ctypes.c_char_p, []),
@@ -108,6 +119,19 @@ SIGNATURES = {
     "gsv_halo_accumulate": (
         ctypes.c_int, [_I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P,
                        _P, _P]),
+    "gsv_softmax_ce_workspace_bytes": (_SZ, [_I64, _I32]),
+    "gsv_softmax_ce_forward": (
+        ctypes.c_int, [_I64, _I32, _I32, _P, _P, _OPT, _P, _P, _P, _P, _SZ, _P]),
+    "gsv_softmax_ce_backward": (
+        ctypes.c_int, [_I64, _I32, _I32, _P, _P, _OPT, _P, _P, _P, _P, _P]),
+    "gsv_linear_ce_state_bytes": (_SZ, [_I64]),
+    "gsv_linear_ce_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _OPT, _I32]),
+    "gsv_linear_ce_forward": (
+        ctypes.c_int, [_I64, _I32, _I32, _I32, _P, _P, _P, _OPT, _P, _P, _P, _SZ,
+                       _P]),
+    "gsv_linear_ce_backward": (
+        ctypes.c_int, [_I64, _I32, _I32, _I32, _P, _P, _P, _OPT, _P, _P, _P, _P,
+                       _P, _SZ, _P]),
 }
 
 HALO_RECORD_FLOATS = 20

@@ -17,7 +17,11 @@ SRC = HERE / "csrc"
 BUILD = HERE / "_build"
 LIB = HERE / "libgsvox.so"
 SOURCES = ["projection.cu", "binning.cu", "voxelize.cu", "bwd_tc.cu", "loss.cu",
-           "ssim.cu", "noalloc.cu", "halo.cu", "capi.cu"]
+           "ssim.cu", "noalloc.cu", "halo.cu", "softmax_ce.cu", "linear_ce.cu",
+           "ce_gemm.cu", "capi.cu"]
+# Sources compiled with IEEE arithmetic and math functions: their scores
+# reach the hundreds and their exponents may be infinite on purpose.
+PRECISE = {"softmax_ce.cu", "linear_ce.cu", "ce_gemm.cu"}
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -37,7 +41,7 @@ def _run(cmd: list[str]) -> None:
 
 def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
-    deps = [SRC / "common.cuh", HERE.parent / "include" / "gsvox.h"]
+    deps = [*SRC.glob("*.cuh"), HERE.parent / "include" / "gsvox.h"]
     dep_mtime = max(p.stat().st_mtime for p in deps)
     objs = []
     for name in SOURCES:
@@ -47,7 +51,8 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
         if obj.exists() and obj.stat().st_mtime > max(src.stat().st_mtime, dep_mtime) \
                 and not ptxas_info:
             continue
-        cmd = [NVCC, *ARCH, *FLAGS, "-c", str(src), "-o", str(obj)]
+        flags = [f for f in FLAGS if f != "-use_fast_math" or name not in PRECISE]
+        cmd = [NVCC, *ARCH, *flags, "-c", str(src), "-o", str(obj)]
         if ptxas_info:
             cmd.insert(1, "-Xptxas=-v")
         if verbose:

@@ -8,7 +8,7 @@
 #include <string>
 
 #include "../../include/gsvox.h"
-#include "common.cuh"
+#include "ce.cuh"
 
 namespace gsv {
 cudaError_t launch_project_fwd(int n, int channels, const float *pos3d,
@@ -134,6 +134,23 @@ cudaError_t launch_vox_backward_voxel(const Geom &g, int C, int n,
                                       float *int_grad, void *ws,
                                       cudaStream_t stream);
 void enable_large_smem();
+size_t softmax_ce_workspace_bytes(long long rows, int V);
+cudaError_t launch_softmax_ce(bool fwd, int type, long long rows, int V, const void *scores,
+                              const long long *labels, const CeOpt &o, float *loss,
+                              float *lse, float *count, const float *grad_loss, void *grad,
+                              void *ws, cudaStream_t st);
+size_t linear_ce_state_bytes(long long rows);
+size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
+                                 const CeOpt &o);
+cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
+                                     const void *features, const void *weight,
+                                     const long long *labels, const CeOpt &o, float *loss,
+                                     void *state, void *workspace, cudaStream_t st);
+cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
+                                      const void *features, const void *weight,
+                                      const long long *labels, const CeOpt &o, void *state,
+                                      const float *grad_loss, void *grad_features,
+                                      void *grad_weight, void *workspace, cudaStream_t st);
 }  // namespace gsv
 
 namespace gsv {
@@ -1054,3 +1071,136 @@ extern "C" int gsv_peer_barrier(int32_t world, int32_t rank, const int64_t *sig_
                            epoch, as_stream(stream)),
                        fn);
 }
+
+// ------------------------------------------------------------ class losses
+
+namespace {
+
+int check_ce(const char *fn, int64_t rows, int32_t classes, int32_t channels, int32_t dtype,
+             const gsv_ce_options *o) {
+    GSV_REQUIRE(o, GSV_ERR_INVALID_ARGUMENT, "%s: options are null", fn);
+    GSV_REQUIRE(rows >= 1 && classes >= 1 && channels >= 1, GSV_ERR_INVALID_ARGUMENT,
+                "%s: rows, classes and channels must be positive", fn);
+    GSV_REQUIRE(rows < INT32_MAX - 1024 && classes <= (1 << 30) && channels <= (1 << 20),
+                GSV_ERR_SIZE_OVERFLOW, "%s: sizes beyond the 32-bit index formats", fn);
+    GSV_REQUIRE(dtype >= GSV_F32 && dtype <= GSV_F16, GSV_ERR_INVALID_ARGUMENT,
+                "%s: unknown dtype %d", fn, dtype);
+    GSV_REQUIRE(o->label_smoothing >= 0.f && o->label_smoothing < 1.f,
+                GSV_ERR_INVALID_ARGUMENT, "%s: label_smoothing must be in [0, 1)", fn);
+    GSV_REQUIRE(o->softcap >= 0.f && o->softcap <= 1e30f && o->z_loss >= 0.f &&
+                    o->z_loss <= 1e30f,
+                GSV_ERR_INVALID_ARGUMENT,
+                "%s: softcap and z_loss must be finite and not negative", fn);
+    GSV_REQUIRE(o->reduction >= GSV_REDUCE_NONE && o->reduction <= GSV_REDUCE_MEAN,
+                GSV_ERR_INVALID_ARGUMENT, "%s: unknown reduction %d", fn, o->reduction);
+    return GSV_OK;
+}
+
+gsv::CeOpt ce_opt(const gsv_ce_options *o) {
+    return {(long long)o->ignore_index, o->label_smoothing, o->softcap, o->z_loss,
+            o->reduction};
+}
+
+const long long *as_ll(const int64_t *p) { return reinterpret_cast<const long long *>(p); }
+
+}  // namespace
+
+extern "C" {
+
+size_t gsv_softmax_ce_workspace_bytes(int64_t rows, int32_t classes) {
+    if (rows < 1 || classes < 1) return 0;
+    return gsv::softmax_ce_workspace_bytes(rows, classes);
+}
+
+int gsv_softmax_ce_forward(int64_t rows, int32_t classes, int32_t dtype, const void *scores,
+                           const int64_t *labels, const gsv_ce_options *options, float *loss,
+                           float *lse, float *count, void *ws, size_t ws_bytes,
+                           void *stream) {
+    const char *fn = "gsv_softmax_ce_forward";
+    if (const int st = check_ce(fn, rows, classes, 1, dtype, options)) return st;
+    GSV_REQUIRE(scores && labels && loss && lse && count, GSV_ERR_INVALID_ARGUMENT,
+                "%s: null pointer", fn);
+    const size_t need = gsv_softmax_ce_workspace_bytes(rows, classes);
+    GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
+                "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
+    return cuda_status(gsv::launch_softmax_ce(true, dtype, rows, classes, scores,
+                                              as_ll(labels), ce_opt(options), loss, lse,
+                                              count, nullptr, nullptr, ws, as_stream(stream)),
+                       fn);
+}
+
+int gsv_softmax_ce_backward(int64_t rows, int32_t classes, int32_t dtype, const void *scores,
+                            const int64_t *labels, const gsv_ce_options *options,
+                            const float *lse, const float *count, const float *grad_loss,
+                            void *grad_scores, void *stream) {
+    const char *fn = "gsv_softmax_ce_backward";
+    if (const int st = check_ce(fn, rows, classes, 1, dtype, options)) return st;
+    GSV_REQUIRE(scores && labels && lse && count && grad_loss && grad_scores,
+                GSV_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+    return cuda_status(gsv::launch_softmax_ce(
+                           false, dtype, rows, classes, scores, as_ll(labels),
+                           ce_opt(options), nullptr, const_cast<float *>(lse),
+                           const_cast<float *>(count), grad_loss, grad_scores, nullptr,
+                           as_stream(stream)),
+                       fn);
+}
+
+size_t gsv_linear_ce_state_bytes(int64_t rows) {
+    if (rows < 1 || rows >= INT32_MAX - 1024) return 0;
+    return gsv::linear_ce_state_bytes(rows);
+}
+
+size_t gsv_linear_ce_workspace_bytes(int64_t rows, int32_t classes, int32_t channels,
+                                     int32_t dtype, const gsv_ce_options *options,
+                                     int32_t backward) {
+    if (check_ce("gsv_linear_ce_workspace_bytes", rows, classes, channels, dtype, options))
+        return 0;
+    return gsv::linear_ce_workspace_bytes(rows, classes, channels, dtype, backward != 0,
+                                          ce_opt(options));
+}
+
+int gsv_linear_ce_forward(int64_t rows, int32_t classes, int32_t channels, int32_t dtype,
+                          const void *features, const void *weight, const int64_t *labels,
+                          const gsv_ce_options *options, float *loss, void *state, void *ws,
+                          size_t ws_bytes, void *stream) {
+    const char *fn = "gsv_linear_ce_forward";
+    if (const int st = check_ce(fn, rows, classes, channels, dtype, options)) return st;
+    GSV_REQUIRE(features && weight && labels && loss && state, GSV_ERR_INVALID_ARGUMENT,
+                "%s: null pointer", fn);
+    const size_t need =
+        gsv_linear_ce_workspace_bytes(rows, classes, channels, dtype, options, 0);
+    GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
+                "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
+    GSV_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0 &&
+                    (reinterpret_cast<uintptr_t>(state) & 15) == 0,
+                GSV_ERR_INVALID_ARGUMENT, "%s: workspace or state not aligned", fn);
+    return cuda_status(gsv::launch_linear_ce_forward(rows, classes, channels, dtype, features,
+                                                     weight, as_ll(labels), ce_opt(options),
+                                                     loss, state, ws, as_stream(stream)),
+                       fn);
+}
+
+int gsv_linear_ce_backward(int64_t rows, int32_t classes, int32_t channels, int32_t dtype,
+                           const void *features, const void *weight, const int64_t *labels,
+                           const gsv_ce_options *options, void *state,
+                           const float *grad_loss, void *grad_features, void *grad_weight,
+                           void *ws, size_t ws_bytes, void *stream) {
+    const char *fn = "gsv_linear_ce_backward";
+    if (const int st = check_ce(fn, rows, classes, channels, dtype, options)) return st;
+    GSV_REQUIRE(features && weight && labels && state && grad_loss, GSV_ERR_INVALID_ARGUMENT,
+                "%s: null pointer", fn);
+    const size_t need =
+        gsv_linear_ce_workspace_bytes(rows, classes, channels, dtype, options, 1);
+    GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
+                "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
+    GSV_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0 &&
+                    (reinterpret_cast<uintptr_t>(state) & 15) == 0,
+                GSV_ERR_INVALID_ARGUMENT, "%s: workspace or state not aligned", fn);
+    return cuda_status(gsv::launch_linear_ce_backward(
+                           rows, classes, channels, dtype, features, weight, as_ll(labels),
+                           ce_opt(options), state, grad_loss, grad_features, grad_weight, ws,
+                           as_stream(stream)),
+                       fn);
+}
+
+}  // extern "C"

@@ -1,0 +1,130 @@
+// Shared pieces of the class losses (softmax_ce.cu, linear_ce.cu, ce_gemm.cu).
+//
+// With z_ij the scores of row i (capped: z = c tanh(s / c) when c > 0),
+//     lse_i  = log sum_j exp z_ij
+//     loss_i = lse_i - (1 - eps) z_iy - eps / V sum_j z_ij + zeta lse_i^2
+//     dloss_i / dz_ij = (1 + 2 zeta lse_i) exp(z_ij - lse_i)
+//                       - (1 - eps) [j = y_i] - eps / V
+// and, through the cap, ds = dz (1 - (z / c)^2). Scores, maxima, sums and
+// losses are float32 whatever the type of the inputs.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace gsv {
+
+enum CeType { kCeF32 = 0, kCeBf16 = 1, kCeF16 = 2 };
+enum CeReduction { kCeNone = 0, kCeSum = 1, kCeMean = 2 };
+
+// Options of a class loss, by value into the kernels.
+struct CeOpt {
+    long long ignore;
+    float eps, cap, zeta;
+    int reduction;
+};
+
+// What a row's label stands for: a class >= 0, or one of these.
+constexpr int kCeInvalid = -1;  // outside [0, V): the row's loss is NaN
+constexpr int kCeIgnored = -2;  // no label: the row takes no part
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kCeLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ int ce_label(long long y, long long ignore, int V) {
+    if (y == ignore) return kCeIgnored;
+    return (y < 0 || y >= V) ? kCeInvalid : (int)y;
+}
+
+__device__ __forceinline__ float ce_nan() { return __int_as_float(0x7fc00000); }
+__device__ __forceinline__ float ce_neg_inf() { return __int_as_float(0xff800000); }
+
+__device__ __forceinline__ float ce_cap(float s, float cap) {
+    return cap > 0.f ? cap * tanhf(s / cap) : s;
+}
+
+// Running maximum, sum of exponentials (relative to the maximum) and plain
+// sum of a row's scores.
+struct CeAcc {
+    float m, s, sz;
+    __device__ __forceinline__ void init() {
+        m = ce_neg_inf();
+        s = 0.f;
+        sz = 0.f;
+    }
+    // m stays -inf while every score is -inf: the exponent is taken against
+    // 0 then, so that each term is exp(-inf) = 0 and not NaN
+    __device__ __forceinline__ static float base(float m) {
+        return m == ce_neg_inf() ? 0.f : m * kLog2e;
+    }
+    __device__ __forceinline__ void merge(float om, float os, float osz) {
+        const float nm = fmaxf(m, om);
+        const float b = base(nm);
+        s = s * ex2(fmaf(m, kLog2e, -b)) + os * ex2(fmaf(om, kLog2e, -b));
+        m = nm;
+        sz += osz;
+    }
+    __device__ __forceinline__ float lse() const {
+        return (m == ce_neg_inf() ? 0.f : m) + logf(s);
+    }
+};
+
+// loss of a labelled row
+__device__ __forceinline__ float ce_row_loss(float lse, float zy, float sz, int V,
+                                             const CeOpt &o) {
+    float l = lse - (1.f - o.eps) * zy;
+    if (o.eps > 0.f) l -= o.eps / (float)V * sz;
+    if (o.zeta > 0.f) l += o.zeta * lse * lse;
+    return l;
+}
+
+template <typename T> __device__ __forceinline__ float ce_to_float(T v);
+template <> __device__ __forceinline__ float ce_to_float(float v) { return v; }
+template <> __device__ __forceinline__ float ce_to_float(__nv_bfloat16 v) {
+    return __bfloat162float(v);
+}
+template <> __device__ __forceinline__ float ce_to_float(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T ce_from_float(float v);
+template <> __device__ __forceinline__ float ce_from_float(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 ce_from_float(float v) {
+    return __float2bfloat16_rn(v);
+}
+template <> __device__ __forceinline__ __half ce_from_float(float v) {
+    return __float2half_rn(v);
+}
+
+// Sums (loss, labelled rows) over a block of NT threads; valid in thread 0.
+template <int NT>
+__device__ __forceinline__ float2 ce_block_sum(float loss, float cnt, float2 *sh) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        loss += __shfl_xor_sync(0xffffffffu, loss, o);
+        cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+    }
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(loss, cnt);
+    __syncthreads();
+    float2 r = make_float2(0.f, 0.f);
+    if (threadIdx.x == 0)
+        for (int w = 0; w < NT / 32; ++w) {
+            r.x += sh[w].x;
+            r.y += sh[w].y;
+        }
+    return r;
+}
+
+// loss[0] from per-block (loss, rows) sums; count[0] = max(rows, 1), by which
+// the mean and its gradient are divided (no labelled row: loss 0).
+cudaError_t launch_ce_finish(const float2 *partials, int n, int reduction,
+                             float *loss, float *count, cudaStream_t stream);
+
+__device__ __forceinline__ void ce_finish(double loss, double rows, int reduction,
+                                          float *out, float *count) {
+    const double c = rows > 1.0 ? rows : 1.0;
+    count[0] = (float)c;
+    if (reduction != kCeNone)
+        out[0] = (float)(reduction == kCeMean ? loss / c : loss);
+}
+
+}  // namespace gsv

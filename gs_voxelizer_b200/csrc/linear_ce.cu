@@ -1,0 +1,610 @@
+// Softmax cross entropy of a linear map: scores X W^T of N feature rows
+// against a table of V classes, without keeping the N x V scores.
+//
+// Forward: the labelled rows are packed into whole 128-row tiles (rows
+// without a label cost nothing and cannot leak what they hold), the product
+// runs tile by tile and leaves one (maximum, sum) pair per row and class
+// tile, and a merge turns the pairs into lse and loss.
+// Backward: the scores are computed again in pieces of rows x classes that a
+// bounded workspace holds, as P = dloss/dscore in 16 bits, and each piece is
+// multiplied into both gradients: dX += P W, dW += P^T X, accumulated in
+// float32 and rounded once.
+//
+// Rounding P to 16 bits costs at most half a unit of its last place
+// (2^-9 of the value in bf16, 2^-12 in fp16), which is below the rounding of
+// the gradients themselves to the same type. fp16 keeps P times a power of
+// two (see p_scale_of) so that small probabilities stay normal numbers.
+// float32 inputs keep three bf16 planes of every operand, which hold all 24
+// bits.
+#include "ce_gemm.cuh"
+
+namespace gsv {
+namespace {
+
+constexpr int kIdxNT = 1024;
+constexpr size_t kPieceBytes = (size_t)256 << 20;  // of P
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+long long up(long long v, long long a) { return (v + a - 1) / a * a; }
+
+// ------------------------------------------------------------ packed rows
+
+__global__ void __launch_bounds__(kIdxNT)
+count_labels_kernel(long long n, const long long *__restrict__ labels, long long ignore,
+                    int *__restrict__ counts) {
+    const long long i = (long long)blockIdx.x * kIdxNT + threadIdx.x;
+    const int c = __syncthreads_count(i < n && labels[i] != ignore);
+    if (threadIdx.x == 0) counts[blockIdx.x] = c;
+}
+
+// idx / lab of the packed rows in their order; positions from the number of
+// labelled rows up to padded are kCeIgnored. total[0] = labelled rows.
+__global__ void __launch_bounds__(kIdxNT)
+index_kernel(long long n, long long padded, int V, const long long *__restrict__ labels,
+             long long ignore, const int *__restrict__ counts, int nblocks,
+             int *__restrict__ total, int *__restrict__ idx, int *__restrict__ lab) {
+    __shared__ long long s_before[32], s_all[32];
+    __shared__ int s_warp[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long i = (long long)blockIdx.x * kIdxNT + threadIdx.x;
+    const long long y = i < n ? labels[i] : ignore;
+    const bool keep = i < n && y != ignore;
+    long long before = 0, all = 0;
+    if (nblocks > 1) {
+        for (int b = threadIdx.x; b < nblocks; b += kIdxNT) {
+            const int c = counts[b];
+            all += c;
+            if (b < (int)blockIdx.x) before += c;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+            all += __shfl_xor_sync(0xffffffffu, all, o);
+        }
+        if (lane == 0) {
+            s_before[warp] = before;
+            s_all[warp] = all;
+        }
+    }
+    const unsigned ballot = __ballot_sync(0xffffffffu, keep);
+    if (lane == 0) s_warp[warp] = __popc(ballot);
+    __syncthreads();
+    before = all = 0;
+    if (nblocks > 1) {
+        for (int w = 0; w < 32; ++w) {
+            before += s_before[w];
+            all += s_all[w];
+        }
+    }
+    int here = 0, block_total = 0;
+    for (int w = 0; w < 32; ++w) {
+        if (w < warp) here += s_warp[w];
+        block_total += s_warp[w];
+    }
+    if (nblocks == 1) all = block_total;
+    if (keep) {
+        const long long r = before + here + __popc(ballot & ((1u << lane) - 1u));
+        idx[r] = (int)i;
+        lab[r] = ce_label(y, ignore, V);
+    }
+    if (i >= all && i < padded) lab[i] = kCeIgnored;
+    if (i == 0) total[0] = (int)all;
+}
+
+// Splits a float into bf16 planes whose sum it is. Infinities and NaN live
+// in the first plane alone; a finite value that would round to infinity is
+// held at the largest bf16 and the remainder follows.
+__device__ __forceinline__ void split3(float v, __nv_bfloat16 (&h)[3]) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        h[p] = __float2bfloat16_rn(v);
+        float f = __bfloat162float(h[p]);
+        if (!isfinite(f)) {
+            if (!isfinite(v)) {
+                v = 0.f;
+                continue;
+            }
+            h[p] = __ushort_as_bfloat16(v < 0.f ? 0xff7f : 0x7f7f);
+            f = __bfloat162float(h[p]);
+        }
+        v -= f;
+    }
+}
+
+// Per-row factor of the table's gradient: the row's upstream gradient
+// (reduction "none"), in fp16 over the largest one, so that it cannot
+// overflow or vanish.
+struct RowScale {
+    const float *g;       // by original row, or null
+    const float *gmax;    // or null
+};
+
+// dst[plane][padded rows][ld] = src[idx[r]] (times the row's factor), rows
+// past the count and columns past D zero. One warp a row.
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(256)
+pack_kernel(long long rows, int D, long long ld, long long plane, const T *__restrict__ src,
+            const int *__restrict__ idx, const int *__restrict__ total, RowScale sc,
+            void *__restrict__ dst) {
+    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const int lane = threadIdx.x & 31;
+    long long from = r;
+    float k = 1.f;
+    if (ROWS) {
+        const long long live = *total;
+        if (r >= (live + kCeTileM - 1) / kCeTileM * kCeTileM) return;
+        from = r < live ? idx[r] : -1;
+        if (sc.g && from >= 0) {
+            k = sc.g[from];
+            if (sc.gmax && *sc.gmax > 0.f) k /= *sc.gmax;
+        }
+    }
+    for (long long c = lane; c < ld; c += 32) {
+        T v = ce_from_float<T>(0.f);
+        if (from >= 0 && c < D) v = src[from * D + c];
+        if constexpr (sizeof(T) == 4) {
+            __nv_bfloat16 h[3];
+            split3(sc.g ? v * k : v, h);
+            __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(dst) + r * ld + c;
+            o[0] = h[0];
+            o[plane] = h[1];
+            o[2 * plane] = h[2];
+        } else {
+            if (sc.g) v = ce_from_float<T>(ce_to_float(v) * k);
+            static_cast<T *>(dst)[r * ld + c] = v;
+        }
+    }
+}
+
+// --------------------------------------------------------- merge and loss
+
+constexpr int kMergeRows = 32, kMergeSlices = 8;
+
+// One row's (max, sum) pairs of all class tiles -> lse and loss. Eight
+// slices of the tiles run side by side for 32 rows.
+__global__ void __launch_bounds__(kMergeRows *kMergeSlices)
+merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
+             const float *__restrict__ psum, const float *__restrict__ zt,
+             const int *__restrict__ total, const int *__restrict__ idx,
+             const int *__restrict__ lab, const long long *__restrict__ labels, CeOpt o,
+             float *__restrict__ loss, float *__restrict__ lse_out,
+             float *__restrict__ count, float2 *__restrict__ block_sums) {
+    __shared__ float sm[kMergeSlices][kMergeRows], ss[kMergeSlices][kMergeRows],
+        sz[kMergeSlices][kMergeRows];
+    const int lane = threadIdx.x % kMergeRows, slice = threadIdx.x / kMergeRows;
+    const long long r = (long long)blockIdx.x * kMergeRows + lane;
+    const bool live = r < rows && (!total || r < *total);
+    CeAcc a;
+    a.init();
+    if (live)
+        for (int t = slice; t < tiles; t += kMergeSlices) {
+            const float2 p = part[t * rows + r];
+            a.merge(p.x, p.y, psum ? psum[t * rows + r] : 0.f);
+        }
+    sm[slice][lane] = a.m;
+    ss[slice][lane] = a.s;
+    sz[slice][lane] = a.sz;
+    __syncthreads();
+    if (slice) return;
+    float l = 0.f, c = 0.f;
+    if (live) {
+        for (int s = 1; s < kMergeSlices; ++s) a.merge(sm[s][lane], ss[s][lane], sz[s][lane]);
+        const int y = lab ? lab[r] : ce_label(labels[r], o.ignore, V);
+        float lse = a.lse();
+        if (y >= 0)
+            l = ce_row_loss(lse, zt[r], a.sz, V, o);
+        else if (y == kCeInvalid)
+            l = lse = ce_nan();
+        c = y == kCeIgnored ? 0.f : 1.f;
+        const long long dst = idx ? idx[r] : r;
+        lse_out[dst] = lse;
+        if (o.reduction == kCeNone) loss[dst] = l;
+    }
+#pragma unroll
+    for (int k = 16; k; k >>= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, k);
+        c += __shfl_xor_sync(0xffffffffu, c, k);
+    }
+    if (lane == 0) {
+        if (gridDim.x == 1)
+            ce_finish(l, c, o.reduction, loss, count);
+        else
+            block_sums[blockIdx.x] = make_float2(l, c);
+    }
+}
+
+// -------------------------------------------------------------- gradients
+
+// out[0] (zero before) = largest |g| of the labelled rows; the bits of
+// non-negative floats order as integers, and a maximum has no order
+__global__ void __launch_bounds__(256)
+max_abs_kernel(const float *__restrict__ g, const int *__restrict__ idx,
+               const int *__restrict__ total, float *__restrict__ out) {
+    float m = 0.f;
+    const long long n = *total;
+    for (long long r = blockIdx.x * 256LL + threadIdx.x; r < n; r += gridDim.x * 256LL)
+        m = fmaxf(m, fabsf(g[idx[r]]));
+#pragma unroll
+    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    if ((threadIdx.x & 31) == 0 && m > 0.f)
+        atomicMax(reinterpret_cast<int *>(out), __float_as_int(m));
+}
+
+// factor of the accumulated gradients: 1 / p_scale times the upstream
+// gradient (of the row, with reduction "none": `row` is the original row)
+__device__ __forceinline__ float out_scale(const float *g, const float *count, int reduction,
+                                           float inv_p, long long row, const float *gmax) {
+    if (reduction == kCeNone) {
+        if (row >= 0) return g[row] * inv_p;
+        return (gmax && *gmax > 0.f ? *gmax : 1.f) * inv_p;
+    }
+    return (reduction == kCeMean ? g[0] / count[0] : g[0]) * inv_p;
+}
+
+// dst[idx[r]] = scale * sum over splits of acc[s][r]; one warp a row. The
+// rows are those of a piece: packed rows row0 .. row0 + rows.
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(256)
+finish_grad_kernel(long long row0, long long rows, int D, const float *__restrict__ acc,
+                   long long split, int splits, const int *__restrict__ idx,
+                   const int *__restrict__ total, const float *__restrict__ g,
+                   const float *__restrict__ count, int reduction, float inv_p,
+                   const float *__restrict__ gmax, T *__restrict__ dst) {
+    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    long long to = r;
+    if (ROWS) {
+        if (row0 + r >= *total) return;
+        to = idx[row0 + r];
+    }
+    const float k = out_scale(g, count, reduction, inv_p, ROWS ? to : -1, gmax);
+    for (long long c = threadIdx.x & 31; c < D; c += 32) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += acc[s * split + r * D + c];
+        dst[to * D + c] = ce_from_float<T>(v * k);
+    }
+}
+
+// rows without a label: zero gradient
+template <typename T>
+__global__ void __launch_bounds__(256)
+zero_ignored_kernel(long long n, int D, const long long *__restrict__ labels,
+                    long long ignore, T *__restrict__ dst) {
+    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= n || labels[r] != ignore) return;
+    for (long long c = threadIdx.x & 31; c < D; c += 32) dst[r * D + c] = ce_from_float<T>(0.f);
+}
+
+// ------------------------------------------------------------------- plan
+
+unsigned blocks8(long long rows) { return (unsigned)((rows + 7) / 8); }
+
+struct Plan {
+    long long N, Np;      // rows, rows in whole tiles
+    int V, D, type, planes;
+    long long ld;         // of packed features / table
+    bool pack_w;          // the table cannot be read in place
+    int tiles;            // class tiles of the forward
+    // backward: pieces and splits
+    long long piece_rows, ldp;
+    int piece_classes;
+    bool one_row_piece, one_class_piece;
+    int split_x, split_w;
+    // workspace offsets (bytes)
+    size_t xp, xs, wp, part, psum, zt, sums, gmax, p, dx, dw, bytes;
+};
+
+// state (kept between the two directions): count (float, padded to 4 words),
+// lse [N], packed total (int, padded to 4 words), idx [Np], lab [Np],
+// block counts
+struct State {
+    float *count, *lse;
+    int *total, *idx, *lab, *counts;
+};
+
+long long state_words(long long N) {
+    const long long Np = up(N, kCeTileM);
+    return 4 + up(N, 4) + 4 + 2 * Np + up((N + kIdxNT - 1) / kIdxNT, 4);
+}
+
+State state_of(void *p, long long N) {
+    const long long Np = up(N, kCeTileM);
+    float *f = static_cast<float *>(p);
+    State s;
+    s.count = f;
+    s.lse = f + 4;
+    s.total = reinterpret_cast<int *>(s.lse + up(N, 4));
+    s.idx = s.total + 4;
+    s.lab = s.idx + Np;
+    s.counts = s.lab + Np;
+    return s;
+}
+
+// |dloss / dscore| <= 1 + 2 zeta |lse|: the largest power of two, up to 2^14,
+// that keeps fp16 finite for |lse| <= 4096. The other types have the range
+// of float32.
+float p_scale_of(int type, const CeOpt &o) {
+    if (type != kCeF16) return 1.f;
+    float s = 16384.f;
+    while (s > 1.f / 1024.f && s * (1.f + 8192.f * o.zeta) > 65504.f) s *= 0.5f;
+    return s;
+}
+
+int splits_for(long long tiles, long long depth) {
+    // enough blocks for the device when the product has few tiles, each
+    // split keeping at least 512 of the summed axis
+    const long long want = tiles > 0 ? kSMs / tiles : 1;
+    return (int)std::max(1LL, std::min(want, depth / 512));
+}
+
+Plan make_plan(long long N, int V, int D, int type, const void *weight, bool backward,
+               const CeOpt &o) {
+    Plan p{};
+    p.N = N;
+    p.Np = up(N, kCeTileM);
+    p.V = V;
+    p.D = D;
+    p.type = type;
+    p.planes = type == kCeF32 ? 3 : 1;
+    p.ld = up(D, 8);
+    // `weight` null: the workspace query, which allows for any alignment
+    p.pack_w = p.planes == 3 || D % 8 != 0 || weight == nullptr ||
+               (reinterpret_cast<uintptr_t>(weight) & 15) != 0;
+    p.tiles = (V + kCeScoreTile - 1) / kCeScoreTile;
+    size_t at = 0;
+    auto take = [&](size_t b) {
+        const size_t o = at;
+        at += align256(b);
+        return o;
+    };
+    p.sums = take(sizeof(float2) * (size_t)((N + kMergeRows - 1) / kMergeRows));
+    p.xp = take((size_t)p.planes * p.Np * p.ld * 2);
+    p.wp = take(p.pack_w ? (size_t)p.planes * V * p.ld * 2 : 0);
+    if (!backward) {
+        p.part = take(sizeof(float2) * (size_t)p.tiles * p.Np);
+        p.psum = take(o.eps > 0.f ? sizeof(float) * (size_t)p.tiles * p.Np : 0);
+        p.zt = take(sizeof(float) * (size_t)p.Np);
+        p.bytes = at;
+        return p;
+    }
+    p.gmax = take(sizeof(float));
+    p.xs = take(o.reduction == kCeNone ? (size_t)p.planes * p.Np * p.ld * 2 : 0);
+    // pieces of P: all rows while at least 4096 classes (or all) fit, else
+    // 8192 classes (or all) and the rows that fit
+    const long long Vp = up(V, 64);
+    const long long fit = (long long)(kPieceBytes / (2 * p.planes * p.Np)) / 256 * 256;
+    if (fit >= std::min(Vp, 4096LL)) {
+        p.piece_rows = p.Np;
+        p.ldp = std::min(Vp, fit);
+    } else {
+        p.ldp = std::min(Vp, 8192LL);
+        p.piece_rows = std::max(
+            (long long)kCeTileM,
+            (long long)(kPieceBytes / (2 * p.planes * p.ldp)) / kCeTileM * kCeTileM);
+    }
+    p.piece_classes = (int)std::min((long long)V, p.ldp);
+    p.one_row_piece = p.piece_rows >= p.Np;
+    p.one_class_piece = p.piece_classes >= V;
+    p.piece_rows = std::min(p.piece_rows, p.Np);
+    p.p = take((size_t)p.planes * p.piece_rows * p.ldp * 2);
+    const long long tn = (D + 255) / 256;
+    p.split_x = splits_for(p.piece_rows / kCeTileM * tn, p.piece_classes);
+    p.split_w = splits_for(up(p.piece_classes, kCeTileM) / kCeTileM * tn, p.piece_rows);
+    p.dx = take(sizeof(float) * (size_t)p.split_x * p.piece_rows * D);
+    p.dw = take(sizeof(float) * (size_t)p.split_w * (p.one_row_piece ? p.piece_classes : V) * D);
+    p.bytes = at;
+    return p;
+}
+
+template <typename T>
+cudaError_t pack(const Plan &p, bool rows, const void *src, const State &s, const float *g,
+                 const float *gmax, void *dst, cudaStream_t st) {
+    const RowScale sc{g, gmax};
+    if (rows)
+        pack_kernel<T, true><<<blocks8(p.Np), 256, 0, st>>>(
+            p.Np, p.D, p.ld, p.Np * p.ld, static_cast<const T *>(src), s.idx, s.total, sc, dst);
+    else
+        pack_kernel<T, false><<<blocks8(p.V), 256, 0, st>>>(
+            p.V, p.D, p.ld, p.V * p.ld, static_cast<const T *>(src), nullptr, nullptr, sc, dst);
+    count_launches(1);
+    return cudaGetLastError();
+}
+
+cudaError_t pack_any(const Plan &p, bool rows, const void *src, const State &s,
+                     const float *g, const float *gmax, void *dst, cudaStream_t st) {
+    switch (p.type) {
+        case kCeF32: return pack<float>(p, rows, src, s, g, gmax, dst, st);
+        case kCeBf16: return pack<__nv_bfloat16>(p, rows, src, s, g, gmax, dst, st);
+        default: return pack<__half>(p, rows, src, s, g, gmax, dst, st);
+    }
+}
+
+template <typename T>
+cudaError_t finish_grad(const Plan &p, bool rows, long long row0, long long n,
+                        const float *acc, long long split, int splits, const State &s,
+                        const float *g, int reduction, float inv_p, const float *gmax,
+                        void *dst, cudaStream_t st) {
+    if (rows)
+        finish_grad_kernel<T, true><<<blocks8(n), 256, 0, st>>>(
+            row0, n, p.D, acc, split, splits, s.idx, s.total, g, s.count, reduction, inv_p,
+            gmax, static_cast<T *>(dst));
+    else
+        finish_grad_kernel<T, false><<<blocks8(n), 256, 0, st>>>(
+            0, n, p.D, acc, split, splits, nullptr, nullptr, g, s.count, reduction, inv_p,
+            gmax, static_cast<T *>(dst) + row0 * p.D);
+    count_launches(1);
+    return cudaGetLastError();
+}
+
+cudaError_t finish_any(const Plan &p, bool rows, long long row0, long long n,
+                       const float *acc, long long split, int splits, const State &s,
+                       const float *g, int reduction, float inv_p, const float *gmax,
+                       void *dst, cudaStream_t st) {
+#define GSV_CE_T(T) \
+    finish_grad<T>(p, rows, row0, n, acc, split, splits, s, g, reduction, inv_p, gmax, dst, st)
+    switch (p.type) {
+        case kCeF32: return GSV_CE_T(float);
+        case kCeBf16: return GSV_CE_T(__nv_bfloat16);
+        default: return GSV_CE_T(__half);
+    }
+#undef GSV_CE_T
+}
+
+#define GSV_CE_TRY(expr)                              \
+    do {                                              \
+        const cudaError_t err_ = (expr);              \
+        if (err_ != cudaSuccess) return err_;         \
+    } while (0)
+
+CeGemm gemm_of(const Plan &p, const State &s, const void *weight, unsigned char *ws,
+               const CeOpt &o) {
+    CeGemm g{};
+    g.bf16 = p.type != kCeF16;
+    g.planes = p.planes;
+    g.V = p.V;
+    g.D = p.D;
+    g.opt = o;
+    g.splits = 1;
+    g.X = {ws + p.xp, p.Np, p.D, p.ld, p.Np * p.ld};
+    g.W = p.pack_w ? CeMat{ws + p.wp, p.V, p.D, p.ld, p.V * p.ld}
+                   : CeMat{weight, p.V, p.D, p.D, 0};
+    g.count = s.total;
+    g.lab = s.lab;
+    g.idx = s.idx;
+    return g;
+}
+
+}  // namespace
+
+size_t linear_ce_state_bytes(long long rows) { return (size_t)state_words(rows) * 4; }
+
+size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
+                                 const CeOpt &o) {
+    return make_plan(N, V, D, type, nullptr, backward, o).bytes;
+}
+
+cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
+                                     const void *features, const void *weight,
+                                     const long long *labels, const CeOpt &o, float *loss,
+                                     void *state, void *workspace, cudaStream_t st) {
+    const Plan p = make_plan(N, V, D, type, weight, false, o);
+    const State s = state_of(state, N);
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    const int nb = (int)((p.Np + kIdxNT - 1) / kIdxNT);
+    if (o.reduction == kCeNone)
+        GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
+    if (nb > 1) {
+        count_labels_kernel<<<nb, kIdxNT, 0, st>>>(N, labels, o.ignore, s.counts);
+        count_launches(1);
+    }
+    index_kernel<<<nb, kIdxNT, 0, st>>>(N, p.Np, V, labels, o.ignore, s.counts, nb, s.total,
+                                        s.idx, s.lab);
+    count_launches(1);
+    GSV_CE_TRY(cudaGetLastError());
+    GSV_CE_TRY(pack_any(p, true, features, s, nullptr, nullptr, ws + p.xp, st));
+    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, nullptr, nullptr, ws + p.wp, st));
+    CeGemm g = gemm_of(p, s, weight, ws, o);
+    g.product = kCeScores;
+    g.rows = p.Np;
+    g.nv = V;
+    g.part = reinterpret_cast<float2 *>(ws + p.part);
+    g.psum = o.eps > 0.f ? reinterpret_cast<float *>(ws + p.psum) : nullptr;
+    g.zt = reinterpret_cast<float *>(ws + p.zt);
+    GSV_CE_TRY(launch_ce_gemm(g, st));
+    const int mb = (int)((N + kMergeRows - 1) / kMergeRows);
+    float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
+    merge_kernel<<<mb, kMergeRows * kMergeSlices, 0, st>>>(
+        p.Np, p.tiles, V, g.part, g.psum, g.zt, s.total, s.idx, s.lab, labels, o, loss, s.lse,
+        s.count, sums);
+    count_launches(1);
+    GSV_CE_TRY(cudaGetLastError());
+    if (mb > 1) GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));
+    return cudaSuccess;
+}
+
+cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
+                                      const void *features, const void *weight,
+                                      const long long *labels, const CeOpt &o, void *state,
+                                      const float *grad_loss, void *grad_features,
+                                      void *grad_weight, void *workspace, cudaStream_t st) {
+    const Plan p = make_plan(N, V, D, type, weight, true, o);
+    const State s = state_of(state, N);
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    float *gmax = type == kCeF16 ? reinterpret_cast<float *>(ws + p.gmax) : nullptr;
+    const bool none = o.reduction == kCeNone;
+    GSV_CE_TRY(pack_any(p, true, features, s, nullptr, nullptr, ws + p.xp, st));
+    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, nullptr, nullptr, ws + p.wp, st));
+    if (none && grad_weight) {
+        if (gmax) {
+            GSV_CE_TRY(cudaMemsetAsync(gmax, 0, sizeof(float), st));
+            const int nb = (int)std::min<long long>(kSMs, (N + 1023) / 1024);
+            max_abs_kernel<<<nb, 256, 0, st>>>(grad_loss, s.idx, s.total, gmax);
+            count_launches(1);
+            GSV_CE_TRY(cudaGetLastError());
+        }
+        GSV_CE_TRY(pack_any(p, true, features, s, grad_loss, gmax, ws + p.xs, st));
+    }
+    if (grad_features) {
+        switch (type) {
+            case kCeF32:
+                zero_ignored_kernel<<<blocks8(N), 256, 0, st>>>(
+                    N, D, labels, o.ignore, static_cast<float *>(grad_features));
+                break;
+            default:
+                zero_ignored_kernel<<<blocks8(N), 256, 0, st>>>(
+                    N, D, labels, o.ignore, static_cast<__half *>(grad_features));
+        }
+        count_launches(1);
+        GSV_CE_TRY(cudaGetLastError());
+    }
+    CeGemm g = gemm_of(p, s, weight, ws, o);
+    g.lse = s.lse;
+    g.p_out = ws + p.p;
+    g.p_scale = p_scale_of(type, o);
+    const float inv_p = 1.f / g.p_scale;
+    float *dx = reinterpret_cast<float *>(ws + p.dx);
+    float *dw = reinterpret_cast<float *>(ws + p.dw);
+    for (long long r0 = 0; r0 < p.Np; r0 += p.piece_rows) {
+        g.row0 = r0;
+        g.rows = std::min(p.piece_rows, p.Np - r0);
+        for (int v0 = 0; v0 < V; v0 += p.piece_classes) {
+            g.v0 = v0;
+            g.nv = std::min(p.piece_classes, V - v0);
+            g.P = {ws + p.p, g.rows, g.nv, p.ldp, p.piece_rows * p.ldp};
+            g.product = kCeProbs;
+            GSV_CE_TRY(launch_ce_gemm(g, st));
+            if (grad_features) {
+                CeGemm x = g;
+                x.product = kCeGradX;
+                x.out = dx;
+                x.out_split = p.piece_rows * D;
+                x.splits = p.split_x;
+                x.add = v0 > 0;
+                GSV_CE_TRY(launch_ce_gemm(x, st));
+            }
+            if (grad_weight) {
+                CeGemm w = g;
+                w.product = kCeGradW;
+                if (none) w.X.ptr = ws + p.xs;
+                w.out = p.one_row_piece ? dw : dw + (long long)v0 * D;
+                w.out_split = (long long)(p.one_row_piece ? p.piece_classes : V) * D;
+                w.splits = p.split_w;
+                w.add = r0 > 0;
+                GSV_CE_TRY(launch_ce_gemm(w, st));
+                if (p.one_row_piece)
+                    GSV_CE_TRY(finish_any(p, false, v0, g.nv, dw, w.out_split, p.split_w, s,
+                                          grad_loss, o.reduction, inv_p, gmax, grad_weight, st));
+            }
+        }
+        if (grad_features)
+            GSV_CE_TRY(finish_any(p, true, r0, g.rows, dx, p.piece_rows * D, p.split_x, s,
+                                  grad_loss, o.reduction, inv_p, gmax, grad_features, st));
+    }
+    if (grad_weight && !p.one_row_piece)
+        GSV_CE_TRY(finish_any(p, false, 0, V, dw, (long long)V * D, p.split_w, s, grad_loss,
+                              o.reduction, inv_p, gmax, grad_weight, st));
+    return cudaSuccess;
+}
+
+}  // namespace gsv

@@ -13,6 +13,11 @@ kernels:
   flow from the loss to the Gaussians (the volume output is not
   differentiable). With a ``SlabPlan`` it voxelizes one z-slab and, in the
   backward, all-reduces the per-Gaussian gradients over the process group.
+
+Further losses of a volume: ``fused_ssim3d`` and ``tv3d``, and the class
+losses ``softmax_cross_entropy`` (the channels are class scores) and
+``linear_cross_entropy`` (the channels are features, scored against a table of
+class embeddings without keeping the scores).
 """
 from __future__ import annotations
 
@@ -20,9 +25,10 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import cuda as _C
-from ._lib import check, i3, lib
+from ._lib import CeOptions, check, i3, lib
 from .slab import SlabPlan, allreduce_gaussian_grads, tile_layers
 
 
@@ -273,3 +279,217 @@ def tv3d(vol: torch.Tensor, isotropic: bool = True, eps: float = 1e-8) -> torch.
     if isotropic and not eps > 0:
         raise ValueError("isotropic TV needs eps > 0")
     return _Tv3d.apply(vol, isotropic, eps)
+
+
+# ---------------------------------------------------------- class losses
+
+_CE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_CE_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _ce_args(named, labels, ignore_index, label_smoothing, softcap, z_loss,
+             reduction):
+    """Checks what both class losses take; returns (labels as contiguous
+    int64, options)."""
+    first_name, first = named[0]
+    for name, t in named:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor")
+        if t.dtype not in _CE_DTYPES:
+            raise RuntimeError(f"{name} must be float32, bfloat16 or float16, "
+                               f"got {t.dtype}")
+        if t.dtype != first.dtype or t.device != first.device:
+            raise RuntimeError(f"{name} must share dtype and device with "
+                               f"{first_name}")
+    if first.dim() < 1:
+        raise ValueError(f"{first_name} must have at least one dimension")
+    if labels.device != first.device:
+        raise RuntimeError(f"labels must be on the device of {first_name}")
+    if labels.dtype.is_floating_point or labels.dtype.is_complex \
+            or labels.dtype == torch.bool:
+        raise RuntimeError(f"labels must be integers, got {labels.dtype}")
+    if labels.shape != first.shape[:-1]:
+        raise ValueError(f"labels shape {tuple(labels.shape)} != "
+                         f"{tuple(first.shape[:-1])}")
+    if reduction not in _CE_REDUCTIONS:
+        raise ValueError(f"unsupported reduction {reduction!r}")
+    if not 0.0 <= label_smoothing < 1.0:
+        raise ValueError("label_smoothing must be in [0, 1)")
+    if not (0.0 <= softcap <= 1e30 and 0.0 <= z_loss <= 1e30):
+        raise ValueError("softcap and z_loss must be finite and >= 0")
+    opt = CeOptions(int(ignore_index), label_smoothing, softcap, z_loss,
+                    _CE_REDUCTIONS[reduction])
+    return labels.to(torch.int64).contiguous(), opt
+
+
+def _ce_loss_out(labels, opt, dev):
+    shape = labels.shape if opt.reduction == 0 else ()
+    return torch.empty(shape, dtype=torch.float32, device=dev)
+
+
+def _ce_grad_loss(grad_loss):
+    return grad_loss.to(torch.float32).contiguous()
+
+
+class _SoftmaxCe(Function):
+    @staticmethod
+    def forward(ctx, scores, labels, opt):
+        dev, V = scores.device, int(scores.shape[-1])
+        rows = labels.numel()
+        loss = _ce_loss_out(labels, opt, dev)
+        ctx.opt = opt
+        if rows == 0:
+            ctx.save_for_backward(scores)
+            return loss.zero_()
+        stats = torch.empty((rows + 1,), dtype=torch.float32, device=dev)
+        nbytes = lib.gsv_softmax_ce_workspace_bytes(rows, V)
+        with torch.cuda.device(dev):
+            ws = _C._workspace(nbytes, dev)
+            check(lib.gsv_softmax_ce_forward(
+                rows, V, _CE_DTYPES[scores.dtype], scores.data_ptr(),
+                labels.data_ptr(), opt, loss.data_ptr(), stats.data_ptr(),
+                stats.data_ptr() + 4 * rows, ws.data_ptr(), ws.numel(),
+                _C._stream(dev)))
+        ctx.save_for_backward(scores, labels, stats)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        if len(ctx.saved_tensors) == 1:
+            return torch.zeros_like(ctx.saved_tensors[0]), None, None
+        scores, labels, stats = ctx.saved_tensors
+        dev, rows, V = scores.device, labels.numel(), int(scores.shape[-1])
+        grad_loss = _ce_grad_loss(grad_loss)
+        g = torch.empty_like(scores)
+        with torch.cuda.device(dev):
+            check(lib.gsv_softmax_ce_backward(
+                rows, V, _CE_DTYPES[scores.dtype], scores.data_ptr(),
+                labels.data_ptr(), ctx.opt, stats.data_ptr(),
+                stats.data_ptr() + 4 * rows, grad_loss.data_ptr(),
+                g.data_ptr(), _C._stream(dev)))
+        return g, None, None
+
+
+def softmax_cross_entropy(
+    scores: torch.Tensor,
+    labels: torch.Tensor,
+    ignore_index: int = -100,
+    label_smoothing: float = 0.0,
+    softcap: float = 0.0,
+    z_loss: float = 0.0,
+    reduction: str = "mean",
+) -> torch.Tensor:
+    """Softmax cross entropy of class scores against labels, e.g. of a
+    [Z, Y, X, C] volume whose channels are class scores.
+
+    With z = scores (or softcap * tanh(scores / softcap)) over the V classes
+    of the last dimension and lse = log sum exp z, a row's loss is
+    ``lse - (1 - s) z[label] - s mean(z) + z_loss lse^2`` with s =
+    label_smoothing.
+
+    Args:
+        scores: [..., V] float32, bfloat16 or float16.
+        labels: [...] integers. Rows labelled ``ignore_index`` have loss 0 and
+            a zero gradient whatever they hold; any other label outside
+            [0, V) makes the row's loss and gradient NaN.
+        ignore_index, label_smoothing, softcap, z_loss: see above.
+        reduction: "mean" over the labelled rows (0 if there is none), "sum"
+            or "none" (the losses in the shape of labels).
+    Returns:
+        float32 loss, differentiable once in scores (gradient in their type).
+    """
+    labels, opt = _ce_args([("scores", scores)], labels, ignore_index,
+                           label_smoothing, softcap, z_loss, reduction)
+    if scores.shape[-1] < 1:
+        raise ValueError("scores must have at least one class")
+    return _SoftmaxCe.apply(scores.contiguous(), labels, opt)
+
+
+class _LinearCe(Function):
+    @staticmethod
+    def forward(ctx, features, weight, labels, opt):
+        dev = features.device
+        rows, (V, D) = labels.numel(), weight.shape
+        loss = _ce_loss_out(labels, opt, dev)
+        ctx.opt = opt
+        if rows == 0:
+            ctx.save_for_backward(features, weight)
+            return loss.zero_()
+        dtype = _CE_DTYPES[features.dtype]
+        with torch.cuda.device(dev):
+            state = _C._workspace(lib.gsv_linear_ce_state_bytes(rows), dev)
+            ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
+                rows, V, D, dtype, opt, 0), dev)
+            check(lib.gsv_linear_ce_forward(
+                rows, V, D, dtype, features.data_ptr(), weight.data_ptr(),
+                labels.data_ptr(), opt, loss.data_ptr(), state.data_ptr(),
+                ws.data_ptr(), ws.numel(), _C._stream(dev)))
+        ctx.save_for_backward(features, weight, labels, state)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if len(ctx.saved_tensors) == 2:
+            return (*(torch.zeros_like(t) if need else None for t, need in
+                      zip(ctx.saved_tensors, (need_x, need_w))), None, None)
+        features, weight, labels, state = ctx.saved_tensors
+        dev = features.device
+        rows, (V, D) = labels.numel(), weight.shape
+        dtype = _CE_DTYPES[features.dtype]
+        grad_loss = _ce_grad_loss(grad_loss)
+        gx = torch.empty_like(features) if need_x else None
+        gw = torch.empty_like(weight) if need_w else None
+        with torch.cuda.device(dev):
+            ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
+                rows, V, D, dtype, ctx.opt, 1), dev)
+            check(lib.gsv_linear_ce_backward(
+                rows, V, D, dtype, features.data_ptr(), weight.data_ptr(),
+                labels.data_ptr(), ctx.opt, state.data_ptr(),
+                grad_loss.data_ptr(), _C._ptr(gx), _C._ptr(gw), ws.data_ptr(),
+                ws.numel(), _C._stream(dev)))
+        return gx, gw, None, None
+
+
+def linear_cross_entropy(
+    features: torch.Tensor,
+    weight: torch.Tensor,
+    labels: torch.Tensor,
+    ignore_index: int = -100,
+    label_smoothing: float = 0.0,
+    softcap: float = 0.0,
+    z_loss: float = 0.0,
+    reduction: str = "mean",
+) -> torch.Tensor:
+    """``softmax_cross_entropy(features @ weight.T, labels, ...)`` without the
+    scores in memory: e.g. a [Z, Y, X, C] volume decoded by a table of V class
+    embeddings, or the hidden states of a model against a vocabulary.
+
+    The scores are products of the inputs summed in float32 and are not
+    rounded to the inputs' type. The forward keeps 12 bytes a row; the
+    backward computes the scores again in pieces, with a workspace of a few
+    hundred MB beside float32 copies of what it accumulates. With
+    ``reduction="none"`` and no gradient it is minus the log-probability of
+    each row's label.
+
+    Args:
+        features: [..., D] float32, bfloat16 or float16.
+        weight: [V, D] of the same type.
+        labels, ignore_index, label_smoothing, softcap, z_loss, reduction: as
+            for ``softmax_cross_entropy``.
+    Returns:
+        float32 loss, differentiable once in features and weight (gradients
+        in their type).
+    """
+    labels, opt = _ce_args([("features", features), ("weight", weight)], labels,
+                           ignore_index, label_smoothing, softcap, z_loss,
+                           reduction)
+    if weight.dim() != 2 or weight.shape[1] != features.shape[-1]:
+        raise ValueError(f"weight shape {tuple(weight.shape)} does not match "
+                         f"features {tuple(features.shape)}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError("weight must have at least one class and one channel")
+    return _LinearCe.apply(features.contiguous(), weight.contiguous(), labels,
+                           opt)

@@ -497,6 +497,76 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
                                 const float *loss, const float *flags,
                                 float *out, void *stream);
 
+/*
+ * Class losses: softmax cross entropy of scores in memory (gsv_softmax_ce_*)
+ * and of the scores features . weight^T, which are never in memory
+ * (gsv_linear_ce_*), each with its gradient. No reference counterpart.
+ *
+ * Of row i with scores s_ij (capped to z = cap tanh(s / cap) when softcap =
+ * cap > 0, else z = s), label y and lse_i = log sum_j exp z_ij:
+ *   loss_i = lse_i - (1 - eps) z_iy - eps / classes * sum_j z_ij
+ *            + z_loss lse_i^2,         eps = label_smoothing.
+ * A row whose label is ignore_index has loss 0 and a zero gradient, whatever
+ * it holds; any other label outside [0, classes) makes the row's loss and the
+ * gradients that it enters NaN. GSV_REDUCE_MEAN divides by the number of
+ * labelled rows (by 1 if there is none).
+ *
+ * scores [rows, classes], features [rows, channels] and weight [classes,
+ * channels] are contiguous and of one type (gsv_dtype), labels int64 [rows],
+ * loss float32 ([1], or [rows] with GSV_REDUCE_NONE), grad_loss float32 of
+ * the same size. Arithmetic is float32 or wider; the products of 16-bit
+ * types are exact and summed in float32, those of float32 are taken with all
+ * their bits. 1 <= rows < 2^31 - 1024, 1 <= classes <= 2^30, 1 <= channels <=
+ * 2^20.
+ *
+ * The forward leaves what the backward needs in `lse` / `count` (device
+ * float32 [rows] and [1]) or in `state` (gsv_linear_ce_state_bytes, 16-byte
+ * aligned); the backward is called with the same sizes, inputs and options.
+ * Workspaces are scratch of one call, 256-byte aligned. A null gradient output
+ * of gsv_linear_ce_backward is not computed.
+ */
+enum gsv_dtype { GSV_F32 = 0, GSV_BF16 = 1, GSV_F16 = 2 };
+enum gsv_reduction { GSV_REDUCE_NONE = 0, GSV_REDUCE_SUM = 1, GSV_REDUCE_MEAN = 2 };
+
+typedef struct gsv_ce_options {
+    int64_t ignore_index;
+    float label_smoothing; /* 0 <= . < 1 */
+    float softcap;         /* >= 0; 0: no cap */
+    float z_loss;          /* >= 0 */
+    int32_t reduction;     /* gsv_reduction */
+} gsv_ce_options;
+
+GSV_API size_t gsv_softmax_ce_workspace_bytes(int64_t rows, int32_t classes);
+GSV_API int gsv_softmax_ce_forward(int64_t rows, int32_t classes, int32_t dtype,
+                                   const void *scores, const int64_t *labels,
+                                   const gsv_ce_options *options, float *loss,
+                                   float *lse, float *count, void *workspace,
+                                   size_t workspace_bytes, void *stream);
+GSV_API int gsv_softmax_ce_backward(int64_t rows, int32_t classes, int32_t dtype,
+                                    const void *scores, const int64_t *labels,
+                                    const gsv_ce_options *options, const float *lse,
+                                    const float *count, const float *grad_loss,
+                                    void *grad_scores, void *stream);
+
+GSV_API size_t gsv_linear_ce_state_bytes(int64_t rows);
+GSV_API size_t gsv_linear_ce_workspace_bytes(int64_t rows, int32_t classes,
+                                             int32_t channels, int32_t dtype,
+                                             const gsv_ce_options *options,
+                                             int32_t backward);
+GSV_API int gsv_linear_ce_forward(int64_t rows, int32_t classes, int32_t channels,
+                                  int32_t dtype, const void *features,
+                                  const void *weight, const int64_t *labels,
+                                  const gsv_ce_options *options, float *loss,
+                                  void *state, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+GSV_API int gsv_linear_ce_backward(int64_t rows, int32_t classes, int32_t channels,
+                                   int32_t dtype, const void *features,
+                                   const void *weight, const int64_t *labels,
+                                   const gsv_ce_options *options, void *state,
+                                   const float *grad_loss, void *grad_features,
+                                   void *grad_weight, void *workspace,
+                                   size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
