@@ -83,6 +83,7 @@ cudaError_t launch_vox_backward_tc(const Geom &g, const int *ids,
                                    const float *grad_loss, float inv_denom,
                                    cudaStream_t stream);
 int tc_error_flag(bool clear);
+int ce_error_flag(bool clear);
 int peer_error_flag(bool clear);
 cudaError_t launch_peer_barrier(int world, int rank, const long long *sig_ptrs,
                                 int *epoch, cudaStream_t stream);
@@ -137,7 +138,7 @@ void enable_large_smem();
 size_t softmax_ce_workspace_bytes(long long rows, int V);
 cudaError_t launch_softmax_ce(bool fwd, int type, long long rows, int V, const void *scores,
                               const long long *labels, const CeOpt &o, float *loss,
-                              float *lse, float *count, const float *grad_loss, void *grad,
+                              float2 *lse, float *count, const float *grad_loss, void *grad,
                               void *ws, cudaStream_t st);
 size_t linear_ce_state_bytes(long long rows);
 size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
@@ -797,9 +798,10 @@ int gsv_device_error(int32_t *flag_out, int32_t clear) {
     GSV_REQUIRE(flag_out, GSV_ERR_INVALID_ARGUMENT, "%s: flag_out is null", fn);
     const int a = gsv::tc_error_flag(clear != 0);
     const int b = gsv::peer_error_flag(clear != 0);
-    GSV_REQUIRE(a >= 0 && b >= 0, GSV_ERR_CUDA, "%s: could not read the device flags",
-                fn);
-    *flag_out = (a ? 1 : 0) | (b ? 2 : 0);
+    const int c = gsv::ce_error_flag(clear != 0);
+    GSV_REQUIRE(a >= 0 && b >= 0 && c >= 0, GSV_ERR_CUDA,
+                "%s: could not read the device flags", fn);
+    *flag_out = (a ? 1 : 0) | (b ? 2 : 0) | (c ? 4 : 0);
     return GSV_OK;
 }
 
@@ -1123,9 +1125,11 @@ int gsv_softmax_ce_forward(int64_t rows, int32_t classes, int32_t dtype, const v
     const size_t need = gsv_softmax_ce_workspace_bytes(rows, classes);
     GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
                 "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
+    GSV_REQUIRE((reinterpret_cast<uintptr_t>(lse) & 7) == 0, GSV_ERR_INVALID_ARGUMENT,
+                "%s: lse not aligned", fn);
     return cuda_status(gsv::launch_softmax_ce(true, dtype, rows, classes, scores,
-                                              as_ll(labels), ce_opt(options), loss, lse,
-                                              count, nullptr, nullptr, ws, as_stream(stream)),
+                                              as_ll(labels), ce_opt(options), loss,
+                                              reinterpret_cast<float2 *>(lse), count, nullptr, nullptr, ws, as_stream(stream)),
                        fn);
 }
 
@@ -1139,7 +1143,8 @@ int gsv_softmax_ce_backward(int64_t rows, int32_t classes, int32_t dtype, const 
                 GSV_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
     return cuda_status(gsv::launch_softmax_ce(
                            false, dtype, rows, classes, scores, as_ll(labels),
-                           ce_opt(options), nullptr, const_cast<float *>(lse),
+                           ce_opt(options), nullptr,
+                           reinterpret_cast<float2 *>(const_cast<float *>(lse)),
                            const_cast<float *>(count), grad_loss, grad_scores, nullptr,
                            as_stream(stream)),
                        fn);

@@ -45,8 +45,9 @@ __device__ __forceinline__ float ce_cap(float s, float cap) {
     return cap > 0.f ? cap * tanhf(s / cap) : s;
 }
 
-// Running maximum, sum of exponentials (relative to the maximum) and plain
-// sum of a row's scores.
+// Running maximum m, sum of exp(z - m) and plain sum of a row's scores. The
+// difference is taken before the product with log2 e: a maximum that stays
+// rescales by exactly 1, and rows of huge scores keep their digits.
 struct CeAcc {
     float m, s, sz;
     __device__ __forceinline__ void init() {
@@ -54,29 +55,35 @@ struct CeAcc {
         s = 0.f;
         sz = 0.f;
     }
-    // m stays -inf while every score is -inf: the exponent is taken against
-    // 0 then, so that each term is exp(-inf) = 0 and not NaN
+    // m stays -inf while every score is -inf: exponents are taken against 0
+    // then, so that each term is exp(-inf) = 0 and not NaN
     __device__ __forceinline__ static float base(float m) {
-        return m == ce_neg_inf() ? 0.f : m * kLog2e;
+        return m == ce_neg_inf() ? 0.f : m;
     }
     __device__ __forceinline__ void merge(float om, float os, float osz) {
-        const float nm = fmaxf(m, om);
-        const float b = base(nm);
-        s = s * ex2(fmaf(m, kLog2e, -b)) + os * ex2(fmaf(om, kLog2e, -b));
+        const float nm = fmaxf(m, om), e = base(nm);
+        s = s * ex2((m - e) * kLog2e) + os * ex2((om - e) * kLog2e);
         m = nm;
         sz += osz;
     }
-    __device__ __forceinline__ float lse() const {
-        return (m == ce_neg_inf() ? 0.f : m) + logf(s);
-    }
+    // A row's logsumexp, kept as (maximum, log2 of the sum): of scores at the
+    // type's lowest value the one alone would lose the other.
+    __device__ __forceinline__ float2 lse() const { return make_float2(base(m), log2f(s)); }
 };
 
+__device__ __forceinline__ float ce_lse(float2 l) { return fmaf(l.y, kCeLn2, l.x); }
+
+// probability of score z in a row of logsumexp l
+__device__ __forceinline__ float ce_prob(float z, float2 l) {
+    return ex2(fmaf(z - l.x, kLog2e, -l.y));
+}
+
 // loss of a labelled row
-__device__ __forceinline__ float ce_row_loss(float lse, float zy, float sz, int V,
+__device__ __forceinline__ float ce_row_loss(float2 lse, float zy, float sz, int V,
                                              const CeOpt &o) {
-    float l = lse - (1.f - o.eps) * zy;
-    if (o.eps > 0.f) l -= o.eps / (float)V * sz;
-    if (o.zeta > 0.f) l += o.zeta * lse * lse;
+    float l = fmaf(1.f - o.eps, lse.x - zy, lse.y * kCeLn2);
+    if (o.eps > 0.f) l += o.eps * (lse.x - sz / (float)V);
+    if (o.zeta > 0.f) l += o.zeta * ce_lse(lse) * ce_lse(lse);
     return l;
 }
 

@@ -1,145 +1,694 @@
-// The matrix products of the linear class loss: plain tiles on the CUDA
-// cores. A block computes 64 x 64 of the product from 16-deep slices staged
-// in shared memory as float32 (the planes of a float32 operand summed), then
-// each of 64 threads takes one row of the tile through the epilogue.
+// The matrix products of the linear class loss on the 5th-generation tensor
+// cores: 256 x 256 tiles by pairs of SMs (tcgen05 cta_group::2), operands
+// staged by TMA, accumulators in tensor memory, the loss in the epilogue.
+//
+// Work: a CTA pair takes units of the product one after another (persistent,
+// one CTA a SM). Each CTA stages its 128 rows of A and its half of B, 64 deep
+// a stage; the leader's MMA thread multiplies both halves. 256 x 256 tiles
+// need 32 KB of operands a stage and SM for 2 x 256 x 256 x 64 products, two
+// thirds of what 128 x 256 tiles of a single SM load: the L2 could not feed
+// those at the tensor cores' rate. Two accumulators alternate, so that the
+// epilogue of a tile (eight warps) runs under the next tile's products.
+//
+// Operand layouts: X W^T reads both operands along the contiguous axis
+// (K-major); the gradients sum over rows or classes, the strided axis, and
+// read P, W and X in place as MN-major tiles. No operand is transposed.
+//
+// Waits are bounded: on a timeout a role sets g_ce_error, leaves its loop and
+// the kernel ends, its tensor memory freed; the result is invalid.
+#include <cuda.h>
+
 #include "ce_gemm.cuh"
 
 namespace gsv {
+
+// Nonzero after a product gave up on a barrier wait; read and cleared
+// through the C ABI (gsv_device_error).
+__device__ int g_ce_error = 0;
+
 namespace {
 
-constexpr int kT = 64, kKB = 16;
+constexpr int kStages = 6;
+constexpr int kDepth = 64;                       // K a stage
+constexpr int kABytes = 128 * kDepth * 2;        // per CTA
+constexpr int kStageBytes = 2 * kABytes;         // A and B halves
+constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (4 + kEpiWarps) * 32;
+constexpr int kCols = 512;
+constexpr int kSpinLimit = 1 << 24;
 
-__device__ __forceinline__ float load16(const void *p, long long i, bool bf16) {
-    return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i])
-                : __half2float(static_cast<const __half *>(p)[i]);
+struct Barriers {
+    uint64_t full[kStages], empty[kStages], tfull[2], tempty[2];
+    uint32_t tmem;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-
-__device__ __forceinline__ float at(const CeMat &m, long long r, long long c, int planes,
-                                    bool bf16) {
-    if (r >= m.rows || c >= m.cols) return 0.f;
-    float v = 0.f;
-    for (int p = planes - 1; p >= 0; --p)
-        v += load16(m.ptr, p * m.plane + r * m.ld + c, bf16);
-    return v;
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
 }
-
-__global__ void __launch_bounds__(256)
-gemm_kernel(CeGemm g) {
-    __shared__ float As[kKB][kT + 1], Bs[kKB][kT + 1], C[kT][kT + 1];
-    const long long m0 = (long long)blockIdx.x * kT, n0 = (long long)blockIdx.y * kT;
-    long long live = g.rows;
-    if (g.count) live = max(0LL, min(live, (long long)*g.count - g.row0));
-    const bool scores = g.product <= kCeProbs;
-    long long k0 = 0, k1 = scores ? g.D : g.product == kCeGradX ? g.nv : live;
-    // the probabilities are written (as zeros) up to whole 128-row tiles
-    if (g.product != kCeGradW && m0 >= (live + 127) / 128 * 128) return;
-    if (!scores) {
-        const long long per = ((k1 + g.splits - 1) / g.splits + kKB - 1) / kKB * kKB;
-        k0 = min(k1, per * blockIdx.z);
-        k1 = min(k1, k0 + per);
+// address of the leader's copy of a barrier
+__device__ __forceinline__ uint32_t in_leader(uint32_t a) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ void bar_init(uint64_t *b, int n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(n));
+}
+__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity) {
+    const uint32_t a = smem_addr(b);
+    for (int it = 0; it < kSpinLimit; ++it) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (done) return true;
     }
-    float acc[4][4] = {};
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    for (long long k = k0; k < k1; k += kKB) {
-        for (int e = threadIdx.x; e < kKB * kT; e += 256) {
-            const int i = e % kT, kk = e / kT;
-            float a = 0.f, b = 0.f;
-            if (k + kk < k1) {
-                if (scores) {
-                    a = at(g.X, g.row0 + m0 + i, k + kk, g.planes, g.bf16);
-                    b = at(g.W, g.v0 + n0 + i, k + kk, g.planes, g.bf16);
-                } else if (g.product == kCeGradX) {
-                    a = at(g.P, m0 + i, k + kk, g.planes, g.bf16);
-                    b = at(g.W, g.v0 + k + kk, n0 + i, g.planes, g.bf16);
-                } else {
-                    a = at(g.P, k + kk, m0 + i, g.planes, g.bf16);
-                    b = at(g.X, g.row0 + k + kk, n0 + i, g.planes, g.bf16);
+    atomicExch(&g_ce_error, 1);
+    return false;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
+                 "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void fence_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+
+// box of 64 columns from column x, rows from y on, plane z, into shared
+// memory at dst; its bytes are counted at the leader's barrier
+__device__ __forceinline__ void tma_load(const CUtensorMap *map, uint32_t dst, uint32_t bar,
+                                         int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile"
+        ".mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// Shared-memory descriptors of 128-byte-swizzled tiles (8 rows of 128 bytes
+// repeat every 1024). K-major: rows of the tile, 64 K each; MN-major: rows
+// of K, 64 of M or N each, the next 64 in another box 8 KB on.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, bool mn_major) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(mn_major ? 8192 >> 4 : 1) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// 16 K further: 32 bytes of a row, or 16 rows
+__device__ __forceinline__ uint64_t k_step(bool mn_major) { return mn_major ? 128 : 2; }
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                    uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// arrives at the barrier of both CTAs when the MMAs so far are done
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster"
+        ".multicast::cluster.b64 [%0], %1;"
+        ::"r"(smem_addr(bar)), "h"((unsigned short)3)
+        : "memory");
+}
+
+__device__ __forceinline__ void load32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void load_wait(uint32_t (&r)[32]) {
+    // the registers pass through, so that no use moves above the wait
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
+                   "+r"(r[27]), "+r"(r[28])
+                 ::"memory");
+    asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+__device__ __forceinline__ void store8(void *p, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void fetch8(const float *p, float *v) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]),
+                   "=f"(v[6]), "=f"(v[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return reinterpret_cast<const uint32_t &>(h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return reinterpret_cast<const uint32_t &>(h);
+}
+
+// The grid's work, the same for every role: units (m tile, n tile, split or
+// run), each `tiles` accumulators long.
+struct Work {
+    int mtiles, ntiles, units;
+    int kblocks;          // 64-deep blocks a plane pair
+    long long K;
+    long long live;       // rows in use of the piece
+};
+
+template <int PRODUCT>
+__device__ __forceinline__ Work work_of(const CeGemm &g, int nt) {
+    Work w;
+    w.live = g.rows;
+    if (g.count) w.live = max(0LL, min(w.live, (long long)*g.count - g.row0));
+    const long long M = PRODUCT == kCeGradW ? g.nv : w.live;
+    w.mtiles = (int)((M + kCeTileM - 1) / kCeTileM);
+    w.ntiles = ((PRODUCT <= kCeProbs ? g.nv : g.D) + nt - 1) / nt;
+    w.K = PRODUCT <= kCeProbs ? g.D : PRODUCT == kCeGradX ? g.nv : w.live;
+    w.kblocks = (int)((w.K + kDepth - 1) / kDepth);
+    w.units = w.mtiles * (PRODUCT == kCeScores ? g.runs : w.ntiles * g.splits);
+    return w;
+}
+
+struct Unit {
+    int m, n0, n1, split, k0, k1;  // n tiles [n0, n1), K blocks [k0, k1)
+};
+
+// m fastest: the pairs in flight share class tiles, and each keeps to rows
+// that stay in L2
+template <int PRODUCT>
+__device__ __forceinline__ Unit unit_of(const CeGemm &g, const Work &w, int u) {
+    Unit t;
+    t.m = u % w.mtiles;
+    u /= w.mtiles;
+    t.split = 0;
+    t.k0 = 0;
+    t.k1 = w.kblocks;
+    if (PRODUCT == kCeScores) {
+        t.n0 = (int)((long long)w.ntiles * u / g.runs);
+        t.n1 = (int)((long long)w.ntiles * (u + 1) / g.runs);
+        t.split = u;
+    } else {
+        t.n0 = u % w.ntiles;
+        t.n1 = t.n0 + 1;
+        t.split = u / w.ntiles;
+        t.k0 = (int)((long long)w.kblocks * t.split / g.splits);
+        t.k1 = (int)((long long)w.kblocks * (t.split + 1) / g.splits);
+    }
+    return t;
+}
+
+// Plane pairs of a float32 product, least first: (2,0) (0,2) (1,1) (1,0)
+// (0,1) (0,0). The pairs left out are below 2^-26 of the whole.
+__device__ __forceinline__ int pairs_of(int planes) { return planes == 3 ? 6 : 1; }
+__device__ __forceinline__ int plane_a(int planes, int p) {
+    return planes == 3 ? (0x001102 >> (4 * p)) & 3 : 0;
+}
+__device__ __forceinline__ int plane_b(int planes, int p) {
+    return planes == 3 ? (0x010120 >> (4 * p)) & 3 : 0;
+}
+
+template <int PRODUCT, bool CAP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const CeGemm g, const int nt) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ Barriers S;
+    // the same offset in both CTAs: the MMA reads both through one descriptor
+    const uint32_t smem0 = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    constexpr bool kAMn = PRODUCT == kCeGradW;
+    constexpr bool kBMn = PRODUCT >= kCeGradX;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            bar_init(&S.full[i], 1);
+            bar_init(&S.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&S.tfull[i], 1);
+            bar_init(&S.tempty[i], 2 * kEpiWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_addr(&S.tmem)),
+                     "r"(kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        fence_before();
+    }
+    __syncthreads();
+    cluster_sync();
+    fence_after();
+    const uint32_t tmem = S.tmem;
+    const Work w = work_of<PRODUCT>(g, nt);
+    const int pairs = pairs_of(g.planes);
+
+    if (warp == 0 && lane == 0) {
+        // ------------------------------------------------------ producer
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const uint32_t bytes = 2 * (kABytes + nt / 2 * kDepth * 2);
+        for (int u = first; ok && u < w.units; u += step) {
+            const Unit t = unit_of<PRODUCT>(g, w, u);
+            for (int n = t.n0; ok && n < t.n1; ++n) {
+                const int m_at = t.m * kCeTileM + (int)rank * 128;
+                const int n_at = n * nt + (int)rank * (nt / 2);
+                for (int p = 0; ok && p < pairs; ++p) {
+                    const int pa = plane_a(g.planes, p), pb = plane_b(g.planes, p);
+                    for (int k = t.k0; k < t.k1; ++k) {
+                        if (!bar_wait(&S.empty[stage], phase ^ 1)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t bar = in_leader(smem_addr(&S.full[stage]));
+                        const uint32_t a = smem0 + stage * kStageBytes, b = a + kABytes;
+                        if (rank == 0)
+                            asm volatile(
+                                "mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                                    smem_addr(&S.full[stage])),
+                                "r"(bytes)
+                                : "memory");
+                        const int kk = k * kDepth;
+                        if (kAMn) {
+                            tma_load(&map_a, a, bar, m_at, kk, pa);
+                            tma_load(&map_a, a + 8192, bar, m_at + 64, kk, pa);
+                        } else {
+                            const long long r0 = PRODUCT == kCeGradX ? 0 : g.row0;
+                            tma_load(&map_a, a, bar, kk, (int)(r0 + m_at), pa);
+                        }
+                        if (kBMn) {
+                            const int r0 = PRODUCT == kCeGradX ? g.v0 : (int)g.row0;
+                            for (int h = 0; h < nt / 2; h += 64)
+                                tma_load(&map_b, b + h * 128, bar, n_at + h, r0 + kk, pb);
+                        } else {
+                            tma_load(&map_b, b, bar, kk, g.v0 + n_at, pb);
+                        }
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
                 }
             }
-            As[kk][i] = a;
-            Bs[kk][i] = b;
         }
-        __syncthreads();
-        for (int kk = 0; kk < kKB; ++kk)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = fmaf(As[kk][ty * 4 + i], Bs[kk][tx * 4 + j], acc[i][j]);
-        __syncthreads();
-    }
-    if (!scores) {
-        const long long M = g.product == kCeGradX ? g.rows : g.nv;
-        float *out = g.out + blockIdx.z * g.out_split;
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const long long m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-                if (m < M && n < g.D)
-                    out[m * g.D + n] = (g.add ? out[m * g.D + n] : 0.f) + acc[i][j];
+        // Every load is consumed, and every arrival at this CTA's barriers
+        // has come, before the CTA may end.
+        for (int i = 0; ok && i < kStages; ++i) {
+            ok = bar_wait(&S.empty[stage], phase ^ 1);
+            if (++stage == kStages) {
+                stage = 0;
+                phase ^= 1;
             }
-        return;
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // ----------------------------------------------------------- MMA
+        // D float32, A and B bf16 or fp16, M = 256
+        const uint32_t type = g.bf16 ? 1u : 0u;
+        const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)kAMn << 15) |
+                               ((uint32_t)kBMn << 16) | ((uint32_t)(nt >> 3) << 17) |
+                               ((256u >> 4) << 24);
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int u = first; ok && u < w.units; u += step) {
+            const Unit t = unit_of<PRODUCT>(g, w, u);
+            if (t.k0 == t.k1) continue;
+            for (int n = t.n0; ok && n < t.n1; ++n) {
+                if (!bar_wait(&S.tempty[acc], acc_phase ^ 1)) {
+                    ok = false;
+                    break;
+                }
+                fence_after();
+                uint32_t accumulate = 0;
+                for (int p = 0; ok && p < pairs; ++p)
+                    for (int k = t.k0; k < t.k1; ++k) {
+                        if (!bar_wait(&S.full[stage], phase)) {
+                            ok = false;
+                            break;
+                        }
+                        fence_after();
+                        const uint32_t a = smem0 + stage * kStageBytes;
+                        uint64_t da = tile_desc(a, kAMn), db = tile_desc(a + kABytes, kBMn);
+                        // the last block may end early (its rest is zeros)
+                        const long long left = w.K - (long long)k * kDepth;
+                        const int steps = left >= kDepth ? 4 : (int)((left + 15) / 16);
+                        for (int i = 0; i < steps; ++i) {
+                            mma(tmem + acc * kCeTileN, da, db, idesc, accumulate);
+                            accumulate = 1;
+                            da += k_step(kAMn);
+                            db += k_step(kBMn);
+                        }
+                        commit(&S.empty[stage]);
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                commit(&S.tfull[acc]);
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1;
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------ epilogue
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t tlane = tmem + ((uint32_t)(q * 32) << 16);
+        const int chunks = (nt + 31) / 32;
+        const CeOpt o = g.opt;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        float scale = 1.f;
+        if (PRODUCT >= kCeGradX && g.dst) scale = ce_grad_scale(g.up);
+        for (int u = first; ok && u < w.units; u += step) {
+            const Unit t = unit_of<PRODUCT>(g, w, u);
+            const long long r = (long long)t.m * kCeTileM + rank * 128 + q * 32 + lane;
+            // per-row state
+            int y = kCeIgnored;
+            float top = ce_neg_inf(), s = 0.f, sz = 0.f;
+            float2 lse = make_float2(0.f, 0.f);
+            float kz = 1.f, e = 0.f, hit = 0.f;
+            if (PRODUCT <= kCeProbs && r < w.live) {
+                y = g.lab ? g.lab[g.row0 + r] : ce_label(g.labels[g.row0 + r], o.ignore, g.V);
+                if (PRODUCT == kCeProbs && y != kCeIgnored) {
+                    const long long src = g.idx ? g.idx[g.row0 + r] : g.row0 + r;
+                    lse = g.lse[src];
+                    float f = g.p_scale;
+                    if (g.grow) {
+                        f *= g.grow[src];
+                        if (g.gmax && *g.gmax > 0.f) f /= *g.gmax;
+                    }
+                    kz = (1.f + 2.f * o.zeta * ce_lse(lse)) * f;
+                    e = o.eps / (float)g.V * f;
+                    hit = (1.f - o.eps) * f;
+                }
+            }
+            for (int n = t.n0; ok && n < t.n1; ++n) {
+                const bool empty = t.k0 == t.k1;
+                if (!empty) {
+                    ok = __all_sync(0xffffffffu, bar_wait(&S.tfull[acc], acc_phase));
+                    if (!ok) break;
+                    fence_after();
+                }
+                uint32_t v[32];
+                for (int c = half; c < chunks; c += 2) {
+                    const int col0 = n * nt + c * 32;  // within the piece
+                    if (empty) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = 0;
+                    } else {
+                        load32(tlane + acc * kCeTileN + c * 32, v);
+                        load_wait(v);
+                    }
+                    if constexpr (PRODUCT == kCeScores) {
+                        const int valid = g.nv - col0;
+                        float z[32], m = top;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            z[j] = __uint_as_float(v[j]);
+                            if (CAP) z[j] = ce_cap(z[j], o.cap);
+                        }
+                        if (y >= col0 && y < col0 + 32) {
+                            float zy = 0.f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) zy = y == col0 + j ? z[j] : zy;
+                            g.zt[r] = zy;
+                        }
+                        if (g.psum) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sz += j < valid ? z[j] : 0.f;
+                        }
+                        if (valid < 32) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (j >= valid) z[j] = ce_neg_inf();
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) m = fmaxf(m, z[j]);
+                        const float base = CeAcc::base(m);
+                        s *= ex2((top - base) * kLog2e);
+                        top = m;
+                        float s4[4] = {s, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            s4[j & 3] += ex2((z[j] - base) * kLog2e);
+                        s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    } else if constexpr (PRODUCT == kCeProbs) {
+                        if (col0 < g.P.ld) {
+                            float d[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                float z = __uint_as_float(v[j]), slope = 1.f;
+                                if (CAP) {
+                                    z = ce_cap(z, o.cap);
+                                    slope = 1.f - (z / o.cap) * (z / o.cap);
+                                }
+                                float x = fmaf(kz, ce_prob(z, lse), -e);
+                                if (y == g.v0 + col0 + j) x -= hit;
+                                if (CAP) x *= slope;
+                                d[j] = y != kCeIgnored && col0 + j < g.nv ? x : 0.f;
+                            }
+                            for (int p = 0; p < g.planes; ++p) {
+                                uint32_t h[16];
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) {
+                                    h[j] = pack2(d[2 * j], d[2 * j + 1], g.bf16);
+                                    if (g.planes > 1) {
+                                        d[2 * j] -= __uint_as_float(h[j] << 16);
+                                        d[2 * j + 1] -= __uint_as_float(h[j] & 0xffff0000u);
+                                    }
+                                }
+                                char *out = static_cast<char *>(g.p_out) +
+                                            2 * (p * g.P.plane + r * g.P.ld + col0);
+                                store8(out, h);
+                                store8(out + 32, h + 8);
+                            }
+                        }
+                    } else {
+                        const long long M = PRODUCT == kCeGradW ? g.nv : w.live;
+                        if (r < M && col0 < g.D) {
+                            const int cols = min(32, g.D - col0);
+                            if (g.dst) {
+                                long long to = r;
+                                if (PRODUCT == kCeGradX)
+                                    to = g.idx ? g.idx[g.row0 + r] : g.row0 + r;
+                                else
+                                    to += g.v0;
+                                const long long at = to * g.D + col0;
+                                if (g.dst_type == kCeF32) {
+                                    float *p = static_cast<float *>(g.dst) + at;
+                                    for (int j = 0; j < 32; ++j)
+                                        if (j < cols) p[j] = __uint_as_float(v[j]) * scale;
+                                } else {
+                                    uint32_t h[16];
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j)
+                                        h[j] = pack2(__uint_as_float(v[2 * j]) * scale,
+                                                     __uint_as_float(v[2 * j + 1]) * scale,
+                                                     g.bf16);
+                                    uint16_t *p = static_cast<uint16_t *>(g.dst) + at;
+                                    if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+                                        store8(p, h);
+                                        store8(p + 16, h + 8);
+                                    } else {
+#pragma unroll
+                                        for (int j = 0; j < 32; ++j)
+                                            if (j < cols)
+                                                p[j] = (uint16_t)(h[j / 2] >> (16 * (j & 1)));
+                                    }
+                                }
+                            } else {
+                                float *p = g.acc + t.split * g.acc_split + r * g.D + col0;
+                                if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+#pragma unroll
+                                    for (int j = 0; j < 32; j += 8) {
+                                        if (g.add) {
+                                            float old[8];
+                                            fetch8(p + j, old);
+#pragma unroll
+                                            for (int i = 0; i < 8; ++i)
+                                                v[j + i] = __float_as_uint(
+                                                    __uint_as_float(v[j + i]) + old[i]);
+                                        }
+                                        store8(p + j, v + j);
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 32; ++j)
+                                        if (j < cols)
+                                            p[j] = (g.add ? p[j] : 0.f) + __uint_as_float(v[j]);
+                                }
+                            }
+                        }
+                    }
+                }
+                if (!empty) {
+                    // this warp has read its part of the accumulator
+                    fence_before();
+                    if (lane == 0)
+                        asm volatile(
+                            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                in_leader(smem_addr(&S.tempty[acc])))
+                            : "memory");
+                    __syncwarp();
+                    if (++acc == 2) {
+                        acc = 0;
+                        acc_phase ^= 1;
+                    }
+                }
+            }
+            if (PRODUCT == kCeScores && r < w.live) {
+                const long long at = (2LL * t.split + half) * g.rows + r;
+                g.part[at] = make_float2(top, s);
+                if (g.psum) g.psum[at] = sz;
+            }
+        }
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) C[ty * 4 + i][tx * 4 + j] = acc[i][j];
+    __syncwarp();
+    fence_before();
     __syncthreads();
-    if (threadIdx.x >= kT) return;
-    const long long r = m0 + threadIdx.x;  // row of the piece
-    if (r >= g.rows) return;
-    const float *c = C[threadIdx.x];
-    int y = kCeIgnored;
-    if (r < live)
-        y = g.lab ? g.lab[g.row0 + r] : ce_label(g.labels[g.row0 + r], g.opt.ignore, g.V);
-    const int ncols = (int)min((long long)kT, g.nv - n0);
-    if (g.product == kCeScores) {
-        CeAcc a;
-        a.init();
-        for (int j = 0; j < ncols; ++j) {
-            const float z = ce_cap(c[j], g.opt.cap);
-            a.merge(z, 1.f, z);
-            if (y == g.v0 + n0 + j) g.zt[r] = z;
-        }
-        g.part[blockIdx.y * g.rows + r] = make_float2(a.m, a.s);
-        if (g.psum) g.psum[blockIdx.y * g.rows + r] = a.sz;
-        return;
-    }
-    const long long src = r < live ? (g.idx ? g.idx[g.row0 + r] : g.row0 + r) : 0;
-    const float lse = y == kCeIgnored ? 0.f : g.lse[src];
-    for (int j = 0; j < kT; ++j) {
-        const long long col = n0 + j;
-        if (col >= g.P.ld) break;
-        float d = 0.f;
-        if (y != kCeIgnored && col < g.nv) {
-            const float z = ce_cap(c[j], g.opt.cap);
-            d = (1.f + 2.f * g.opt.zeta * lse) * ex2(fmaf(z, kLog2e, -lse * kLog2e)) -
-                g.opt.eps / (float)g.V;
-            if (y == g.v0 + col) d -= 1.f - g.opt.eps;
-            if (g.opt.cap > 0.f) d *= 1.f - (z / g.opt.cap) * (z / g.opt.cap);
-        }
-        d *= g.p_scale;
-        for (int p = 0; p < g.planes; ++p) {
-            const long long o = p * g.P.plane + r * g.P.ld + col;
-            if (g.bf16) {
-                const __nv_bfloat16 h = __float2bfloat16_rn(d);
-                static_cast<__nv_bfloat16 *>(g.p_out)[o] = h;
-                d -= __bfloat162float(h);
-            } else {
-                static_cast<__half *>(g.p_out)[o] = __float2half_rn(d);
-            }
-        }
-    }
+    cluster_sync();
+    fence_after();
+    if (warp == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(kCols));
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                              const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                              const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult st;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000,
+                                             cudaEnableDefault, &st) != cudaSuccess ||
+            st != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// boxes of 64 columns x box_rows rows of one plane, 128-byte swizzle, zeros
+// outside the matrix
+bool make_map(CUtensorMap *map, const CeMat &m, int planes, bool bf16, int box_rows) {
+    const EncodeFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t plane = planes > 1 ? (cuuint64_t)m.plane : (cuuint64_t)m.ld * m.rows;
+    const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)m.ld * 2, plane * 2};
+    const cuuint32_t box[3] = {kDepth, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+              const_cast<void *>(m.ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// columns of a tile: a multiple of 32 (K-major B) or of 128 (MN-major B)
+int tile_n(int cols, int unit) {
+    return std::min(kCeTileN, (int)(((long long)cols + unit - 1) / unit * unit));
+}
+
+template <int PRODUCT, bool CAP>
+cudaError_t launch(const CeGemm &g, cudaStream_t st) {
+    constexpr bool kAMn = PRODUCT == kCeGradW, kBMn = PRODUCT >= kCeGradX;
+    const int nt = kBMn ? tile_n(g.D, 128) : tile_n(g.nv, 32);
+    CUtensorMap a, b;
+    const CeMat &ma = PRODUCT >= kCeGradX ? g.P : g.X;
+    const CeMat &mb = PRODUCT == kCeGradW ? g.X : g.W;
+    if (!make_map(&a, ma, g.planes, g.bf16, kAMn ? 64 : 128) ||
+        !make_map(&b, mb, g.planes, g.bf16, kBMn ? 64 : nt / 2))
+        return cudaErrorInvalidValue;
+    auto kernel = ce_gemm_kernel<PRODUCT, CAP>;
+    const cudaError_t err =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (err != cudaSuccess) return err;
+    const long long M = PRODUCT == kCeGradW ? g.nv : g.rows;
+    const long long mt = (M + kCeTileM - 1) / kCeTileM;
+    const long long n = (PRODUCT <= kCeProbs ? g.nv : g.D);
+    const long long units =
+        mt * (PRODUCT == kCeScores ? g.runs : (n + nt - 1) / nt * g.splits);
+    const int grid = 2 * (int)std::min<long long>(kCePairs, units);
+    kernel<<<grid, kThreads, kSmemBytes, st>>>(a, b, g, nt);
+    count_launches(1);
+    return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_ce_gemm(const CeGemm &g, cudaStream_t stream) {
-    long long m = g.rows, n = g.nv;
-    int z = 1;
-    if (g.product == kCeProbs) n = g.P.ld;
-    if (g.product == kCeGradX) n = g.D;
-    if (g.product == kCeGradW) m = g.nv, n = g.D;
-    if (g.product >= kCeGradX) z = g.splits;
-    gemm_kernel<<<dim3((unsigned)((m + kT - 1) / kT), (unsigned)((n + kT - 1) / kT), z), 256, 0,
-                  stream>>>(g);
-    count_launches(1);
-    return cudaGetLastError();
+int ce_runs(long long rows, int V) {
+    const long long mt = (rows + kCeTileM - 1) / kCeTileM;
+    const int tiles = (V + kCeTileN - 1) / kCeTileN;
+    // the longest pair's tiles, and about a third of a tile to begin a run
+    int best = 1;
+    double cost = 1e300;
+    for (int r = 1; r <= std::min(tiles, 2 * kCePairs); ++r) {
+        const double c = (double)((mt * r + kCePairs - 1) / kCePairs) *
+                         ((tiles + r - 1) / r + 0.33);
+        if (c < cost - 1e-9) {
+            cost = c;
+            best = r;
+        }
+    }
+    return best;
+}
+
+int ce_error_flag(bool clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_ce_error, sizeof(v)) != cudaSuccess) return -1;
+    if (clear && v) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(g_ce_error, &zero, sizeof(zero));
+    }
+    return v;
+}
+
+cudaError_t launch_ce_gemm(const CeGemm &g, cudaStream_t st) {
+    const bool cap = g.opt.cap > 0.f;
+    switch (g.product) {
+        case kCeScores: return cap ? launch<kCeScores, true>(g, st) : launch<kCeScores, false>(g, st);
+        case kCeProbs: return cap ? launch<kCeProbs, true>(g, st) : launch<kCeProbs, false>(g, st);
+        case kCeGradX: return launch<kCeGradX, false>(g, st);
+        default: return launch<kCeGradW, false>(g, st);
+    }
 }
 
 }  // namespace gsv

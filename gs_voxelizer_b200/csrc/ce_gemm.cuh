@@ -9,55 +9,82 @@
 namespace gsv {
 
 enum CeProduct {
-    kCeScores = 0,  // X W^T, kept as a (max, sum) pair per row and class tile
+    kCeScores = 0,  // X W^T, kept as (maximum, sum) pairs
     kCeProbs = 1,   // X W^T, stored as the loss's derivative in the scores
-    kCeGradX = 2,   // P W: accumulated for the features
-    kCeGradW = 3,   // P^T X: accumulated for the table
+    kCeGradX = 2,   // P W
+    kCeGradW = 3,   // P^T X
 };
 
 // rows x cols, cols contiguous; plane p starts at ptr + p * plane (elements).
-// ld, plane and ptr keep 16-byte alignment.
+// ptr, ld and plane keep 16-byte alignment.
 struct CeMat {
     const void *ptr;
     long long rows, cols, ld, plane;
 };
 
+// Factor of the summed gradients. With reduction "none" each row's upstream
+// gradient is in P already, over the largest one (gmax) in fp16.
+struct CeUpstream {
+    const float *g;      // [1]
+    const float *count;  // labelled rows, at least 1
+    const float *gmax;   // or null
+    float inv_p;         // 1 / p_scale
+    int reduction;
+};
+
+__device__ __forceinline__ float ce_grad_scale(const CeUpstream &u) {
+    if (u.reduction == kCeNone)
+        return (u.gmax && *u.gmax > 0.f ? *u.gmax : 1.f) * u.inv_p;
+    return (u.reduction == kCeMean ? u.g[0] / u.count[0] : u.g[0]) * u.inv_p;
+}
+
 struct CeGemm {
     int product;
     bool bf16;
     int planes;         // 1 or 3
-    CeMat X;            // kCeScores, kCeProbs: [rows, D]; kCeGradW: [rows, D]
+    CeMat X;            // [rows, D]
     CeMat W;            // [V, D]
     CeMat P;            // [rows of the piece, classes of the piece]
-    long long row0;     // first row of the piece within the packed rows
+    long long row0;     // first row of the piece within X
     long long rows;     // rows of the piece
     int v0, nv;         // classes of the piece
     int V, D;
-    const int *count;   // packed rows in use (device), or null: all of them
+    const int *count;   // rows of X in use (device), or null: rows
 
-    // rows: packed class (>= 0, kCeInvalid, kCeIgnored), or raw labels
+    // a row's class: packed (lab), or from the caller's labels
     const int *lab;
     const long long *labels;
-    const int *idx;     // packed row -> original row (lse is by original row)
+    const int *idx;     // packed row -> original row, or null
     CeOpt opt;
 
-    // kCeScores
-    float2 *part;       // [tiles][rows] (max, sum)
-    float *psum;        // [tiles][rows] plain sums (label smoothing) or null
+    // kCeScores: class tiles in `runs` runs
+    int runs;
+    float2 *part;       // [2 * runs][rows] (maximum, sum)
+    float *psum;        // [2 * runs][rows] plain sums (label smoothing) or null
     float *zt;          // [rows] score of the row's class
-    // kCeProbs
-    const float *lse;
+    // kCeProbs: derivative * p_scale * (row's upstream gradient / gmax)
+    const float2 *lse;  // by original row
     void *p_out;        // P's storage (P describes it)
-    float p_scale;      // stored = p_scale * derivative
-    // kCeGradX, kCeGradW: out[split][m][D] (+)= product
-    float *out;
-    long long out_split;  // elements between splits
+    float p_scale;
+    const float *grow;  // upstream gradient by original row, or null
+    const float *gmax;  // or null
+    // kCeGradX, kCeGradW: acc[split][m][D] (+)= product, or, with dst set,
+    // dst[row of m][D] = scale * product in the inputs' type
+    float *acc;
+    long long acc_split;  // elements between splits
     int splits;
     bool add;
+    void *dst;
+    int dst_type;
+    CeUpstream up;
 };
 
-constexpr int kCeTileM = 128;    // packed rows come in whole tiles of these
-constexpr int kCeScoreTile = 64; // classes behind one (max, sum) pair
+constexpr int kCeTileM = 256;     // rows a tile: packed rows come in whole tiles
+constexpr int kCeTileN = 256;     // classes (or channels) a tile, at most
+constexpr int kCePairs = kSMs / 2;  // tiles in flight: a pair of SMs each
+
+// runs of class tiles for the forward: (rows of) partial sums and balance
+int ce_runs(long long rows, int V);
 
 cudaError_t launch_ce_gemm(const CeGemm &g, cudaStream_t stream);
 

@@ -111,47 +111,33 @@ __device__ __forceinline__ void split3(float v, __nv_bfloat16 (&h)[3]) {
     }
 }
 
-// Per-row factor of the table's gradient: the row's upstream gradient
-// (reduction "none"), in fp16 over the largest one, so that it cannot
-// overflow or vanish.
-struct RowScale {
-    const float *g;       // by original row, or null
-    const float *gmax;    // or null
-};
-
-// dst[plane][padded rows][ld] = src[idx[r]] (times the row's factor), rows
-// past the count and columns past D zero. One warp a row.
+// dst[plane][rows][ld] = src[idx[r]], rows past the count (up to whole tiles)
+// and columns past D zero. One warp a row.
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(256)
 pack_kernel(long long rows, int D, long long ld, long long plane, const T *__restrict__ src,
-            const int *__restrict__ idx, const int *__restrict__ total, RowScale sc,
+            const int *__restrict__ idx, const int *__restrict__ total,
             void *__restrict__ dst) {
     const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (r >= rows) return;
     const int lane = threadIdx.x & 31;
     long long from = r;
-    float k = 1.f;
     if (ROWS) {
         const long long live = *total;
         if (r >= (live + kCeTileM - 1) / kCeTileM * kCeTileM) return;
         from = r < live ? idx[r] : -1;
-        if (sc.g && from >= 0) {
-            k = sc.g[from];
-            if (sc.gmax && *sc.gmax > 0.f) k /= *sc.gmax;
-        }
     }
     for (long long c = lane; c < ld; c += 32) {
         T v = ce_from_float<T>(0.f);
         if (from >= 0 && c < D) v = src[from * D + c];
         if constexpr (sizeof(T) == 4) {
             __nv_bfloat16 h[3];
-            split3(sc.g ? v * k : v, h);
+            split3(v, h);
             __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(dst) + r * ld + c;
             o[0] = h[0];
             o[plane] = h[1];
             o[2 * plane] = h[2];
         } else {
-            if (sc.g) v = ce_from_float<T>(ce_to_float(v) * k);
             static_cast<T *>(dst)[r * ld + c] = v;
         }
     }
@@ -161,14 +147,14 @@ pack_kernel(long long rows, int D, long long ld, long long plane, const T *__res
 
 constexpr int kMergeRows = 32, kMergeSlices = 8;
 
-// One row's (max, sum) pairs of all class tiles -> lse and loss. Eight
-// slices of the tiles run side by side for 32 rows.
+// One row's (maximum, sum) pairs of all class runs -> lse and loss. Eight
+// slices of the pairs run side by side for 32 rows.
 __global__ void __launch_bounds__(kMergeRows *kMergeSlices)
 merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
              const float *__restrict__ psum, const float *__restrict__ zt,
              const int *__restrict__ total, const int *__restrict__ idx,
              const int *__restrict__ lab, const long long *__restrict__ labels, CeOpt o,
-             float *__restrict__ loss, float *__restrict__ lse_out,
+             float *__restrict__ loss, float2 *__restrict__ lse_out,
              float *__restrict__ count, float2 *__restrict__ block_sums) {
     __shared__ float sm[kMergeSlices][kMergeRows], ss[kMergeSlices][kMergeRows],
         sz[kMergeSlices][kMergeRows];
@@ -191,11 +177,11 @@ merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
     if (live) {
         for (int s = 1; s < kMergeSlices; ++s) a.merge(sm[s][lane], ss[s][lane], sz[s][lane]);
         const int y = lab ? lab[r] : ce_label(labels[r], o.ignore, V);
-        float lse = a.lse();
+        float2 lse = a.lse();
         if (y >= 0)
             l = ce_row_loss(lse, zt[r], a.sz, V, o);
         else if (y == kCeInvalid)
-            l = lse = ce_nan();
+            l = lse.x = ce_nan();
         c = y == kCeIgnored ? 0.f : 1.f;
         const long long dst = idx ? idx[r] : r;
         lse_out[dst] = lse;
@@ -231,26 +217,13 @@ max_abs_kernel(const float *__restrict__ g, const int *__restrict__ idx,
         atomicMax(reinterpret_cast<int *>(out), __float_as_int(m));
 }
 
-// factor of the accumulated gradients: 1 / p_scale times the upstream
-// gradient (of the row, with reduction "none": `row` is the original row)
-__device__ __forceinline__ float out_scale(const float *g, const float *count, int reduction,
-                                           float inv_p, long long row, const float *gmax) {
-    if (reduction == kCeNone) {
-        if (row >= 0) return g[row] * inv_p;
-        return (gmax && *gmax > 0.f ? *gmax : 1.f) * inv_p;
-    }
-    return (reduction == kCeMean ? g[0] / count[0] : g[0]) * inv_p;
-}
-
 // dst[idx[r]] = scale * sum over splits of acc[s][r]; one warp a row. The
 // rows are those of a piece: packed rows row0 .. row0 + rows.
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(256)
 finish_grad_kernel(long long row0, long long rows, int D, const float *__restrict__ acc,
                    long long split, int splits, const int *__restrict__ idx,
-                   const int *__restrict__ total, const float *__restrict__ g,
-                   const float *__restrict__ count, int reduction, float inv_p,
-                   const float *__restrict__ gmax, T *__restrict__ dst) {
+                   const int *__restrict__ total, CeUpstream upstream, T *__restrict__ dst) {
     const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (r >= rows) return;
     long long to = r;
@@ -258,7 +231,7 @@ finish_grad_kernel(long long row0, long long rows, int D, const float *__restric
         if (row0 + r >= *total) return;
         to = idx[row0 + r];
     }
-    const float k = out_scale(g, count, reduction, inv_p, ROWS ? to : -1, gmax);
+    const float k = ce_grad_scale(upstream);
     for (long long c = threadIdx.x & 31; c < D; c += 32) {
         float v = 0.f;
         for (int s = 0; s < splits; ++s) v += acc[s * split + r * D + c];
@@ -285,27 +258,29 @@ struct Plan {
     int V, D, type, planes;
     long long ld;         // of packed features / table
     bool pack_w;          // the table cannot be read in place
-    int tiles;            // class tiles of the forward
+    int runs;             // runs of class tiles in the forward
     // backward: pieces and splits
     long long piece_rows, ldp;
     int piece_classes;
-    bool one_row_piece, one_class_piece;
+    bool one_row_piece;
+    bool direct_x, direct_w;  // gradients straight from the product
     int split_x, split_w;
     // workspace offsets (bytes)
-    size_t xp, xs, wp, part, psum, zt, sums, gmax, p, dx, dw, bytes;
+    size_t xp, wp, part, psum, zt, sums, gmax, p, dx, dw, bytes;
 };
 
 // state (kept between the two directions): count (float, padded to 4 words),
-// lse [N], packed total (int, padded to 4 words), idx [Np], lab [Np],
+// lse [N] (two floats), packed total (int, padded to 4 words), idx [Np], lab [Np],
 // block counts
 struct State {
-    float *count, *lse;
+    float *count;
+    float2 *lse;
     int *total, *idx, *lab, *counts;
 };
 
 long long state_words(long long N) {
     const long long Np = up(N, kCeTileM);
-    return 4 + up(N, 4) + 4 + 2 * Np + up((N + kIdxNT - 1) / kIdxNT, 4);
+    return 4 + up(2 * N, 4) + 4 + 2 * Np + up((N + kIdxNT - 1) / kIdxNT, 4);
 }
 
 State state_of(void *p, long long N) {
@@ -313,8 +288,8 @@ State state_of(void *p, long long N) {
     float *f = static_cast<float *>(p);
     State s;
     s.count = f;
-    s.lse = f + 4;
-    s.total = reinterpret_cast<int *>(s.lse + up(N, 4));
+    s.lse = reinterpret_cast<float2 *>(f + 4);
+    s.total = reinterpret_cast<int *>(f + 4 + up(2 * N, 4));
     s.idx = s.total + 4;
     s.lab = s.idx + Np;
     s.counts = s.lab + Np;
@@ -334,7 +309,7 @@ float p_scale_of(int type, const CeOpt &o) {
 int splits_for(long long tiles, long long depth) {
     // enough blocks for the device when the product has few tiles, each
     // split keeping at least 512 of the summed axis
-    const long long want = tiles > 0 ? kSMs / tiles : 1;
+    const long long want = tiles > 0 ? kCePairs / tiles : 1;
     return (int)std::max(1LL, std::min(want, depth / 512));
 }
 
@@ -351,7 +326,7 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     // `weight` null: the workspace query, which allows for any alignment
     p.pack_w = p.planes == 3 || D % 8 != 0 || weight == nullptr ||
                (reinterpret_cast<uintptr_t>(weight) & 15) != 0;
-    p.tiles = (V + kCeScoreTile - 1) / kCeScoreTile;
+    p.runs = ce_runs(N, V);
     size_t at = 0;
     auto take = [&](size_t b) {
         const size_t o = at;
@@ -362,14 +337,13 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     p.xp = take((size_t)p.planes * p.Np * p.ld * 2);
     p.wp = take(p.pack_w ? (size_t)p.planes * V * p.ld * 2 : 0);
     if (!backward) {
-        p.part = take(sizeof(float2) * (size_t)p.tiles * p.Np);
-        p.psum = take(o.eps > 0.f ? sizeof(float) * (size_t)p.tiles * p.Np : 0);
+        p.part = take(sizeof(float2) * 2 * (size_t)p.runs * p.Np);
+        p.psum = take(o.eps > 0.f ? sizeof(float) * 2 * (size_t)p.runs * p.Np : 0);
         p.zt = take(sizeof(float) * (size_t)p.Np);
         p.bytes = at;
         return p;
     }
     p.gmax = take(sizeof(float));
-    p.xs = take(o.reduction == kCeNone ? (size_t)p.planes * p.Np * p.ld * 2 : 0);
     // pieces of P: all rows while at least 4096 classes (or all) fit, else
     // 8192 classes (or all) and the rows that fit
     const long long Vp = up(V, 64);
@@ -385,64 +359,64 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     }
     p.piece_classes = (int)std::min((long long)V, p.ldp);
     p.one_row_piece = p.piece_rows >= p.Np;
-    p.one_class_piece = p.piece_classes >= V;
+    const bool one_class_piece = p.piece_classes >= V;
     p.piece_rows = std::min(p.piece_rows, p.Np);
     p.p = take((size_t)p.planes * p.piece_rows * p.ldp * 2);
-    const long long tn = (D + 255) / 256;
+    const long long tn = (D + kCeTileN - 1) / kCeTileN;
     p.split_x = splits_for(p.piece_rows / kCeTileM * tn, p.piece_classes);
     p.split_w = splits_for(up(p.piece_classes, kCeTileM) / kCeTileM * tn, p.piece_rows);
-    p.dx = take(sizeof(float) * (size_t)p.split_x * p.piece_rows * D);
-    p.dw = take(sizeof(float) * (size_t)p.split_w * (p.one_row_piece ? p.piece_classes : V) * D);
+    p.direct_x = one_class_piece && p.split_x == 1;
+    p.direct_w = p.one_row_piece && p.split_w == 1;
+    p.dx = take(p.direct_x ? 0 : sizeof(float) * (size_t)p.split_x * p.piece_rows * D);
+    p.dw = take(p.direct_w ? 0
+                           : sizeof(float) * (size_t)p.split_w *
+                                 (p.one_row_piece ? p.piece_classes : V) * D);
     p.bytes = at;
     return p;
 }
 
 template <typename T>
-cudaError_t pack(const Plan &p, bool rows, const void *src, const State &s, const float *g,
-                 const float *gmax, void *dst, cudaStream_t st) {
-    const RowScale sc{g, gmax};
+cudaError_t pack(const Plan &p, bool rows, const void *src, const State &s, void *dst,
+                 cudaStream_t st) {
     if (rows)
         pack_kernel<T, true><<<blocks8(p.Np), 256, 0, st>>>(
-            p.Np, p.D, p.ld, p.Np * p.ld, static_cast<const T *>(src), s.idx, s.total, sc, dst);
+            p.Np, p.D, p.ld, p.Np * p.ld, static_cast<const T *>(src), s.idx, s.total, dst);
     else
         pack_kernel<T, false><<<blocks8(p.V), 256, 0, st>>>(
-            p.V, p.D, p.ld, p.V * p.ld, static_cast<const T *>(src), nullptr, nullptr, sc, dst);
+            p.V, p.D, p.ld, p.V * p.ld, static_cast<const T *>(src), nullptr, nullptr, dst);
     count_launches(1);
     return cudaGetLastError();
 }
 
-cudaError_t pack_any(const Plan &p, bool rows, const void *src, const State &s,
-                     const float *g, const float *gmax, void *dst, cudaStream_t st) {
+cudaError_t pack_any(const Plan &p, bool rows, const void *src, const State &s, void *dst,
+                     cudaStream_t st) {
     switch (p.type) {
-        case kCeF32: return pack<float>(p, rows, src, s, g, gmax, dst, st);
-        case kCeBf16: return pack<__nv_bfloat16>(p, rows, src, s, g, gmax, dst, st);
-        default: return pack<__half>(p, rows, src, s, g, gmax, dst, st);
+        case kCeF32: return pack<float>(p, rows, src, s, dst, st);
+        case kCeBf16: return pack<__nv_bfloat16>(p, rows, src, s, dst, st);
+        default: return pack<__half>(p, rows, src, s, dst, st);
     }
 }
 
 template <typename T>
 cudaError_t finish_grad(const Plan &p, bool rows, long long row0, long long n,
                         const float *acc, long long split, int splits, const State &s,
-                        const float *g, int reduction, float inv_p, const float *gmax,
-                        void *dst, cudaStream_t st) {
+                        const CeUpstream &u, void *dst, cudaStream_t st) {
     if (rows)
         finish_grad_kernel<T, true><<<blocks8(n), 256, 0, st>>>(
-            row0, n, p.D, acc, split, splits, s.idx, s.total, g, s.count, reduction, inv_p,
-            gmax, static_cast<T *>(dst));
+            row0, n, p.D, acc, split, splits, s.idx, s.total, u, static_cast<T *>(dst));
     else
         finish_grad_kernel<T, false><<<blocks8(n), 256, 0, st>>>(
-            0, n, p.D, acc, split, splits, nullptr, nullptr, g, s.count, reduction, inv_p,
-            gmax, static_cast<T *>(dst) + row0 * p.D);
+            0, n, p.D, acc, split, splits, nullptr, nullptr, u,
+            static_cast<T *>(dst) + row0 * p.D);
     count_launches(1);
     return cudaGetLastError();
 }
 
 cudaError_t finish_any(const Plan &p, bool rows, long long row0, long long n,
                        const float *acc, long long split, int splits, const State &s,
-                       const float *g, int reduction, float inv_p, const float *gmax,
-                       void *dst, cudaStream_t st) {
+                       const CeUpstream &u, void *dst, cudaStream_t st) {
 #define GSV_CE_T(T) \
-    finish_grad<T>(p, rows, row0, n, acc, split, splits, s, g, reduction, inv_p, gmax, dst, st)
+    finish_grad<T>(p, rows, row0, n, acc, split, splits, s, u, dst, st)
     switch (p.type) {
         case kCeF32: return GSV_CE_T(float);
         case kCeBf16: return GSV_CE_T(__nv_bfloat16);
@@ -502,12 +476,13 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
                                         s.idx, s.lab);
     count_launches(1);
     GSV_CE_TRY(cudaGetLastError());
-    GSV_CE_TRY(pack_any(p, true, features, s, nullptr, nullptr, ws + p.xp, st));
-    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, nullptr, nullptr, ws + p.wp, st));
+    GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
+    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, ws + p.wp, st));
     CeGemm g = gemm_of(p, s, weight, ws, o);
     g.product = kCeScores;
     g.rows = p.Np;
     g.nv = V;
+    g.runs = p.runs;
     g.part = reinterpret_cast<float2 *>(ws + p.part);
     g.psum = o.eps > 0.f ? reinterpret_cast<float *>(ws + p.psum) : nullptr;
     g.zt = reinterpret_cast<float *>(ws + p.zt);
@@ -515,7 +490,7 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     const int mb = (int)((N + kMergeRows - 1) / kMergeRows);
     float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
     merge_kernel<<<mb, kMergeRows * kMergeSlices, 0, st>>>(
-        p.Np, p.tiles, V, g.part, g.psum, g.zt, s.total, s.idx, s.lab, labels, o, loss, s.lse,
+        p.Np, 2 * p.runs, V, g.part, g.psum, g.zt, s.total, s.idx, s.lab, labels, o, loss, s.lse,
         s.count, sums);
     count_launches(1);
     GSV_CE_TRY(cudaGetLastError());
@@ -533,17 +508,14 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     float *gmax = type == kCeF16 ? reinterpret_cast<float *>(ws + p.gmax) : nullptr;
     const bool none = o.reduction == kCeNone;
-    GSV_CE_TRY(pack_any(p, true, features, s, nullptr, nullptr, ws + p.xp, st));
-    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, nullptr, nullptr, ws + p.wp, st));
-    if (none && grad_weight) {
-        if (gmax) {
-            GSV_CE_TRY(cudaMemsetAsync(gmax, 0, sizeof(float), st));
-            const int nb = (int)std::min<long long>(kSMs, (N + 1023) / 1024);
-            max_abs_kernel<<<nb, 256, 0, st>>>(grad_loss, s.idx, s.total, gmax);
-            count_launches(1);
-            GSV_CE_TRY(cudaGetLastError());
-        }
-        GSV_CE_TRY(pack_any(p, true, features, s, grad_loss, gmax, ws + p.xs, st));
+    GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
+    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, ws + p.wp, st));
+    if (none && gmax) {
+        GSV_CE_TRY(cudaMemsetAsync(gmax, 0, sizeof(float), st));
+        const int nb = (int)std::min<long long>(kSMs, (N + 1023) / 1024);
+        max_abs_kernel<<<nb, 256, 0, st>>>(grad_loss, s.idx, s.total, gmax);
+        count_launches(1);
+        GSV_CE_TRY(cudaGetLastError());
     }
     if (grad_features) {
         switch (type) {
@@ -562,9 +534,14 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
     g.lse = s.lse;
     g.p_out = ws + p.p;
     g.p_scale = p_scale_of(type, o);
-    const float inv_p = 1.f / g.p_scale;
+    g.grow = none ? grad_loss : nullptr;
+    g.gmax = gmax;
+    g.dst_type = type;
+    g.up = {grad_loss, s.count, gmax, 1.f / g.p_scale, o.reduction};
     float *dx = reinterpret_cast<float *>(ws + p.dx);
     float *dw = reinterpret_cast<float *>(ws + p.dw);
+    const long long x_split = p.piece_rows * D;
+    const long long w_split = (long long)(p.one_row_piece ? p.piece_classes : V) * D;
     for (long long r0 = 0; r0 < p.Np; r0 += p.piece_rows) {
         g.row0 = r0;
         g.rows = std::min(p.piece_rows, p.Np - r0);
@@ -577,33 +554,33 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
             if (grad_features) {
                 CeGemm x = g;
                 x.product = kCeGradX;
-                x.out = dx;
-                x.out_split = p.piece_rows * D;
                 x.splits = p.split_x;
+                x.acc = dx;
+                x.acc_split = x_split;
                 x.add = v0 > 0;
+                x.dst = p.direct_x ? grad_features : nullptr;
                 GSV_CE_TRY(launch_ce_gemm(x, st));
             }
             if (grad_weight) {
                 CeGemm w = g;
                 w.product = kCeGradW;
-                if (none) w.X.ptr = ws + p.xs;
-                w.out = p.one_row_piece ? dw : dw + (long long)v0 * D;
-                w.out_split = (long long)(p.one_row_piece ? p.piece_classes : V) * D;
                 w.splits = p.split_w;
+                w.acc = p.one_row_piece ? dw : dw + (long long)v0 * D;
+                w.acc_split = w_split;
                 w.add = r0 > 0;
+                w.dst = p.direct_w ? grad_weight : nullptr;
                 GSV_CE_TRY(launch_ce_gemm(w, st));
-                if (p.one_row_piece)
-                    GSV_CE_TRY(finish_any(p, false, v0, g.nv, dw, w.out_split, p.split_w, s,
-                                          grad_loss, o.reduction, inv_p, gmax, grad_weight, st));
+                if (p.one_row_piece && !p.direct_w)
+                    GSV_CE_TRY(finish_any(p, false, v0, g.nv, dw, w_split, p.split_w, s, g.up,
+                                          grad_weight, st));
             }
         }
-        if (grad_features)
-            GSV_CE_TRY(finish_any(p, true, r0, g.rows, dx, p.piece_rows * D, p.split_x, s,
-                                  grad_loss, o.reduction, inv_p, gmax, grad_features, st));
+        if (grad_features && !p.direct_x)
+            GSV_CE_TRY(finish_any(p, true, r0, g.rows, dx, x_split, p.split_x, s, g.up,
+                                  grad_features, st));
     }
     if (grad_weight && !p.one_row_piece)
-        GSV_CE_TRY(finish_any(p, false, 0, V, dw, (long long)V * D, p.split_w, s, grad_loss,
-                              o.reduction, inv_p, gmax, grad_weight, st));
+        GSV_CE_TRY(finish_any(p, false, 0, V, dw, w_split, p.split_w, s, g.up, grad_weight, st));
     return cudaSuccess;
 }
 

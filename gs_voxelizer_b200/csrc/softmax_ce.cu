@@ -41,7 +41,7 @@ template <typename T, int G>
 __global__ void __launch_bounds__(kNT)
 staged_fwd_kernel(long long rows, int V, const T *__restrict__ scores,
                   const long long *__restrict__ labels, CeOpt o, bool vec,
-                  float *__restrict__ loss, float *__restrict__ lse_out,
+                  float *__restrict__ loss, float2 *__restrict__ lse_out,
                   float *__restrict__ count, float2 *__restrict__ partials) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float2 sh[kNT / 32];
@@ -66,7 +66,7 @@ staged_fwd_kernel(long long rows, int V, const T *__restrict__ scores,
         const float b = CeAcc::base(a.m);
         for (int j = lane; j < V; j += G) {
             const float z = ce_cap(ce_to_float(p[j]), o.cap);
-            a.s += ex2(fmaf(z, kLog2e, -b));
+            a.s += ex2((z - b) * kLog2e);
             a.sz += z;
         }
 #pragma unroll
@@ -75,11 +75,11 @@ staged_fwd_kernel(long long rows, int V, const T *__restrict__ scores,
             a.sz += __shfl_xor_sync(mask, a.sz, k);
         }
         if (lane == 0) {
-            float lse = a.lse();
+            float2 lse = a.lse();
             if (y >= 0) {
                 l = ce_row_loss(lse, ce_cap(ce_to_float(p[y]), o.cap), a.sz, V, o);
             } else if (y == kCeInvalid) {
-                l = lse = ce_nan();
+                l = lse.x = ce_nan();
             }
             cnt = y == kCeIgnored ? 0.f : 1.f;
             lse_out[row0 + r] = lse;
@@ -96,10 +96,10 @@ staged_fwd_kernel(long long rows, int V, const T *__restrict__ scores,
 }
 
 // gradient of one score: k = 1 + 2 zeta lse, e = eps / V
-__device__ __forceinline__ float grad_of(float s, bool hit, float lse2, float k, float e,
+__device__ __forceinline__ float grad_of(float s, bool hit, float2 lse, float k, float e,
                                          float g, const CeOpt &o) {
     const float z = ce_cap(s, o.cap);
-    float d = k * ex2(fmaf(z, kLog2e, -lse2)) - e;
+    float d = k * ce_prob(z, lse) - e;
     if (hit) d -= 1.f - o.eps;
     if (o.cap > 0.f) {
         const float t = z / o.cap;
@@ -118,7 +118,7 @@ template <typename T, int G>
 __global__ void __launch_bounds__(kNT)
 staged_bwd_kernel(long long rows, int V, const T *__restrict__ scores,
                   const long long *__restrict__ labels, CeOpt o, bool vec,
-                  const float *__restrict__ lse_in, const float *__restrict__ count,
+                  const float2 *__restrict__ lse_in, const float *__restrict__ count,
                   const float *__restrict__ grad_loss, T *__restrict__ grad) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     T *tile = reinterpret_cast<T *>(smem_raw);
@@ -131,13 +131,13 @@ staged_bwd_kernel(long long rows, int V, const T *__restrict__ scores,
     if (r < nr) {
         T *p = tile + r * V;
         const int y = ce_label(labels[row0 + r], o.ignore, V);
-        const float lse = lse_in[row0 + r];
-        const float lse2 = lse * kLog2e, k = 1.f + 2.f * o.zeta * lse;
+        const float2 lse = lse_in[row0 + r];
+        const float k = 1.f + 2.f * o.zeta * ce_lse(lse);
         const float e = o.eps / (float)V;
         const float g = upstream(grad_loss, row0 + r, count, o);
         for (int j = lane; j < V; j += G)
             p[j] = ce_from_float<T>(y == kCeIgnored ? 0.f
-                                                    : grad_of(ce_to_float(p[j]), j == y, lse2,
+                                                    : grad_of(ce_to_float(p[j]), j == y, lse,
                                                               k, e, g, o));
     }
     __syncthreads();
@@ -154,7 +154,7 @@ __device__ __forceinline__ int head_of(const T *p, int V) {
 template <typename T>
 __global__ void __launch_bounds__(kNT)
 row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict__ labels,
-               CeOpt o, float *__restrict__ loss, float *__restrict__ lse_out,
+               CeOpt o, float *__restrict__ loss, float2 *__restrict__ lse_out,
                float *__restrict__ count, float2 *__restrict__ partials) {
     constexpr int kN = Vec16<T>::kN;
     const long long row = blockIdx.x;
@@ -173,10 +173,10 @@ row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
             a.sz += z[k];
         }
         const float b = CeAcc::base(m);
-        a.s *= ex2(fmaf(a.m, kLog2e, -b));
+        a.s *= ex2((a.m - b) * kLog2e);
         a.m = m;
 #pragma unroll
-        for (int k = 0; k < kN; ++k) a.s += ex2(fmaf(z[k], kLog2e, -b));
+        for (int k = 0; k < kN; ++k) a.s += ex2((z[k] - b) * kLog2e);
     }
     if ((int)threadIdx.x < head) one(ce_to_float(p[threadIdx.x]));
     const int tail = head + nv * kN + (int)threadIdx.x;
@@ -195,11 +195,12 @@ row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
     if (threadIdx.x) return;
     for (int w = 1; w < kNT / 32; ++w) a.merge(sm[w], ss[w], sz[w]);
     const int y = ce_label(labels[row], o.ignore, V);
-    float lse = a.lse(), l = 0.f;
+    float2 lse = a.lse();
+    float l = 0.f;
     if (y >= 0)
         l = ce_row_loss(lse, ce_cap(ce_to_float(p[y]), o.cap), a.sz, V, o);
     else if (y == kCeInvalid)
-        l = lse = ce_nan();
+        l = lse.x = ce_nan();
     lse_out[row] = lse;
     if (o.reduction == kCeNone) loss[row] = l;
     const float c = y == kCeIgnored ? 0.f : 1.f;
@@ -212,7 +213,7 @@ row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
 template <typename T>
 __global__ void __launch_bounds__(kNT)
 row_bwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict__ labels,
-               CeOpt o, const float *__restrict__ lse_in, const float *__restrict__ count,
+               CeOpt o, const float2 *__restrict__ lse_in, const float *__restrict__ count,
                const float *__restrict__ grad_loss, T *__restrict__ grad, bool same_head) {
     constexpr int kN = Vec16<T>::kN;
     const long long row = blockIdx.x;
@@ -221,12 +222,12 @@ row_bwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
     const int head = same_head ? head_of(p, V) : V;
     const int nv = (V - head) / kN;
     const int y = ce_label(labels[row], o.ignore, V);
-    const float lse = lse_in[row];
-    const float lse2 = lse * kLog2e, k = 1.f + 2.f * o.zeta * lse, e = o.eps / (float)V;
+    const float2 lse = lse_in[row];
+    const float k = 1.f + 2.f * o.zeta * ce_lse(lse), e = o.eps / (float)V;
     const float g = upstream(grad_loss, row, count, o);
     auto one = [&](int j) {
         q[j] = ce_from_float<T>(
-            y == kCeIgnored ? 0.f : grad_of(ce_to_float(p[j]), j == y, lse2, k, e, g, o));
+            y == kCeIgnored ? 0.f : grad_of(ce_to_float(p[j]), j == y, lse, k, e, g, o));
     };
     for (int i = threadIdx.x; i < nv; i += kNT) {
         Vec16<T> v = reinterpret_cast<const Vec16<T> *>(p + head)[i];
@@ -234,7 +235,7 @@ row_bwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
         for (int t = 0; t < kN; ++t)
             v.v[t] = ce_from_float<T>(
                 y == kCeIgnored ? 0.f
-                                : grad_of(ce_to_float(v.v[t]), head + i * kN + t == y, lse2,
+                                : grad_of(ce_to_float(v.v[t]), head + i * kN + t == y, lse,
                                           k, e, g, o));
         reinterpret_cast<Vec16<T> *>(q + head)[i] = v;
     }
@@ -280,7 +281,7 @@ int lanes_of(int V) {
 
 template <typename T, int G>
 cudaError_t staged(bool fwd, long long rows, int V, const void *scores,
-                   const long long *labels, const CeOpt &o, float *loss, float *lse,
+                   const long long *labels, const CeOpt &o, float *loss, float2 *lse,
                    float *count, const float *grad_loss, void *grad, float2 *partials,
                    cudaStream_t st) {
     constexpr int R = kNT / G;
@@ -304,7 +305,7 @@ cudaError_t staged(bool fwd, long long rows, int V, const void *scores,
 
 template <typename T>
 cudaError_t run(bool fwd, long long rows, int V, const void *scores, const long long *labels,
-                const CeOpt &o, float *loss, float *lse, float *count,
+                const CeOpt &o, float *loss, float2 *lse, float *count,
                 const float *grad_loss, void *grad, float2 *partials, cudaStream_t st) {
     if (V <= kStagedV) {
         switch (lanes_of(V)) {
@@ -355,7 +356,7 @@ size_t softmax_ce_workspace_bytes(long long rows, int V) {
 
 cudaError_t launch_softmax_ce(bool fwd, int type, long long rows, int V, const void *scores,
                               const long long *labels, const CeOpt &o, float *loss,
-                              float *lse, float *count, const float *grad_loss, void *grad,
+                              float2 *lse, float *count, const float *grad_loss, void *grad,
                               void *ws, cudaStream_t st) {
     float2 *partials = static_cast<float2 *>(ws);
     switch (type) {

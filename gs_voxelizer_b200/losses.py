@@ -341,14 +341,14 @@ class _SoftmaxCe(Function):
         if rows == 0:
             ctx.save_for_backward(scores)
             return loss.zero_()
-        stats = torch.empty((rows + 1,), dtype=torch.float32, device=dev)
+        stats = torch.empty((2 * rows + 1,), dtype=torch.float32, device=dev)
         nbytes = lib.gsv_softmax_ce_workspace_bytes(rows, V)
         with torch.cuda.device(dev):
             ws = _C._workspace(nbytes, dev)
             check(lib.gsv_softmax_ce_forward(
                 rows, V, _CE_DTYPES[scores.dtype], scores.data_ptr(),
                 labels.data_ptr(), opt, loss.data_ptr(), stats.data_ptr(),
-                stats.data_ptr() + 4 * rows, ws.data_ptr(), ws.numel(),
+                stats.data_ptr() + 8 * rows, ws.data_ptr(), ws.numel(),
                 _C._stream(dev)))
         ctx.save_for_backward(scores, labels, stats)
         return loss
@@ -366,7 +366,7 @@ class _SoftmaxCe(Function):
             check(lib.gsv_softmax_ce_backward(
                 rows, V, _CE_DTYPES[scores.dtype], scores.data_ptr(),
                 labels.data_ptr(), ctx.opt, stats.data_ptr(),
-                stats.data_ptr() + 4 * rows, grad_loss.data_ptr(),
+                stats.data_ptr() + 8 * rows, grad_loss.data_ptr(),
                 g.data_ptr(), _C._stream(dev)))
         return g, None, None
 
@@ -468,7 +468,7 @@ def linear_cross_entropy(
     embeddings, or the hidden states of a model against a vocabulary.
 
     The scores are products of the inputs summed in float32 and are not
-    rounded to the inputs' type. The forward keeps 12 bytes a row; the
+    rounded to the inputs' type. The forward keeps 16 bytes a row; the
     backward computes the scores again in pieces, with a workspace of a few
     hundred MB beside float32 copies of what it accumulates. With
     ``reduction="none"`` and no gradient it is minus the log-probability of

@@ -355,8 +355,9 @@ GSV_API int gsv_set_tensor_core_backward(int32_t enable);
 /*
  * Device error flags of this library's kernels on the current device, as
  * bits: 1 after a tensor-core backward launch gave up waiting on one of its
- * internal barriers, 2 after a gsv_peer_barrier gave up waiting for a peer
- * (results of those launches are invalid); 0 if none. clear != 0 resets
+ * internal barriers, 2 after a gsv_peer_barrier gave up waiting for a peer,
+ * 4 after a product of gsv_linear_ce_* gave up waiting on one of its internal
+ * barriers (results of those launches are invalid); 0 if none. clear != 0 resets
  * them. Synchronises with the device. No reference counterpart.
  */
 GSV_API int gsv_device_error(int32_t *flag_out, int32_t clear);
@@ -520,7 +521,7 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
  * 2^20.
  *
  * The forward leaves what the backward needs in `lse` / `count` (device
- * float32 [rows] and [1]) or in `state` (gsv_linear_ce_state_bytes, 16-byte
+ * float32 [rows][2], 8-byte aligned, and [1]) or in `state` (gsv_linear_ce_state_bytes, 16-byte
  * aligned); the backward is called with the same sizes, inputs and options.
  * Workspaces are scratch of one call, 256-byte aligned. A null gradient output
  * of gsv_linear_ce_backward is not computed.
