@@ -17,6 +17,7 @@
 // float32 inputs keep three bf16 planes of every operand, which hold all 24
 // bits.
 #include "ce_gemm.cuh"
+#include "ce_narrow.cuh"
 
 namespace gsv {
 namespace {
@@ -239,6 +240,25 @@ finish_grad_kernel(long long row0, long long rows, int D, const float *__restric
     }
 }
 
+// dst[i] = scale * sum over many splits of acc[s][i]: 32 values a block, 32
+// slices of the splits side by side
+template <typename T>
+__global__ void __launch_bounds__(1024)
+reduce_splits_kernel(long long n, const float *__restrict__ acc, int splits,
+                     T *__restrict__ dst) {
+    __shared__ float sh[32][33];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const long long i = (long long)blockIdx.x * 32 + lane;
+    float v = 0.f;
+    if (i < n)
+        for (int s = slice; s < splits; s += 32) v += acc[s * n + i];
+    sh[slice][lane] = v;
+    __syncthreads();
+    if (slice || i >= n) return;
+    for (int s = 1; s < 32; ++s) v += sh[s][lane];
+    dst[i] = ce_from_float<T>(v);
+}
+
 // rows without a label: zero gradient
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -453,8 +473,94 @@ CeGemm gemm_of(const Plan &p, const State &s, const void *weight, unsigned char 
 
 size_t linear_ce_state_bytes(long long rows) { return (size_t)state_words(rows) * 4; }
 
+namespace {
+
+// Workspace of the narrow path: per-block sums, parts of the class splits,
+// parts of dX, parts of dW.
+struct NarrowPlan {
+    int splits, dw_splits;
+    size_t sums, part, psum, zt, dx, dw, bytes;
+};
+
+NarrowPlan narrow_plan(long long N, int V, int D, bool backward, const CeOpt &o) {
+    NarrowPlan p{};
+    p.splits = narrow_class_splits(N, V);
+    p.dw_splits = narrow_dw_splits(N, V);
+    size_t at = 0;
+    auto take = [&](size_t b) {
+        const size_t a = at;
+        at += align256(b);
+        return a;
+    };
+    const size_t parts = p.splits > 1 ? (size_t)p.splits * N : 0;
+    if (backward) {
+        p.dx = take(parts * D * sizeof(float));
+        p.dw = take(sizeof(float) * (size_t)p.dw_splits * V * D);
+    } else {
+        p.sums = take(sizeof(float2) * (size_t)std::max(
+                          narrow_fwd_blocks(N), (N + kMergeRows - 1) / kMergeRows));
+        p.part = take(parts * sizeof(float2));
+        p.psum = take(o.eps > 0.f ? parts * sizeof(float) : 0);
+        p.zt = take(parts ? sizeof(float) * (size_t)N : 0);
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <typename T>
+cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
+                           cudaStream_t st) {
+    const NarrowPlan p = narrow_plan(a.N, a.V, a.D, false, a.opt);
+    float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
+    float2 *part = reinterpret_cast<float2 *>(ws + p.part);
+    float *psum = a.opt.eps > 0.f ? reinterpret_cast<float *>(ws + p.psum) : nullptr;
+    float *zt = reinterpret_cast<float *>(ws + p.zt);
+    GSV_CE_TRY(launch_narrow_fwd<T>(a, loss, sums, part, psum, zt, st));
+    long long blocks = narrow_fwd_blocks(a.N);
+    if (p.splits > 1) {
+        blocks = (a.N + kMergeRows - 1) / kMergeRows;
+        merge_kernel<<<(unsigned)blocks, kMergeRows * kMergeSlices, 0, st>>>(
+            a.N, p.splits, a.V, part, psum, zt, nullptr, nullptr, nullptr, a.labels, a.opt,
+            loss, a.lse, a.count, sums);
+        count_launches(1);
+        GSV_CE_TRY(cudaGetLastError());
+    }
+    if (blocks > 1)
+        GSV_CE_TRY(launch_ce_finish(sums, (int)blocks, a.opt.reduction, loss, a.count, st));
+    return cudaSuccess;
+}
+
+template <typename T>
+cudaError_t reduce_splits(long long n, const float *acc, int splits, void *dst,
+                          cudaStream_t st) {
+    reduce_splits_kernel<T><<<(unsigned)((n + 31) / 32), 1024, 0, st>>>(n, acc, splits,
+                                                                        static_cast<T *>(dst));
+    count_launches(1);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t narrow_backward(const NarrowArgs &a, const float *grad_loss, void *gx, void *gw,
+                            unsigned char *ws, cudaStream_t st) {
+    const NarrowPlan p = narrow_plan(a.N, a.V, a.D, true, a.opt);
+    const CeUpstream u{grad_loss, a.count, nullptr, 1.f, a.opt.reduction};
+    float *dx = reinterpret_cast<float *>(ws + p.dx), *dw = reinterpret_cast<float *>(ws + p.dw);
+    if (gx) {
+        GSV_CE_TRY(launch_narrow_dx<T>(a, u, gx, dx, st));
+        if (p.splits > 1) GSV_CE_TRY(reduce_splits<T>(a.N * a.D, dx, p.splits, gx, st));
+    }
+    if (gw) {
+        GSV_CE_TRY(launch_narrow_dw<T>(a, u, dw, st));
+        GSV_CE_TRY(reduce_splits<T>((long long)a.V * a.D, dw, p.dw_splits, gw, st));
+    }
+    return cudaSuccess;
+}
+
+}  // namespace
+
 size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
                                  const CeOpt &o) {
+    if (D <= kNarrowD) return narrow_plan(N, V, D, backward, o).bytes;
     return make_plan(N, V, D, type, nullptr, backward, o).bytes;
 }
 
@@ -462,9 +568,17 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
                                      const void *features, const void *weight,
                                      const long long *labels, const CeOpt &o, float *loss,
                                      void *state, void *workspace, cudaStream_t st) {
-    const Plan p = make_plan(N, V, D, type, weight, false, o);
     const State s = state_of(state, N);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
+    if (D <= kNarrowD) {
+        const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
+        switch (type) {
+            case kCeF32: return narrow_forward<float>(a, loss, ws, st);
+            case kCeBf16: return narrow_forward<__nv_bfloat16>(a, loss, ws, st);
+            default: return narrow_forward<__half>(a, loss, ws, st);
+        }
+    }
+    const Plan p = make_plan(N, V, D, type, weight, false, o);
     const int nb = (int)((p.Np + kIdxNT - 1) / kIdxNT);
     if (o.reduction == kCeNone)
         GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
@@ -503,9 +617,19 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
                                       const long long *labels, const CeOpt &o, void *state,
                                       const float *grad_loss, void *grad_features,
                                       void *grad_weight, void *workspace, cudaStream_t st) {
-    const Plan p = make_plan(N, V, D, type, weight, true, o);
     const State s = state_of(state, N);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
+    if (D <= kNarrowD) {
+        const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
+#define GSV_CE_T(T) narrow_backward<T>(a, grad_loss, grad_features, grad_weight, ws, st)
+        switch (type) {
+            case kCeF32: return GSV_CE_T(float);
+            case kCeBf16: return GSV_CE_T(__nv_bfloat16);
+            default: return GSV_CE_T(__half);
+        }
+#undef GSV_CE_T
+    }
+    const Plan p = make_plan(N, V, D, type, weight, true, o);
     float *gmax = type == kCeF16 ? reinterpret_cast<float *>(ws + p.gmax) : nullptr;
     const bool none = o.reduction == kCeNone;
     GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
