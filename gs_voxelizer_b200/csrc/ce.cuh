@@ -41,8 +41,22 @@ __device__ __forceinline__ int ce_label(long long y, long long ignore, int V) {
 __device__ __forceinline__ float ce_nan() { return __int_as_float(0x7fc00000); }
 __device__ __forceinline__ float ce_neg_inf() { return __int_as_float(0xff800000); }
 
+// tanh(s / cap). FAST: 1 - 2 / (1 + e^2x) on the special-function unit, off by
+// at most 2^-22 absolutely - scores enter through differences, so this is
+// what counts - against tanhf's correct digits for float32 inputs.
+template <bool FAST>
+__device__ __forceinline__ float ce_tanh(float s, float cap) {
+    if (!FAST) return tanhf(s / cap);
+    const float u = ex2(fabsf(s) * __fdividef(2.f * kLog2e, cap));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + u));
+    return copysignf(fmaf(-2.f, r, 1.f), s);
+}
+
+// the capped score, and the slope dz / ds that goes with it
+template <bool FAST>
 __device__ __forceinline__ float ce_cap(float s, float cap) {
-    return cap > 0.f ? cap * tanhf(s / cap) : s;
+    return cap > 0.f ? cap * ce_tanh<FAST>(s, cap) : s;
 }
 
 // Running maximum m, sum of exp(z - m) and plain sum of a row's scores. The

@@ -235,7 +235,8 @@ __device__ __forceinline__ int plane_b(int planes, int p) {
     return planes == 3 ? (0x010120 >> (4 * p)) & 3 : 0;
 }
 
-template <int PRODUCT, bool CAP>
+// CAP: 0 no cap, 1 tanh of float32 inputs, 2 of 16-bit inputs
+template <int PRODUCT, int CAP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const CeGemm g, const int nt) {
@@ -441,7 +442,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             z[j] = __uint_as_float(v[j]);
-                            if (CAP) z[j] = ce_cap(z[j], o.cap);
+                            if (CAP) z[j] = o.cap * ce_tanh<CAP == 2>(z[j], o.cap);
                         }
                         if (y >= col0 && y < col0 + 32) {
                             float zy = 0.f;
@@ -475,8 +476,9 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             for (int j = 0; j < 32; ++j) {
                                 float z = __uint_as_float(v[j]), slope = 1.f;
                                 if (CAP) {
-                                    z = ce_cap(z, o.cap);
-                                    slope = 1.f - (z / o.cap) * (z / o.cap);
+                                    const float th = ce_tanh<CAP == 2>(z, o.cap);
+                                    z = o.cap * th;
+                                    slope = fmaf(-th, th, 1.f);
                                 }
                                 float x = fmaf(kz, ce_prob(z, lse), -e);
                                 if (y == g.v0 + col0 + j) x -= hit;
@@ -627,7 +629,7 @@ int tile_n(int cols, int unit) {
     return std::min(kCeTileN, (int)(((long long)cols + unit - 1) / unit * unit));
 }
 
-template <int PRODUCT, bool CAP>
+template <int PRODUCT, int CAP>
 cudaError_t launch(const CeGemm &g, cudaStream_t st) {
     constexpr bool kAMn = PRODUCT == kCeGradW, kBMn = PRODUCT >= kCeGradX;
     const int nt = kBMn ? tile_n(g.D, 128) : tile_n(g.nv, 32);
@@ -682,12 +684,18 @@ int ce_error_flag(bool clear) {
 }
 
 cudaError_t launch_ce_gemm(const CeGemm &g, cudaStream_t st) {
-    const bool cap = g.opt.cap > 0.f;
+    const int cap = g.opt.cap > 0.f ? (g.planes == 3 ? 1 : 2) : 0;
     switch (g.product) {
-        case kCeScores: return cap ? launch<kCeScores, true>(g, st) : launch<kCeScores, false>(g, st);
-        case kCeProbs: return cap ? launch<kCeProbs, true>(g, st) : launch<kCeProbs, false>(g, st);
-        case kCeGradX: return launch<kCeGradX, false>(g, st);
-        default: return launch<kCeGradW, false>(g, st);
+        case kCeScores:
+            return cap == 0   ? launch<kCeScores, 0>(g, st)
+                   : cap == 1 ? launch<kCeScores, 1>(g, st)
+                              : launch<kCeScores, 2>(g, st);
+        case kCeProbs:
+            return cap == 0   ? launch<kCeProbs, 0>(g, st)
+                   : cap == 1 ? launch<kCeProbs, 1>(g, st)
+                              : launch<kCeProbs, 2>(g, st);
+        case kCeGradX: return launch<kCeGradX, 0>(g, st);
+        default: return launch<kCeGradW, 0>(g, st);
     }
 }
 

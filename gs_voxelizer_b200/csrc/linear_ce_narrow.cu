@@ -110,7 +110,7 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
 #pragma unroll
                     for (int k = 0; k < kRows; ++k) {
                         z[k][j] = dot<DP>(x[k], w);
-                        if (CAP) z[k][j] = ce_cap(z[k][j], o.cap);
+                        if (CAP) z[k][j] = ce_cap<sizeof(T) == 2>(z[k][j], o.cap);
                     }
                 } else {
 #pragma unroll
@@ -203,13 +203,13 @@ __device__ __forceinline__ RowGrad row_grad(long long r, int y, const float2 *ls
     return q;
 }
 
-template <bool CAP>
+template <bool CAP, bool FAST>
 __device__ __forceinline__ float derivative(float s, bool is_class, const RowGrad &q,
                                             float cap) {
-    const float z = CAP ? ce_cap(s, cap) : s;
-    float d = fmaf(q.kz, ce_prob(z, q.lse), -q.e);
+    const float t = CAP ? ce_tanh<FAST>(s, cap) : 0.f;
+    float d = fmaf(q.kz, ce_prob(CAP ? cap * t : s, q.lse), -q.e);
     if (is_class) d -= q.hit;
-    if (CAP) d *= 1.f - (z / cap) * (z / cap);
+    if (CAP) d *= fmaf(-t, t, 1.f);
     return d;
 }
 
@@ -245,7 +245,7 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
             const Row<DP> w = sw[j];
 #pragma unroll
             for (int k = 0; k < kRows; ++k) {
-                const float d = derivative<CAP>(dot<DP>(x[k], w), y[k] == v0 + j, q[k], o.cap);
+                const float d = derivative<CAP, sizeof(T) == 2>(dot<DP>(x[k], w), y[k] == v0 + j, q[k], o.cap);
 #pragma unroll
                 for (int i = 0; i < DP; ++i) dx[k].v[i] = fmaf(d, w.v[i], dx[k].v[i]);
             }
@@ -331,13 +331,16 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
         for (int i = slice; i < n; i += slices) {
             const DwRow<DP> s = rows[i];
             const float2 l = make_float2(s.m, s.l2);
-            float z = dot<DP>(s.x, w);
-            if (CAP) z = ce_cap(z, o.cap);
+            float z = dot<DP>(s.x, w), t = 0.f;
+            if (CAP) {
+                t = ce_tanh<sizeof(T) == 2>(z, o.cap);
+                z = o.cap * t;
+            }
             float d = ce_prob(z, l);
             if (!plain) d = fmaf(1.f + 2.f * o.zeta * ce_lse(l), d, -ev);
             if (s.y == j) d -= hv;
             d *= s.g;
-            if (CAP) d *= 1.f - (z / o.cap) * (z / o.cap);
+            if (CAP) d *= fmaf(-t, t, 1.f);
 #pragma unroll
             for (int k = 0; k < DP; ++k) dw.v[k] = fmaf(d, s.x.v[k], dw.v[k]);
         }

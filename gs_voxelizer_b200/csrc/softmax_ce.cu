@@ -3,8 +3,9 @@
 // Both directions are bound by HBM: V b bytes a row are read forward, read
 // and written backward (b bytes a score, V classes). Two layouts:
 //  * V <= kStagedV: a block stages the contiguous scores of its rows in
-//    shared memory with 16-byte accesses - rows of odd lengths have no
-//    alignment of their own - and G lanes share a row;
+//    shared memory with asynchronous 16-byte copies - rows of odd lengths
+//    have no alignment of their own - about 32 KB at once, which is what
+//    keeps enough loads in flight, and G lanes share a row;
 //  * longer rows: one block a row, 16-byte accesses from the first aligned
 //    element on, the running maximum and sum kept per thread and merged.
 #include "ce.cuh"
@@ -21,54 +22,95 @@ struct alignas(16) Vec16 {
     T v[kN];
 };
 
-// n contiguous elements, 16 bytes an access when `vec` (both sides aligned;
-// n * sizeof(T) need not be a multiple of 16)
+// n contiguous elements into shared memory, 16 bytes a copy when `vec`
+// (src aligned; n * sizeof(T) need not be a multiple of 16)
 template <typename T>
-__device__ __forceinline__ void copy_block(T *dst, const T *src, int n, bool vec) {
+__device__ __forceinline__ void stage(T *dst, const T *src, int n, bool vec) {
+    int done = 0;
+    if (vec) {
+        constexpr int kN = Vec16<T>::kN;
+        const int nv = n / kN;
+        const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+        for (int i = threadIdx.x; i < nv; i += kNT)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + 16 * i),
+                         "l"(src + i * kN)
+                         : "memory");
+        done = nv * kN;
+    }
+    for (int i = done + threadIdx.x; i < n; i += kNT) dst[i] = src[i];
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void unstage(T *dst, const T *src, int n, bool vec) {
+    int done = 0;
     if (vec) {
         constexpr int kN = Vec16<T>::kN;
         const int nv = n / kN;
         for (int i = threadIdx.x; i < nv; i += kNT)
-            reinterpret_cast<Vec16<T> *>(dst)[i] =
-                reinterpret_cast<const Vec16<T> *>(src)[i];
-        for (int i = nv * kN + threadIdx.x; i < n; i += kNT) dst[i] = src[i];
-    } else {
-        for (int i = threadIdx.x; i < n; i += kNT) dst[i] = src[i];
+            __stcs(reinterpret_cast<int4 *>(dst) + i, reinterpret_cast<const int4 *>(src)[i]);
+        done = nv * kN;
+    }
+    for (int i = done + threadIdx.x; i < n; i += kNT) dst[i] = src[i];
+}
+
+// Elements of a row that a lane of its group takes: lane, lane + G, ... from
+// a start that differs between the groups of a warp, as rows of V = 2^k
+// would otherwise all begin in the same bank.
+template <int G, typename F>
+__device__ __forceinline__ void each_of_row(int V, F f) {
+    const int lane = threadIdx.x % G, n = (V + G - 1) / G;
+    int k = G == 32 ? 0 : ((threadIdx.x & 31) / G) % n;
+    for (int i = 0; i < n; ++i) {
+        const int j = k * G + lane;
+        if (G == 1 || j < V) f(j);
+        if (++k == n) k = 0;
     }
 }
 
-template <typename T, int G>
+template <int G>
+__device__ __forceinline__ unsigned group_mask() {
+    return G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G);
+}
+
+// kPass rows at once (one a group of G lanes), `passes` times
+template <typename T, int G, bool CAP>
 __global__ void __launch_bounds__(kNT)
-staged_fwd_kernel(long long rows, int V, const T *__restrict__ scores,
+staged_fwd_kernel(long long rows, int V, int passes, const T *__restrict__ scores,
                   const long long *__restrict__ labels, CeOpt o, bool vec,
                   float *__restrict__ loss, float2 *__restrict__ lse_out,
                   float *__restrict__ count, float2 *__restrict__ partials) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float2 sh[kNT / 32];
     T *tile = reinterpret_cast<T *>(smem_raw);
-    constexpr int R = kNT / G;
-    const long long row0 = (long long)blockIdx.x * R;
-    const int nr = (int)min((long long)R, rows - row0);
-    copy_block(tile, scores + row0 * V, nr * V, vec);
+    constexpr int kPass = kNT / G;
+    const long long row0 = (long long)blockIdx.x * kPass * passes;
+    const int nr = (int)min((long long)kPass * passes, rows - row0);
+    const int r0 = threadIdx.x / G, lane = threadIdx.x % G;
+    long long y_next = r0 < nr ? labels[row0 + r0] : o.ignore;
+    stage(tile, scores + row0 * V, nr * V, vec);
     __syncthreads();
-    const int r = threadIdx.x / G, lane = threadIdx.x % G;
-    float l = 0.f, cnt = 0.f;
-    if (r < nr) {  // whole groups of G lanes take the same branch
-        const unsigned mask = G == 32 ? 0xffffffffu
-                                      : ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G);
+    const unsigned mask = group_mask<G>();
+    auto score = [&](T v) {
+        const float s = ce_to_float(v);
+        return CAP ? o.cap * ce_tanh<sizeof(T) == 2>(s, o.cap) : s;
+    };
+    float lsum = 0.f, cnt = 0.f;
+    for (int r = r0; r < nr; r += kPass) {  // whole groups take the same path
         const T *p = tile + r * V;
-        const int y = ce_label(labels[row0 + r], o.ignore, V);
+        const int y = ce_label(y_next, o.ignore, V);
+        if (r + kPass < nr) y_next = labels[row0 + r + kPass];
         CeAcc a;
         a.init();
-        for (int j = lane; j < V; j += G) a.m = fmaxf(a.m, ce_cap(ce_to_float(p[j]), o.cap));
+        each_of_row<G>(V, [&](int j) { a.m = fmaxf(a.m, score(p[j])); });
 #pragma unroll
         for (int k = G / 2; k; k >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(mask, a.m, k));
         const float b = CeAcc::base(a.m);
-        for (int j = lane; j < V; j += G) {
-            const float z = ce_cap(ce_to_float(p[j]), o.cap);
+        each_of_row<G>(V, [&](int j) {
+            const float z = score(p[j]);
             a.s += ex2((z - b) * kLog2e);
             a.sz += z;
-        }
+        });
 #pragma unroll
         for (int k = G / 2; k; k >>= 1) {
             a.s += __shfl_xor_sync(mask, a.s, k);
@@ -76,17 +118,18 @@ staged_fwd_kernel(long long rows, int V, const T *__restrict__ scores,
         }
         if (lane == 0) {
             float2 lse = a.lse();
-            if (y >= 0) {
-                l = ce_row_loss(lse, ce_cap(ce_to_float(p[y]), o.cap), a.sz, V, o);
-            } else if (y == kCeInvalid) {
+            float l = 0.f;
+            if (y >= 0)
+                l = ce_row_loss(lse, score(p[y]), a.sz, V, o);
+            else if (y == kCeInvalid)
                 l = lse.x = ce_nan();
-            }
-            cnt = y == kCeIgnored ? 0.f : 1.f;
+            cnt += y == kCeIgnored ? 0.f : 1.f;
+            lsum += l;
             lse_out[row0 + r] = lse;
             if (o.reduction == kCeNone) loss[row0 + r] = l;
         }
     }
-    const float2 t = ce_block_sum<kNT>(l, cnt, sh);
+    const float2 t = ce_block_sum<kNT>(lsum, cnt, sh);
     if (threadIdx.x == 0) {
         if (gridDim.x == 1)
             ce_finish(t.x, t.y, o.reduction, loss, count);
@@ -95,53 +138,67 @@ staged_fwd_kernel(long long rows, int V, const T *__restrict__ scores,
     }
 }
 
-// gradient of one score: k = 1 + 2 zeta lse, e = eps / V
-__device__ __forceinline__ float grad_of(float s, bool hit, float2 lse, float k, float e,
-                                         float g, const CeOpt &o) {
-    const float z = ce_cap(s, o.cap);
-    float d = k * ce_prob(z, lse) - e;
-    if (hit) d -= 1.f - o.eps;
-    if (o.cap > 0.f) {
-        const float t = z / o.cap;
-        d *= 1.f - t * t;
-    }
-    return d * g;
+// A row's share of the gradient of its scores: kz prob - e (- hit at its
+// class), the upstream gradient in all three.
+struct RowGrad {
+    float2 lse;
+    float kz, e, hit;
+};
+
+__device__ __forceinline__ RowGrad row_grad(long long row, float2 lse, int V, const float *g,
+                                            const float *count, const CeOpt &o) {
+    const float f = o.reduction == kCeNone ? g[row]
+                    : o.reduction == kCeMean ? g[0] / count[0]
+                                             : g[0];
+    return {lse, (1.f + 2.f * o.zeta * ce_lse(lse)) * f, o.eps / (float)V * f,
+            (1.f - o.eps) * f};
 }
 
-__device__ __forceinline__ float upstream(const float *g, long long row,
-                                          const float *count, const CeOpt &o) {
-    if (o.reduction == kCeNone) return g[row];
-    return o.reduction == kCeMean ? g[0] / count[0] : g[0];
+template <typename T, bool CAP>
+__device__ __forceinline__ float grad_of(T v, bool is_class, const RowGrad &q, float cap) {
+    const float s = ce_to_float(v);
+    const float t = CAP ? ce_tanh<sizeof(T) == 2>(s, cap) : 0.f;
+    float d = fmaf(q.kz, ce_prob(CAP ? cap * t : s, q.lse), -q.e);
+    if (is_class) d -= q.hit;
+    if (CAP) d *= fmaf(-t, t, 1.f);
+    return d;
 }
 
-template <typename T, int G>
+template <typename T, int G, bool CAP>
 __global__ void __launch_bounds__(kNT)
-staged_bwd_kernel(long long rows, int V, const T *__restrict__ scores,
+staged_bwd_kernel(long long rows, int V, int passes, const T *__restrict__ scores,
                   const long long *__restrict__ labels, CeOpt o, bool vec,
                   const float2 *__restrict__ lse_in, const float *__restrict__ count,
                   const float *__restrict__ grad_loss, T *__restrict__ grad) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     T *tile = reinterpret_cast<T *>(smem_raw);
-    constexpr int R = kNT / G;
-    const long long row0 = (long long)blockIdx.x * R;
-    const int nr = (int)min((long long)R, rows - row0);
-    copy_block(tile, scores + row0 * V, nr * V, vec);
+    constexpr int kPass = kNT / G;
+    const long long row0 = (long long)blockIdx.x * kPass * passes;
+    const int nr = (int)min((long long)kPass * passes, rows - row0);
+    const int r0 = threadIdx.x / G;
+    long long y_next = o.ignore;
+    float2 lse_next = make_float2(0.f, 0.f);
+    if (r0 < nr) {
+        y_next = labels[row0 + r0];
+        lse_next = lse_in[row0 + r0];
+    }
+    stage(tile, scores + row0 * V, nr * V, vec);
     __syncthreads();
-    const int r = threadIdx.x / G, lane = threadIdx.x % G;
-    if (r < nr) {
+    for (int r = r0; r < nr; r += kPass) {
         T *p = tile + r * V;
-        const int y = ce_label(labels[row0 + r], o.ignore, V);
-        const float2 lse = lse_in[row0 + r];
-        const float k = 1.f + 2.f * o.zeta * ce_lse(lse);
-        const float e = o.eps / (float)V;
-        const float g = upstream(grad_loss, row0 + r, count, o);
-        for (int j = lane; j < V; j += G)
-            p[j] = ce_from_float<T>(y == kCeIgnored ? 0.f
-                                                    : grad_of(ce_to_float(p[j]), j == y, lse,
-                                                              k, e, g, o));
+        const int y = ce_label(y_next, o.ignore, V);
+        const RowGrad q = row_grad(row0 + r, lse_next, V, grad_loss, count, o);
+        if (r + kPass < nr) {
+            y_next = labels[row0 + r + kPass];
+            lse_next = lse_in[row0 + r + kPass];
+        }
+        each_of_row<G>(V, [&](int j) {
+            const float d = grad_of<T, CAP>(p[j], j == y, q, o.cap);
+            p[j] = ce_from_float<T>(y == kCeIgnored ? 0.f : d);
+        });
     }
     __syncthreads();
-    copy_block(grad + row0 * V, tile, nr * V, vec);
+    unstage(grad + row0 * V, tile, nr * V, vec);
 }
 
 // One block a row. `head`: elements before the first 16-byte boundary.
@@ -151,7 +208,7 @@ __device__ __forceinline__ int head_of(const T *p, int V) {
     return mis ? min(V, (16 - mis) / (int)sizeof(T)) : 0;
 }
 
-template <typename T>
+template <typename T, bool CAP>
 __global__ void __launch_bounds__(kNT)
 row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict__ labels,
                CeOpt o, float *__restrict__ loss, float2 *__restrict__ lse_out,
@@ -162,13 +219,20 @@ row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
     const int head = head_of(p, V), nv = (V - head) / kN;
     CeAcc a;
     a.init();
-    auto one = [&](float s) { const float z = ce_cap(s, o.cap); a.merge(z, 1.f, z); };
+    auto score = [&](T v) {
+        const float s = ce_to_float(v);
+        return CAP ? o.cap * ce_tanh<sizeof(T) == 2>(s, o.cap) : s;
+    };
+    auto one = [&](T v) {
+        const float z = score(v);
+        a.merge(z, 1.f, z);
+    };
     for (int i = threadIdx.x; i < nv; i += kNT) {
         const Vec16<T> q = reinterpret_cast<const Vec16<T> *>(p + head)[i];
         float z[kN], m = a.m;
 #pragma unroll
         for (int k = 0; k < kN; ++k) {
-            z[k] = ce_cap(ce_to_float(q.v[k]), o.cap);
+            z[k] = score(q.v[k]);
             m = fmaxf(m, z[k]);
             a.sz += z[k];
         }
@@ -178,9 +242,9 @@ row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
 #pragma unroll
         for (int k = 0; k < kN; ++k) a.s += ex2((z[k] - b) * kLog2e);
     }
-    if ((int)threadIdx.x < head) one(ce_to_float(p[threadIdx.x]));
+    if ((int)threadIdx.x < head) one(p[threadIdx.x]);
     const int tail = head + nv * kN + (int)threadIdx.x;
-    if (tail < V) one(ce_to_float(p[tail]));
+    if (tail < V) one(p[tail]);
     __shared__ float sm[kNT / 32], ss[kNT / 32], sz[kNT / 32];
 #pragma unroll
     for (int k = 16; k; k >>= 1)
@@ -198,7 +262,7 @@ row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
     float2 lse = a.lse();
     float l = 0.f;
     if (y >= 0)
-        l = ce_row_loss(lse, ce_cap(ce_to_float(p[y]), o.cap), a.sz, V, o);
+        l = ce_row_loss(lse, score(p[y]), a.sz, V, o);
     else if (y == kCeInvalid)
         l = lse.x = ce_nan();
     lse_out[row] = lse;
@@ -210,7 +274,7 @@ row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
         partials[row] = make_float2(l, c);
 }
 
-template <typename T>
+template <typename T, bool CAP>
 __global__ void __launch_bounds__(kNT)
 row_bwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict__ labels,
                CeOpt o, const float2 *__restrict__ lse_in, const float *__restrict__ count,
@@ -218,26 +282,28 @@ row_bwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
     constexpr int kN = Vec16<T>::kN;
     const long long row = blockIdx.x;
     const T *p = scores + row * (long long)V;
-    T *q = grad + row * (long long)V;
+    T *out = grad + row * (long long)V;
     const int head = same_head ? head_of(p, V) : V;
     const int nv = (V - head) / kN;
     const int y = ce_label(labels[row], o.ignore, V);
-    const float2 lse = lse_in[row];
-    const float k = 1.f + 2.f * o.zeta * ce_lse(lse), e = o.eps / (float)V;
-    const float g = upstream(grad_loss, row, count, o);
+    const RowGrad q = row_grad(row, lse_in[row], V, grad_loss, count, o);
     auto one = [&](int j) {
-        q[j] = ce_from_float<T>(
-            y == kCeIgnored ? 0.f : grad_of(ce_to_float(p[j]), j == y, lse, k, e, g, o));
+        const float d = grad_of<T, CAP>(p[j], j == y, q, o.cap);
+        out[j] = ce_from_float<T>(y == kCeIgnored ? 0.f : d);
     };
-    for (int i = threadIdx.x; i < nv; i += kNT) {
-        Vec16<T> v = reinterpret_cast<const Vec16<T> *>(p + head)[i];
+    int4 *o16 = reinterpret_cast<int4 *>(out + head);
+    if (y == kCeIgnored) {  // nothing of the row is read
+        for (int i = threadIdx.x; i < nv; i += kNT) __stcs(o16 + i, make_int4(0, 0, 0, 0));
+    } else {
+#pragma unroll 2
+        for (int i = threadIdx.x; i < nv; i += kNT) {
+            Vec16<T> v = reinterpret_cast<const Vec16<T> *>(p + head)[i];
+            const int at = y - (head + i * kN);
 #pragma unroll
-        for (int t = 0; t < kN; ++t)
-            v.v[t] = ce_from_float<T>(
-                y == kCeIgnored ? 0.f
-                                : grad_of(ce_to_float(v.v[t]), head + i * kN + t == y, lse,
-                                          k, e, g, o));
-        reinterpret_cast<Vec16<T> *>(q + head)[i] = v;
+            for (int t = 0; t < kN; ++t)
+                v.v[t] = ce_from_float<T>(grad_of<T, CAP>(v.v[t], t == at, q, o.cap));
+            __stcs(o16 + i, reinterpret_cast<const int4 &>(v));
+        }
     }
     for (int j = threadIdx.x; j < head; j += kNT) one(j);
     for (int j = head + nv * kN + (int)threadIdx.x; j < V; j += kNT) one(j);
@@ -272,71 +338,86 @@ finish_kernel(const float2 *__restrict__ partials, int n, int reduction,
     }
 }
 
-// lanes a row: about eight scores each
+// lanes a row: at most 32 scores each
 int lanes_of(int V) {
     int g = 1;
-    while (g < 32 && g * 8 < V) g *= 2;
+    while (g < 32 && g * 32 < V) g *= 2;
     return g;
 }
 
-template <typename T, int G>
-cudaError_t staged(bool fwd, long long rows, int V, const void *scores,
-                   const long long *labels, const CeOpt &o, float *loss, float2 *lse,
-                   float *count, const float *grad_loss, void *grad, float2 *partials,
-                   cudaStream_t st) {
-    constexpr int R = kNT / G;
-    const long long blocks = (rows + R - 1) / R;
-    const size_t smem = (size_t)R * V * sizeof(T);  // <= 32 KB
-    const bool vec = ((reinterpret_cast<uintptr_t>(scores) |
-                       reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
+// Times that a block's groups go over its rows: as many as 32 KB of scores
+// hold (at most 8), while the blocks still fill the device twice.
+int passes_of(long long rows, int V, size_t bytes) {
+    const long long pass = kNT / lanes_of(V);
+    const long long fit = (32 << 10) / (pass * V * (long long)bytes);
+    return (int)std::max(1LL, std::min({8LL, fit, rows / (pass * 2 * kSMs)}));
+}
+
+// Every argument of both directions.
+struct Args {
+    long long rows;
+    int V;
+    const void *scores;
+    const long long *labels;
+    CeOpt o;
+    float *loss;
+    float2 *lse;
+    float *count;
+    const float *grad_loss;
+    void *grad;
+    float2 *partials;
+    cudaStream_t st;
+};
+
+template <typename T, int G, bool CAP>
+cudaError_t staged(bool fwd, const Args &a) {
+    const int passes = passes_of(a.rows, a.V, sizeof(T));
+    const long long per = (long long)(kNT / G) * passes, blocks = (a.rows + per - 1) / per;
+    const size_t smem = (size_t)per * a.V * sizeof(T);  // <= 32 KB
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.scores) |
+                       reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
     if (fwd)
-        staged_fwd_kernel<T, G><<<(unsigned)blocks, kNT, smem, st>>>(
-            rows, V, static_cast<const T *>(scores), labels, o, vec, loss, lse, count, partials);
+        staged_fwd_kernel<T, G, CAP><<<(unsigned)blocks, kNT, smem, a.st>>>(
+            a.rows, a.V, passes, static_cast<const T *>(a.scores), a.labels, a.o, vec, a.loss,
+            a.lse, a.count, a.partials);
     else
-        staged_bwd_kernel<T, G><<<(unsigned)blocks, kNT, smem, st>>>(
-            rows, V, static_cast<const T *>(scores), labels, o, vec, lse, count, grad_loss,
-            static_cast<T *>(grad));
+        staged_bwd_kernel<T, G, CAP><<<(unsigned)blocks, kNT, smem, a.st>>>(
+            a.rows, a.V, passes, static_cast<const T *>(a.scores), a.labels, a.o, vec, a.lse,
+            a.count, a.grad_loss, static_cast<T *>(a.grad));
     count_launches(1);
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess && fwd && blocks > 1)
-        err = launch_ce_finish(partials, (int)blocks, o.reduction, loss, count, st);
+        err = launch_ce_finish(a.partials, (int)blocks, a.o.reduction, a.loss, a.count, a.st);
     return err;
 }
 
-template <typename T>
-cudaError_t run(bool fwd, long long rows, int V, const void *scores, const long long *labels,
-                const CeOpt &o, float *loss, float2 *lse, float *count,
-                const float *grad_loss, void *grad, float2 *partials, cudaStream_t st) {
-    if (V <= kStagedV) {
-        switch (lanes_of(V)) {
-#define GSV_CE_G(G)                                                                     \
-    case G:                                                                             \
-        return staged<T, G>(fwd, rows, V, scores, labels, o, loss, lse, count, grad_loss, \
-                            grad, partials, st)
-            GSV_CE_G(1);
-            GSV_CE_G(2);
-            GSV_CE_G(4);
-            GSV_CE_G(8);
-            GSV_CE_G(16);
-            default:
-            GSV_CE_G(32);
-#undef GSV_CE_G
+template <typename T, bool CAP>
+cudaError_t run(bool fwd, const Args &a) {
+    if (a.V <= kStagedV) {
+        switch (lanes_of(a.V)) {
+            case 1: return staged<T, 1, CAP>(fwd, a);
+            case 2: return staged<T, 2, CAP>(fwd, a);
+            case 4: return staged<T, 4, CAP>(fwd, a);
+            case 8: return staged<T, 8, CAP>(fwd, a);
+            case 16: return staged<T, 16, CAP>(fwd, a);
+            default: return staged<T, 32, CAP>(fwd, a);
         }
     }
+    const T *scores = static_cast<const T *>(a.scores);
     if (fwd) {
-        row_fwd_kernel<T><<<(unsigned)rows, kNT, 0, st>>>(V, static_cast<const T *>(scores),
-                                                          labels, o, loss, lse, count, partials);
+        row_fwd_kernel<T, CAP><<<(unsigned)a.rows, kNT, 0, a.st>>>(
+            a.V, scores, a.labels, a.o, a.loss, a.lse, a.count, a.partials);
     } else {
-        const bool same = ((reinterpret_cast<uintptr_t>(scores) ^
-                            reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
-        row_bwd_kernel<T><<<(unsigned)rows, kNT, 0, st>>>(V, static_cast<const T *>(scores),
-                                                          labels, o, lse, count, grad_loss,
-                                                          static_cast<T *>(grad), same);
+        const bool same = ((reinterpret_cast<uintptr_t>(a.scores) ^
+                            reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
+        row_bwd_kernel<T, CAP><<<(unsigned)a.rows, kNT, 0, a.st>>>(
+            a.V, scores, a.labels, a.o, a.lse, a.count, a.grad_loss,
+            static_cast<T *>(a.grad), same);
     }
     count_launches(1);
     cudaError_t err = cudaGetLastError();
-    if (err == cudaSuccess && fwd && rows > 1)
-        err = launch_ce_finish(partials, (int)rows, o.reduction, loss, count, st);
+    if (err == cudaSuccess && fwd && a.rows > 1)
+        err = launch_ce_finish(a.partials, (int)a.rows, a.o.reduction, a.loss, a.count, a.st);
     return err;
 }
 
@@ -350,6 +431,7 @@ cudaError_t launch_ce_finish(const float2 *partials, int n, int reduction, float
 }
 
 size_t softmax_ce_workspace_bytes(long long rows, int V) {
+    // with one pass a block, the most blocks there can be
     const long long r = V <= kStagedV ? kNT / lanes_of(V) : 1;
     return sizeof(float2) * (size_t)((rows + r - 1) / r);
 }
@@ -358,17 +440,15 @@ cudaError_t launch_softmax_ce(bool fwd, int type, long long rows, int V, const v
                               const long long *labels, const CeOpt &o, float *loss,
                               float2 *lse, float *count, const float *grad_loss, void *grad,
                               void *ws, cudaStream_t st) {
-    float2 *partials = static_cast<float2 *>(ws);
+    const Args a{rows, V,     scores,    labels, o,
+                 loss, lse,   count,     grad_loss, grad,
+                 static_cast<float2 *>(ws), st};
+    const bool cap = o.cap > 0.f;
     switch (type) {
-        case kCeF32:
-            return run<float>(fwd, rows, V, scores, labels, o, loss, lse, count, grad_loss,
-                              grad, partials, st);
+        case kCeF32: return cap ? run<float, true>(fwd, a) : run<float, false>(fwd, a);
         case kCeBf16:
-            return run<__nv_bfloat16>(fwd, rows, V, scores, labels, o, loss, lse, count,
-                                      grad_loss, grad, partials, st);
-        default:
-            return run<__half>(fwd, rows, V, scores, labels, o, loss, lse, count, grad_loss,
-                               grad, partials, st);
+            return cap ? run<__nv_bfloat16, true>(fwd, a) : run<__nv_bfloat16, false>(fwd, a);
+        default: return cap ? run<__half, true>(fwd, a) : run<__half, false>(fwd, a);
     }
 }
 
