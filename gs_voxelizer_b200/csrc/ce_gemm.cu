@@ -51,6 +51,18 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// One lane of the warp. The compiler knows it for one thread, which a test of
+// the lane number does not tell it: with that test each tcgen05.mma was
+// issued behind a loop over the active lanes, and the MMAs ran at 190 clocks
+// each instead of 128 (256 x 256 x 16), whatever fed them.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
 // address of the leader's copy of a barrier
 __device__ __forceinline__ uint32_t in_leader(uint32_t a) {
     uint32_t r;
@@ -276,7 +288,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const Work w = work_of<PRODUCT>(g, nt);
     const int pairs = pairs_of(g.planes);
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
         // ------------------------------------------------------ producer
         int stage = 0;
         uint32_t phase = 0;
@@ -334,7 +346,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 phase ^= 1;
             }
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0 && elect_one()) {
         // ----------------------------------------------------------- MMA
         // D float32, A and B bf16 or fp16, M = 256
         const uint32_t type = g.bf16 ? 1u : 0u;
