@@ -211,11 +211,20 @@ __device__ __forceinline__ Work work_of(const CeGemm &g, int nt) {
 
 struct Unit {
     int m, n0, n1, split, k0, k1;  // n tiles [n0, n1), K blocks [k0, k1)
+    int chunks;                    // parts of [k0, k1), see kChunk
+    // the unit's accumulators, one after another
+    __device__ __forceinline__ int steps() const { return (n1 - n0) * chunks; }
 };
+
+// float32 products are accumulated in tensor memory over 512 of K at most
+// and summed in registers or memory from there: the tensor cores truncate
+// each addition, which over 4000 of K cost 4e-6 of the result (16 at a time;
+// 5e-7 over 512). 16-bit results do not see it.
+constexpr int kChunk = 512 / kDepth;
 
 // m fastest: the pairs in flight share class tiles, and each keeps to rows
 // that stay in L2
-template <int PRODUCT>
+template <int PRODUCT, bool F32>
 __device__ __forceinline__ Unit unit_of(const CeGemm &g, const Work &w, int u) {
     Unit t;
     t.m = u % w.mtiles;
@@ -234,21 +243,23 @@ __device__ __forceinline__ Unit unit_of(const CeGemm &g, const Work &w, int u) {
         t.k0 = (int)((long long)w.kblocks * t.split / g.splits);
         t.k1 = (int)((long long)w.kblocks * (t.split + 1) / g.splits);
     }
+    t.chunks = F32 ? max(1, (t.k1 - t.k0 + kChunk - 1) / kChunk) : 1;
     return t;
 }
 
 // Plane pairs of a float32 product, least first: (2,0) (0,2) (1,1) (1,0)
 // (0,1) (0,0). The pairs left out are below 2^-26 of the whole.
-__device__ __forceinline__ int pairs_of(int planes) { return planes == 3 ? 6 : 1; }
-__device__ __forceinline__ int plane_a(int planes, int p) {
-    return planes == 3 ? (0x001102 >> (4 * p)) & 3 : 0;
+template <bool F32>
+__device__ __forceinline__ int plane_a(int p) {
+    return F32 ? (0x001102 >> (4 * p)) & 3 : 0;
 }
-__device__ __forceinline__ int plane_b(int planes, int p) {
-    return planes == 3 ? (0x010120 >> (4 * p)) & 3 : 0;
+template <bool F32>
+__device__ __forceinline__ int plane_b(int p) {
+    return F32 ? (0x010120 >> (4 * p)) & 3 : 0;
 }
 
-// CAP: 0 no cap, 1 tanh of float32 inputs, 2 of 16-bit inputs
-template <int PRODUCT, int CAP>
+// F32: three planes
+template <int PRODUCT, bool CAP, bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const CeGemm g, const int nt) {
@@ -286,7 +297,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     fence_after();
     const uint32_t tmem = S.tmem;
     const Work w = work_of<PRODUCT>(g, nt);
-    const int pairs = pairs_of(g.planes);
+    const int pairs = F32 ? 6 : 1;
 
     if (warp == 0 && elect_one()) {
         // ------------------------------------------------------ producer
@@ -295,13 +306,15 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         bool ok = true;
         const uint32_t bytes = 2 * (kABytes + nt / 2 * kDepth * 2);
         for (int u = first; ok && u < w.units; u += step) {
-            const Unit t = unit_of<PRODUCT>(g, w, u);
-            for (int n = t.n0; ok && n < t.n1; ++n) {
-                const int m_at = t.m * kCeTileM + (int)rank * 128;
-                const int n_at = n * nt + (int)rank * (nt / 2);
+            const Unit t = unit_of<PRODUCT, F32>(g, w, u);
+            const int m_at = t.m * kCeTileM + (int)rank * 128;
+            for (int i = 0; ok && i < t.steps(); ++i) {
+                const int n_at = (t.n0 + i / t.chunks) * nt + (int)rank * (nt / 2);
+                const int k0 = t.k0 + (F32 ? i % t.chunks * kChunk : 0);
+                const int k1 = F32 ? min(t.k1, k0 + kChunk) : t.k1;
                 for (int p = 0; ok && p < pairs; ++p) {
-                    const int pa = plane_a(g.planes, p), pb = plane_b(g.planes, p);
-                    for (int k = t.k0; k < t.k1; ++k) {
+                    const int pa = plane_a<F32>(p), pb = plane_b<F32>(p);
+                    for (int k = k0; k < k1; ++k) {
                         if (!bar_wait(&S.empty[stage], phase ^ 1)) {
                             ok = false;
                             break;
@@ -357,9 +370,11 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
         for (int u = first; ok && u < w.units; u += step) {
-            const Unit t = unit_of<PRODUCT>(g, w, u);
+            const Unit t = unit_of<PRODUCT, F32>(g, w, u);
             if (t.k0 == t.k1) continue;
-            for (int n = t.n0; ok && n < t.n1; ++n) {
+            for (int i = 0; ok && i < t.steps(); ++i) {
+                const int k0 = t.k0 + (F32 ? i % t.chunks * kChunk : 0);
+                const int k1 = F32 ? min(t.k1, k0 + kChunk) : t.k1;
                 if (!bar_wait(&S.tempty[acc], acc_phase ^ 1)) {
                     ok = false;
                     break;
@@ -367,7 +382,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 fence_after();
                 uint32_t accumulate = 0;
                 for (int p = 0; ok && p < pairs; ++p)
-                    for (int k = t.k0; k < t.k1; ++k) {
+                    for (int k = k0; k < k1; ++k) {
                         if (!bar_wait(&S.full[stage], phase)) {
                             ok = false;
                             break;
@@ -378,7 +393,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         // the last block may end early (its rest is zeros)
                         const long long left = w.K - (long long)k * kDepth;
                         const int steps = left >= kDepth ? 4 : (int)((left + 15) / 16);
-                        for (int i = 0; i < steps; ++i) {
+                        for (int j = 0; j < steps; ++j) {
                             mma(tmem + acc * kCeTileN, da, db, idesc, accumulate);
                             accumulate = 1;
                             da += k_step(kAMn);
@@ -409,7 +424,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         float scale = 1.f;
         if (PRODUCT >= kCeGradX && g.dst) scale = ce_grad_scale(g.up);
         for (int u = first; ok && u < w.units; u += step) {
-            const Unit t = unit_of<PRODUCT>(g, w, u);
+            const Unit t = unit_of<PRODUCT, F32>(g, w, u);
             const long long r = (long long)t.m * kCeTileM + rank * 128 + q * 32 + lane;
             // per-row state
             int y = kCeIgnored;
@@ -431,7 +446,10 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     hit = (1.f - o.eps) * f;
                 }
             }
-            for (int n = t.n0; ok && n < t.n1; ++n) {
+            float sum[F32 && PRODUCT <= kCeProbs ? 2 : 1][32];
+            for (int i = 0; ok && i < t.steps(); ++i) {
+                const int n = t.n0 + i / t.chunks, chunk = i % t.chunks;
+                const bool last = chunk == t.chunks - 1;
                 const bool empty = t.k0 == t.k1;
                 if (!empty) {
                     ok = __all_sync(0xffffffffu, bar_wait(&S.tfull[acc], acc_phase));
@@ -439,7 +457,10 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     fence_after();
                 }
                 uint32_t v[32];
-                for (int c = half; c < chunks; c += 2) {
+#pragma unroll(F32 && PRODUCT <= kCeProbs ? 2 : 1)
+                for (int h = 0; h < (F32 && PRODUCT <= kCeProbs ? 2 : 4); ++h) {
+                    const int c = 2 * h + half;
+                    if (c >= chunks) continue;
                     const int col0 = n * nt + c * 32;  // within the piece
                     if (empty) {
 #pragma unroll
@@ -448,13 +469,25 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         load32(tlane + acc * kCeTileN + c * 32, v);
                         load_wait(v);
                     }
+                    if constexpr (F32 && PRODUCT <= kCeProbs) {
+                        if (t.chunks > 1) {
+                            // the chunks of K, summed in float32
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const float a = __uint_as_float(v[j]);
+                                sum[h][j] = chunk ? sum[h][j] + a : a;
+                                v[j] = __float_as_uint(sum[h][j]);
+                            }
+                            if (!last) continue;
+                        }
+                    }
                     if constexpr (PRODUCT == kCeScores) {
                         const int valid = g.nv - col0;
                         float z[32], m = top;
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             z[j] = __uint_as_float(v[j]);
-                            if (CAP) z[j] = o.cap * ce_tanh<CAP == 2>(z[j], o.cap);
+                            if (CAP) z[j] = o.cap * ce_tanh<!F32>(z[j], o.cap);
                         }
                         if (y >= col0 && y < col0 + 32) {
                             float zy = 0.f;
@@ -488,7 +521,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             for (int j = 0; j < 32; ++j) {
                                 float z = __uint_as_float(v[j]), slope = 1.f;
                                 if (CAP) {
-                                    const float th = ce_tanh<CAP == 2>(z, o.cap);
+                                    const float th = ce_tanh<!F32>(z, o.cap);
                                     z = o.cap * th;
                                     slope = fmaf(-th, th, 1.f);
                                 }
@@ -497,61 +530,54 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                                 if (CAP) x *= slope;
                                 d[j] = y != kCeIgnored && col0 + j < g.nv ? x : 0.f;
                             }
-                            for (int p = 0; p < g.planes; ++p) {
-                                uint32_t h[16];
+                            for (int p = 0; p < (F32 ? 3 : 1); ++p) {
+                                uint32_t out[16];
 #pragma unroll
                                 for (int j = 0; j < 16; ++j) {
-                                    h[j] = pack2(d[2 * j], d[2 * j + 1], g.bf16);
-                                    if (g.planes > 1) {
-                                        d[2 * j] -= __uint_as_float(h[j] << 16);
-                                        d[2 * j + 1] -= __uint_as_float(h[j] & 0xffff0000u);
+                                    out[j] = pack2(d[2 * j], d[2 * j + 1], F32 || g.bf16);
+                                    if (F32) {
+                                        d[2 * j] -= __uint_as_float(out[j] << 16);
+                                        d[2 * j + 1] -= __uint_as_float(out[j] & 0xffff0000u);
                                     }
                                 }
-                                char *out = static_cast<char *>(g.p_out) +
-                                            2 * (p * g.P.plane + r * g.P.ld + col0);
-                                store8(out, h);
-                                store8(out + 32, h + 8);
+                                char *to = static_cast<char *>(g.p_out) +
+                                           2 * (p * g.P.plane + r * g.P.ld + col0);
+                                store8(to, out);
+                                store8(to + 32, out + 8);
                             }
                         }
                     } else {
                         const long long M = PRODUCT == kCeGradW ? g.nv : w.live;
                         if (r < M && col0 < g.D) {
                             const int cols = min(32, g.D - col0);
-                            if (g.dst) {
+                            if (!F32 && g.dst) {
                                 long long to = r;
                                 if (PRODUCT == kCeGradX)
                                     to = g.idx ? g.idx[g.row0 + r] : g.row0 + r;
                                 else
                                     to += g.v0;
-                                const long long at = to * g.D + col0;
-                                if (g.dst_type == kCeF32) {
-                                    float *p = static_cast<float *>(g.dst) + at;
-                                    for (int j = 0; j < 32; ++j)
-                                        if (j < cols) p[j] = __uint_as_float(v[j]) * scale;
+                                uint32_t out[16];
+#pragma unroll
+                                for (int j = 0; j < 16; ++j)
+                                    out[j] = pack2(__uint_as_float(v[2 * j]) * scale,
+                                                   __uint_as_float(v[2 * j + 1]) * scale, g.bf16);
+                                uint16_t *p = static_cast<uint16_t *>(g.dst) + to * g.D + col0;
+                                if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+                                    store8(p, out);
+                                    store8(p + 16, out + 8);
                                 } else {
-                                    uint32_t h[16];
 #pragma unroll
-                                    for (int j = 0; j < 16; ++j)
-                                        h[j] = pack2(__uint_as_float(v[2 * j]) * scale,
-                                                     __uint_as_float(v[2 * j + 1]) * scale,
-                                                     g.bf16);
-                                    uint16_t *p = static_cast<uint16_t *>(g.dst) + at;
-                                    if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
-                                        store8(p, h);
-                                        store8(p + 16, h + 8);
-                                    } else {
-#pragma unroll
-                                        for (int j = 0; j < 32; ++j)
-                                            if (j < cols)
-                                                p[j] = (uint16_t)(h[j / 2] >> (16 * (j & 1)));
-                                    }
+                                    for (int j = 0; j < 32; ++j)
+                                        if (j < cols)
+                                            p[j] = (uint16_t)(out[j / 2] >> (16 * (j & 1)));
                                 }
                             } else {
+                                const bool add = g.add || chunk > 0;
                                 float *p = g.acc + t.split * g.acc_split + r * g.D + col0;
                                 if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
 #pragma unroll
                                     for (int j = 0; j < 32; j += 8) {
-                                        if (g.add) {
+                                        if (add) {
                                             float old[8];
                                             fetch8(p + j, old);
 #pragma unroll
@@ -565,7 +591,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                                     for (int j = 0; j < 32; ++j)
                                         if (j < cols)
-                                            p[j] = (g.add ? p[j] : 0.f) + __uint_as_float(v[j]);
+                                            p[j] = (add ? p[j] : 0.f) + __uint_as_float(v[j]);
                                 }
                             }
                         }
@@ -641,17 +667,18 @@ int tile_n(int cols, int unit) {
     return std::min(kCeTileN, (int)(((long long)cols + unit - 1) / unit * unit));
 }
 
-template <int PRODUCT, int CAP>
+template <int PRODUCT, bool CAP, bool F32>
 cudaError_t launch(const CeGemm &g, cudaStream_t st) {
     constexpr bool kAMn = PRODUCT == kCeGradW, kBMn = PRODUCT >= kCeGradX;
-    const int nt = kBMn ? tile_n(g.D, 128) : tile_n(g.nv, 32);
+    // float32 scores keep a tile's sums in registers: 64 a thread
+    const int nt = kBMn ? tile_n(g.D, 128) : std::min(tile_n(g.nv, 32), F32 ? 128 : kCeTileN);
     CUtensorMap a, b;
     const CeMat &ma = PRODUCT >= kCeGradX ? g.P : g.X;
     const CeMat &mb = PRODUCT == kCeGradW ? g.X : g.W;
     if (!make_map(&a, ma, g.planes, g.bf16, kAMn ? 64 : 128) ||
         !make_map(&b, mb, g.planes, g.bf16, kBMn ? 64 : nt / 2))
         return cudaErrorInvalidValue;
-    auto kernel = ce_gemm_kernel<PRODUCT, CAP>;
+    auto kernel = ce_gemm_kernel<PRODUCT, CAP, F32>;
     const cudaError_t err =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (err != cudaSuccess) return err;
@@ -696,18 +723,26 @@ int ce_error_flag(bool clear) {
 }
 
 cudaError_t launch_ce_gemm(const CeGemm &g, cudaStream_t st) {
-    const int cap = g.opt.cap > 0.f ? (g.planes == 3 ? 1 : 2) : 0;
+    const bool cap = g.opt.cap > 0.f, f32 = g.planes == 3;
     switch (g.product) {
         case kCeScores:
-            return cap == 0   ? launch<kCeScores, 0>(g, st)
-                   : cap == 1 ? launch<kCeScores, 1>(g, st)
-                              : launch<kCeScores, 2>(g, st);
+            if (f32)
+                return cap ? launch<kCeScores, true, true>(g, st)
+                           : launch<kCeScores, false, true>(g, st);
+            return cap ? launch<kCeScores, true, false>(g, st)
+                       : launch<kCeScores, false, false>(g, st);
         case kCeProbs:
-            return cap == 0   ? launch<kCeProbs, 0>(g, st)
-                   : cap == 1 ? launch<kCeProbs, 1>(g, st)
-                              : launch<kCeProbs, 2>(g, st);
-        case kCeGradX: return launch<kCeGradX, 0>(g, st);
-        default: return launch<kCeGradW, 0>(g, st);
+            if (f32)
+                return cap ? launch<kCeProbs, true, true>(g, st)
+                           : launch<kCeProbs, false, true>(g, st);
+            return cap ? launch<kCeProbs, true, false>(g, st)
+                       : launch<kCeProbs, false, false>(g, st);
+        case kCeGradX:
+            return f32 ? launch<kCeGradX, false, true>(g, st)
+                       : launch<kCeGradX, false, false>(g, st);
+        default:
+            return f32 ? launch<kCeGradW, false, true>(g, st)
+                       : launch<kCeGradW, false, false>(g, st);
     }
 }
 

@@ -68,14 +68,13 @@ struct CeGemm {
     float p_scale;
     const float *grow;  // upstream gradient by original row, or null
     const float *gmax;  // or null
-    // kCeGradX, kCeGradW: acc[split][m][D] (+)= product, or, with dst set,
-    // dst[row of m][D] = scale * product in the inputs' type
+    // kCeGradX, kCeGradW: acc[split][m][D] (+)= product, or, with dst set (one
+    // plane), dst[row of m][D] = scale * product in the inputs' type
     float *acc;
     long long acc_split;  // elements between splits
     int splits;
     bool add;
     void *dst;
-    int dst_type;
     CeUpstream up;
 };
 

@@ -385,8 +385,8 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     const long long tn = (D + kCeTileN - 1) / kCeTileN;
     p.split_x = splits_for(p.piece_rows / kCeTileM * tn, p.piece_classes);
     p.split_w = splits_for(up(p.piece_classes, kCeTileM) / kCeTileM * tn, p.piece_rows);
-    p.direct_x = one_class_piece && p.split_x == 1;
-    p.direct_w = p.one_row_piece && p.split_w == 1;
+    p.direct_x = p.planes == 1 && one_class_piece && p.split_x == 1;
+    p.direct_w = p.planes == 1 && p.one_row_piece && p.split_w == 1;
     p.dx = take(p.direct_x ? 0 : sizeof(float) * (size_t)p.split_x * p.piece_rows * D);
     p.dw = take(p.direct_w ? 0
                            : sizeof(float) * (size_t)p.split_w *
@@ -660,7 +660,6 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
     g.p_scale = p_scale_of(type, o);
     g.grow = none ? grad_loss : nullptr;
     g.gmax = gmax;
-    g.dst_type = type;
     g.up = {grad_loss, s.count, gmax, 1.f / g.p_scale, o.reduction};
     float *dx = reinterpret_cast<float *>(ws + p.dx);
     float *dw = reinterpret_cast<float *>(ws + p.dw);
