@@ -1170,7 +1170,7 @@ int gsv_linear_ce_forward(int64_t rows, int32_t classes, int32_t channels, int32
                           size_t ws_bytes, void *stream) {
     const char *fn = "gsv_linear_ce_forward";
     if (const int st = check_ce(fn, rows, classes, channels, dtype, options)) return st;
-    GSV_REQUIRE(features && weight && labels && loss && state, GSV_ERR_INVALID_ARGUMENT,
+    GSV_REQUIRE(features && weight && labels && loss, GSV_ERR_INVALID_ARGUMENT,
                 "%s: null pointer", fn);
     const size_t need =
         gsv_linear_ce_workspace_bytes(rows, classes, channels, dtype, options, 0);

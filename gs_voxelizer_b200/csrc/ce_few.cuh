@@ -1,0 +1,23 @@
+// Linear class loss of a few rows (linear_ce_few.cu).
+#pragma once
+
+#include "ce.cuh"
+
+namespace gsv {
+
+constexpr int kFewRows = 4;  // rows at most
+
+struct FewArgs {
+    int N, V, D;
+    const void *features, *weight;
+    const long long *labels;
+    CeOpt opt;
+    float2 *lse;
+    float *count;
+};
+
+size_t few_workspace_bytes(int N, int V);
+cudaError_t launch_few_forward(const FewArgs &a, int type, float *loss, void *workspace,
+                               cudaStream_t st);
+
+}  // namespace gsv

@@ -16,6 +16,7 @@
 // two (see p_scale_of) so that small probabilities stay normal numbers.
 // float32 inputs keep three bf16 planes of every operand, which hold all 24
 // bits.
+#include "ce_few.cuh"
 #include "ce_gemm.cuh"
 #include "ce_narrow.cuh"
 
@@ -558,19 +559,46 @@ cudaError_t narrow_backward(const NarrowArgs &a, const float *grad_loss, void *g
 
 }  // namespace
 
+namespace {
+
+// Which forward serves N rows of D channels.
+enum Path { kNarrow, kFew, kTiles };
+Path path_of(long long N, int D) {
+    return D <= kNarrowD ? kNarrow : N <= kFewRows ? kFew : kTiles;
+}
+
+// Rows that the tiles read in place when no gradient is to follow: no more
+// than one tile, which packing could not make fewer, of 16 bits and aligned
+// for TMA.
+bool in_place(long long N, int D, int type, const void *features) {
+    return N <= kCeTileM && type != kCeF32 && D % 8 == 0 &&
+           (reinterpret_cast<uintptr_t>(features) & 15) == 0;
+}
+
+}  // namespace
+
 size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
                                  const CeOpt &o) {
-    if (D <= kNarrowD) return narrow_plan(N, V, D, backward, o).bytes;
-    return make_plan(N, V, D, type, nullptr, backward, o).bytes;
+    // a forward without a state keeps its statistics (and, of tiles, the
+    // packed rows' index) here
+    const size_t own = backward ? 0 : align256(linear_ce_state_bytes(N));
+    switch (backward && D > kNarrowD ? kTiles : path_of(N, D)) {
+        case kNarrow: return own + narrow_plan(N, V, D, backward, o).bytes;
+        case kFew: return own + few_workspace_bytes((int)N, V);
+        default: return own + make_plan(N, V, D, type, nullptr, backward, o).bytes;
+    }
 }
 
 cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
                                      const void *features, const void *weight,
                                      const long long *labels, const CeOpt &o, float *loss,
                                      void *state, void *workspace, cudaStream_t st) {
-    const State s = state_of(state, N);
+    const bool forward_only = state == nullptr;
     unsigned char *ws = static_cast<unsigned char *>(workspace);
-    if (D <= kNarrowD) {
+    const State s = state_of(forward_only ? ws : state, N);
+    ws += align256(linear_ce_state_bytes(N));
+    const Path path = path_of(N, D);
+    if (path == kNarrow) {
         const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
         switch (type) {
             case kCeF32: return narrow_forward<float>(a, loss, ws, st);
@@ -579,18 +607,27 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         }
     }
     const Plan p = make_plan(N, V, D, type, weight, false, o);
-    const int nb = (int)((p.Np + kIdxNT - 1) / kIdxNT);
-    if (o.reduction == kCeNone)
-        GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
-    if (nb > 1) {
-        count_labels_kernel<<<nb, kIdxNT, 0, st>>>(N, labels, o.ignore, s.counts);
+    const bool direct = forward_only && in_place(N, D, type, features);
+    if (!direct && (path == kTiles || !forward_only)) {
+        const int nb = (int)((p.Np + kIdxNT - 1) / kIdxNT);
+        if (nb > 1) {
+            count_labels_kernel<<<nb, kIdxNT, 0, st>>>(N, labels, o.ignore, s.counts);
+            count_launches(1);
+        }
+        index_kernel<<<nb, kIdxNT, 0, st>>>(N, p.Np, V, labels, o.ignore, s.counts, nb, s.total,
+                                            s.idx, s.lab);
         count_launches(1);
+        GSV_CE_TRY(cudaGetLastError());
     }
-    index_kernel<<<nb, kIdxNT, 0, st>>>(N, p.Np, V, labels, o.ignore, s.counts, nb, s.total,
-                                        s.idx, s.lab);
-    count_launches(1);
-    GSV_CE_TRY(cudaGetLastError());
-    GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
+    if (path == kFew) {
+        const FewArgs a{(int)N, V, D, features, weight, labels, o, s.lse, s.count};
+        return launch_few_forward(a, type, loss, ws, st);
+    }
+    if (!direct) {
+        if (o.reduction == kCeNone)
+            GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
+        GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
+    }
     if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, ws + p.wp, st));
     CeGemm g = gemm_of(p, s, weight, ws, o);
     g.product = kCeScores;
@@ -600,12 +637,18 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     g.part = reinterpret_cast<float2 *>(ws + p.part);
     g.psum = o.eps > 0.f ? reinterpret_cast<float *>(ws + p.psum) : nullptr;
     g.zt = reinterpret_cast<float *>(ws + p.zt);
+    if (direct) {
+        g.X = {features, N, D, D, 0};
+        g.rows = N;
+        g.count = g.lab = g.idx = nullptr;
+        g.labels = labels;
+    }
     GSV_CE_TRY(launch_ce_gemm(g, st));
     const int mb = (int)((N + kMergeRows - 1) / kMergeRows);
     float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
     merge_kernel<<<mb, kMergeRows * kMergeSlices, 0, st>>>(
-        p.Np, 2 * p.runs, V, g.part, g.psum, g.zt, s.total, s.idx, s.lab, labels, o, loss, s.lse,
-        s.count, sums);
+        g.rows, 2 * p.runs, V, g.part, g.psum, g.zt, g.count, g.idx, g.lab, labels, o, loss,
+        s.lse, s.count, sums);
     count_launches(1);
     GSV_CE_TRY(cudaGetLastError());
     if (mb > 1) GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));

@@ -331,26 +331,40 @@ def _ce_grad_loss(grad_loss):
     return grad_loss.to(torch.float32).contiguous()
 
 
+def _ce_call(fn, dev, *args):
+    """fn(*args, stream) on the current stream of dev."""
+    if torch.cuda.current_device() == dev.index:
+        check(fn(*args, _C._stream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _C._stream(dev)))
+
+
+def _softmax_ce(scores, labels, opt):
+    """(loss, stats): per row (maximum, log2 of the sum), then the number of
+    labelled rows, then the call's workspace."""
+    dev, V, rows = scores.device, int(scores.shape[-1]), labels.numel()
+    loss = _ce_loss_out(labels, opt, dev)
+    if rows == 0:
+        return loss.zero_(), None
+    nbytes = lib.gsv_softmax_ce_workspace_bytes(rows, V)
+    stats = torch.empty((8 * rows + 8 + nbytes,), dtype=torch.uint8, device=dev)
+    p = stats.data_ptr()
+    _ce_call(lib.gsv_softmax_ce_forward, dev, rows, V, _CE_DTYPES[scores.dtype],
+             scores.data_ptr(), labels.data_ptr(), opt, loss.data_ptr(), p,
+             p + 8 * rows, p + 8 * rows + 8, nbytes)
+    return loss, stats
+
+
 class _SoftmaxCe(Function):
     @staticmethod
     def forward(ctx, scores, labels, opt):
-        dev, V = scores.device, int(scores.shape[-1])
-        rows = labels.numel()
-        loss = _ce_loss_out(labels, opt, dev)
         ctx.opt = opt
-        if rows == 0:
+        loss, stats = _softmax_ce(scores, labels, opt)
+        if stats is None:
             ctx.save_for_backward(scores)
-            return loss.zero_()
-        stats = torch.empty((2 * rows + 1,), dtype=torch.float32, device=dev)
-        nbytes = lib.gsv_softmax_ce_workspace_bytes(rows, V)
-        with torch.cuda.device(dev):
-            ws = _C._workspace(nbytes, dev)
-            check(lib.gsv_softmax_ce_forward(
-                rows, V, _CE_DTYPES[scores.dtype], scores.data_ptr(),
-                labels.data_ptr(), opt, loss.data_ptr(), stats.data_ptr(),
-                stats.data_ptr() + 8 * rows, ws.data_ptr(), ws.numel(),
-                _C._stream(dev)))
-        ctx.save_for_backward(scores, labels, stats)
+        else:
+            ctx.save_for_backward(scores, labels, stats)
         return loss
 
     @staticmethod
@@ -362,12 +376,10 @@ class _SoftmaxCe(Function):
         dev, rows, V = scores.device, labels.numel(), int(scores.shape[-1])
         grad_loss = _ce_grad_loss(grad_loss)
         g = torch.empty_like(scores)
-        with torch.cuda.device(dev):
-            check(lib.gsv_softmax_ce_backward(
-                rows, V, _CE_DTYPES[scores.dtype], scores.data_ptr(),
-                labels.data_ptr(), ctx.opt, stats.data_ptr(),
-                stats.data_ptr() + 8 * rows, grad_loss.data_ptr(),
-                g.data_ptr(), _C._stream(dev)))
+        p = stats.data_ptr()
+        _ce_call(lib.gsv_softmax_ce_backward, dev, rows, V,
+                 _CE_DTYPES[scores.dtype], scores.data_ptr(), labels.data_ptr(),
+                 ctx.opt, p, p + 8 * rows, grad_loss.data_ptr(), g.data_ptr())
         return g, None, None
 
 
@@ -403,29 +415,39 @@ def softmax_cross_entropy(
                            label_smoothing, softcap, z_loss, reduction)
     if scores.shape[-1] < 1:
         raise ValueError("scores must have at least one class")
-    return _SoftmaxCe.apply(scores.contiguous(), labels, opt)
+    scores = scores.contiguous()
+    if not (scores.requires_grad and torch.is_grad_enabled()):
+        return _softmax_ce(scores, labels, opt)[0]
+    return _SoftmaxCe.apply(scores, labels, opt)
+
+
+def _linear_ce(features, weight, labels, opt, with_state):
+    """(loss, state for the backward or None)."""
+    dev, rows, (V, D) = features.device, labels.numel(), weight.shape
+    loss = _ce_loss_out(labels, opt, dev)
+    if rows == 0:
+        return loss.zero_(), None
+    dtype = _CE_DTYPES[features.dtype]
+    state = None
+    if with_state:
+        state = _C._workspace(lib.gsv_linear_ce_state_bytes(rows), dev)
+    ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
+        rows, V, D, dtype, opt, 0), dev)
+    _ce_call(lib.gsv_linear_ce_forward, dev, rows, V, D, dtype,
+             features.data_ptr(), weight.data_ptr(), labels.data_ptr(), opt,
+             loss.data_ptr(), _C._ptr(state), ws.data_ptr(), ws.numel())
+    return loss, state
 
 
 class _LinearCe(Function):
     @staticmethod
     def forward(ctx, features, weight, labels, opt):
-        dev = features.device
-        rows, (V, D) = labels.numel(), weight.shape
-        loss = _ce_loss_out(labels, opt, dev)
         ctx.opt = opt
-        if rows == 0:
+        loss, state = _linear_ce(features, weight, labels, opt, True)
+        if state is None:
             ctx.save_for_backward(features, weight)
-            return loss.zero_()
-        dtype = _CE_DTYPES[features.dtype]
-        with torch.cuda.device(dev):
-            state = _C._workspace(lib.gsv_linear_ce_state_bytes(rows), dev)
-            ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
-                rows, V, D, dtype, opt, 0), dev)
-            check(lib.gsv_linear_ce_forward(
-                rows, V, D, dtype, features.data_ptr(), weight.data_ptr(),
-                labels.data_ptr(), opt, loss.data_ptr(), state.data_ptr(),
-                ws.data_ptr(), ws.numel(), _C._stream(dev)))
-        ctx.save_for_backward(features, weight, labels, state)
+        else:
+            ctx.save_for_backward(features, weight, labels, state)
         return loss
 
     @staticmethod
@@ -442,14 +464,12 @@ class _LinearCe(Function):
         grad_loss = _ce_grad_loss(grad_loss)
         gx = torch.empty_like(features) if need_x else None
         gw = torch.empty_like(weight) if need_w else None
-        with torch.cuda.device(dev):
-            ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
-                rows, V, D, dtype, ctx.opt, 1), dev)
-            check(lib.gsv_linear_ce_backward(
-                rows, V, D, dtype, features.data_ptr(), weight.data_ptr(),
-                labels.data_ptr(), ctx.opt, state.data_ptr(),
-                grad_loss.data_ptr(), _C._ptr(gx), _C._ptr(gw), ws.data_ptr(),
-                ws.numel(), _C._stream(dev)))
+        ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
+            rows, V, D, dtype, ctx.opt, 1), dev)
+        _ce_call(lib.gsv_linear_ce_backward, dev, rows, V, D, dtype,
+                 features.data_ptr(), weight.data_ptr(), labels.data_ptr(),
+                 ctx.opt, state.data_ptr(), grad_loss.data_ptr(), _C._ptr(gx),
+                 _C._ptr(gw), ws.data_ptr(), ws.numel())
         return gx, gw, None, None
 
 
@@ -491,5 +511,8 @@ def linear_cross_entropy(
                          f"features {tuple(features.shape)}")
     if weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError("weight must have at least one class and one channel")
-    return _LinearCe.apply(features.contiguous(), weight.contiguous(), labels,
-                           opt)
+    features, weight = features.contiguous(), weight.contiguous()
+    if not ((features.requires_grad or weight.requires_grad)
+            and torch.is_grad_enabled()):
+        return _linear_ce(features, weight, labels, opt, False)[0]
+    return _LinearCe.apply(features, weight, labels, opt)

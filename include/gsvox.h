@@ -523,6 +523,7 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
  * The forward leaves what the backward needs in `lse` / `count` (device
  * float32 [rows][2], 8-byte aligned, and [1]) or in `state` (gsv_linear_ce_state_bytes, 16-byte
  * aligned); the backward is called with the same sizes, inputs and options.
+ * A null state: no backward follows.
  * Workspaces are scratch of one call, 256-byte aligned. A null gradient output
  * of gsv_linear_ce_backward is not computed.
  */

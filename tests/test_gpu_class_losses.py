@@ -473,3 +473,35 @@ def test_voxelize_then_class_loss(decode):
     for x, y in zip(ga, gb):
         tol = 1e-4 * y.abs() + 1e-4 * y.abs().max()
         assert ((x - y).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 130, 256, 257])
+@pytest.mark.parametrize("V,D", [(1, 24), (7, 33), (5003, 64), (20021, 136)])
+def test_loss_without_gradient(n, V, D, dtype):
+    """Scoring: the forward alone, for single rows up to more than a tile."""
+    for i, opt in enumerate([dict(reduction="none"), dict(),
+                             dict(reduction="sum", smoothing=0.1, softcap=9.0, z_loss=1e-3)]):
+        data, labels = make(n, V, D, dtype, n + V + i, 0.3 if i else 0.0)
+        if i == 2:
+            labels[0] = -100
+        loss, _ = call(data, labels, opt)
+        assert not loss.requires_grad
+        check(data, labels, opt, None, loss, [])
+        with torch.no_grad():
+            leaves = [t.clone().requires_grad_(True) for t in data]
+            from gs_voxelizer_b200.losses import linear_cross_entropy
+            assert not linear_cross_entropy(*leaves, labels).requires_grad
+
+
+def test_loss_without_gradient_unaligned():
+    from gs_voxelizer_b200.losses import linear_cross_entropy
+    for n in (2, 100):
+        data, labels = make(n, 300, 64, BF16, 40)
+        flat = [torch.empty(t.numel() + 1, dtype=BF16, device="cuda") for t in data]
+        views = []
+        for f, t in zip(flat, data):
+            f[1:] = t.reshape(-1)
+            views.append(f[1:].view(t.shape))
+        loss = linear_cross_entropy(*views, labels)
+        check(data, labels, {}, None, loss, [])
