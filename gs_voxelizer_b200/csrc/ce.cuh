@@ -74,9 +74,12 @@ struct CeAcc {
     __device__ __forceinline__ static float base(float m) {
         return m == ce_neg_inf() ? 0.f : m;
     }
+    // LOG2: the scores are exponents of two already
+    template <bool LOG2 = false>
     __device__ __forceinline__ void merge(float om, float os, float osz) {
+        constexpr float k = LOG2 ? 1.f : kLog2e;
         const float nm = fmaxf(m, om), e = base(nm);
-        s = s * ex2((m - e) * kLog2e) + os * ex2((om - e) * kLog2e);
+        s = s * ex2((m - e) * k) + os * ex2((om - e) * k);
         m = nm;
         sz += osz;
     }

@@ -150,7 +150,9 @@ pack_kernel(long long rows, int D, long long ld, long long plane, const T *__res
 constexpr int kMergeRows = 32, kMergeSlices = 8;
 
 // One row's (maximum, sum) pairs of all class runs -> lse and loss. Eight
-// slices of the pairs run side by side for 32 rows.
+// slices of the pairs run side by side for 32 rows. LOG2: the maxima are
+// exponents of two, and stay so in lse.
+template <bool LOG2>
 __global__ void __launch_bounds__(kMergeRows *kMergeSlices)
 merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
              const float *__restrict__ psum, const float *__restrict__ zt,
@@ -168,7 +170,7 @@ merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
     if (live)
         for (int t = slice; t < tiles; t += kMergeSlices) {
             const float2 p = part[t * rows + r];
-            a.merge(p.x, p.y, psum ? psum[t * rows + r] : 0.f);
+            a.merge<LOG2>(p.x, p.y, psum ? psum[t * rows + r] : 0.f);
         }
     sm[slice][lane] = a.m;
     ss[slice][lane] = a.s;
@@ -177,11 +179,12 @@ merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
     if (slice) return;
     float l = 0.f, c = 0.f;
     if (live) {
-        for (int s = 1; s < kMergeSlices; ++s) a.merge(sm[s][lane], ss[s][lane], sz[s][lane]);
+        for (int s = 1; s < kMergeSlices; ++s) a.merge<LOG2>(sm[s][lane], ss[s][lane], sz[s][lane]);
         const int y = lab ? lab[r] : ce_label(labels[r], o.ignore, V);
         float2 lse = a.lse();
         if (y >= 0)
-            l = ce_row_loss(lse, zt[r], a.sz, V, o);
+            l = ce_row_loss(make_float2(LOG2 ? lse.x * kCeLn2 : lse.x, lse.y), zt[r], a.sz, V,
+                            o);
         else if (y == kCeInvalid)
             l = lse.x = ce_nan();
         c = y == kCeIgnored ? 0.f : 1.f;
@@ -520,7 +523,8 @@ cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
     long long blocks = narrow_fwd_blocks(a.N);
     if (p.splits > 1) {
         blocks = (a.N + kMergeRows - 1) / kMergeRows;
-        merge_kernel<<<(unsigned)blocks, kMergeRows * kMergeSlices, 0, st>>>(
+        const auto merge = a.opt.cap > 0.f ? merge_kernel<false> : merge_kernel<true>;
+        merge<<<(unsigned)blocks, kMergeRows * kMergeSlices, 0, st>>>(
             a.N, p.splits, a.V, part, psum, zt, nullptr, nullptr, nullptr, a.labels, a.opt,
             loss, a.lse, a.count, sums);
         count_launches(1);
@@ -646,7 +650,7 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     GSV_CE_TRY(launch_ce_gemm(g, st));
     const int mb = (int)((N + kMergeRows - 1) / kMergeRows);
     float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
-    merge_kernel<<<mb, kMergeRows * kMergeSlices, 0, st>>>(
+    merge_kernel<false><<<mb, kMergeRows * kMergeSlices, 0, st>>>(
         g.rows, 2 * p.runs, V, g.part, g.psum, g.zt, g.count, g.idx, g.lab, labels, o, loss,
         s.lse, s.count, sums);
     count_launches(1);
