@@ -323,27 +323,29 @@ def _ce_args(named, labels, ignore_index, label_smoothing, softcap, z_loss,
 
 
 def _ce_loss_out(labels, opt, dev):
-    shape = labels.shape if opt.reduction == 0 else ()
-    return torch.empty(shape, dtype=torch.float32, device=dev)
-
-
-def _ce_grad_loss(grad_loss):
-    return grad_loss.to(torch.float32).contiguous()
+    return torch.empty(labels.shape if opt.reduction == 0 else (),
+                       dtype=torch.float32, device=dev)
 
 
 def _ce_call(fn, dev, *args):
-    """fn(*args, stream) on the current stream of dev."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, _C._stream(dev)))
+    """fn(*args, stream) on the current stream of dev. These losses may be of
+    a few rows, where a call's own microseconds count: the stream is asked for
+    by number and the device is set only where it is not the current one."""
+    i = dev.index
+    stream = torch._C._cuda_getCurrentRawStream(i)
+    if torch.cuda.current_device() == i:
+        status = fn(*args, stream)
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, _C._stream(dev)))
+        with torch.cuda.device(i):
+            status = fn(*args, stream)
+    if status:
+        check(status)
 
 
 def _softmax_ce(scores, labels, opt):
     """(loss, stats): per row (maximum, log2 of the sum), then the number of
     labelled rows, then the call's workspace."""
-    dev, V, rows = scores.device, int(scores.shape[-1]), labels.numel()
+    dev, V, rows = scores.device, scores.size(-1), labels.numel()
     loss = _ce_loss_out(labels, opt, dev)
     if rows == 0:
         return loss.zero_(), None
@@ -370,11 +372,12 @@ class _SoftmaxCe(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
-        if len(ctx.saved_tensors) == 1:
-            return torch.zeros_like(ctx.saved_tensors[0]), None, None
-        scores, labels, stats = ctx.saved_tensors
-        dev, rows, V = scores.device, labels.numel(), int(scores.shape[-1])
-        grad_loss = _ce_grad_loss(grad_loss)
+        saved = ctx.saved_tensors
+        if len(saved) == 1:
+            return torch.zeros_like(saved[0]), None, None
+        scores, labels, stats = saved
+        dev, rows, V = scores.device, labels.numel(), scores.size(-1)
+        grad_loss = grad_loss.contiguous()  # float32, as the loss is
         g = torch.empty_like(scores)
         p = stats.data_ptr()
         _ce_call(lib.gsv_softmax_ce_backward, dev, rows, V,
@@ -454,14 +457,15 @@ class _LinearCe(Function):
     @once_differentiable
     def backward(ctx, grad_loss):
         need_x, need_w = ctx.needs_input_grad[:2]
-        if len(ctx.saved_tensors) == 2:
+        saved = ctx.saved_tensors
+        if len(saved) == 2:
             return (*(torch.zeros_like(t) if need else None for t, need in
-                      zip(ctx.saved_tensors, (need_x, need_w))), None, None)
-        features, weight, labels, state = ctx.saved_tensors
+                      zip(saved, (need_x, need_w))), None, None)
+        features, weight, labels, state = saved
         dev = features.device
         rows, (V, D) = labels.numel(), weight.shape
         dtype = _CE_DTYPES[features.dtype]
-        grad_loss = _ce_grad_loss(grad_loss)
+        grad_loss = grad_loss.contiguous()  # float32, as the loss is
         gx = torch.empty_like(features) if need_x else None
         gw = torch.empty_like(weight) if need_w else None
         ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
