@@ -32,8 +32,9 @@ constexpr int kStages = 6;
 constexpr int kDepth = 64;                       // K a stage
 constexpr int kABytes = 128 * kDepth * 2;        // per CTA
 constexpr int kStageBytes = 2 * kABytes;         // A and B halves
-constexpr int kSmemBytes = kStages * kStageBytes + 1024;
 constexpr int kEpiWarps = 8;
+// stages, their alignment, and a 32 x 32 turn a warp for the gradients
+constexpr int kSmemBytes = kStages * kStageBytes + 1024 + kEpiWarps * 32 * 33 * 4;
 constexpr int kThreads = (4 + kEpiWarps) * 32;
 constexpr int kCols = 512;
 constexpr int kSpinLimit = 1 << 24;
@@ -422,7 +423,14 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         uint32_t acc_phase = 0;
         bool ok = true;
         float scale = 1.f;
-        if (PRODUCT >= kCeGradX && g.dst) scale = ce_grad_scale(g.up);
+        bool wide = true;  // output rows aligned to 32 bytes
+        float *stage_out = reinterpret_cast<float *>(
+            smem_raw + (smem0 - smem_addr(smem_raw)) + kStages * kStageBytes);
+        if (PRODUCT >= kCeGradX) {
+            wide = g.dst ? g.D % 16 == 0 && (reinterpret_cast<uintptr_t>(g.dst) & 31) == 0
+                         : g.D % 8 == 0;
+            if (g.dst) scale = ce_grad_scale(g.up);
+        }
         for (int u = first; ok && u < w.units; u += step) {
             const Unit t = unit_of<PRODUCT, F32>(g, w, u);
             const long long r = (long long)t.m * kCeTileM + rank * 128 + q * 32 + lane;
@@ -548,52 +556,68 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         }
                     } else {
                         const long long M = PRODUCT == kCeGradW ? g.nv : w.live;
-                        if (r < M && col0 < g.D) {
-                            const int cols = min(32, g.D - col0);
-                            if (!F32 && g.dst) {
-                                long long to = r;
-                                if (PRODUCT == kCeGradX)
-                                    to = g.idx ? g.idx[g.row0 + r] : g.row0 + r;
-                                else
-                                    to += g.v0;
-                                uint32_t out[16];
+                        const int cols = min(32, g.D - col0);
+                        const bool direct = !F32 && g.dst;
+                        const bool add = g.add || chunk > 0;
+                        long long to = r;  // row of the output
+                        if (direct && PRODUCT == kCeGradX && r < M)
+                            to = g.idx ? g.idx[g.row0 + r] : g.row0 + r;
+                        if (direct && PRODUCT == kCeGradW) to += g.v0;
+                        to *= g.D;
+                        float *acc_out = g.acc + t.split * g.acc_split;
+                        uint16_t *dst = static_cast<uint16_t *>(g.dst);
+                        if (wide) {
+                            if (r < M) {
 #pragma unroll
-                                for (int j = 0; j < 16; ++j)
-                                    out[j] = pack2(__uint_as_float(v[2 * j]) * scale,
-                                                   __uint_as_float(v[2 * j + 1]) * scale, g.bf16);
-                                uint16_t *p = static_cast<uint16_t *>(g.dst) + to * g.D + col0;
-                                if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
-                                    store8(p, out);
-                                    store8(p + 16, out + 8);
-                                } else {
+                                for (int j = 0; j < 32; j += 16) {
+                                    if (direct) {
+                                        uint32_t out[8];
 #pragma unroll
-                                    for (int j = 0; j < 32; ++j)
-                                        if (j < cols)
-                                            p[j] = (uint16_t)(out[j / 2] >> (16 * (j & 1)));
-                                }
-                            } else {
-                                const bool add = g.add || chunk > 0;
-                                float *p = g.acc + t.split * g.acc_split + r * g.D + col0;
-                                if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+                                        for (int i = 0; i < 8; ++i)
+                                            out[i] = pack2(
+                                                __uint_as_float(v[j + 2 * i]) * scale,
+                                                __uint_as_float(v[j + 2 * i + 1]) * scale,
+                                                g.bf16);
+                                        if (j < cols) store8(dst + to + col0 + j, out);
+                                        continue;
+                                    }
 #pragma unroll
-                                    for (int j = 0; j < 32; j += 8) {
+                                    for (int q = j; q < j + 16; q += 8) {
+                                        if (q >= cols) continue;
+                                        float *p = acc_out + to + col0 + q;
                                         if (add) {
                                             float old[8];
-                                            fetch8(p + j, old);
+                                            fetch8(p, old);
 #pragma unroll
                                             for (int i = 0; i < 8; ++i)
-                                                v[j + i] = __float_as_uint(
-                                                    __uint_as_float(v[j + i]) + old[i]);
+                                                v[q + i] = __float_as_uint(
+                                                    __uint_as_float(v[q + i]) + old[i]);
                                         }
-                                        store8(p + j, v + j);
+                                        store8(p, v + q);
                                     }
-                                } else {
-#pragma unroll
-                                    for (int j = 0; j < 32; ++j)
-                                        if (j < cols)
-                                            p[j] = (add ? p[j] : 0.f) + __uint_as_float(v[j]);
                                 }
                             }
+                        } else if (cols > 0) {
+                            // rows of no alignment: the warp turns its 32 x 32
+                            // and writes row by row
+                            float *turn = stage_out + (warp - 4) * 32 * 33;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                turn[lane * 33 + j] = __uint_as_float(v[j]) * scale;
+                            __syncwarp();
+                            const long long first_row = r - lane;
+                            const int n_rows = (int)max(0LL, min(32LL, M - first_row));
+                            for (int i = 0; i < n_rows; ++i) {
+                                const long long at = __shfl_sync(0xffffffffu, to, i) + col0 + lane;
+                                const float x = turn[i * 33 + lane];
+                                if (lane < cols) {
+                                    if (direct)
+                                        dst[at] = (uint16_t)pack2(x, 0.f, g.bf16);
+                                    else
+                                        acc_out[at] = (add ? acc_out[at] : 0.f) + x;
+                                }
+                            }
+                            __syncwarp();
                         }
                     }
                 }

@@ -113,73 +113,104 @@ __device__ __forceinline__ void split3(float v, __nv_bfloat16 (&h)[3]) {
     }
 }
 
+// How 256 threads cover rows of `chunks` chunks: cx side by side in a row,
+// 256 / cx rows.
+struct RowShape {
+    int cx;
+    unsigned blocks;
+};
+RowShape row_shape(long long rows, long long chunks) {
+    int cx = 1;
+    while (cx < 256 && cx < chunks) cx *= 2;
+    return {cx, (unsigned)((rows + 256 / cx - 1) / (256 / cx))};
+}
+
 // dst[plane][rows][ld] = src[idx[r]], rows past the count (up to whole tiles)
-// and columns past D zero. One warp a row.
-template <typename T, bool ROWS>
+// and columns past D zero, eight columns a thread. VEC: rows of src are
+// aligned to 16 bytes and D is a multiple of eight.
+template <typename T, bool ROWS, bool VEC>
 __global__ void __launch_bounds__(256)
-pack_kernel(long long rows, int D, long long ld, long long plane, const T *__restrict__ src,
-            const int *__restrict__ idx, const int *__restrict__ total,
-            void *__restrict__ dst) {
-    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+pack_kernel(long long rows, int D, long long ld, long long plane, int cx,
+            const T *__restrict__ src, const int *__restrict__ idx,
+            const int *__restrict__ total, void *__restrict__ dst) {
+    const long long r = (long long)blockIdx.x * (256 / cx) + threadIdx.x / cx;
     if (r >= rows) return;
-    const int lane = threadIdx.x & 31;
     long long from = r;
     if (ROWS) {
         const long long live = *total;
         if (r >= (live + kCeTileM - 1) / kCeTileM * kCeTileM) return;
         from = r < live ? idx[r] : -1;
     }
-    for (long long c = lane; c < ld; c += 32) {
-        T v = ce_from_float<T>(0.f);
-        if (from >= 0 && c < D) v = src[from * D + c];
-        if constexpr (sizeof(T) == 4) {
-            __nv_bfloat16 h[3];
-            split3(v, h);
-            __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(dst) + r * ld + c;
-            o[0] = h[0];
-            o[plane] = h[1];
-            o[2 * plane] = h[2];
+    const T *in = src + from * D;
+    for (long long c = 8 * (threadIdx.x % cx); c < ld; c += 8 * cx) {
+        struct alignas(16) Vec { T t[8]; };
+        Vec v;
+        if (VEC && from >= 0) {
+            v = *reinterpret_cast<const Vec *>(in + c);
         } else {
-            static_cast<T *>(dst)[r * ld + c] = v;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v.t[k] = from >= 0 && c + k < D ? in[c + k] : ce_from_float<T>(0.f);
+        }
+        if constexpr (sizeof(T) == 4) {
+            struct alignas(16) Out { __nv_bfloat16 t[8]; };
+            Out h[3];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                __nv_bfloat16 q[3];
+                split3(v.t[k], q);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) h[p].t[k] = q[p];
+            }
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                *reinterpret_cast<Out *>(static_cast<__nv_bfloat16 *>(dst) + p * plane + r * ld +
+                                         c) = h[p];
+        } else {
+            *reinterpret_cast<Vec *>(static_cast<T *>(dst) + r * ld + c) = v;
         }
     }
 }
 
 // --------------------------------------------------------- merge and loss
 
-constexpr int kMergeRows = 32, kMergeSlices = 8;
+constexpr int kMergeNT = 256;
 
-// One row's (maximum, sum) pairs of all class runs -> lse and loss. Eight
-// slices of the pairs run side by side for 32 rows. LOG2: the maxima are
-// exponents of two, and stay so in lse.
-template <bool LOG2>
-__global__ void __launch_bounds__(kMergeRows *kMergeSlices)
+// One row's (maximum, sum) pairs of all class runs -> lse and loss. SLICES
+// parts of the pairs run side by side for 256 / SLICES rows (a warp's, so
+// that one warp ends each row). LOG2: the maxima are exponents of two, and
+// stay so in lse.
+template <bool LOG2, int SLICES>
+__global__ void __launch_bounds__(kMergeNT)
 merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
              const float *__restrict__ psum, const float *__restrict__ zt,
              const int *__restrict__ total, const int *__restrict__ idx,
              const int *__restrict__ lab, const long long *__restrict__ labels, CeOpt o,
              float *__restrict__ loss, float2 *__restrict__ lse_out,
              float *__restrict__ count, float2 *__restrict__ block_sums) {
-    __shared__ float sm[kMergeSlices][kMergeRows], ss[kMergeSlices][kMergeRows],
-        sz[kMergeSlices][kMergeRows];
-    const int lane = threadIdx.x % kMergeRows, slice = threadIdx.x / kMergeRows;
-    const long long r = (long long)blockIdx.x * kMergeRows + lane;
+    constexpr int kRows = kMergeNT / SLICES;
+    __shared__ float sm[SLICES][kRows], ss[SLICES][kRows], sz[SLICES][kRows];
+    __shared__ float2 sh[kMergeNT / 32];
+    const int lane = threadIdx.x % kRows, slice = threadIdx.x / kRows;
+    const long long r = (long long)blockIdx.x * kRows + lane;
     const bool live = r < rows && (!total || r < *total);
     CeAcc a;
     a.init();
     if (live)
-        for (int t = slice; t < tiles; t += kMergeSlices) {
+        for (int t = slice; t < tiles; t += SLICES) {
             const float2 p = part[t * rows + r];
             a.merge<LOG2>(p.x, p.y, psum ? psum[t * rows + r] : 0.f);
         }
-    sm[slice][lane] = a.m;
-    ss[slice][lane] = a.s;
-    sz[slice][lane] = a.sz;
-    __syncthreads();
-    if (slice) return;
+    if (SLICES > 1) {
+        sm[slice][lane] = a.m;
+        ss[slice][lane] = a.s;
+        sz[slice][lane] = a.sz;
+        __syncthreads();
+    }
     float l = 0.f, c = 0.f;
-    if (live) {
-        for (int s = 1; s < kMergeSlices; ++s) a.merge<LOG2>(sm[s][lane], ss[s][lane], sz[s][lane]);
+    if (live && slice == 0) {
+        for (int s = 1; s < SLICES; ++s)
+            a.merge<LOG2>(sm[s][lane], ss[s][lane], sz[s][lane]);
         const int y = lab ? lab[r] : ce_label(labels[r], o.ignore, V);
         float2 lse = a.lse();
         if (y >= 0)
@@ -192,17 +223,29 @@ merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
         lse_out[dst] = lse;
         if (o.reduction == kCeNone) loss[dst] = l;
     }
-#pragma unroll
-    for (int k = 16; k; k >>= 1) {
-        l += __shfl_xor_sync(0xffffffffu, l, k);
-        c += __shfl_xor_sync(0xffffffffu, c, k);
-    }
-    if (lane == 0) {
+    const float2 t = ce_block_sum<kMergeNT>(l, c, sh);
+    if (threadIdx.x == 0) {
         if (gridDim.x == 1)
-            ce_finish(l, c, o.reduction, loss, count);
+            ce_finish(t.x, t.y, o.reduction, loss, count);
         else
-            block_sums[blockIdx.x] = make_float2(l, c);
+            block_sums[blockIdx.x] = t;
     }
+}
+
+// few pairs a row: a thread a row; many: eight threads
+int merge_rows(int parts) { return parts <= 4 ? kMergeNT : kMergeNT / 8; }
+
+template <bool LOG2>
+void launch_merge(long long rows, long long grid_rows, int parts, int V, const float2 *part,
+                  const float *psum, const float *zt, const int *total, const int *idx,
+                  const int *lab, const long long *labels, const CeOpt &o, float *loss,
+                  float2 *lse, float *count, float2 *sums, cudaStream_t st) {
+    const int per = merge_rows(parts);
+    const unsigned blocks = (unsigned)((grid_rows + per - 1) / per);
+    const auto kernel = per == kMergeNT ? merge_kernel<LOG2, 1> : merge_kernel<LOG2, 8>;
+    kernel<<<blocks, kMergeNT, 0, st>>>(rows, parts, V, part, psum, zt, total, idx, lab, labels,
+                                        o, loss, lse, count, sums);
+    count_launches(1);
 }
 
 // -------------------------------------------------------------- gradients
@@ -222,14 +265,15 @@ max_abs_kernel(const float *__restrict__ g, const int *__restrict__ idx,
         atomicMax(reinterpret_cast<int *>(out), __float_as_int(m));
 }
 
-// dst[idx[r]] = scale * sum over splits of acc[s][r]; one warp a row. The
-// rows are those of a piece: packed rows row0 .. row0 + rows.
-template <typename T, bool ROWS>
+// dst[idx[r]] = scale * sum over splits of acc[s][r], four columns a thread.
+// The rows are those of a piece: packed rows row0 .. row0 + rows. VEC: D is a
+// multiple of four and dst aligned to four elements.
+template <typename T, bool ROWS, bool VEC>
 __global__ void __launch_bounds__(256)
-finish_grad_kernel(long long row0, long long rows, int D, const float *__restrict__ acc,
+finish_grad_kernel(long long row0, long long rows, int D, int cx, const float *__restrict__ acc,
                    long long split, int splits, const int *__restrict__ idx,
                    const int *__restrict__ total, CeUpstream upstream, T *__restrict__ dst) {
-    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const long long r = (long long)blockIdx.x * (256 / cx) + threadIdx.x / cx;
     if (r >= rows) return;
     long long to = r;
     if (ROWS) {
@@ -237,10 +281,31 @@ finish_grad_kernel(long long row0, long long rows, int D, const float *__restric
         to = idx[row0 + r];
     }
     const float k = ce_grad_scale(upstream);
-    for (long long c = threadIdx.x & 31; c < D; c += 32) {
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += acc[s * split + r * D + c];
-        dst[to * D + c] = ce_from_float<T>(v * k);
+    for (long long c = 4 * (threadIdx.x % cx); c < D; c += 4 * cx) {
+        const float *p = acc + r * D + c;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (VEC) {
+#pragma unroll 4
+            for (int s = 0; s < splits; ++s) {
+                const float4 q = *reinterpret_cast<const float4 *>(p + s * split);
+                v[0] += q.x;
+                v[1] += q.y;
+                v[2] += q.z;
+                v[3] += q.w;
+            }
+            struct alignas(4 * sizeof(T)) Out { T t[4]; };
+            Out out;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out.t[i] = ce_from_float<T>(v[i] * k);
+            *reinterpret_cast<Out *>(dst + to * D + c) = out;
+        } else {
+            for (int s = 0; s < splits; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += c + i < D ? p[s * split + i] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < D) dst[to * D + c + i] = ce_from_float<T>(v[i] * k);
+        }
     }
 }
 
@@ -263,19 +328,30 @@ reduce_splits_kernel(long long n, const float *__restrict__ acc, int splits,
     dst[i] = ce_from_float<T>(v);
 }
 
-// rows without a label: zero gradient
-template <typename T>
+// Rows without a label: zero gradient. A warp reads 32 labels and writes the
+// rows among them, `bytes` each.
 __global__ void __launch_bounds__(256)
-zero_ignored_kernel(long long n, int D, const long long *__restrict__ labels,
-                    long long ignore, T *__restrict__ dst) {
-    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (r >= n || labels[r] != ignore) return;
-    for (long long c = threadIdx.x & 31; c < D; c += 32) dst[r * D + c] = ce_from_float<T>(0.f);
+zero_ignored_kernel(long long n, long long bytes, const long long *__restrict__ labels,
+                    long long ignore, unsigned char *__restrict__ dst) {
+    const long long r = blockIdx.x * 256LL + threadIdx.x;
+    const int lane = threadIdx.x & 31;
+    unsigned rows = __ballot_sync(0xffffffffu, r < n && labels[r] == ignore);
+    while (rows) {
+        unsigned char *p = dst + (r - lane + __ffs(rows) - 1) * bytes;
+        rows &= rows - 1;
+        // whole words from the first aligned byte on (rows are of 2-byte
+        // elements at least)
+        const int head = (int)min((long long)(-reinterpret_cast<uintptr_t>(p) & 15), bytes);
+        for (int i = 2 * lane; i < head; i += 64) *reinterpret_cast<uint16_t *>(p + i) = 0;
+        const long long words = (bytes - head) / 16;
+        for (long long i = lane; i < words; i += 32)
+            reinterpret_cast<int4 *>(p + head)[i] = make_int4(0, 0, 0, 0);
+        for (long long i = head + 16 * words + 2 * lane; i < bytes; i += 64)
+            *reinterpret_cast<uint16_t *>(p + i) = 0;
+    }
 }
 
 // ------------------------------------------------------------------- plan
-
-unsigned blocks8(long long rows) { return (unsigned)((rows + 7) / 8); }
 
 struct Plan {
     long long N, Np;      // rows, rows in whole tiles
@@ -357,7 +433,7 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
         at += align256(b);
         return o;
     };
-    p.sums = take(sizeof(float2) * (size_t)((N + kMergeRows - 1) / kMergeRows));
+    p.sums = take(sizeof(float2) * (size_t)(N / 32 + 1));
     p.xp = take((size_t)p.planes * p.Np * p.ld * 2);
     p.wp = take(p.pack_w ? (size_t)p.planes * V * p.ld * 2 : 0);
     if (!backward) {
@@ -402,12 +478,13 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
 template <typename T>
 cudaError_t pack(const Plan &p, bool rows, const void *src, const State &s, void *dst,
                  cudaStream_t st) {
-    if (rows)
-        pack_kernel<T, true><<<blocks8(p.Np), 256, 0, st>>>(
-            p.Np, p.D, p.ld, p.Np * p.ld, static_cast<const T *>(src), s.idx, s.total, dst);
-    else
-        pack_kernel<T, false><<<blocks8(p.V), 256, 0, st>>>(
-            p.V, p.D, p.ld, p.V * p.ld, static_cast<const T *>(src), nullptr, nullptr, dst);
+    const bool vec = p.D % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+    const long long n = rows ? p.Np : p.V;
+    const RowShape g = row_shape(n, p.ld / 8);
+    const T *in = static_cast<const T *>(src);
+    const auto kernel = rows ? (vec ? pack_kernel<T, true, true> : pack_kernel<T, true, false>)
+                             : (vec ? pack_kernel<T, false, true> : pack_kernel<T, false, false>);
+    kernel<<<g.blocks, 256, 0, st>>>(n, p.D, p.ld, n * p.ld, g.cx, in, s.idx, s.total, dst);
     count_launches(1);
     return cudaGetLastError();
 }
@@ -425,13 +502,14 @@ template <typename T>
 cudaError_t finish_grad(const Plan &p, bool rows, long long row0, long long n,
                         const float *acc, long long split, int splits, const State &s,
                         const CeUpstream &u, void *dst, cudaStream_t st) {
-    if (rows)
-        finish_grad_kernel<T, true><<<blocks8(n), 256, 0, st>>>(
-            row0, n, p.D, acc, split, splits, s.idx, s.total, u, static_cast<T *>(dst));
-    else
-        finish_grad_kernel<T, false><<<blocks8(n), 256, 0, st>>>(
-            0, n, p.D, acc, split, splits, nullptr, nullptr, u,
-            static_cast<T *>(dst) + row0 * p.D);
+    const bool vec = p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & (4 * sizeof(T) - 1)) == 0;
+    const RowShape g = row_shape(n, (p.D + 3) / 4);
+    const auto kernel =
+        rows ? (vec ? finish_grad_kernel<T, true, true> : finish_grad_kernel<T, true, false>)
+             : (vec ? finish_grad_kernel<T, false, true> : finish_grad_kernel<T, false, false>);
+    T *out = static_cast<T *>(dst) + (rows ? 0 : row0 * p.D);
+    kernel<<<g.blocks, 256, 0, st>>>(rows ? row0 : 0, n, p.D, g.cx, acc, split, splits, s.idx,
+                                     s.total, u, out);
     count_launches(1);
     return cudaGetLastError();
 }
@@ -501,8 +579,7 @@ NarrowPlan narrow_plan(long long N, int V, int D, bool backward, const CeOpt &o)
         p.dx = take(parts * D * sizeof(float));
         p.dw = take(sizeof(float) * (size_t)p.dw_splits * V * D);
     } else {
-        p.sums = take(sizeof(float2) * (size_t)std::max(
-                          narrow_fwd_blocks(N), (N + kMergeRows - 1) / kMergeRows));
+        p.sums = take(sizeof(float2) * (size_t)std::max(narrow_fwd_blocks(N), N / 32 + 1));
         p.part = take(parts * sizeof(float2));
         p.psum = take(o.eps > 0.f ? parts * sizeof(float) : 0);
         p.zt = take(parts ? sizeof(float) * (size_t)N : 0);
@@ -522,12 +599,10 @@ cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
     GSV_CE_TRY(launch_narrow_fwd<T>(a, loss, sums, part, psum, zt, st));
     long long blocks = narrow_fwd_blocks(a.N);
     if (p.splits > 1) {
-        blocks = (a.N + kMergeRows - 1) / kMergeRows;
-        const auto merge = a.opt.cap > 0.f ? merge_kernel<false> : merge_kernel<true>;
-        merge<<<(unsigned)blocks, kMergeRows * kMergeSlices, 0, st>>>(
-            a.N, p.splits, a.V, part, psum, zt, nullptr, nullptr, nullptr, a.labels, a.opt,
-            loss, a.lse, a.count, sums);
-        count_launches(1);
+        blocks = (a.N + merge_rows(p.splits) - 1) / merge_rows(p.splits);
+        const auto merge = a.opt.cap > 0.f ? launch_merge<false> : launch_merge<true>;
+        merge(a.N, a.N, p.splits, a.V, part, psum, zt, nullptr, nullptr, nullptr, a.labels,
+              a.opt, loss, a.lse, a.count, sums, st);
         GSV_CE_TRY(cudaGetLastError());
     }
     if (blocks > 1)
@@ -648,12 +723,10 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         g.labels = labels;
     }
     GSV_CE_TRY(launch_ce_gemm(g, st));
-    const int mb = (int)((N + kMergeRows - 1) / kMergeRows);
+    const int per = merge_rows(2 * p.runs), mb = (int)((N + per - 1) / per);
     float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
-    merge_kernel<false><<<mb, kMergeRows * kMergeSlices, 0, st>>>(
-        g.rows, 2 * p.runs, V, g.part, g.psum, g.zt, g.count, g.idx, g.lab, labels, o, loss,
-        s.lse, s.count, sums);
-    count_launches(1);
+    launch_merge<false>(g.rows, N, 2 * p.runs, V, g.part, g.psum, g.zt, g.count, g.idx, g.lab,
+                        labels, o, loss, s.lse, s.count, sums, st);
     GSV_CE_TRY(cudaGetLastError());
     if (mb > 1) GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));
     return cudaSuccess;
@@ -689,15 +762,9 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
         GSV_CE_TRY(cudaGetLastError());
     }
     if (grad_features) {
-        switch (type) {
-            case kCeF32:
-                zero_ignored_kernel<<<blocks8(N), 256, 0, st>>>(
-                    N, D, labels, o.ignore, static_cast<float *>(grad_features));
-                break;
-            default:
-                zero_ignored_kernel<<<blocks8(N), 256, 0, st>>>(
-                    N, D, labels, o.ignore, static_cast<__half *>(grad_features));
-        }
+        zero_ignored_kernel<<<(unsigned)((N + 255) / 256), 256, 0, st>>>(
+            N, (long long)D * (type == kCeF32 ? 4 : 2), labels, o.ignore,
+            static_cast<unsigned char *>(grad_features));
         count_launches(1);
         GSV_CE_TRY(cudaGetLastError());
     }
