@@ -99,7 +99,7 @@ __device__ __forceinline__ float ce_prob(float z, float2 l) {
 __device__ __forceinline__ float ce_row_loss(float2 lse, float zy, float sz, int V,
                                              const CeOpt &o) {
     float l = fmaf(1.f - o.eps, lse.x - zy, lse.y * kCeLn2);
-    if (o.eps > 0.f) l += o.eps * (lse.x - sz / (float)V);
+    if (o.eps > 0.f) l += o.eps * (lse.x - __fdividef(sz, (float)V));
     if (o.zeta > 0.f) l += o.zeta * ce_lse(lse) * ce_lse(lse);
     return l;
 }

@@ -646,11 +646,13 @@ Path path_of(long long N, int D) {
     return D <= kNarrowD ? kNarrow : N <= kFewRows ? kFew : kTiles;
 }
 
-// Rows that the tiles read in place when no gradient is to follow: no more
-// than one tile, which packing could not make fewer, of 16 bits and aligned
-// for TMA.
-bool in_place(long long N, int D, int type, const void *features) {
-    return N <= kCeTileM && type != kCeF32 && D % 8 == 0 &&
+// Rows that the forward's tiles read in place, 16 bits and aligned for TMA:
+// where packing them costs more than the products of unlabelled rows that it
+// saves. Packing moves 4 N D bytes, a share f of unlabelled rows takes
+// 2 f N V D operations: at 5 TB/s and 1.4 PFLOP/s they meet at f V = 570.
+// One tile of rows cannot become fewer.
+bool in_place(long long N, int V, int D, int type, const void *features) {
+    return (N <= kCeTileM || V <= 1024) && type != kCeF32 && D % 8 == 0 &&
            (reinterpret_cast<uintptr_t>(features) & 15) == 0;
 }
 
@@ -686,8 +688,8 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         }
     }
     const Plan p = make_plan(N, V, D, type, weight, false, o);
-    const bool direct = forward_only && in_place(N, D, type, features);
-    if (!direct && (path == kTiles || !forward_only)) {
+    const bool direct = in_place(N, V, D, type, features);
+    if (!forward_only || (path == kTiles && !direct)) {
         const int nb = (int)((p.Np + kIdxNT - 1) / kIdxNT);
         if (nb > 1) {
             count_labels_kernel<<<nb, kIdxNT, 0, st>>>(N, labels, o.ignore, s.counts);

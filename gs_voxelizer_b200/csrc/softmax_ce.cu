@@ -5,7 +5,9 @@
 //  * V <= kStagedV: a block stages the contiguous scores of its rows in
 //    shared memory with asynchronous 16-byte copies - rows of odd lengths
 //    have no alignment of their own - about 32 KB at once, which is what
-//    keeps enough loads in flight, and G lanes share a row;
+//    keeps enough loads in flight. G lanes share a row and hold it in
+//    registers, E scores each. The backward forms the row's maximum and sum
+//    again, which costs less than the 16 bytes a row of keeping them;
 //  * longer rows: one block a row, 16-byte accesses from the first aligned
 //    element on, the running maximum and sum kept per thread and merged.
 #include "ce.cuh"
@@ -54,78 +56,178 @@ __device__ __forceinline__ void unstage(T *dst, const T *src, int n, bool vec) {
     for (int i = done + threadIdx.x; i < n; i += kNT) dst[i] = src[i];
 }
 
-// Elements of a row that a lane of its group takes: lane, lane + G, ... from
-// a start that differs between the groups of a warp, as rows of V = 2^k
-// would otherwise all begin in the same bank.
-template <int G, typename F>
-__device__ __forceinline__ void each_of_row(int V, F f) {
-    const int lane = threadIdx.x % G, n = (V + G - 1) / G;
-    int k = G == 32 ? 0 : ((threadIdx.x & 31) / G) % n;
-    for (int i = 0; i < n; ++i) {
-        const int j = k * G + lane;
-        if (G == 1 || j < V) f(j);
-        if (++k == n) k = 0;
-    }
-}
-
 template <int G>
 __device__ __forceinline__ unsigned group_mask() {
     return G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G);
 }
 
+// A staged row in the registers of its G lanes, at most E scores each; slots
+// past the row hold -inf. WORDS: rows of whole 16-byte words, of which a lane
+// takes every G-th, in an order that starts elsewhere in each group of a warp
+// (rows of V = 2^k would all begin in the same bank). Else a lane takes every
+// G-th score: rows that are no whole words conflict twofold at most, and the
+// addresses are one register and constants. Slots go in fours, skipped
+// together past the row.
+template <typename T, int G, int E, bool CAP, bool WORDS>
+struct RowRegs {
+    static constexpr int kN = WORDS ? Vec16<T>::kN : 1;  // scores a slot word
+    static constexpr int kWords = E / kN;
+    float z[E], t[CAP ? E : 1];
+    int lane, n, rot, limit;
+
+    __device__ __forceinline__ RowRegs(int V) {
+        lane = threadIdx.x % G;
+        n = (V / kN + G - 1) / G;  // words a lane
+        rot = WORDS && G < 32 ? ((threadIdx.x & 31) / G) % n : 0;
+        limit = V / kN - lane;     // word k of the lane exists if k G < limit
+    }
+    // word of slot word k, in units of words; false past the row
+    __device__ __forceinline__ bool at(int k, int &w) const {
+        if (!WORDS) {
+            w = k * G + lane;
+            return k * G < limit;
+        }
+        int s = k + rot;
+        if (s >= n) s -= n;
+        w = s * G + lane;
+        return k < n && s * G < limit;
+    }
+    __device__ __forceinline__ void load(const T *p, float cap) {
+        constexpr int kStep = WORDS ? 1 : 4;
+#pragma unroll
+        for (int k0 = 0; k0 < kWords; k0 += kStep) {
+            if (k0 >= n) {
+#pragma unroll
+                for (int k = k0 * kN; k < (k0 + kStep) * kN; ++k) z[k] = ce_neg_inf();
+                continue;
+            }
+#pragma unroll
+            for (int k = k0; k < k0 + kStep; ++k) {
+                int w;
+                const bool ok = at(k, w);
+                float s[kN];
+#pragma unroll
+                for (int i = 0; i < kN; ++i) s[i] = ce_neg_inf();
+                if (ok) {
+                    if constexpr (WORDS) {
+                        const Vec16<T> v = reinterpret_cast<const Vec16<T> *>(p)[w];
+#pragma unroll
+                        for (int i = 0; i < kN; ++i) s[i] = ce_to_float(v.v[i]);
+                    } else {
+                        s[0] = ce_to_float(p[w]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kN; ++i) {
+                    const int e = k * kN + i;
+                    if (CAP) {
+                        t[CAP ? e : 0] = ce_tanh<sizeof(T) == 2>(s[i], cap);
+                        s[i] = ok ? cap * t[CAP ? e : 0] : ce_neg_inf();
+                    }
+                    z[e] = s[i];
+                }
+            }
+        }
+    }
+    // f(slot, element) -> the element's new value
+    template <typename F>
+    __device__ __forceinline__ void store(T *p, F f) {
+        constexpr int kStep = WORDS ? 1 : 4;
+#pragma unroll
+        for (int k0 = 0; k0 < kWords; k0 += kStep) {
+            if (k0 >= n) break;
+#pragma unroll
+            for (int k = k0; k < k0 + kStep; ++k) {
+                int w;
+                const bool ok = at(k, w);
+                if constexpr (WORDS) {
+                    Vec16<T> v;
+#pragma unroll
+                    for (int i = 0; i < kN; ++i)
+                        v.v[i] = ce_from_float<T>(f(k * kN + i, w * kN + i));
+                    if (ok) reinterpret_cast<Vec16<T> *>(p)[w] = v;
+                } else if (ok) {
+                    p[w] = ce_from_float<T>(f(k, w));
+                }
+            }
+        }
+    }
+    // maximum and sum over the group
+    __device__ __forceinline__ CeAcc reduce() const {
+        const unsigned mask = group_mask<G>();
+        CeAcc a;
+        a.init();
+#pragma unroll
+        for (int k = 0; k < E; ++k) a.m = fmaxf(a.m, z[k]);
+#pragma unroll
+        for (int k = G / 2; k; k >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(mask, a.m, k));
+        const float b = CeAcc::base(a.m);
+#pragma unroll
+        for (int k0 = 0; k0 < E; k0 += 4) {
+            if (k0 >= n * kN) break;
+#pragma unroll
+            for (int k = k0; k < k0 + 4; ++k) a.s += ex2((z[k] - b) * kLog2e);
+        }
+#pragma unroll
+        for (int k = G / 2; k; k >>= 1) a.s += __shfl_xor_sync(mask, a.s, k);
+        return a;
+    }
+    __device__ __forceinline__ float plain_sum() const {
+        const unsigned mask = group_mask<G>();
+        float sz = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+            int w;
+            if (k >= n) break;
+            if (at(k, w)) {
+#pragma unroll
+                for (int i = 0; i < kN; ++i) sz += z[k * kN + i];
+            }
+        }
+#pragma unroll
+        for (int k = G / 2; k; k >>= 1) sz += __shfl_xor_sync(mask, sz, k);
+        return sz;
+    }
+};
+
 // kPass rows at once (one a group of G lanes), `passes` times
-template <typename T, int G, bool CAP>
+template <typename T, int G, int E, bool CAP, bool WORDS>
 __global__ void __launch_bounds__(kNT)
 staged_fwd_kernel(long long rows, int V, int passes, const T *__restrict__ scores,
                   const long long *__restrict__ labels, CeOpt o, bool vec,
-                  float *__restrict__ loss, float2 *__restrict__ lse_out,
-                  float *__restrict__ count, float2 *__restrict__ partials) {
+                  float *__restrict__ loss, float *__restrict__ count,
+                  float2 *__restrict__ partials) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float2 sh[kNT / 32];
     T *tile = reinterpret_cast<T *>(smem_raw);
     constexpr int kPass = kNT / G;
     const long long row0 = (long long)blockIdx.x * kPass * passes;
     const int nr = (int)min((long long)kPass * passes, rows - row0);
-    const int r0 = threadIdx.x / G, lane = threadIdx.x % G;
+    const int r0 = threadIdx.x / G;
     long long y_next = r0 < nr ? labels[row0 + r0] : o.ignore;
     stage(tile, scores + row0 * V, nr * V, vec);
     __syncthreads();
-    const unsigned mask = group_mask<G>();
-    auto score = [&](T v) {
-        const float s = ce_to_float(v);
-        return CAP ? o.cap * ce_tanh<sizeof(T) == 2>(s, o.cap) : s;
-    };
+    RowRegs<T, G, E, CAP, WORDS> row(V);
     float lsum = 0.f, cnt = 0.f;
     for (int r = r0; r < nr; r += kPass) {  // whole groups take the same path
         const T *p = tile + r * V;
         const int y = ce_label(y_next, o.ignore, V);
         if (r + kPass < nr) y_next = labels[row0 + r + kPass];
-        CeAcc a;
-        a.init();
-        each_of_row<G>(V, [&](int j) { a.m = fmaxf(a.m, score(p[j])); });
-#pragma unroll
-        for (int k = G / 2; k; k >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(mask, a.m, k));
-        const float b = CeAcc::base(a.m);
-        each_of_row<G>(V, [&](int j) {
-            const float z = score(p[j]);
-            a.s += ex2((z - b) * kLog2e);
-            a.sz += z;
-        });
-#pragma unroll
-        for (int k = G / 2; k; k >>= 1) {
-            a.s += __shfl_xor_sync(mask, a.s, k);
-            a.sz += __shfl_xor_sync(mask, a.sz, k);
-        }
-        if (lane == 0) {
-            float2 lse = a.lse();
+        row.load(p, o.cap);
+        const CeAcc a = row.reduce();
+        const float sz = o.eps > 0.f ? row.plain_sum() : 0.f;
+        if (row.lane == 0) {
             float l = 0.f;
-            if (y >= 0)
-                l = ce_row_loss(lse, score(p[y]), a.sz, V, o);
-            else if (y == kCeInvalid)
-                l = lse.x = ce_nan();
+            if (y >= 0) {
+                const float s = ce_to_float(p[y]);
+                l = ce_row_loss(make_float2(CeAcc::base(a.m), __log2f(a.s)),
+                                CAP ? o.cap * ce_tanh<sizeof(T) == 2>(s, o.cap) : s, sz,
+                                V, o);
+            } else if (y == kCeInvalid) {
+                l = ce_nan();
+            }
             cnt += y == kCeIgnored ? 0.f : 1.f;
             lsum += l;
-            lse_out[row0 + r] = lse;
             if (o.reduction == kCeNone) loss[row0 + r] = l;
         }
     }
@@ -145,11 +247,8 @@ struct RowGrad {
     float kz, e, hit;
 };
 
-__device__ __forceinline__ RowGrad row_grad(long long row, float2 lse, int V, const float *g,
-                                            const float *count, const CeOpt &o) {
-    const float f = o.reduction == kCeNone ? g[row]
-                    : o.reduction == kCeMean ? g[0] / count[0]
-                                             : g[0];
+// f: the row's upstream gradient
+__device__ __forceinline__ RowGrad row_grad(float2 lse, int V, float f, const CeOpt &o) {
     return {lse, (1.f + 2.f * o.zeta * ce_lse(lse)) * f, o.eps / (float)V * f,
             (1.f - o.eps) * f};
 }
@@ -164,37 +263,40 @@ __device__ __forceinline__ float grad_of(T v, bool is_class, const RowGrad &q, f
     return d;
 }
 
-template <typename T, int G, bool CAP>
+template <typename T, int G, int E, bool CAP, bool WORDS>
 __global__ void __launch_bounds__(kNT)
 staged_bwd_kernel(long long rows, int V, int passes, const T *__restrict__ scores,
                   const long long *__restrict__ labels, CeOpt o, bool vec,
-                  const float2 *__restrict__ lse_in, const float *__restrict__ count,
-                  const float *__restrict__ grad_loss, T *__restrict__ grad) {
+                  const float *__restrict__ count, const float *__restrict__ grad_loss,
+                  T *__restrict__ grad) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     T *tile = reinterpret_cast<T *>(smem_raw);
     constexpr int kPass = kNT / G;
     const long long row0 = (long long)blockIdx.x * kPass * passes;
     const int nr = (int)min((long long)kPass * passes, rows - row0);
     const int r0 = threadIdx.x / G;
-    long long y_next = o.ignore;
-    float2 lse_next = make_float2(0.f, 0.f);
-    if (r0 < nr) {
-        y_next = labels[row0 + r0];
-        lse_next = lse_in[row0 + r0];
-    }
+    long long y_next = r0 < nr ? labels[row0 + r0] : o.ignore;
+    const float common = o.reduction == kCeNone ? 0.f
+                         : o.reduction == kCeMean ? grad_loss[0] / count[0]
+                                                  : grad_loss[0];
     stage(tile, scores + row0 * V, nr * V, vec);
     __syncthreads();
+    RowRegs<T, G, E, CAP, WORDS> row(V);
     for (int r = r0; r < nr; r += kPass) {
         T *p = tile + r * V;
         const int y = ce_label(y_next, o.ignore, V);
-        const RowGrad q = row_grad(row0 + r, lse_next, V, grad_loss, count, o);
-        if (r + kPass < nr) {
-            y_next = labels[row0 + r + kPass];
-            lse_next = lse_in[row0 + r + kPass];
-        }
-        each_of_row<G>(V, [&](int j) {
-            const float d = grad_of<T, CAP>(p[j], j == y, q, o.cap);
-            p[j] = ce_from_float<T>(y == kCeIgnored ? 0.f : d);
+        if (r + kPass < nr) y_next = labels[row0 + r + kPass];
+        row.load(p, o.cap);
+        const CeAcc a = row.reduce();
+        float2 lse = make_float2(CeAcc::base(a.m), __log2f(a.s));
+        if (y == kCeInvalid) lse.x = ce_nan();
+        const RowGrad q = row_grad(
+            lse, V, o.reduction == kCeNone ? grad_loss[row0 + r] : common, o);
+        row.store(p, [&](int k, int j) {
+            float d = fmaf(q.kz, ce_prob(row.z[k], q.lse), -q.e);
+            if (j == y) d -= q.hit;
+            if (CAP) d *= fmaf(-row.t[CAP ? k : 0], row.t[CAP ? k : 0], 1.f);
+            return y == kCeIgnored ? 0.f : d;
         });
     }
     __syncthreads();
@@ -286,7 +388,10 @@ row_bwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
     const int head = same_head ? head_of(p, V) : V;
     const int nv = (V - head) / kN;
     const int y = ce_label(labels[row], o.ignore, V);
-    const RowGrad q = row_grad(row, lse_in[row], V, grad_loss, count, o);
+    const float f = o.reduction == kCeNone ? grad_loss[row]
+                    : o.reduction == kCeMean ? grad_loss[0] / count[0]
+                                             : grad_loss[0];
+    const RowGrad q = row_grad(lse_in[row], V, f, o);
     auto one = [&](int j) {
         const float d = grad_of<T, CAP>(p[j], j == y, q, o.cap);
         out[j] = ce_from_float<T>(y == kCeIgnored ? 0.f : d);
@@ -338,7 +443,9 @@ finish_kernel(const float2 *__restrict__ partials, int n, int reduction,
     }
 }
 
-// lanes a row: at most 32 scores each
+// lanes a row: up to 32 scores each. What a row costs besides its scores (its
+// label, the shuffles, its loss) is paid by every lane, so few lanes are best:
+// 37 classes took 66 us with eight lanes and 40 with two (786k rows).
 int lanes_of(int V) {
     int g = 1;
     while (g < 32 && g * 32 < V) g *= 2;
@@ -369,7 +476,7 @@ struct Args {
     cudaStream_t st;
 };
 
-template <typename T, int G, bool CAP>
+template <typename T, int G, int E, bool CAP, bool WORDS>
 cudaError_t staged(bool fwd, const Args &a) {
     const int passes = passes_of(a.rows, a.V, sizeof(T));
     const long long per = (long long)(kNT / G) * passes, blocks = (a.rows + per - 1) / per;
@@ -377,13 +484,13 @@ cudaError_t staged(bool fwd, const Args &a) {
     const bool vec = ((reinterpret_cast<uintptr_t>(a.scores) |
                        reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
     if (fwd)
-        staged_fwd_kernel<T, G, CAP><<<(unsigned)blocks, kNT, smem, a.st>>>(
+        staged_fwd_kernel<T, G, E, CAP, WORDS><<<(unsigned)blocks, kNT, smem, a.st>>>(
             a.rows, a.V, passes, static_cast<const T *>(a.scores), a.labels, a.o, vec, a.loss,
-            a.lse, a.count, a.partials);
+            a.count, a.partials);
     else
-        staged_bwd_kernel<T, G, CAP><<<(unsigned)blocks, kNT, smem, a.st>>>(
-            a.rows, a.V, passes, static_cast<const T *>(a.scores), a.labels, a.o, vec, a.lse,
-            a.count, a.grad_loss, static_cast<T *>(a.grad));
+        staged_bwd_kernel<T, G, E, CAP, WORDS><<<(unsigned)blocks, kNT, smem, a.st>>>(
+            a.rows, a.V, passes, static_cast<const T *>(a.scores), a.labels, a.o, vec, a.count,
+            a.grad_loss, static_cast<T *>(a.grad));
     count_launches(1);
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess && fwd && blocks > 1)
@@ -391,18 +498,26 @@ cudaError_t staged(bool fwd, const Args &a) {
     return err;
 }
 
+template <typename T, bool CAP, bool WORDS>
+cudaError_t staged_any(bool fwd, const Args &a) {
+    switch (lanes_of(a.V)) {
+        case 1:
+            return a.V <= 8    ? staged<T, 1, 8, CAP, WORDS>(fwd, a)
+                   : a.V <= 16 ? staged<T, 1, 16, CAP, WORDS>(fwd, a)
+                               : staged<T, 1, 32, CAP, WORDS>(fwd, a);
+        case 2: return staged<T, 2, 32, CAP, WORDS>(fwd, a);
+        case 4: return staged<T, 4, 32, CAP, WORDS>(fwd, a);
+        case 8: return staged<T, 8, 32, CAP, WORDS>(fwd, a);
+        case 16: return staged<T, 16, 32, CAP, WORDS>(fwd, a);
+        default: return staged<T, 32, 32, CAP, WORDS>(fwd, a);
+    }
+}
+
 template <typename T, bool CAP>
 cudaError_t run(bool fwd, const Args &a) {
-    if (a.V <= kStagedV) {
-        switch (lanes_of(a.V)) {
-            case 1: return staged<T, 1, CAP>(fwd, a);
-            case 2: return staged<T, 2, CAP>(fwd, a);
-            case 4: return staged<T, 4, CAP>(fwd, a);
-            case 8: return staged<T, 8, CAP>(fwd, a);
-            case 16: return staged<T, 16, CAP>(fwd, a);
-            default: return staged<T, 32, CAP>(fwd, a);
-        }
-    }
+    if (a.V <= kStagedV)
+        return a.V * sizeof(T) % 16 == 0 ? staged_any<T, CAP, true>(fwd, a)
+                                         : staged_any<T, CAP, false>(fwd, a);
     const T *scores = static_cast<const T *>(a.scores);
     if (fwd) {
         row_fwd_kernel<T, CAP><<<(unsigned)a.rows, kNT, 0, a.st>>>(
