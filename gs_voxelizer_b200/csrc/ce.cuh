@@ -35,7 +35,7 @@ constexpr float kCeLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ int ce_label(long long y, long long ignore, int V) {
     if (y == ignore) return kCeIgnored;
-    return (y < 0 || y >= V) ? kCeInvalid : (int)y;
+    return (unsigned long long)y < (unsigned long long)V ? (int)y : kCeInvalid;
 }
 
 __device__ __forceinline__ float ce_nan() { return __int_as_float(0x7fc00000); }

@@ -17,9 +17,9 @@ struct NarrowArgs {
     float *count;  // labelled rows, at least 1
 };
 
-int narrow_class_splits(long long N, int V);
-long long narrow_fwd_blocks(long long N);
-int narrow_dw_splits(long long N, int V);
+int narrow_class_splits(long long N, int V, int D);
+long long narrow_fwd_blocks(long long N, int D);
+int narrow_dw_splits(long long N, int V, int D);
 
 // One class split: lse, per-block sums (several blocks) or the loss itself.
 // Several: part [splits][N], psum, zt, to be merged.

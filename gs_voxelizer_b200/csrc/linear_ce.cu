@@ -566,8 +566,8 @@ struct NarrowPlan {
 
 NarrowPlan narrow_plan(long long N, int V, int D, bool backward, const CeOpt &o) {
     NarrowPlan p{};
-    p.splits = narrow_class_splits(N, V);
-    p.dw_splits = narrow_dw_splits(N, V);
+    p.splits = narrow_class_splits(N, V, D);
+    p.dw_splits = narrow_dw_splits(N, V, D);
     size_t at = 0;
     auto take = [&](size_t b) {
         const size_t a = at;
@@ -579,7 +579,7 @@ NarrowPlan narrow_plan(long long N, int V, int D, bool backward, const CeOpt &o)
         p.dx = take(parts * D * sizeof(float));
         p.dw = take(sizeof(float) * (size_t)p.dw_splits * V * D);
     } else {
-        p.sums = take(sizeof(float2) * (size_t)std::max(narrow_fwd_blocks(N), N / 32 + 1));
+        p.sums = take(sizeof(float2) * (size_t)std::max(narrow_fwd_blocks(N, D), N / 32 + 1));
         p.part = take(parts * sizeof(float2));
         p.psum = take(o.eps > 0.f ? parts * sizeof(float) : 0);
         p.zt = take(parts ? sizeof(float) * (size_t)N : 0);
@@ -597,7 +597,7 @@ cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
     float *psum = a.opt.eps > 0.f ? reinterpret_cast<float *>(ws + p.psum) : nullptr;
     float *zt = reinterpret_cast<float *>(ws + p.zt);
     GSV_CE_TRY(launch_narrow_fwd<T>(a, loss, sums, part, psum, zt, st));
-    long long blocks = narrow_fwd_blocks(a.N);
+    long long blocks = narrow_fwd_blocks(a.N, a.D);
     if (p.splits > 1) {
         blocks = (a.N + merge_rows(p.splits) - 1) / merge_rows(p.splits);
         const auto merge = a.opt.cap > 0.f ? launch_merge<false> : launch_merge<true>;

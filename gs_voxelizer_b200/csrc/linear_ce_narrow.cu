@@ -24,7 +24,8 @@ namespace {
 
 constexpr int kNT = 256;
 constexpr int kPairs = 1;                // pairs of rows a thread
-constexpr int kPerSM = 4;                // blocks an SM
+// blocks an SM, as many as registers hold without spills
+constexpr int per_sm(int dp) { return dp == 4 ? 3 : 2; }
 constexpr int kBlockRows = kNT * 2 * kPairs;
 constexpr int kChunk = 256;              // classes staged at once
 constexpr int kTile = 256;               // rows staged at once (dW)
@@ -101,6 +102,34 @@ __device__ __forceinline__ float2 dot2(const Row2<DP> &a, const Row2<DP> &b) {
     for (int d = 1; d < DP; ++d) s = __ffma2_rn(a.v[d], b.v[d], s);
     return s;
 }
+// What a thread reads of its rows, one tile ahead of their use: the loads of
+// a tile cost as long as its classes otherwise.
+template <int DP, int R>
+struct Ahead {
+    Row<DP> x[R];
+    long long label[R];
+    float2 lse[R];
+};
+
+template <typename T, int DP, bool VEC, int R>
+__device__ __forceinline__ void read_ahead(Ahead<DP, R> &a, long long t0, long long N, int D,
+                                           const T *features, const long long *labels,
+                                           long long ignore, const float2 *lse) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const long long r = t0 + k * kNT + threadIdx.x;
+        a.label[k] = ignore;
+        a.lse[k] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int d = 0; d < DP; ++d) a.x[k].v[d] = 0.f;
+        if (r < N) {
+            a.x[k] = load_row<T, DP, VEC>(features, r, D);
+            a.label[k] = labels[r];
+            if (lse) a.lse[k] = lse[r];
+        }
+    }
+}
+
 struct Span {
     int v0, v1;
 };
@@ -141,7 +170,7 @@ template <bool CAP>
 __device__ __forceinline__ float exp_of(float d) { return ex2(CAP ? d * kLog2e : d); }
 
 template <typename T, int DP, bool CAP, bool VEC>
-__global__ void __launch_bounds__(kNT, kPerSM)
+__global__ void __launch_bounds__(kNT, per_sm(DP))
 narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
                   const T *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
                   float *__restrict__ loss, float2 *__restrict__ lse_out,
@@ -157,27 +186,24 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
     if (smooth && !CAP) table_sum<T, DP, VEC>(wsum, sh_sum, weight, span, D);
     float lsum = 0.f, cnt = 0.f;
     bool staged = false;
-    for (long long t0 = (long long)blockIdx.x * kBlockRows; t0 < N;
-         t0 += (long long)gridDim.x * kBlockRows) {
+    const long long stride = (long long)gridDim.x * kBlockRows;
+    Ahead<DP, 2 * kPairs> next;
+    read_ahead<T, DP, VEC>(next, (long long)blockIdx.x * kBlockRows, N, D, features, labels,
+                           o.ignore, nullptr);
+    for (long long t0 = (long long)blockIdx.x * kBlockRows; t0 < N; t0 += stride) {
         Row2<DP> x[kPairs];
         float2 m[kPairs], s[kPairs], sz[kPairs];
-        long long label[2 * kPairs];
+        int label[2 * kPairs];
 #pragma unroll
         for (int k = 0; k < 2 * kPairs; ++k) {
-            const long long r = t0 + k * kNT + threadIdx.x;
-            Row<DP> q;
+            label[k] = ce_label(next.label[k], o.ignore, V);
 #pragma unroll
-            for (int d = 0; d < DP; ++d) q.v[d] = 0.f;
-            label[k] = o.ignore;
-            if (r < N) {
-                q = load_row<T, DP, VEC>(features, r, D);
-                label[k] = labels[r];
-            }
-#pragma unroll
-            for (int d = 0; d < DP; ++d) (k & 1 ? x[k / 2].v[d].y : x[k / 2].v[d].x) = q.v[d];
+            for (int d = 0; d < DP; ++d)
+                (k & 1 ? x[k / 2].v[d].y : x[k / 2].v[d].x) = next.x[k].v[d];
             m[k / 2] = f2(ce_neg_inf());
             s[k / 2] = sz[k / 2] = f2(0.f);
         }
+        read_ahead<T, DP, VEC>(next, t0 + stride, N, D, features, labels, o.ignore, nullptr);
         for (int v0 = span.v0; v0 < span.v1; v0 += kChunk) {
             const int n = min(kChunk, span.v1 - v0);
             if (!staged) {
@@ -210,13 +236,11 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
                         top.x = fmaxf(top.x, z[k][j].x);
                         top.y = fmaxf(top.y, z[k][j].y);
                     }
-                    const float2 b = make_float2(CeAcc::base(top.x), CeAcc::base(top.y));
-                    if (top.x != m[k].x || top.y != m[k].y) {
-                        s[k].x *= exp_of<CAP>(m[k].x - b.x);
-                        s[k].y *= exp_of<CAP>(m[k].y - b.y);
-                        m[k] = top;
-                    }
-                    const float2 nb = make_float2(-b.x, -b.y);
+                    // (all scores at -inf: not a distribution, NaN like theirs)
+                    s[k].x *= exp_of<CAP>(m[k].x - top.x);
+                    s[k].y *= exp_of<CAP>(m[k].y - top.y);
+                    m[k] = top;
+                    const float2 nb = make_float2(-top.x, -top.y);
                     float2 e = f2(0.f);
 #pragma unroll
                     for (int j = 0; j < kG; ++j) {
@@ -238,7 +262,7 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
         for (int k = 0; k < 2 * kPairs; ++k) {
             const long long r = t0 + k * kNT + threadIdx.x;
             if (r >= N) continue;
-            const int y = ce_label(label[k], o.ignore, V);
+            const int y = label[k];
             Row<DP> q;
 #pragma unroll
             for (int d = 0; d < DP; ++d) q.v[d] = k & 1 ? x[k / 2].v[d].y : x[k / 2].v[d].x;
@@ -295,11 +319,11 @@ __device__ __forceinline__ float common_grad(const CeUpstream &u) {
 }
 
 template <bool CAP>
-__device__ __forceinline__ RowGrad row_grad(long long r, int y, const float2 *lse, CeOpt o,
+__device__ __forceinline__ RowGrad row_grad(long long r, int y, float2 lse, const CeOpt &o,
                                             const float *per_row, float common, float smooth) {
     RowGrad q{make_float2(0.f, 0.f), 0.f, 0.f, 0.f};
     if (y == kCeIgnored) return q;
-    q.lse = lse[r];
+    q.lse = lse;
     const float g = per_row ? per_row[r] : common;
     q.kz = g;
     if (o.zeta > 0.f)
@@ -311,7 +335,7 @@ __device__ __forceinline__ RowGrad row_grad(long long r, int y, const float2 *ls
 }
 
 template <typename T, int DP, bool CAP, bool VEC>
-__global__ void __launch_bounds__(kNT, kPerSM)
+__global__ void __launch_bounds__(kNT, per_sm(DP))
 narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
                  const T *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
                  const float2 *__restrict__ lse, CeUpstream u, T *__restrict__ grad,
@@ -325,8 +349,11 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
     bool staged = false;
     const float common = common_grad(u), ev = o.eps / (float)V;
     const float *per_row = u.reduction == kCeNone ? u.g : nullptr;
-    for (long long t0 = (long long)blockIdx.x * kBlockRows; t0 < N;
-         t0 += (long long)gridDim.x * kBlockRows) {
+    const long long stride = (long long)gridDim.x * kBlockRows;
+    Ahead<DP, 2 * kPairs> next;
+    read_ahead<T, DP, VEC>(next, (long long)blockIdx.x * kBlockRows, N, D, features, labels,
+                           o.ignore, lse);
+    for (long long t0 = (long long)blockIdx.x * kBlockRows; t0 < N; t0 += stride) {
         Row2<DP> x[kPairs], dx[kPairs];
         float2 nm[kPairs], nl[kPairs], kz[kPairs], e[kPairs];
         RowGrad q[2 * kPairs];
@@ -334,17 +361,12 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
 #pragma unroll
         for (int k = 0; k < 2 * kPairs; ++k) {
             const long long r = t0 + k * kNT + threadIdx.x;
-            y[k] = r < N ? ce_label(labels[r], o.ignore, V) : kCeIgnored;
-            q[k] = row_grad<CAP>(r, y[k], lse, o, per_row, common, ev);
-            Row<DP> v;
-#pragma unroll
-            for (int d = 0; d < DP; ++d) v.v[d] = 0.f;
-            // an unlabelled row keeps x = 0: nothing of it is read
-            if (y[k] != kCeIgnored) v = load_row<T, DP, VEC>(features, r, D);
+            y[k] = ce_label(next.label[k], o.ignore, V);
+            q[k] = row_grad<CAP>(r, y[k], next.lse[k], o, per_row, common, ev);
             auto put = [&](float2 &a, float b) { (k & 1 ? a.y : a.x) = b; };
 #pragma unroll
             for (int d = 0; d < DP; ++d) {
-                put(x[k / 2].v[d], v.v[d]);
+                put(x[k / 2].v[d], next.x[k].v[d]);
                 dx[k / 2].v[d] = f2(0.f);
             }
             put(nm[k / 2], -q[k].lse.x);
@@ -352,6 +374,7 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
             put(kz[k / 2], q[k].kz);
             put(e[k / 2], -q[k].e);
         }
+        read_ahead<T, DP, VEC>(next, t0 + stride, N, D, features, labels, o.ignore, lse);
         for (int v0 = span.v0; v0 < span.v1; v0 += kChunk) {
             const int n = min(kChunk, span.v1 - v0);
             if (!staged) {
@@ -433,13 +456,13 @@ struct alignas(16) DwPair {
 // the staged rows; two classes a thread halve the shared-memory reads, which
 // bound it with one.
 template <typename T, int DP, bool CAP, bool VEC>
-__global__ void __launch_bounds__(kNT, kPerSM)
+__global__ void __launch_bounds__(kNT, per_sm(DP))
 narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ features,
                  const T *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
                  const float2 *__restrict__ lse, CeUpstream u, float *__restrict__ acc) {
-    __shared__ DwPair<DP> rows[kTile / 2];
+    // two buffers: a tile is staged while others still read the last one
+    __shared__ DwPair<DP> buffers[2][kTile / 2];
     __shared__ float red[kNT][DP + 1];
-    __shared__ int s_warp[kNT / 32];
     const int slices = kNT / lanes, slice = threadIdx.x / lanes;
     const int j0 = blockIdx.y * 2 * lanes + threadIdx.x % lanes;
     const bool active = slice < slices && j0 < V;
@@ -459,48 +482,35 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
     const bool plain = o.eps == 0.f && o.zeta == 0.f;
     const float common = common_grad(u), ev = o.eps / (float)V;
     const float *per_row = u.reduction == kCeNone ? u.g : nullptr;
-    for (long long t0 = (long long)blockIdx.x * kTile; t0 < N; t0 += (long long)gridDim.x * kTile) {
+    const long long stride = (long long)gridDim.x * kTile;
+    int buffer = 0;
+    Ahead<DP, 1> next;
+    read_ahead<T, DP, VEC>(next, (long long)blockIdx.x * kTile, N, D, features, labels, o.ignore,
+                           lse);
+    for (long long t0 = (long long)blockIdx.x * kTile; t0 < N; t0 += stride) {
         const long long r = t0 + threadIdx.x;
-        __syncthreads();
-        // rows are packed without the unlabelled ones
-        const int y = r < N ? ce_label(labels[r], o.ignore, V) : kCeIgnored;
-        const bool keep = y != kCeIgnored;
-        const unsigned ballot = __ballot_sync(0xffffffffu, keep);
-        if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = __popc(ballot);
-        RowGrad q{};
-        Row<DP> x;
-#pragma unroll
-        for (int d = 0; d < DP; ++d) x.v[d] = 0.f;
-        if (keep) {
-            q = row_grad<CAP>(r, y, lse, o, per_row, common, ev);
-            x = load_row<T, DP, VEC>(features, r, D);
-        }
-        __syncthreads();
-        int at = __popc(ballot & ((1u << (threadIdx.x & 31)) - 1u)), n = 0;
-#pragma unroll
-        for (int k = 0; k < kNT / 32; ++k) {
-            if (k < (int)(threadIdx.x >> 5)) at += s_warp[k];
-            n += s_warp[k];
-        }
-        // an odd row's partner is all zeros: the first thread without a row
-        // of its own writes it (n is odd, so there is one)
-        const bool partner = !keep && (n & 1) && (int)threadIdx.x - at == 0;
-        if (keep || partner) {
-            const int i = keep ? at : n, h = i & 1;
-            DwPair<DP> &p = rows[i / 2];
+        // an unlabelled row is all zeros
+        const int y = ce_label(next.label[0], o.ignore, V);
+        const RowGrad q = row_grad<CAP>(r, y, next.lse[0], o, per_row, common, ev);
+        DwPair<DP> *rows = buffers[buffer];
+        buffer ^= 1;
+        {
+            const int h = threadIdx.x & 1;
+            DwPair<DP> &p = rows[threadIdx.x / 2];
             auto put = [&](float2 &a, float b) { (&a.x)[h] = b; };
 #pragma unroll
-            for (int d = 0; d < DP; ++d) put(p.x.v[d], x.v[d]);
+            for (int d = 0; d < DP; ++d) put(p.x.v[d], y == kCeIgnored ? 0.f : next.x[0].v[d]);
             put(p.nm, -q.lse.x);
             put(p.nl, -q.lse.y);
             put(p.kz, q.kz);
-            (&p.y.x)[h] = keep ? y : kCeIgnored;
+            (&p.y.x)[h] = y;
             put(p.e, -q.e);
             put(p.hit, q.hit);
         }
+        read_ahead<T, DP, VEC>(next, t0 + stride, N, D, features, labels, o.ignore, lse);
         __syncthreads();
         if (!active) continue;
-        for (int i = slice; i < (n + 1) / 2; i += slices) {
+        for (int i = slice; i < kTile / 2; i += slices) {
             const DwPair<DP> &p = rows[i];
             const Row2<DP> xv = p.x;
             const float2 nm = p.nm, nl = p.nl, kz = p.kz;
@@ -552,23 +562,25 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // blocks over the rows, each taking every gridDim.x-th tile of them: a
 // block stages its table once
-long long row_blocks(long long N) {
-    return std::min(ceil_div(N, kBlockRows), (long long)kPerSM * kSMs);
+long long row_blocks(long long N, int D) {
+    return std::min(ceil_div(N, kBlockRows), (long long)per_sm(D <= 4 ? 4 : 8) * kSMs);
 }
-// classes split over blocks until there are four a SM, 64 classes a part at
-// least
-int class_splits(long long N, int V) {
-    return (int)std::max(1LL, std::min({ceil_div(V, 64), (long long)kPerSM * kSMs / row_blocks(N), 1024LL}));
+// classes split over blocks until these fill the device, 64 classes a part
+// at least
+int class_splits(long long N, int V, int D) {
+    return (int)std::max(
+        1LL, std::min({ceil_div(V, 64),
+                       (long long)per_sm(D <= 4 ? 4 : 8) * kSMs / row_blocks(N, D), 1024LL}));
 }
 
 struct DwShape {
     int lanes, chunks, blocks;
 };
-DwShape dw_shape(long long N, int V) {
+DwShape dw_shape(long long N, int V, int D) {
     DwShape s;
     s.lanes = (int)std::min<long long>(ceil_div(V, 2), kNT);
     s.chunks = (int)ceil_div(V, 2 * s.lanes);
-    s.blocks = (int)std::max(1LL, std::min(ceil_div(N, kTile), (long long)kPerSM * kSMs / s.chunks));
+    s.blocks = (int)std::max(1LL, std::min(ceil_div(N, kTile), (long long)per_sm(D <= 4 ? 4 : 8) * kSMs / s.chunks));
     return s;
 }
 
@@ -593,15 +605,15 @@ cudaError_t by_form(const NarrowArgs &a, const void *grad, F f) {
 
 }  // namespace
 
-int narrow_class_splits(long long N, int V) { return class_splits(N, V); }
-long long narrow_fwd_blocks(long long N) { return row_blocks(N); }
-int narrow_dw_splits(long long N, int V) { return dw_shape(N, V).blocks; }
+int narrow_class_splits(long long N, int V, int D) { return class_splits(N, V, D); }
+long long narrow_fwd_blocks(long long N, int D) { return row_blocks(N, D); }
+int narrow_dw_splits(long long N, int V, int D) { return dw_shape(N, V, D).blocks; }
 
 template <typename T>
 cudaError_t launch_narrow_fwd(const NarrowArgs &a, float *loss, float2 *sums, float2 *part,
                               float *psum, float *zt, cudaStream_t st) {
     return by_form<T>(a, nullptr, [&](auto dp, auto cap, auto vec) {
-        const dim3 grid((unsigned)narrow_fwd_blocks(a.N), class_splits(a.N, a.V));
+        const dim3 grid((unsigned)narrow_fwd_blocks(a.N, a.D), class_splits(a.N, a.V, a.D));
         narrow_fwd_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value><<<grid, kNT, 0, st>>>(
             a.N, a.V, a.D, static_cast<const T *>(a.features), static_cast<const T *>(a.weight),
             a.labels, a.opt, loss, a.lse, a.count, sums, part, psum, zt);
@@ -614,7 +626,7 @@ template <typename T>
 cudaError_t launch_narrow_dx(const NarrowArgs &a, const CeUpstream &u, void *grad, float *acc,
                              cudaStream_t st) {
     return by_form<T>(a, grad, [&](auto dp, auto cap, auto vec) {
-        const dim3 grid((unsigned)narrow_fwd_blocks(a.N), class_splits(a.N, a.V));
+        const dim3 grid((unsigned)narrow_fwd_blocks(a.N, a.D), class_splits(a.N, a.V, a.D));
         narrow_dx_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value><<<grid, kNT, 0, st>>>(
             a.N, a.V, a.D, static_cast<const T *>(a.features), static_cast<const T *>(a.weight),
             a.labels, a.opt, a.lse, u, static_cast<T *>(grad), acc);
@@ -627,7 +639,7 @@ template <typename T>
 cudaError_t launch_narrow_dw(const NarrowArgs &a, const CeUpstream &u, float *acc,
                              cudaStream_t st) {
     return by_form<T>(a, nullptr, [&](auto dp, auto cap, auto vec) {
-        const DwShape s = dw_shape(a.N, a.V);
+        const DwShape s = dw_shape(a.N, a.V, a.D);
         narrow_dw_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value>
             <<<dim3(s.blocks, s.chunks), kNT, 0, st>>>(
                 a.N, a.V, a.D, s.lanes, static_cast<const T *>(a.features),
