@@ -248,6 +248,13 @@ __device__ __forceinline__ Unit unit_of(const CeGemm &g, const Work &w, int u) {
     return t;
 }
 
+// What the epilogue needs of a row: its class, logsumexp, upstream gradient.
+struct RowInfo {
+    int y;
+    float2 lse;
+    float g;
+};
+
 // Plane pairs of a float32 product, least first: (2,0) (0,2) (1,1) (1,0)
 // (0,1) (0,0). The pairs left out are below 2^-26 of the whole.
 template <bool F32>
@@ -431,28 +438,38 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                          : g.D % 8 == 0;
             if (g.dst) scale = ce_grad_scale(g.up);
         }
+        // a unit's row, read a unit ahead: units of few classes and channels
+        // take no longer than these loads
+        auto row_of = [&](int u) {
+            RowInfo x{kCeIgnored, make_float2(0.f, 0.f), 1.f};
+            if (PRODUCT > kCeProbs || u >= w.units) return x;
+            const Unit t = unit_of<PRODUCT, F32>(g, w, u);
+            const long long r = (long long)t.m * kCeTileM + rank * 128 + q * 32 + lane;
+            if (r >= w.live) return x;
+            x.y = g.lab ? g.lab[g.row0 + r] : ce_label(g.labels[g.row0 + r], o.ignore, g.V);
+            if (PRODUCT == kCeProbs) {
+                x.lse = g.lse[g.row0 + r];
+                if (g.grow) x.g = g.grow[g.idx[g.row0 + r]];
+            }
+            return x;
+        };
+        float unit_scale = g.p_scale;
+        if (PRODUCT == kCeProbs && g.grow && g.gmax && *g.gmax > 0.f) unit_scale /= *g.gmax;
+        RowInfo next = row_of(first);
         for (int u = first; ok && u < w.units; u += step) {
             const Unit t = unit_of<PRODUCT, F32>(g, w, u);
             const long long r = (long long)t.m * kCeTileM + rank * 128 + q * 32 + lane;
-            // per-row state
-            int y = kCeIgnored;
+            const RowInfo row = next;
+            next = row_of(u + step);
+            const int y = row.y;
+            const float2 lse = row.lse;
             float top = ce_neg_inf(), s = 0.f, sz = 0.f;
-            float2 lse = make_float2(0.f, 0.f);
             float kz = 1.f, e = 0.f, hit = 0.f;
-            if (PRODUCT <= kCeProbs && r < w.live) {
-                y = g.lab ? g.lab[g.row0 + r] : ce_label(g.labels[g.row0 + r], o.ignore, g.V);
-                if (PRODUCT == kCeProbs && y != kCeIgnored) {
-                    const long long src = g.idx ? g.idx[g.row0 + r] : g.row0 + r;
-                    lse = g.lse[src];
-                    float f = g.p_scale;
-                    if (g.grow) {
-                        f *= g.grow[src];
-                        if (g.gmax && *g.gmax > 0.f) f /= *g.gmax;
-                    }
-                    kz = (1.f + 2.f * o.zeta * ce_lse(lse)) * f;
-                    e = o.eps / (float)g.V * f;
-                    hit = (1.f - o.eps) * f;
-                }
+            if (PRODUCT == kCeProbs) {
+                const float f = unit_scale * row.g;
+                kz = (1.f + 2.f * o.zeta * ce_lse(lse)) * f;
+                e = o.eps / (float)g.V * f;
+                hit = (1.f - o.eps) * f;
             }
             float sum[F32 && PRODUCT <= kCeProbs ? 2 : 1][32];
             for (int i = 0; ok && i < t.steps(); ++i) {

@@ -63,7 +63,7 @@ struct CeGemm {
     float *psum;        // [2 * runs][rows] plain sums (label smoothing) or null
     float *zt;          // [rows] score of the row's class
     // kCeProbs: derivative * p_scale * (row's upstream gradient / gmax)
-    const float2 *lse;  // by original row
+    const float2 *lse;  // as X's rows
     void *p_out;        // P's storage (P describes it)
     float p_scale;
     const float *grow;  // upstream gradient by original row, or null

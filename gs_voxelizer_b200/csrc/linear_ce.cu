@@ -179,10 +179,11 @@ constexpr int kMergeNT = 256;
 // One row's (maximum, sum) pairs of all class runs -> lse and loss. SLICES
 // parts of the pairs run side by side for 256 / SLICES rows (a warp's, so
 // that one warp ends each row). LOG2: the maxima are exponents of two, and
-// stay so in lse.
+// stay so in lse. Rows are packed ones where idx is given: lse is kept as
+// they are, loss by original row, and the pairs are found by either (PACKED).
 template <bool LOG2, int SLICES>
 __global__ void __launch_bounds__(kMergeNT)
-merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
+merge_kernel(long long rows, int tiles, int V, bool packed, const float2 *__restrict__ part,
              const float *__restrict__ psum, const float *__restrict__ zt,
              const int *__restrict__ total, const int *__restrict__ idx,
              const int *__restrict__ lab, const long long *__restrict__ labels, CeOpt o,
@@ -196,10 +197,11 @@ merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
     const bool live = r < rows && (!total || r < *total);
     CeAcc a;
     a.init();
+    const long long src = live && idx && !packed ? idx[r] : r;
     if (live)
         for (int t = slice; t < tiles; t += SLICES) {
-            const float2 p = part[t * rows + r];
-            a.merge<LOG2>(p.x, p.y, psum ? psum[t * rows + r] : 0.f);
+            const float2 p = part[t * rows + src];
+            a.merge<LOG2>(p.x, p.y, psum ? psum[t * rows + src] : 0.f);
         }
     if (SLICES > 1) {
         sm[slice][lane] = a.m;
@@ -214,14 +216,13 @@ merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
         const int y = lab ? lab[r] : ce_label(labels[r], o.ignore, V);
         float2 lse = a.lse();
         if (y >= 0)
-            l = ce_row_loss(make_float2(LOG2 ? lse.x * kCeLn2 : lse.x, lse.y), zt[r], a.sz, V,
+            l = ce_row_loss(make_float2(LOG2 ? lse.x * kCeLn2 : lse.x, lse.y), zt[src], a.sz, V,
                             o);
         else if (y == kCeInvalid)
             l = lse.x = ce_nan();
         c = y == kCeIgnored ? 0.f : 1.f;
-        const long long dst = idx ? idx[r] : r;
-        lse_out[dst] = lse;
-        if (o.reduction == kCeNone) loss[dst] = l;
+        lse_out[r] = lse;
+        if (o.reduction == kCeNone) loss[idx ? idx[r] : r] = l;
     }
     const float2 t = ce_block_sum<kMergeNT>(l, c, sh);
     if (threadIdx.x == 0) {
@@ -236,14 +237,15 @@ merge_kernel(long long rows, int tiles, int V, const float2 *__restrict__ part,
 int merge_rows(int parts) { return parts <= 4 ? kMergeNT : kMergeNT / 8; }
 
 template <bool LOG2>
-void launch_merge(long long rows, long long grid_rows, int parts, int V, const float2 *part,
+void launch_merge(long long rows, long long grid_rows, int parts, int V, bool packed,
+                  const float2 *part,
                   const float *psum, const float *zt, const int *total, const int *idx,
                   const int *lab, const long long *labels, const CeOpt &o, float *loss,
                   float2 *lse, float *count, float2 *sums, cudaStream_t st) {
     const int per = merge_rows(parts);
     const unsigned blocks = (unsigned)((grid_rows + per - 1) / per);
     const auto kernel = per == kMergeNT ? merge_kernel<LOG2, 1> : merge_kernel<LOG2, 8>;
-    kernel<<<blocks, kMergeNT, 0, st>>>(rows, parts, V, part, psum, zt, total, idx, lab, labels,
+    kernel<<<blocks, kMergeNT, 0, st>>>(rows, parts, V, packed, part, psum, zt, total, idx, lab, labels,
                                         o, loss, lse, count, sums);
     count_launches(1);
 }
@@ -309,8 +311,20 @@ finish_grad_kernel(long long row0, long long rows, int D, int cx, const float *_
     }
 }
 
-// dst[i] = scale * sum over many splits of acc[s][i]: 32 values a block, 32
-// slices of the splits side by side
+// dst[i] = sum over splits of acc[s][i], a thread each
+template <typename T>
+__global__ void __launch_bounds__(256)
+sum_splits_kernel(long long n, const float *__restrict__ acc, int splits, T *__restrict__ dst) {
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
+    if (i >= n) return;
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) v += acc[s * n + i];
+    dst[i] = ce_from_float<T>(v);
+}
+
+// the same of few values and many splits: 32 values a block, 32 slices of the
+// splits side by side
 template <typename T>
 __global__ void __launch_bounds__(1024)
 reduce_splits_kernel(long long n, const float *__restrict__ acc, int splits,
@@ -370,7 +384,7 @@ struct Plan {
 };
 
 // state (kept between the two directions): count (float, padded to 4 words),
-// lse [N] (two floats), packed total (int, padded to 4 words), idx [Np], lab [Np],
+// lse [N] (two floats; of packed rows but on the narrow path), packed total (int, padded to 4 words), idx [Np], lab [Np],
 // block counts
 struct State {
     float *count;
@@ -601,7 +615,7 @@ cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
     if (p.splits > 1) {
         blocks = (a.N + merge_rows(p.splits) - 1) / merge_rows(p.splits);
         const auto merge = a.opt.cap > 0.f ? launch_merge<false> : launch_merge<true>;
-        merge(a.N, a.N, p.splits, a.V, part, psum, zt, nullptr, nullptr, nullptr, a.labels,
+        merge(a.N, a.N, p.splits, a.V, false, part, psum, zt, nullptr, nullptr, nullptr, a.labels,
               a.opt, loss, a.lse, a.count, sums, st);
         GSV_CE_TRY(cudaGetLastError());
     }
@@ -613,8 +627,12 @@ cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
 template <typename T>
 cudaError_t reduce_splits(long long n, const float *acc, int splits, void *dst,
                           cudaStream_t st) {
-    reduce_splits_kernel<T><<<(unsigned)((n + 31) / 32), 1024, 0, st>>>(n, acc, splits,
-                                                                        static_cast<T *>(dst));
+    if (n >= 64 * 1024)  // two threads a lane of the device
+        sum_splits_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(
+            n, acc, splits, static_cast<T *>(dst));
+    else
+        reduce_splits_kernel<T><<<(unsigned)((n + 31) / 32), 1024, 0, st>>>(
+            n, acc, splits, static_cast<T *>(dst));
     count_launches(1);
     return cudaGetLastError();
 }
@@ -704,11 +722,10 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         const FewArgs a{(int)N, V, D, features, weight, labels, o, s.lse, s.count};
         return launch_few_forward(a, type, loss, ws, st);
     }
-    if (!direct) {
-        if (o.reduction == kCeNone)
-            GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
-        GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
-    }
+    // merged by packed rows, which leaves out those without a label
+    if (o.reduction == kCeNone && !(direct && forward_only))
+        GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
+    if (!direct) GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
     if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, ws + p.wp, st));
     CeGemm g = gemm_of(p, s, weight, ws, o);
     g.product = kCeScores;
@@ -727,8 +744,10 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     GSV_CE_TRY(launch_ce_gemm(g, st));
     const int per = merge_rows(2 * p.runs), mb = (int)((N + per - 1) / per);
     float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
-    launch_merge<false>(g.rows, N, 2 * p.runs, V, g.part, g.psum, g.zt, g.count, g.idx, g.lab,
-                        labels, o, loss, s.lse, s.count, sums, st);
+    const bool indexed = !forward_only || !direct;
+    launch_merge<false>(g.rows, N, 2 * p.runs, V, !direct, g.part, g.psum, g.zt,
+                        indexed ? s.total : nullptr, indexed ? s.idx : nullptr,
+                        indexed ? s.lab : nullptr, labels, o, loss, s.lse, s.count, sums, st);
     GSV_CE_TRY(cudaGetLastError());
     if (mb > 1) GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));
     return cudaSuccess;

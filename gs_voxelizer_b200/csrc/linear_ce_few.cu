@@ -149,7 +149,10 @@ few_merge_kernel(int N, int V, int parts, const float2 *__restrict__ part,
             l = ce_row_loss(lse, zt[r], a.sz, V, o);
         else if (y == kCeInvalid)
             l = lse.x = ce_nan();
-        lse_out[r] = lse;
+        // lse goes by the labelled rows alone, as the backward's rows do
+        int before = 0;
+        for (int k = 0; k < r; ++k) before += labels[k] != o.ignore;
+        if (y != kCeIgnored) lse_out[before] = lse;
         if (o.reduction == kCeNone) loss[r] = l;
         s_loss[r] = l;
         s_count[r] = y == kCeIgnored ? 0.f : 1.f;
