@@ -234,15 +234,18 @@ __device__ __forceinline__ Unit unit_of(const CeGemm &g, const Work &w, int u) {
     t.k0 = 0;
     t.k1 = w.kblocks;
     if (PRODUCT == kCeScores) {
-        t.n0 = (int)((long long)w.ntiles * u / g.runs);
-        t.n1 = (int)((long long)w.ntiles * (u + 1) / g.runs);
+        // products below 2^32 (2^22 tiles at most, 2 kCePairs runs), divided
+        // in 32 bits: every role does this for every unit
+        t.n0 = (int)((unsigned)w.ntiles * (unsigned)u / (unsigned)g.runs);
+        t.n1 = (int)((unsigned)w.ntiles * (unsigned)(u + 1) / (unsigned)g.runs);
         t.split = u;
     } else {
         t.n0 = u % w.ntiles;
         t.n1 = t.n0 + 1;
         t.split = u / w.ntiles;
-        t.k0 = (int)((long long)w.kblocks * t.split / g.splits);
-        t.k1 = (int)((long long)w.kblocks * (t.split + 1) / g.splits);
+        // (2^25 blocks at most, kCePairs splits)
+        t.k0 = (int)((unsigned)w.kblocks * (unsigned)t.split / (unsigned)g.splits);
+        t.k1 = (int)((unsigned)w.kblocks * (unsigned)(t.split + 1) / (unsigned)g.splits);
     }
     t.chunks = F32 ? max(1, (t.k1 - t.k0 + kChunk - 1) / kChunk) : 1;
     return t;

@@ -575,13 +575,16 @@ namespace {
 // parts of dX, parts of dW.
 struct NarrowPlan {
     int splits, dw_splits;
+    long long row_blocks;
     size_t sums, part, psum, zt, dx, dw, bytes;
 };
 
 NarrowPlan narrow_plan(long long N, int V, int D, bool backward, const CeOpt &o) {
     NarrowPlan p{};
-    p.splits = narrow_class_splits(N, V, D);
-    p.dw_splits = narrow_dw_splits(N, V, D);
+    const NarrowShape shape = narrow_shape(N, V, D);
+    p.splits = shape.class_splits;
+    p.dw_splits = shape.dw_blocks;
+    p.row_blocks = shape.row_blocks;
     size_t at = 0;
     auto take = [&](size_t b) {
         const size_t a = at;
@@ -593,7 +596,7 @@ NarrowPlan narrow_plan(long long N, int V, int D, bool backward, const CeOpt &o)
         p.dx = take(parts * D * sizeof(float));
         p.dw = take(sizeof(float) * (size_t)p.dw_splits * V * D);
     } else {
-        p.sums = take(sizeof(float2) * (size_t)std::max(narrow_fwd_blocks(N, D), N / 32 + 1));
+        p.sums = take(sizeof(float2) * (size_t)std::max(p.row_blocks, N / 32 + 1));
         p.part = take(parts * sizeof(float2));
         p.psum = take(o.eps > 0.f ? parts * sizeof(float) : 0);
         p.zt = take(parts ? sizeof(float) * (size_t)N : 0);
@@ -611,7 +614,7 @@ cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
     float *psum = a.opt.eps > 0.f ? reinterpret_cast<float *>(ws + p.psum) : nullptr;
     float *zt = reinterpret_cast<float *>(ws + p.zt);
     GSV_CE_TRY(launch_narrow_fwd<T>(a, loss, sums, part, psum, zt, st));
-    long long blocks = narrow_fwd_blocks(a.N, a.D);
+    long long blocks = p.row_blocks;
     if (p.splits > 1) {
         blocks = (a.N + merge_rows(p.splits) - 1) / merge_rows(p.splits);
         const auto merge = a.opt.cap > 0.f ? launch_merge<false> : launch_merge<true>;
@@ -658,10 +661,22 @@ cudaError_t narrow_backward(const NarrowArgs &a, const float *grad_loss, void *g
 
 namespace {
 
-// Which forward serves N rows of D channels.
+// Which kernels serve a call. kNarrow (linear_ce_narrow.cu, the CUDA cores
+// without tiles): where it is the faster. Kernels' time of a training step,
+// narrow against tiles: 53000 rows x 203 classes, D = 16, 99 against 180 us of
+// float32, 90 against 98 of bf16; D = 32, 156 against 170 and 145 against 80;
+// 10^6 rows x 20 classes, D = 16, 148 against 1311 and 134 against 530, D = 32,
+// 356 and 299 against 530 of bf16; 1000 rows x 50000 classes, D = 16, 267
+// against 472 and 250 against 160, D = 32, 584 against 480 of float32.
+// kFew: the forward alone; its backward takes tiles.
 enum Path { kNarrow, kFew, kTiles };
-Path path_of(long long N, int D) {
-    return D <= kNarrowD ? kNarrow : N <= kFewRows ? kFew : kTiles;
+Path path_of(long long N, int V, int D, int type) {
+    const int most = D <= 8 ? INT_MAX
+                     : D <= 16 ? (type == kCeF32 ? INT_MAX : 128)
+                     : D <= kNarrowD ? (type == kCeF32 ? 256 : 64)
+                                     : 0;
+    if (V <= most) return kNarrow;
+    return N <= kFewRows ? kFew : kTiles;
 }
 
 // Rows that the forward's tiles read in place, 16 bits and aligned for TMA:
@@ -681,7 +696,8 @@ size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backw
     // a forward without a state keeps its statistics (and, of tiles, the
     // packed rows' index) here
     const size_t own = backward ? 0 : align256(linear_ce_state_bytes(N));
-    switch (backward && D > kNarrowD ? kTiles : path_of(N, D)) {
+    const Path path = path_of(N, V, D, type);
+    switch (backward && path == kFew ? kTiles : path) {
         case kNarrow: return own + narrow_plan(N, V, D, backward, o).bytes;
         case kFew: return own + few_workspace_bytes((int)N, V);
         default: return own + make_plan(N, V, D, type, nullptr, backward, o).bytes;
@@ -696,7 +712,7 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const State s = state_of(forward_only ? ws : state, N);
     ws += align256(linear_ce_state_bytes(N));
-    const Path path = path_of(N, D);
+    const Path path = path_of(N, V, D, type);
     if (path == kNarrow) {
         const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
         switch (type) {
@@ -760,7 +776,7 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
                                       void *grad_weight, void *workspace, cudaStream_t st) {
     const State s = state_of(state, N);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
-    if (D <= kNarrowD) {
+    if (path_of(N, V, D, type) == kNarrow) {
         const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
 #define GSV_CE_T(T) narrow_backward<T>(a, grad_loss, grad_features, grad_weight, ws, st)
         switch (type) {

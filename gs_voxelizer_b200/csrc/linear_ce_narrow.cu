@@ -1,123 +1,94 @@
-// Linear class loss of few channels (D <= 8: the channels of a voxelized
-// volume) on the CUDA cores, float32 throughout.
+// Linear class loss of few channels (D <= 32: the channels of a voxelized
+// volume, and small feature volumes) on the CUDA cores, float32 throughout.
 //
-// A score is D multiply-adds here, and the loss's exponential (16 a clock and
-// SM) costs as much as eight of them, so that the tensor cores have nothing to
-// give: they pad D to 16 and, for float32, take six products. The table goes
-// through shared memory in float32, each value twice, and rows go in pairs
-// through the paired FP32 instructions, which leaves the exponentials (two a
-// pair of scores, against 12 to 14 other instructions) as the bound. Forward
-// and dX: a thread owns two rows and walks the classes with the running
-// maximum and sum, or the gradient, in registers. dW: a thread owns a class
-// and walks the rows, so that neither gradient needs atomics. Without a cap
-// the table is held times log2 e, so that a score is an exponent of two, and
-// what is linear stays out of the loops: the label's own term, the sum of all
-// scores (x . sum of the table) and the smoothing's share of dX.
+// Tiles of the tensor cores would be mostly padding here: they take 9 ps a
+// score of float32 (six products of padded planes) and 3 to 25 of 16 bits, the
+// more the fewer the classes, against about (2 + 0.3 D) ps for all of a
+// training step here. A score is D multiply-adds and an exponential (16 a
+// clock and SM, as long as eight multiply-adds). A thread takes two rows
+// (forward, dX) against the classes of the table in shared memory, or one to
+// four classes (dW) against the staged rows, so that each value read serves
+// them all; the paired FP32 instructions run along the channels; the running
+// maximum and sum, or the gradient, stay in registers, and neither gradient
+// needs atomics.
+//
+// What bounds it: issue and latency at the occupancy that the registers leave
+// (256^3 rows x 4 channels, 20 classes, float32: forward 180 us, dX 209 us,
+// dW 258 us; 0.6 instructions a clock and scheduler, 12 to 20 a score, the
+// exponentials alone would take 75 us each). One, two or four rows a thread,
+// three to five blocks an SM and pairs of rows instead of channels came to
+// 636 to 770 us for the three.
+//
+// Without a cap the table is held times log2 e, so that a score is an exponent
+// of two, and what is linear stays out of the loops: the label's own term, the
+// sum of all scores (x . sum of the table) and the smoothing's share of dX.
 // Few rows or many classes: the classes (for dW the rows) are split over
 // blocks and the parts are joined in a fixed order.
-#include <type_traits>
-
 #include "ce_narrow.cuh"
 
 namespace gsv {
 namespace {
 
-constexpr int kNT = 256;
-constexpr int kPairs = 1;                // pairs of rows a thread
+constexpr int kNT = kNarrowNT;
+// rows staged at once (dW), in two buffers of 48 KB at most
+constexpr int dw_rows_of(int dp) { return dp <= 8 ? 256 : 128; }
+constexpr int chunk_of(int dp) { return 4096 / dp; }  // classes staged at once
+constexpr int kRows = 2;                              // rows a thread
+// classes a thread (dW): the registers hold 2 DP each
+constexpr int classes_of(int dp) { return dp == 4 ? 4 : dp == 32 ? 1 : 2; }
 // blocks an SM, as many as registers hold without spills
-constexpr int per_sm(int dp) { return dp == 4 ? 3 : 2; }
-constexpr int kBlockRows = kNT * 2 * kPairs;
-constexpr int kChunk = 256;              // classes staged at once
-constexpr int kTile = 256;               // rows staged at once (dW)
-
-__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+constexpr int per_sm(int dp) { return dp <= 8 ? 3 : dp == 16 ? 2 : 1; }
+constexpr int width_of(int D) { return D <= 4 ? 4 : D <= 8 ? 8 : D <= 16 ? 16 : 32; }
 
 template <int DP>
-struct alignas(16) Row {
-    float v[DP];
-};
-// every value twice, for the paired instructions
-template <int DP>
-struct alignas(16) Row2 {
-    float2 v[DP];
+struct alignas(16) Pairs {
+    float2 v[DP / 2];
 };
 
-// Row r of a [., D] matrix. VEC: D = DP and rows aligned to their size (or
-// 16 bytes), so that a row is one or two wide accesses.
-template <typename T, int DP, bool VEC>
-__device__ __forceinline__ Row<DP> load_row(const T *p, long long r, int D) {
-    constexpr int kBytes = DP * sizeof(T);
-    Row<DP> x;
-    if constexpr (VEC) {
-        struct alignas(kBytes < 16 ? kBytes : 16) Raw { T t[DP]; };
-        const Raw q = reinterpret_cast<const Raw *>(p)[r];
+template <int DP>
+__device__ __forceinline__ Pairs<DP> to_pairs(const Row<DP> &r, float scale) {
+    Pairs<DP> p;
 #pragma unroll
-        for (int d = 0; d < DP; ++d) x.v[d] = ce_to_float(q.t[d]);
-    } else {
-        const T *q = p + r * D;
+    for (int d = 0; d < DP / 2; ++d)
+        p.v[d] = make_float2(r.v[2 * d] * scale, r.v[2 * d + 1] * scale);
+    return p;
+}
+
+// four chains of multiply-adds, two to a register pair
+template <int DP>
+__device__ __forceinline__ float dot_pairs(const Pairs<DP> &a, const Pairs<DP> &b) {
+    float2 s = __fmul2_rn(a.v[0], b.v[0]), t = __fmul2_rn(a.v[1], b.v[1]);
 #pragma unroll
-        for (int d = 0; d < DP; ++d) x.v[d] = d < D ? ce_to_float(q[d]) : 0.f;
+    for (int d = 2; d < DP / 2; d += 2) {
+        s = __ffma2_rn(a.v[d], b.v[d], s);
+        t = __ffma2_rn(a.v[d + 1], b.v[d + 1], t);
     }
-    return x;
+    s = __fadd2_rn(s, t);
+    return s.x + s.y;
 }
 
 template <typename T, int DP, bool VEC>
-__device__ __forceinline__ void store_row(T *p, long long r, int D, const float (&v)[DP]) {
-    constexpr int kBytes = DP * sizeof(T);
-    if constexpr (VEC) {
-        struct alignas(kBytes < 16 ? kBytes : 16) Raw { T t[DP]; };
-        Raw q;
-#pragma unroll
-        for (int d = 0; d < DP; ++d) q.t[d] = ce_from_float<T>(v[d]);
-        reinterpret_cast<Raw *>(p)[r] = q;
-    } else {
-#pragma unroll
-        for (int d = 0; d < DP; ++d)
-            if (d < D) p[r * D + d] = ce_from_float<T>(v[d]);
-    }
-}
-
-// classes [v0, v0 + n) of the table into shared memory, times scale
-template <typename T, int DP, bool VEC>
-__device__ __forceinline__ void stage_table(Row2<DP> *sw, const T *w, long long v0, int n, int D,
+__device__ __forceinline__ void stage_pairs(Pairs<DP> *sw, const T *w, long long v0, int n, int D,
                                             float scale) {
-    for (int j = threadIdx.x; j < n; j += kNT) {
-        const Row<DP> r = load_row<T, DP, VEC>(w, v0 + j, D);
-#pragma unroll
-        for (int d = 0; d < DP; ++d) sw[j].v[d] = f2(r.v[d] * scale);
-    }
+    for (int j = threadIdx.x; j < n; j += kNT)
+        sw[j] = to_pairs<DP>(load_row<T, DP, VEC>(w, v0 + j, D), scale);
 }
 
-template <int DP>
-__device__ __forceinline__ float dot(const Row<DP> &a, const Row<DP> &b) {
-    float s = 0.f;
-#pragma unroll
-    for (int d = 0; d < DP; ++d) s = fmaf(a.v[d], b.v[d], s);
-    return s;
-}
-template <int DP>
-__device__ __forceinline__ float2 dot2(const Row2<DP> &a, const Row2<DP> &b) {
-    float2 s = __fmul2_rn(a.v[0], b.v[0]);
-#pragma unroll
-    for (int d = 1; d < DP; ++d) s = __ffma2_rn(a.v[d], b.v[d], s);
-    return s;
-}
-// What a thread reads of its rows, one tile ahead of their use: the loads of
-// a tile cost as long as its classes otherwise.
+// What a thread reads of its rows, one tile ahead of their use: the loads of a
+// tile take as long as its classes otherwise. LSE: with the rows' statistics.
 template <int DP, int R>
 struct Ahead {
     Row<DP> x[R];
     long long label[R];
     float2 lse[R];
 };
-
-template <typename T, int DP, bool VEC, int R>
-__device__ __forceinline__ void read_ahead(Ahead<DP, R> &a, long long t0, long long N, int D,
-                                           const T *features, const long long *labels,
+template <typename T, int DP, bool VEC, int R, bool LSE>
+__device__ __forceinline__ void read_ahead(Ahead<DP, R> &a, long long t0, int stride, long long N,
+                                           int D, const T *features, const long long *labels,
                                            long long ignore, const float2 *lse) {
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-        const long long r = t0 + k * kNT + threadIdx.x;
+        const long long r = t0 + k * stride + threadIdx.x;
         a.label[k] = ignore;
         a.lse[k] = make_float2(0.f, 0.f);
 #pragma unroll
@@ -125,49 +96,10 @@ __device__ __forceinline__ void read_ahead(Ahead<DP, R> &a, long long t0, long l
         if (r < N) {
             a.x[k] = load_row<T, DP, VEC>(features, r, D);
             a.label[k] = labels[r];
-            if (lse) a.lse[k] = lse[r];
+            if (LSE) a.lse[k] = lse[r];
         }
     }
 }
-
-struct Span {
-    int v0, v1;
-};
-__device__ __forceinline__ Span class_span(int V) {
-    return {(int)((long long)V * blockIdx.y / gridDim.y),
-            (int)((long long)V * (blockIdx.y + 1) / gridDim.y)};
-}
-
-// Sum of a span of the table, by every thread the same, in shared memory.
-template <typename T, int DP, bool VEC>
-__device__ __forceinline__ void table_sum(Row<DP> &out, Row<DP> *sh, const T *w, Span span, int D) {
-    Row<DP> a;
-#pragma unroll
-    for (int d = 0; d < DP; ++d) a.v[d] = 0.f;
-    for (int j = span.v0 + threadIdx.x; j < span.v1; j += kNT) {
-        const Row<DP> r = load_row<T, DP, VEC>(w, j, D);
-#pragma unroll
-        for (int d = 0; d < DP; ++d) a.v[d] += r.v[d];
-    }
-#pragma unroll
-    for (int d = 0; d < DP; ++d)
-#pragma unroll
-        for (int k = 16; k; k >>= 1) a.v[d] += __shfl_xor_sync(0xffffffffu, a.v[d], k);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
-    __syncthreads();
-    a = sh[0];
-    for (int k = 1; k < kNT / 32; ++k)
-#pragma unroll
-        for (int d = 0; d < DP; ++d) a.v[d] += sh[k].v[d];
-    out = a;
-}
-
-// Scores are exponents of two where there is no cap (the table times log2 e),
-// and natural where there is one; so are the maxima that are kept.
-template <bool CAP>
-__device__ __forceinline__ float unit() { return CAP ? 1.f : kLog2e; }
-template <bool CAP>
-__device__ __forceinline__ float exp_of(float d) { return ex2(CAP ? d * kLog2e : d); }
 
 template <typename T, int DP, bool CAP, bool VEC>
 __global__ void __launch_bounds__(kNT, per_sm(DP))
@@ -177,77 +109,74 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
                   float *__restrict__ count, float2 *__restrict__ sums,
                   float2 *__restrict__ part, float *__restrict__ psum,
                   float *__restrict__ zt) {
-    __shared__ Row2<DP> sw[kChunk];
-    __shared__ Row<DP> sh_sum[kNT / 32];
+    constexpr int kChunk = chunk_of(DP), R = kRows;
+    __shared__ Pairs<DP> sw[kChunk];
+    __shared__ Row<DP> sh_sum[kNT / 32], s_wsum;
     __shared__ float2 sh[kNT / 32];
     const Span span = class_span(V);
     const bool smooth = o.eps > 0.f;
-    Row<DP> wsum;
-    if (smooth && !CAP) table_sum<T, DP, VEC>(wsum, sh_sum, weight, span, D);
+    if (smooth && !CAP) {
+        Row<DP> wsum;
+        table_sum<T, DP, VEC>(wsum, sh_sum, weight, span, D);
+        if (threadIdx.x == 0) s_wsum = wsum;
+        __syncthreads();
+    }
     float lsum = 0.f, cnt = 0.f;
     bool staged = false;
-    const long long stride = (long long)gridDim.x * kBlockRows;
-    Ahead<DP, 2 * kPairs> next;
-    read_ahead<T, DP, VEC>(next, (long long)blockIdx.x * kBlockRows, N, D, features, labels,
-                           o.ignore, nullptr);
-    for (long long t0 = (long long)blockIdx.x * kBlockRows; t0 < N; t0 += stride) {
-        Row2<DP> x[kPairs];
-        float2 m[kPairs], s[kPairs], sz[kPairs];
-        int label[2 * kPairs];
+    const long long stride = (long long)gridDim.x * kNT * R;
+    long long t0 = (long long)blockIdx.x * kNT * R;
+    Ahead<DP, R> next;
+    read_ahead<T, DP, VEC, R, false>(next, t0, kNT, N, D, features, labels, o.ignore, nullptr);
+    for (; t0 < N; t0 += stride) {
+        Pairs<DP> x[R];
+        float m[R], s[R], sz[R];
+        int y[R];
 #pragma unroll
-        for (int k = 0; k < 2 * kPairs; ++k) {
-            label[k] = ce_label(next.label[k], o.ignore, V);
-#pragma unroll
-            for (int d = 0; d < DP; ++d)
-                (k & 1 ? x[k / 2].v[d].y : x[k / 2].v[d].x) = next.x[k].v[d];
-            m[k / 2] = f2(ce_neg_inf());
-            s[k / 2] = sz[k / 2] = f2(0.f);
+        for (int k = 0; k < R; ++k) {
+            x[k] = to_pairs<DP>(next.x[k], 1.f);
+            y[k] = ce_label(next.label[k], o.ignore, V);
+            m[k] = ce_neg_inf();
+            s[k] = sz[k] = 0.f;
         }
-        read_ahead<T, DP, VEC>(next, t0 + stride, N, D, features, labels, o.ignore, nullptr);
+        // (of more channels there are no registers to read ahead into)
+        if (DP == 4)
+            read_ahead<T, DP, VEC, R, false>(next, t0 + stride, kNT, N, D, features, labels,
+                                             o.ignore, nullptr);
         for (int v0 = span.v0; v0 < span.v1; v0 += kChunk) {
             const int n = min(kChunk, span.v1 - v0);
             if (!staged) {
                 __syncthreads();
-                stage_table<T, DP, VEC>(sw, weight, v0, n, D, unit<CAP>());
+                stage_pairs<T, DP, VEC>(sw, weight, v0, n, D, unit<CAP>());
                 __syncthreads();
                 staged = span.v1 - span.v0 <= kChunk;
             }
             auto group = [&](int j0, auto size) {
                 constexpr int kG = decltype(size)::value;
-                float2 z[kPairs][kG];
+                float z[R][kG];
 #pragma unroll
                 for (int j = 0; j < kG; ++j) {
-                    const Row2<DP> w = sw[j0 + j];
+                    const Pairs<DP> w = sw[j0 + j];
 #pragma unroll
-                    for (int k = 0; k < kPairs; ++k) {
-                        z[k][j] = dot2<DP>(x[k], w);
+                    for (int k = 0; k < R; ++k) {
+                        z[k][j] = dot_pairs<DP>(x[k], w);
                         if (CAP) {
-                            z[k][j].x = o.cap * ce_tanh<sizeof(T) == 2>(z[k][j].x, o.cap);
-                            z[k][j].y = o.cap * ce_tanh<sizeof(T) == 2>(z[k][j].y, o.cap);
-                            sz[k] = __fadd2_rn(sz[k], z[k][j]);
+                            z[k][j] = o.cap * ce_tanh<sizeof(T) == 2>(z[k][j], o.cap);
+                            sz[k] += z[k][j];
                         }
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < kPairs; ++k) {
-                    float2 top = m[k];
+                for (int k = 0; k < R; ++k) {
+                    float top = m[k];
 #pragma unroll
-                    for (int j = 0; j < kG; ++j) {
-                        top.x = fmaxf(top.x, z[k][j].x);
-                        top.y = fmaxf(top.y, z[k][j].y);
-                    }
-                    // (all scores at -inf: not a distribution, NaN like theirs)
-                    s[k].x *= exp_of<CAP>(m[k].x - top.x);
-                    s[k].y *= exp_of<CAP>(m[k].y - top.y);
+                    for (int j = 0; j < kG; ++j) top = fmaxf(top, z[k][j]);
+                    // (all scores at -inf: no distribution, NaN like theirs)
+                    s[k] *= exp_of<CAP>(m[k] - top);
                     m[k] = top;
-                    const float2 nb = make_float2(-top.x, -top.y);
-                    float2 e = f2(0.f);
+                    float e = 0.f;
 #pragma unroll
-                    for (int j = 0; j < kG; ++j) {
-                        const float2 d = __fadd2_rn(z[k][j], nb);
-                        e = __fadd2_rn(e, make_float2(exp_of<CAP>(d.x), exp_of<CAP>(d.y)));
-                    }
-                    s[k] = __fadd2_rn(s[k], e);
+                    for (int j = 0; j < kG; ++j) e += exp_of<CAP>(z[k][j] - top);
+                    s[k] += e;
                 }
             };
             int j0 = 0;
@@ -259,40 +188,37 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
             for (; j0 < n; ++j0) group(j0, std::integral_constant<int, 1>{});
         }
 #pragma unroll
-        for (int k = 0; k < 2 * kPairs; ++k) {
+        for (int k = 0; k < R; ++k) {
             const long long r = t0 + k * kNT + threadIdx.x;
             if (r >= N) continue;
-            const int y = label[k];
-            Row<DP> q;
-#pragma unroll
-            for (int d = 0; d < DP; ++d) q.v[d] = k & 1 ? x[k / 2].v[d].y : x[k / 2].v[d].x;
-            CeAcc a;
-            a.m = k & 1 ? m[k / 2].y : m[k / 2].x;
-            a.s = k & 1 ? s[k / 2].y : s[k / 2].x;
-            a.sz = k & 1 ? sz[k / 2].y : sz[k / 2].x;
-            if (smooth && !CAP) a.sz = dot<DP>(q, wsum);
+            if (smooth && !CAP) sz[k] = dot_pairs<DP>(x[k], to_pairs<DP>(s_wsum, 1.f));
             float zy = 0.f;
-            if (y >= 0) {
-                zy = dot<DP>(q, load_row<T, DP, VEC>(weight, y, D));
+            if (y[k] >= 0) {
+                zy = dot_pairs<DP>(x[k],
+                                   to_pairs<DP>(load_row<T, DP, VEC>(weight, y[k], D), 1.f));
                 if (CAP) zy = o.cap * ce_tanh<sizeof(T) == 2>(zy, o.cap);
             }
             if (gridDim.y > 1) {
-                part[blockIdx.y * N + r] = make_float2(a.m, a.s);
-                if (psum) psum[blockIdx.y * N + r] = a.sz;
+                part[blockIdx.y * N + r] = make_float2(m[k], s[k]);
+                if (psum) psum[blockIdx.y * N + r] = sz[k];
                 if (blockIdx.y == 0) zt[r] = zy;
                 continue;
             }
             float l = 0.f;
-            float2 lse = make_float2(CeAcc::base(a.m), __log2f(a.s));
-            if (y >= 0)
-                l = ce_row_loss(make_float2(CAP ? lse.x : lse.x * kCeLn2, lse.y), zy, a.sz, V, o);
-            else if (y == kCeInvalid)
+            float2 lse = make_float2(CeAcc::base(m[k]), __log2f(s[k]));
+            if (y[k] >= 0)
+                l = ce_row_loss(make_float2(CAP ? lse.x : lse.x * kCeLn2, lse.y), zy, sz[k], V,
+                                o);
+            else if (y[k] == kCeInvalid)
                 l = lse.x = ce_nan();
             lse_out[r] = lse;
             if (o.reduction == kCeNone) loss[r] = l;
             lsum += l;
-            cnt += y == kCeIgnored ? 0.f : 1.f;
+            cnt += y[k] == kCeIgnored ? 0.f : 1.f;
         }
+        if (DP > 4)
+            read_ahead<T, DP, VEC, R, false>(next, t0 + stride, kNT, N, D, features, labels,
+                                             o.ignore, nullptr);
     }
     if (gridDim.y > 1) return;
     const float2 t = ce_block_sum<kNT>(lsum, cnt, sh);
@@ -304,34 +230,15 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
     }
 }
 
-// A row's part of the derivative: (kz prob - e - hit at its class), all with
-// the row's upstream gradient in them.
-struct RowGrad {
-    float2 lse;
-    float kz, e, hit;
-};
-
-// the upstream gradient that all rows share (a mean's divided by the count)
-__device__ __forceinline__ float common_grad(const CeUpstream &u) {
-    return u.reduction == kCeNone ? 0.f
-           : u.reduction == kCeMean ? u.g[0] / u.count[0]
-                                    : u.g[0];
-}
-
-template <bool CAP>
-__device__ __forceinline__ RowGrad row_grad(long long r, int y, float2 lse, const CeOpt &o,
-                                            const float *per_row, float common, float smooth) {
-    RowGrad q{make_float2(0.f, 0.f), 0.f, 0.f, 0.f};
-    if (y == kCeIgnored) return q;
-    q.lse = lse;
-    const float g = per_row ? per_row[r] : common;
-    q.kz = g;
-    if (o.zeta > 0.f)
-        q.kz *= 1.f + 2.f * o.zeta * ce_lse(make_float2(CAP ? q.lse.x : q.lse.x * kCeLn2,
-                                                       q.lse.y));
-    q.e = smooth * g;
-    q.hit = (1.f - o.eps) * g;
-    return q;
+// 2^(score - logsumexp) of a score before the cap, and the cap's slope
+template <bool CAP, bool FAST>
+__device__ __forceinline__ float prob(float z, float2 lse, float cap, float &slope) {
+    if (CAP) {
+        const float t = ce_tanh<FAST>(z, cap);
+        slope = fmaf(-t, t, 1.f);
+        return ex2(fmaf(cap * t - lse.x, kLog2e, -lse.y));
+    }
+    return ex2((z - lse.x) - lse.y);
 }
 
 template <typename T, int DP, bool CAP, bool VEC>
@@ -340,87 +247,83 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
                  const T *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
                  const float2 *__restrict__ lse, CeUpstream u, T *__restrict__ grad,
                  float *__restrict__ acc) {
-    __shared__ Row2<DP> sw[kChunk];
-    __shared__ Row<DP> sh_sum[kNT / 32];
+    constexpr int kChunk = chunk_of(DP), R = kRows;
+    __shared__ Pairs<DP> sw[kChunk];
+    __shared__ Row<DP> sh_sum[kNT / 32], s_wsum;
     const Span span = class_span(V);
     const bool smooth = o.eps > 0.f;
-    Row<DP> wsum;
-    if (smooth && !CAP) table_sum<T, DP, VEC>(wsum, sh_sum, weight, span, D);
+    if (smooth && !CAP) {
+        Row<DP> wsum;
+        table_sum<T, DP, VEC>(wsum, sh_sum, weight, span, D);
+        if (threadIdx.x == 0) s_wsum = wsum;
+        __syncthreads();
+    }
     bool staged = false;
     const float common = common_grad(u), ev = o.eps / (float)V;
     const float *per_row = u.reduction == kCeNone ? u.g : nullptr;
-    const long long stride = (long long)gridDim.x * kBlockRows;
-    Ahead<DP, 2 * kPairs> next;
-    read_ahead<T, DP, VEC>(next, (long long)blockIdx.x * kBlockRows, N, D, features, labels,
-                           o.ignore, lse);
-    for (long long t0 = (long long)blockIdx.x * kBlockRows; t0 < N; t0 += stride) {
-        Row2<DP> x[kPairs], dx[kPairs];
-        float2 nm[kPairs], nl[kPairs], kz[kPairs], e[kPairs];
-        RowGrad q[2 * kPairs];
-        int y[2 * kPairs];
+    const long long stride = (long long)gridDim.x * kNT * R;
+    long long t0 = (long long)blockIdx.x * kNT * R;
+    Ahead<DP, R> next;
+    read_ahead<T, DP, VEC, R, true>(next, t0, kNT, N, D, features, labels, o.ignore, lse);
+    for (; t0 < N; t0 += stride) {
+        Pairs<DP> x[R], dx[R];
+        RowGrad q[R];
+        int y[R];
 #pragma unroll
-        for (int k = 0; k < 2 * kPairs; ++k) {
+        for (int k = 0; k < R; ++k) {
             const long long r = t0 + k * kNT + threadIdx.x;
             y[k] = ce_label(next.label[k], o.ignore, V);
             q[k] = row_grad<CAP>(r, y[k], next.lse[k], o, per_row, common, ev);
-            auto put = [&](float2 &a, float b) { (k & 1 ? a.y : a.x) = b; };
+            x[k] = to_pairs<DP>(next.x[k], 1.f);
 #pragma unroll
-            for (int d = 0; d < DP; ++d) {
-                put(x[k / 2].v[d], next.x[k].v[d]);
-                dx[k / 2].v[d] = f2(0.f);
-            }
-            put(nm[k / 2], -q[k].lse.x);
-            put(nl[k / 2], -q[k].lse.y);
-            put(kz[k / 2], q[k].kz);
-            put(e[k / 2], -q[k].e);
+            for (int d = 0; d < DP / 2; ++d) dx[k].v[d] = f2(0.f);
         }
-        read_ahead<T, DP, VEC>(next, t0 + stride, N, D, features, labels, o.ignore, lse);
+        if (DP == 4)
+            read_ahead<T, DP, VEC, R, true>(next, t0 + stride, kNT, N, D, features, labels,
+                                            o.ignore, lse);
         for (int v0 = span.v0; v0 < span.v1; v0 += kChunk) {
             const int n = min(kChunk, span.v1 - v0);
             if (!staged) {
                 __syncthreads();
-                stage_table<T, DP, VEC>(sw, weight, v0, n, D, unit<CAP>());
+                stage_pairs<T, DP, VEC>(sw, weight, v0, n, D, unit<CAP>());
                 __syncthreads();
                 staged = span.v1 - span.v0 <= kChunk;
             }
-#pragma unroll 4
+#pragma unroll(DP == 4 ? 2 : 1)
             for (int j = 0; j < n; ++j) {
-                const Row2<DP> w = sw[j];
+                const Pairs<DP> w = sw[j];
 #pragma unroll
-                for (int k = 0; k < kPairs; ++k) {
-                    float2 z = dot2<DP>(x[k], w), t;
-                    if (CAP) {
-                        t = make_float2(ce_tanh<sizeof(T) == 2>(z.x, o.cap),
-                                        ce_tanh<sizeof(T) == 2>(z.y, o.cap));
-                        z = __fmul2_rn(t, f2(o.cap));
-                    }
-                    z = __fadd2_rn(z, nm[k]);
-                    z = CAP ? __ffma2_rn(z, f2(kLog2e), nl[k]) : __fadd2_rn(z, nl[k]);
-                    float2 d = make_float2(ex2(z.x), ex2(z.y));
+                for (int k = 0; k < R; ++k) {
+                    float slope = 1.f;
+                    float d = prob<CAP, sizeof(T) == 2>(dot_pairs<DP>(x[k], w), q[k].lse, o.cap,
+                                                        slope);
                     if (CAP) {  // the whole derivative goes through the slope
-                        d = __ffma2_rn(kz[k], d, e[k]);
-                        if (y[2 * k] == v0 + j) d.x -= q[2 * k].hit;
-                        if (y[2 * k + 1] == v0 + j) d.y -= q[2 * k + 1].hit;
-                        d = __fmul2_rn(d, __ffma2_rn(make_float2(-t.x, -t.y), t, f2(1.f)));
+                        d = fmaf(q[k].kz, d, -q[k].e);
+                        if (y[k] == v0 + j) d -= q[k].hit;
+                        d *= slope;
                     }
 #pragma unroll
-                    for (int i = 0; i < DP; ++i) dx[k].v[i] = __ffma2_rn(d, w.v[i], dx[k].v[i]);
+                    for (int i = 0; i < DP / 2; ++i)
+                        dx[k].v[i] = __ffma2_rn(f2(d), w.v[i], dx[k].v[i]);
                 }
             }
         }
 #pragma unroll
-        for (int k = 0; k < 2 * kPairs; ++k) {
+        for (int k = 0; k < R; ++k) {
             const long long r = t0 + k * kNT + threadIdx.x;
             if (r >= N) continue;
             float out[DP];
+            // the table is times log2 e where there is no cap
+            const float f = CAP ? 1.f : q[k].kz * kCeLn2;
 #pragma unroll
-            for (int d = 0; d < DP; ++d) out[d] = k & 1 ? dx[k / 2].v[d].y : dx[k / 2].v[d].x;
+            for (int d = 0; d < DP / 2; ++d) {
+                out[2 * d] = dx[k].v[d].x * f;
+                out[2 * d + 1] = dx[k].v[d].y * f;
+            }
             if (!CAP) {
-                const float f = q[k].kz * kCeLn2;  // the table is times log2 e
+                if (smooth) {
 #pragma unroll
-                for (int d = 0; d < DP; ++d) {
-                    out[d] *= f;
-                    if (smooth) out[d] = fmaf(-q[k].e, wsum.v[d], out[d]);
+                    for (int d = 0; d < DP; ++d) out[d] = fmaf(-q[k].e, s_wsum.v[d], out[d]);
                 }
                 if (y[k] >= span.v0 && y[k] < span.v1) {
                     const Row<DP> w = load_row<T, DP, VEC>(weight, y[k], D);
@@ -437,186 +340,179 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
             else
                 store_row<T, DP, VEC>(grad, r, D, out);
         }
+        if (DP > 4)
+            read_ahead<T, DP, VEC, R, true>(next, t0 + stride, kNT, N, D, features, labels,
+                                            o.ignore, lse);
     }
 }
 
-// Two staged rows for dW, value by value. `more` is read where smoothing or
-// z-loss make it differ from what kz gives.
+// A staged row for dW; e and hit are read where smoothing or z-loss make them
+// differ from what kz gives.
 template <int DP>
-struct alignas(16) DwPair {
-    Row2<DP> x;
-    float2 nm, nl;
-    float2 kz;
-    int2 y;
-    float2 e, hit;
+struct alignas(16) DwRow {
+    Pairs<DP> x;
+    float2 lse;
+    float kz;
+    int y;
+    float e, hit, unused[2];
 };
 
 // acc[blockIdx.x][V][D]: the block's rows' part of its classes' gradients.
-// Threads: `lanes` pairs of classes (j, j + lanes) x (kNT / lanes) slices of
-// the staged rows; two classes a thread halve the shared-memory reads, which
-// bound it with one.
+// Threads: `lanes` groups of classes (j, j + lanes, ...) x (kNT / lanes)
+// slices of the staged rows.
 template <typename T, int DP, bool CAP, bool VEC>
 __global__ void __launch_bounds__(kNT, per_sm(DP))
 narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ features,
                  const T *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
                  const float2 *__restrict__ lse, CeUpstream u, float *__restrict__ acc) {
-    // two buffers: a tile is staged while others still read the last one
-    __shared__ DwPair<DP> buffers[2][kTile / 2];
-    __shared__ float red[kNT][DP + 1];
+    constexpr int C = classes_of(DP), kDwRows = dw_rows_of(DP);
+    constexpr size_t kRowBytes = sizeof(DwRow<DP>) * kDwRows * 2;
+    constexpr size_t kRedBytes = sizeof(float) * kNT * (DP + 1);
+    // two buffers of rows: a tile is staged while others still read the last
+    // one; and in the end the slices' sums
+    __shared__ __align__(16) unsigned char raw[kRowBytes > kRedBytes ? kRowBytes : kRedBytes];
+    DwRow<DP> *buffers = reinterpret_cast<DwRow<DP> *>(raw);
+    float *red = reinterpret_cast<float *>(raw);
     const int slices = kNT / lanes, slice = threadIdx.x / lanes;
-    const int j0 = blockIdx.y * 2 * lanes + threadIdx.x % lanes;
+    const int j0 = blockIdx.y * C * lanes + threadIdx.x % lanes;
     const bool active = slice < slices && j0 < V;
-    Row2<DP> w[2], dw[2];
+    Pairs<DP> w[C], dw[C];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        Row<DP> q;
+    for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int d = 0; d < DP; ++d) q.v[d] = 0.f;
-        if (active && j0 + c * lanes < V) q = load_row<T, DP, VEC>(weight, j0 + c * lanes, D);
-#pragma unroll
-        for (int d = 0; d < DP; ++d) {
-            w[c].v[d] = f2(q.v[d] * unit<CAP>());
-            dw[c].v[d] = f2(0.f);
-        }
+        for (int d = 0; d < DP / 2; ++d) w[c].v[d] = dw[c].v[d] = f2(0.f);
+        if (active && j0 + c * lanes < V)
+            w[c] = to_pairs<DP>(load_row<T, DP, VEC>(weight, j0 + c * lanes, D), unit<CAP>());
     }
     const bool plain = o.eps == 0.f && o.zeta == 0.f;
     const float common = common_grad(u), ev = o.eps / (float)V;
     const float *per_row = u.reduction == kCeNone ? u.g : nullptr;
-    const long long stride = (long long)gridDim.x * kTile;
+    const long long stride = (long long)gridDim.x * kDwRows;
+    long long t0 = (long long)blockIdx.x * kDwRows;
     int buffer = 0;
+    const bool stager = threadIdx.x < kDwRows;
     Ahead<DP, 1> next;
-    read_ahead<T, DP, VEC>(next, (long long)blockIdx.x * kTile, N, D, features, labels, o.ignore,
-                           lse);
-    for (long long t0 = (long long)blockIdx.x * kTile; t0 < N; t0 += stride) {
-        const long long r = t0 + threadIdx.x;
-        // an unlabelled row is all zeros
-        const int y = ce_label(next.label[0], o.ignore, V);
-        const RowGrad q = row_grad<CAP>(r, y, next.lse[0], o, per_row, common, ev);
-        DwPair<DP> *rows = buffers[buffer];
+    read_ahead<T, DP, VEC, 1, true>(next, stager ? t0 : N, 0, N, D, features, labels, o.ignore,
+                                    lse);
+    for (; t0 < N; t0 += stride) {
+        DwRow<DP> *rows = buffers + buffer * kDwRows;
         buffer ^= 1;
-        {
-            const int h = threadIdx.x & 1;
-            DwPair<DP> &p = rows[threadIdx.x / 2];
-            auto put = [&](float2 &a, float b) { (&a.x)[h] = b; };
-#pragma unroll
-            for (int d = 0; d < DP; ++d) put(p.x.v[d], y == kCeIgnored ? 0.f : next.x[0].v[d]);
-            put(p.nm, -q.lse.x);
-            put(p.nl, -q.lse.y);
-            put(p.kz, q.kz);
-            (&p.y.x)[h] = y;
-            put(p.e, -q.e);
-            put(p.hit, q.hit);
+        if (stager) {
+            // an unlabelled row is all zeros
+            DwRow<DP> s{};
+            s.y = ce_label(next.label[0], o.ignore, V);
+            if (s.y != kCeIgnored) {
+                const RowGrad q = row_grad<CAP>(t0 + threadIdx.x, s.y, next.lse[0], o, per_row,
+                                                common, ev);
+                s.x = to_pairs<DP>(next.x[0], 1.f);
+                s.lse = q.lse;
+                s.kz = q.kz;
+                s.e = q.e;
+                s.hit = q.hit;
+            }
+            rows[threadIdx.x] = s;
+            read_ahead<T, DP, VEC, 1, true>(next, t0 + stride, 0, N, D, features, labels,
+                                            o.ignore, lse);
         }
-        read_ahead<T, DP, VEC>(next, t0 + stride, N, D, features, labels, o.ignore, lse);
         __syncthreads();
         if (!active) continue;
-        for (int i = slice; i < kTile / 2; i += slices) {
-            const DwPair<DP> &p = rows[i];
-            const Row2<DP> xv = p.x;
-            const float2 nm = p.nm, nl = p.nl, kz = p.kz;
-            const int2 yy = p.y;
-            float2 hit = kz, e = f2(0.f);
+        for (int i = slice; i < kDwRows; i += slices) {
+            const Pairs<DP> x = rows[i].x;
+            const float2 l = rows[i].lse;
+            const float kz = rows[i].kz;
+            const int y = rows[i].y;
+            float hit = kz, e = 0.f;
             if (!plain) {
-                hit = p.hit;
-                e = p.e;
+                hit = rows[i].hit;
+                e = rows[i].e;
             }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float2 z = dot2<DP>(xv, w[c]), t;
-                if (CAP) {
-                    t = make_float2(ce_tanh<sizeof(T) == 2>(z.x, o.cap),
-                                    ce_tanh<sizeof(T) == 2>(z.y, o.cap));
-                    z = __fmul2_rn(t, f2(o.cap));
-                }
-                z = __fadd2_rn(z, nm);
-                z = CAP ? __ffma2_rn(z, f2(kLog2e), nl) : __fadd2_rn(z, nl);
-                float2 d = make_float2(ex2(z.x), ex2(z.y));
-                d = __ffma2_rn(kz, d, e);
-                if (yy.x == j0 + c * lanes) d.x -= hit.x;
-                if (yy.y == j0 + c * lanes) d.y -= hit.y;
-                if (CAP) d = __fmul2_rn(d, __ffma2_rn(make_float2(-t.x, -t.y), t, f2(1.f)));
+            for (int c = 0; c < C; ++c) {
+                float slope = 1.f;
+                const float p =
+                    prob<CAP, sizeof(T) == 2>(dot_pairs<DP>(x, w[c]), l, o.cap, slope);
+                float d = fmaf(kz, p, -e);
+                if (y == j0 + c * lanes) d -= hit;
+                if (CAP) d *= slope;
 #pragma unroll
-                for (int k = 0; k < DP; ++k) dw[c].v[k] = __ffma2_rn(d, xv.v[k], dw[c].v[k]);
+                for (int k = 0; k < DP / 2; ++k)
+                    dw[c].v[k] = __ffma2_rn(f2(d), x.v[k], dw[c].v[k]);
             }
         }
     }
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < C; ++c) {
         float out[DP];
         __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DP; ++d)
-            red[threadIdx.x][d] = out[d] = dw[c].v[d].x + dw[c].v[d].y;
+        for (int d = 0; d < DP / 2; ++d) {
+            out[2 * d] = dw[c].v[d].x;
+            out[2 * d + 1] = dw[c].v[d].y;
+        }
+#pragma unroll
+        for (int d = 0; d < DP; ++d) red[threadIdx.x * (DP + 1) + d] = out[d];
         __syncthreads();
         const int j = j0 + c * lanes;
         if (slice == 0 && j < V) {
             for (int s = 1; s < slices; ++s)
 #pragma unroll
-                for (int d = 0; d < DP; ++d) out[d] += red[s * lanes + threadIdx.x][d];
+                for (int d = 0; d < DP; ++d)
+                    out[d] += red[(s * lanes + threadIdx.x) * (DP + 1) + d];
             store_row<float, DP, false>(acc + (long long)blockIdx.x * V * D, j, D, out);
         }
     }
 }
 
-long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-
-// blocks over the rows, each taking every gridDim.x-th tile of them: a
-// block stages its table once
-long long row_blocks(long long N, int D) {
-    return std::min(ceil_div(N, kBlockRows), (long long)per_sm(D <= 4 ? 4 : 8) * kSMs);
-}
-// classes split over blocks until these fill the device, 64 classes a part
-// at least
-int class_splits(long long N, int V, int D) {
-    return (int)std::max(
-        1LL, std::min({ceil_div(V, 64),
-                       (long long)per_sm(D <= 4 ? 4 : 8) * kSMs / row_blocks(N, D), 1024LL}));
-}
-
-struct DwShape {
-    int lanes, chunks, blocks;
-};
-DwShape dw_shape(long long N, int V, int D) {
-    DwShape s;
-    s.lanes = (int)std::min<long long>(ceil_div(V, 2), kNT);
-    s.chunks = (int)ceil_div(V, 2 * s.lanes);
-    s.blocks = (int)std::max(1LL, std::min(ceil_div(N, kTile), (long long)per_sm(D <= 4 ? 4 : 8) * kSMs / s.chunks));
-    return s;
-}
-
-template <typename T, typename F>
-cudaError_t by_form(const NarrowArgs &a, const void *grad, F f) {
-    const int dp = a.D <= 4 ? 4 : 8;
-    const uintptr_t mask = std::min<size_t>(16, dp * sizeof(T)) - 1;
-    const bool vec = a.D == dp && ((reinterpret_cast<uintptr_t>(a.features) |
-                                    reinterpret_cast<uintptr_t>(a.weight) |
-                                    reinterpret_cast<uintptr_t>(grad)) & mask) == 0;
-    std::integral_constant<int, 4> d4;
-    std::integral_constant<int, 8> d8;
-    std::true_type yes;
-    std::false_type no;
-    if (a.opt.cap > 0.f) {
-        if (vec) return dp == 4 ? f(d4, yes, yes) : f(d8, yes, yes);
-        return dp == 4 ? f(d4, yes, no) : f(d8, yes, no);
+template <typename F>
+cudaError_t by_width(int D, F f) {
+    switch (width_of(D)) {
+        case 4: return f(std::integral_constant<int, 4>{});
+        case 8: return f(std::integral_constant<int, 8>{});
+        case 16: return f(std::integral_constant<int, 16>{});
+        default: return f(std::integral_constant<int, 32>{});
     }
-    if (vec) return dp == 4 ? f(d4, no, yes) : f(d8, no, yes);
-    return dp == 4 ? f(d4, no, no) : f(d8, no, no);
+}
+template <typename F>
+cudaError_t by_form(int D, bool cap, bool vec, F f) {
+    return by_width(D, [&](auto dp) {
+        std::true_type yes;
+        std::false_type no;
+        if (cap) return vec ? f(dp, yes, yes) : f(dp, yes, no);
+        return vec ? f(dp, no, yes) : f(dp, no, no);
+    });
 }
 
 }  // namespace
 
-int narrow_class_splits(long long N, int V, int D) { return class_splits(N, V, D); }
-long long narrow_fwd_blocks(long long N, int D) { return row_blocks(N, D); }
-int narrow_dw_splits(long long N, int V, int D) { return dw_shape(N, V, D).blocks; }
+NarrowShape narrow_shape(long long N, int V, int D) {
+    NarrowShape s;
+    const int dp = width_of(D);
+    const long long blocks = (long long)per_sm(dp) * kSMs;
+    // blocks over the rows, each taking every gridDim.x-th tile of them: a
+    // block stages its table once
+    s.row_blocks = std::min(ceil_div(N, kNT * kRows), blocks);
+    // classes split over blocks until these fill the device, 64 a part at
+    // least
+    s.class_splits =
+        (int)std::max(1LL, std::min({ceil_div(V, 64), blocks / s.row_blocks, 1024LL}));
+    s.dw_lanes = (int)std::min<long long>(ceil_div(V, classes_of(dp)), kNT);
+    s.dw_chunks = (int)ceil_div(V, (long long)classes_of(dp) * s.dw_lanes);
+    s.dw_blocks =
+        (int)std::max(1LL, std::min(ceil_div(N, dw_rows_of(dp)), blocks / s.dw_chunks));
+    return s;
+}
 
 template <typename T>
 cudaError_t launch_narrow_fwd(const NarrowArgs &a, float *loss, float2 *sums, float2 *part,
                               float *psum, float *zt, cudaStream_t st) {
-    return by_form<T>(a, nullptr, [&](auto dp, auto cap, auto vec) {
-        const dim3 grid((unsigned)narrow_fwd_blocks(a.N, a.D), class_splits(a.N, a.V, a.D));
-        narrow_fwd_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value><<<grid, kNT, 0, st>>>(
-            a.N, a.V, a.D, static_cast<const T *>(a.features), static_cast<const T *>(a.weight),
-            a.labels, a.opt, loss, a.lse, a.count, sums, part, psum, zt);
+    return by_form(a.D, a.opt.cap > 0.f, a.wide_rows(sizeof(T), nullptr),
+                   [&](auto dp, auto cap, auto vec) {
+        const NarrowShape s = narrow_shape(a.N, a.V, a.D);
+        narrow_fwd_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value>
+            <<<dim3((unsigned)s.row_blocks, s.class_splits), kNT, 0, st>>>(
+                a.N, a.V, a.D, static_cast<const T *>(a.features),
+                static_cast<const T *>(a.weight), a.labels, a.opt, loss, a.lse, a.count, sums,
+                part, psum, zt);
         count_launches(1);
         return cudaGetLastError();
     });
@@ -625,11 +521,14 @@ cudaError_t launch_narrow_fwd(const NarrowArgs &a, float *loss, float2 *sums, fl
 template <typename T>
 cudaError_t launch_narrow_dx(const NarrowArgs &a, const CeUpstream &u, void *grad, float *acc,
                              cudaStream_t st) {
-    return by_form<T>(a, grad, [&](auto dp, auto cap, auto vec) {
-        const dim3 grid((unsigned)narrow_fwd_blocks(a.N, a.D), class_splits(a.N, a.V, a.D));
-        narrow_dx_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value><<<grid, kNT, 0, st>>>(
-            a.N, a.V, a.D, static_cast<const T *>(a.features), static_cast<const T *>(a.weight),
-            a.labels, a.opt, a.lse, u, static_cast<T *>(grad), acc);
+    return by_form(a.D, a.opt.cap > 0.f, a.wide_rows(sizeof(T), grad),
+                   [&](auto dp, auto cap, auto vec) {
+        const NarrowShape s = narrow_shape(a.N, a.V, a.D);
+        narrow_dx_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value>
+            <<<dim3((unsigned)s.row_blocks, s.class_splits), kNT, 0, st>>>(
+                a.N, a.V, a.D, static_cast<const T *>(a.features),
+                static_cast<const T *>(a.weight), a.labels, a.opt, a.lse, u,
+                static_cast<T *>(grad), acc);
         count_launches(1);
         return cudaGetLastError();
     });
@@ -638,11 +537,12 @@ cudaError_t launch_narrow_dx(const NarrowArgs &a, const CeUpstream &u, void *gra
 template <typename T>
 cudaError_t launch_narrow_dw(const NarrowArgs &a, const CeUpstream &u, float *acc,
                              cudaStream_t st) {
-    return by_form<T>(a, nullptr, [&](auto dp, auto cap, auto vec) {
-        const DwShape s = dw_shape(a.N, a.V, a.D);
+    return by_form(a.D, a.opt.cap > 0.f, a.wide_rows(sizeof(T), nullptr),
+                   [&](auto dp, auto cap, auto vec) {
+        const NarrowShape s = narrow_shape(a.N, a.V, a.D);
         narrow_dw_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value>
-            <<<dim3(s.blocks, s.chunks), kNT, 0, st>>>(
-                a.N, a.V, a.D, s.lanes, static_cast<const T *>(a.features),
+            <<<dim3(s.dw_blocks, s.dw_chunks), kNT, 0, st>>>(
+                a.N, a.V, a.D, s.dw_lanes, static_cast<const T *>(a.features),
                 static_cast<const T *>(a.weight), a.labels, a.opt, a.lse, u, acc);
         count_launches(1);
         return cudaGetLastError();
