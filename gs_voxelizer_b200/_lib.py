@@ -124,7 +124,7 @@ SIGNATURES = {
         ctypes.c_int, [_I64, _I32, _I32, _P, _P, _OPT, _P, _P, _P, _P, _SZ, _P]),
     "gsv_softmax_ce_backward": (
         ctypes.c_int, [_I64, _I32, _I32, _P, _P, _OPT, _P, _P, _P, _P, _P]),
-    "gsv_linear_ce_state_bytes": (_SZ, [_I64]),
+    "gsv_linear_ce_state_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
     "gsv_linear_ce_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _OPT, _I32]),
     "gsv_linear_ce_forward": (
         ctypes.c_int, [_I64, _I32, _I32, _I32, _P, _P, _P, _OPT, _P, _P, _P, _SZ,

@@ -140,7 +140,7 @@ cudaError_t launch_softmax_ce(bool fwd, int type, long long rows, int V, const v
                               const long long *labels, const CeOpt &o, float *loss,
                               float2 *lse, float *count, const float *grad_loss, void *grad,
                               void *ws, cudaStream_t st);
-size_t linear_ce_state_bytes(long long rows);
+size_t linear_ce_state_bytes(long long N, int V, int D, int type);
 size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
                                  const CeOpt &o);
 cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
@@ -1150,9 +1150,11 @@ int gsv_softmax_ce_backward(int64_t rows, int32_t classes, int32_t dtype, const 
                        fn);
 }
 
-size_t gsv_linear_ce_state_bytes(int64_t rows) {
-    if (rows < 1 || rows >= INT32_MAX - 1024) return 0;
-    return gsv::linear_ce_state_bytes(rows);
+size_t gsv_linear_ce_state_bytes(int64_t rows, int32_t classes, int32_t channels,
+                                 int32_t dtype) {
+    const gsv_ce_options any = {-1, 0.f, 0.f, 0.f, GSV_REDUCE_SUM};
+    if (check_ce("gsv_linear_ce_state_bytes", rows, classes, channels, dtype, &any)) return 0;
+    return gsv::linear_ce_state_bytes(rows, classes, channels, dtype);
 }
 
 size_t gsv_linear_ce_workspace_bytes(int64_t rows, int32_t classes, int32_t channels,

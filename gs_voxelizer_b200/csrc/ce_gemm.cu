@@ -18,6 +18,8 @@
 // the kernel ends, its tensor memory freed; the result is invalid.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "ce_gemm.cuh"
 
 namespace gsv {
@@ -723,9 +725,17 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
         !make_map(&b, mb, g.planes, g.bf16, kBMn ? 64 : nt / 2))
         return cudaErrorInvalidValue;
     auto kernel = ce_gemm_kernel<PRODUCT, CAP, F32>;
-    const cudaError_t err =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    // once a device (a repeated call is harmless)
+    static std::atomic<unsigned long long> ready{0};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
+    if (!(ready.load() >> (dev & 63) & 1)) {
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   kSmemBytes);
+        if (err != cudaSuccess) return err;
+        ready.fetch_or(1ull << (dev & 63));
+    }
     const long long M = PRODUCT == kCeGradW ? g.nv : g.rows;
     const long long mt = (M + kCeTileM - 1) / kCeTileM;
     const long long n = (PRODUCT <= kCeProbs ? g.nv : g.D);

@@ -372,6 +372,7 @@ struct Plan {
     int V, D, type, planes;
     long long ld;         // of packed features / table
     bool pack_w;          // the table cannot be read in place
+    bool keep_x, keep_w;  // packed in the state, not in the workspace
     int runs;             // runs of class tiles in the forward
     // backward: pieces and splits
     long long piece_rows, ldp;
@@ -383,18 +384,28 @@ struct Plan {
     size_t xp, wp, part, psum, zt, sums, gmax, p, dx, dw, bytes;
 };
 
-// state (kept between the two directions): count (float, padded to 4 words),
-// lse [N] (two floats; of packed rows but on the narrow path), packed total (int, padded to 4 words), idx [Np], lab [Np],
-// block counts
+// State (kept between the two directions): count (float, padded to 4 words),
+// lse [N] (two floats; of packed rows but on the narrow path), packed total
+// (int, padded to 4 words), idx [Np], lab [Np], block counts; then the packed
+// features and the packed table where they are small: their kernels' launches
+// cost more than their memory, and the backward need not repeat them.
 struct State {
     float *count;
     float2 *lse;
     int *total, *idx, *lab, *counts;
+    unsigned char *packed;
 };
+
+constexpr size_t kKeepBytes = (size_t)16 << 20;
+
+size_t packed_bytes(long long rows, int D, int type) {
+    return (size_t)(type == kCeF32 ? 3 : 1) * rows * up(D, 8) * 2;
+}
+bool kept(size_t bytes) { return bytes <= kKeepBytes; }
 
 long long state_words(long long N) {
     const long long Np = up(N, kCeTileM);
-    return 4 + up(2 * N, 4) + 4 + 2 * Np + up((N + kIdxNT - 1) / kIdxNT, 4);
+    return up(4 + up(2 * N, 4) + 4 + 2 * Np + up((N + kIdxNT - 1) / kIdxNT, 4), 64);
 }
 
 State state_of(void *p, long long N) {
@@ -407,6 +418,7 @@ State state_of(void *p, long long N) {
     s.idx = s.total + 4;
     s.lab = s.idx + Np;
     s.counts = s.lab + Np;
+    s.packed = reinterpret_cast<unsigned char *>(f + state_words(N));
     return s;
 }
 
@@ -448,8 +460,12 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
         return o;
     };
     p.sums = take(sizeof(float2) * (size_t)(N / 32 + 1));
-    p.xp = take((size_t)p.planes * p.Np * p.ld * 2);
-    p.wp = take(p.pack_w ? (size_t)p.planes * V * p.ld * 2 : 0);
+    // packed operands: in the state where they are kept
+    const size_t xb = packed_bytes(p.Np, D, type), wb = packed_bytes(V, D, type);
+    p.keep_x = kept(xb);
+    p.keep_w = kept(wb);
+    p.xp = p.keep_x ? 0 : take(xb);
+    p.wp = p.keep_w ? (p.keep_x ? align256(xb) : 0) : take(p.pack_w ? wb : 0);
     if (!backward) {
         p.part = take(sizeof(float2) * 2 * (size_t)p.runs * p.Np);
         p.psum = take(o.eps > 0.f ? sizeof(float) * 2 * (size_t)p.runs * p.Np : 0);
@@ -547,6 +563,13 @@ cudaError_t finish_any(const Plan &p, bool rows, long long row0, long long n,
         if (err_ != cudaSuccess) return err_;         \
     } while (0)
 
+unsigned char *x_of(const Plan &p, const State &s, unsigned char *ws) {
+    return (p.keep_x ? s.packed : ws) + p.xp;
+}
+unsigned char *w_of(const Plan &p, const State &s, unsigned char *ws) {
+    return (p.keep_w ? s.packed : ws) + p.wp;
+}
+
 CeGemm gemm_of(const Plan &p, const State &s, const void *weight, unsigned char *ws,
                const CeOpt &o) {
     CeGemm g{};
@@ -556,8 +579,8 @@ CeGemm gemm_of(const Plan &p, const State &s, const void *weight, unsigned char 
     g.D = p.D;
     g.opt = o;
     g.splits = 1;
-    g.X = {ws + p.xp, p.Np, p.D, p.ld, p.Np * p.ld};
-    g.W = p.pack_w ? CeMat{ws + p.wp, p.V, p.D, p.ld, p.V * p.ld}
+    g.X = {x_of(p, s, ws), p.Np, p.D, p.ld, p.Np * p.ld};
+    g.W = p.pack_w ? CeMat{w_of(p, s, ws), p.V, p.D, p.ld, p.V * p.ld}
                    : CeMat{weight, p.V, p.D, p.D, 0};
     g.count = s.total;
     g.lab = s.lab;
@@ -567,7 +590,6 @@ CeGemm gemm_of(const Plan &p, const State &s, const void *weight, unsigned char 
 
 }  // namespace
 
-size_t linear_ce_state_bytes(long long rows) { return (size_t)state_words(rows) * 4; }
 
 namespace {
 
@@ -691,11 +713,20 @@ bool in_place(long long N, int V, int D, int type, const void *features) {
 
 }  // namespace
 
+size_t linear_ce_state_bytes(long long N, int V, int D, int type) {
+    size_t b = (size_t)state_words(N) * 4;
+    if (path_of(N, V, D, type) == kNarrow) return b;
+    const size_t xb = packed_bytes(up(N, kCeTileM), D, type), wb = packed_bytes(V, D, type);
+    if (kept(xb)) b += align256(xb);
+    if (kept(wb)) b += align256(wb);
+    return b;
+}
+
 size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
                                  const CeOpt &o) {
     // a forward without a state keeps its statistics (and, of tiles, the
     // packed rows' index) here
-    const size_t own = backward ? 0 : align256(linear_ce_state_bytes(N));
+    const size_t own = backward ? 0 : align256(linear_ce_state_bytes(N, V, D, type));
     const Path path = path_of(N, V, D, type);
     switch (backward && path == kFew ? kTiles : path) {
         case kNarrow: return own + narrow_plan(N, V, D, backward, o).bytes;
@@ -711,7 +742,7 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     const bool forward_only = state == nullptr;
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const State s = state_of(forward_only ? ws : state, N);
-    ws += align256(linear_ce_state_bytes(N));
+    ws += align256(linear_ce_state_bytes(N, V, D, type));
     const Path path = path_of(N, V, D, type);
     if (path == kNarrow) {
         const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
@@ -741,8 +772,8 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     // merged by packed rows, which leaves out those without a label
     if (o.reduction == kCeNone && !(direct && forward_only))
         GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
-    if (!direct) GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
-    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, ws + p.wp, st));
+    if (!direct) GSV_CE_TRY(pack_any(p, true, features, s, x_of(p, s, ws), st));
+    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, w_of(p, s, ws), st));
     CeGemm g = gemm_of(p, s, weight, ws, o);
     g.product = kCeScores;
     g.rows = p.Np;
@@ -789,8 +820,12 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
     const Plan p = make_plan(N, V, D, type, weight, true, o);
     float *gmax = type == kCeF16 ? reinterpret_cast<float *>(ws + p.gmax) : nullptr;
     const bool none = o.reduction == kCeNone;
-    GSV_CE_TRY(pack_any(p, true, features, s, ws + p.xp, st));
-    if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, ws + p.wp, st));
+    // what the forward packed and kept is there (kFew packed nothing)
+    const bool tiled = path_of(N, V, D, type) == kTiles;
+    if (!(tiled && p.keep_x && !in_place(N, V, D, type, features)))
+        GSV_CE_TRY(pack_any(p, true, features, s, x_of(p, s, ws), st));
+    if (p.pack_w && !(tiled && p.keep_w))
+        GSV_CE_TRY(pack_any(p, false, weight, s, w_of(p, s, ws), st));
     if (none && gmax) {
         GSV_CE_TRY(cudaMemsetAsync(gmax, 0, sizeof(float), st));
         const int nb = (int)std::min<long long>(kSMs, (N + 1023) / 1024);

@@ -433,7 +433,8 @@ def _linear_ce(features, weight, labels, opt, with_state):
     dtype = _CE_DTYPES[features.dtype]
     state = None
     if with_state:
-        state = _C._workspace(lib.gsv_linear_ce_state_bytes(rows), dev)
+        state = _C._workspace(
+            lib.gsv_linear_ce_state_bytes(rows, V, D, dtype), dev)
     ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
         rows, V, D, dtype, opt, 0), dev)
     _ce_call(lib.gsv_linear_ce_forward, dev, rows, V, D, dtype,
@@ -492,11 +493,11 @@ def linear_cross_entropy(
     embeddings, or the hidden states of a model against a vocabulary.
 
     The scores are products of the inputs summed in float32 and are not
-    rounded to the inputs' type. The forward keeps 16 bytes a row; the
-    backward computes the scores again in pieces, with a workspace of a few
-    hundred MB beside float32 copies of what it accumulates. With
-    ``reduction="none"`` and no gradient it is minus the log-probability of
-    each row's label.
+    rounded to the inputs' type. The forward keeps 16 bytes a row and, up to
+    16 MB each, its packed operands; the backward computes the scores again in
+    pieces, with a workspace of a few hundred MB beside float32 copies of what
+    it accumulates. With ``reduction="none"`` and no gradient it is minus the
+    log-probability of each row's label.
 
     Args:
         features: [..., D] float32, bfloat16 or float16.

@@ -550,7 +550,8 @@ GSV_API int gsv_softmax_ce_backward(int64_t rows, int32_t classes, int32_t dtype
                                     const float *count, const float *grad_loss,
                                     void *grad_scores, void *stream);
 
-GSV_API size_t gsv_linear_ce_state_bytes(int64_t rows);
+GSV_API size_t gsv_linear_ce_state_bytes(int64_t rows, int32_t classes,
+                                         int32_t channels, int32_t dtype);
 GSV_API size_t gsv_linear_ce_workspace_bytes(int64_t rows, int32_t classes,
                                              int32_t channels, int32_t dtype,
                                              const gsv_ce_options *options,

@@ -67,8 +67,13 @@ def test_workspace_queries():
     assert lib.gsv_softmax_ce_workspace_bytes(0, 5) == 0
     assert lib.gsv_softmax_ce_workspace_bytes(1000, 4) >= 8 * 4
     assert lib.gsv_softmax_ce_workspace_bytes(1000, 5000) >= 8 * 1000
-    assert lib.gsv_linear_ce_state_bytes(0) == 0
-    assert lib.gsv_linear_ce_state_bytes(1000) >= 4 * 1000
+    assert lib.gsv_linear_ce_state_bytes(0, 10, 10, 0) == 0
+    assert lib.gsv_linear_ce_state_bytes(1000, 10, 10, 3) == 0
+    assert lib.gsv_linear_ce_state_bytes(1000, 10, 4, 0) >= 8 * 1000
+    # the packed operands are kept up to 16 MB each
+    small = lib.gsv_linear_ce_state_bytes(8192, 1024, 64, 1)
+    assert small >= 2 * 64 * (8192 + 1024)
+    assert lib.gsv_linear_ce_state_bytes(8192, 131072, 4096, 1) < 32 * 8192
     assert lib.gsv_linear_ce_workspace_bytes(10, 0, 4, 1, options(), 0) == 0
     # far below the scores: a long batch over a large vocabulary
     n, V, D = 65536, 131072, 1024
