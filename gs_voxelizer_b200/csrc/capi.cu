@@ -1083,7 +1083,7 @@ int check_ce(const char *fn, int64_t rows, int32_t classes, int32_t channels, in
     GSV_REQUIRE(o, GSV_ERR_INVALID_ARGUMENT, "%s: options are null", fn);
     GSV_REQUIRE(rows >= 1 && classes >= 1 && channels >= 1, GSV_ERR_INVALID_ARGUMENT,
                 "%s: rows, classes and channels must be positive", fn);
-    GSV_REQUIRE(rows < INT32_MAX - 1024 && classes <= (1 << 30) && channels <= (1 << 20),
+    GSV_REQUIRE(rows < INT32_MAX - 1024 && classes <= (1 << 24) && channels <= (1 << 20),
                 GSV_ERR_SIZE_OVERFLOW, "%s: sizes beyond the 32-bit index formats", fn);
     GSV_REQUIRE(dtype >= GSV_F32 && dtype <= GSV_F16, GSV_ERR_INVALID_ARGUMENT,
                 "%s: unknown dtype %d", fn, dtype);

@@ -41,16 +41,19 @@ __device__ __forceinline__ int ce_label(long long y, long long ignore, int V) {
 __device__ __forceinline__ float ce_nan() { return __int_as_float(0x7fc00000); }
 __device__ __forceinline__ float ce_neg_inf() { return __int_as_float(0xff800000); }
 
-// tanh(s / cap). FAST: 1 - 2 / (1 + e^2x) on the special-function unit, off by
-// at most 2^-22 absolutely - scores enter through differences, so this is
-// what counts - against tanhf's correct digits for float32 inputs.
+// tanh(s / cap). FAST (16-bit inputs): 1 - 2 / (1 + e^2x) on the
+// special-function unit, off by at most 2^-22, and below 0.1, where that would
+// be too much of a large cap's scores, the series to x^5 (off by 2^-24 x);
+// float32 inputs take tanhf.
 template <bool FAST>
 __device__ __forceinline__ float ce_tanh(float s, float cap) {
     if (!FAST) return tanhf(s / cap);
-    const float u = ex2(fabsf(s) * __fdividef(2.f * kLog2e, cap));
+    const float x = __fdividef(s, cap), x2 = x * x;
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + u));
-    return copysignf(fmaf(-2.f, r, 1.f), s);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(fabsf(x) * (2.f * kLog2e))));
+    const float far = copysignf(fmaf(-2.f, r, 1.f), x);
+    const float near = x * fmaf(x2, fmaf(x2, 2.f / 15.f, -1.f / 3.f), 1.f);
+    return fabsf(x) < 0.1f ? near : far;
 }
 
 // the capped score, and the slope dz / ds that goes with it

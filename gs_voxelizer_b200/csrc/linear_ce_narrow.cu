@@ -35,7 +35,7 @@ constexpr int dw_rows_of(int dp) { return dp <= 8 ? 256 : 128; }
 constexpr int chunk_of(int dp) { return 4096 / dp; }  // classes staged at once
 constexpr int kRows = 2;                              // rows a thread
 // classes a thread (dW): the registers hold 2 DP each
-constexpr int classes_of(int dp) { return dp == 4 ? 4 : dp == 32 ? 1 : 2; }
+constexpr int classes_of(int dp) { return dp == 4 ? 4 : 2; }
 // blocks an SM, as many as registers hold without spills
 constexpr int per_sm(int dp) { return dp <= 8 ? 3 : dp == 16 ? 2 : 1; }
 constexpr int width_of(int D) { return D <= 4 ? 4 : D <= 8 ? 8 : D <= 16 ? 16 : 32; }
@@ -289,7 +289,7 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
                 __syncthreads();
                 staged = span.v1 - span.v0 <= kChunk;
             }
-#pragma unroll(DP == 4 ? 2 : 1)
+#pragma unroll 2
             for (int j = 0; j < n; ++j) {
                 const Pairs<DP> w = sw[j];
 #pragma unroll
@@ -416,6 +416,7 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
         }
         __syncthreads();
         if (!active) continue;
+#pragma unroll(DP == 8 || DP == 32 ? 2 : 1)
         for (int i = slice; i < kDwRows; i += slices) {
             const Pairs<DP> x = rows[i].x;
             const float2 l = rows[i].lse;

@@ -495,8 +495,8 @@ def linear_cross_entropy(
     The scores are products of the inputs summed in float32 and are not
     rounded to the inputs' type. The forward keeps 16 bytes a row and, up to
     16 MB each, its packed operands; the backward computes the scores again in
-    pieces, with a workspace of a few hundred MB beside float32 copies of what
-    it accumulates. With ``reduction="none"`` and no gradient it is minus the
+    pieces, with a workspace of a few hundred MB beside packed copies of the
+    operands and float32 copies of what it accumulates over several pieces. With ``reduction="none"`` and no gradient it is minus the
     log-probability of each row's label.
 
     Args:

@@ -517,7 +517,7 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
  * loss float32 ([1], or [rows] with GSV_REDUCE_NONE), grad_loss float32 of
  * the same size. Arithmetic is float32 or wider; the products of 16-bit
  * types are exact and summed in float32, those of float32 are taken with all
- * their bits. 1 <= rows < 2^31 - 1024, 1 <= classes <= 2^30, 1 <= channels <=
+ * their bits. 1 <= rows < 2^31 - 1024, 1 <= classes <= 2^24, 1 <= channels <=
  * 2^20.
  *
  * The forward leaves what the backward needs in `lse` / `count` (device

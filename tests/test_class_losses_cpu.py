@@ -44,7 +44,7 @@ def test_c_entries_refuse_bad_arguments():
         assert fn(rows=0) == 1 and b"positive" in lib.gsv_last_error()
         assert fn(V=0) == 1
         assert fn(rows=2 ** 31) == 4
-        assert fn(V=2 ** 30 + 1) == 4
+        assert fn(V=2 ** 24 + 1) == 4
         assert fn(dtype=3) == 1 and fn(dtype=-1) == 1
         assert fn(opt=None) == 1
         for bad in (options(smoothing=1.0), options(smoothing=-0.5), options(cap=-1.0),

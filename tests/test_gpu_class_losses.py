@@ -505,3 +505,102 @@ def test_loss_without_gradient_unaligned():
             views.append(f[1:].view(t.shape))
         loss = linear_cross_entropy(*views, labels)
         check(data, labels, {}, None, loss, [])
+
+
+@pytest.mark.parametrize("D", [0, 4, 24, 64])
+@pytest.mark.parametrize("ignore", [0, 7, 255, 10 ** 12])
+def test_ignore_index(D, ignore):
+    """Any value may mark unlabelled rows, a class's own number and an 8-bit
+    label's 255 too."""
+    from gs_voxelizer_b200 import losses
+    data, labels = make(300, 12, D, F32, 41)
+    labels[::3] = ignore
+    given = labels.to(torch.uint8) if ignore == 255 else labels
+    fn = losses.linear_cross_entropy if D else losses.softmax_cross_entropy
+    leaves = [t.requires_grad_(True) for t in data]
+    loss = fn(*leaves, given, ignore_index=ignore)
+    grads = torch.autograd.grad(loss, leaves)
+    marked = torch.where(labels == ignore, -100, labels)
+    check([t.detach() for t in data], marked, {}, torch.ones((), device="cuda"),
+          loss.detach(), grads)
+
+
+@pytest.mark.parametrize("D", [0, 4, 64])
+def test_sum_of_row_losses_and_single_rows(D):
+    """An expanded upstream gradient, twice through a kept graph; and a row
+    without leading dimensions."""
+    from gs_voxelizer_b200 import losses
+    data, labels = make(200, 30, D, F32, 42, ignored=0.2, garbage=False)
+    fn = losses.linear_cross_entropy if D else losses.softmax_cross_entropy
+    leaves = [t.requires_grad_(True) for t in data]
+    rows = fn(*leaves, labels, reduction="none")
+    one = torch.autograd.grad(rows.sum(), leaves, retain_graph=True)
+    two = torch.autograd.grad(rows.sum(), leaves)
+    for a, b in zip(one, two):
+        assert torch.equal(a, b)
+    check([t.detach() for t in data], labels, dict(reduction="none"),
+          torch.ones(200, device="cuda"), rows.detach(), one)
+    first = [data[0][0].detach().requires_grad_(True), *data[1:]]
+    label = labels[0].clamp_min(0)
+    loss = fn(*first, label)
+    assert loss.shape == ()
+    grads = torch.autograd.grad(loss, first)
+    check([data[0][:1].detach(), *(t.detach() for t in data[1:])], label.view(1), {},
+          torch.ones((), device="cuda"), loss.detach(),
+          [grads[0].view(1, -1), *grads[1:]])
+
+
+@pytest.mark.parametrize("cap", [0.5, 30.0, 1e4, 1e8])
+@pytest.mark.parametrize("D", [0, 4, 64])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_softcap_of_any_size(cap, D, dtype):
+    """A cap far above the scores leaves them as they are (to 2^-22 of a
+    score above a tenth of the cap, 2^-22 of itself below)."""
+    data, labels = make(150, 40, D, dtype, 43)
+    up = torch.tensor(1.0, device="cuda")
+    loss, grads = call(data, labels, dict(softcap=cap), up)
+    # check()'s bound takes 2^-21 of the cap, which says nothing of large ones;
+    # scores below 32 differ from capped ones by s^3 / (3 cap^2) < 2e-4 at 1e4
+    check(data, labels, dict(softcap=cap) if cap < 1e4 else {}, up, loss, grads)
+
+
+def test_no_barrier_timed_out():
+    import ctypes
+    from gs_voxelizer_b200._lib import check as ok
+    from gs_voxelizer_b200._lib import lib
+    flag = ctypes.c_int32(-1)
+    ok(lib.gsv_device_error(ctypes.byref(flag), 0))
+    assert flag.value == 0
+
+
+def test_first_call_of_a_process_in_a_capture():
+    """Nothing needs a call outside the capture first."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from gs_voxelizer_b200.losses import linear_cross_entropy, softmax_cross_entropy
+for D in (0, 4, 64):
+    g = torch.Generator("cuda").manual_seed(1)
+    y = torch.randint(0, 30, (400,), generator=g, device="cuda")
+    x = torch.randn(400, D or 30, generator=g, device="cuda").bfloat16()
+    w = torch.randn(30, D, generator=g, device="cuda").bfloat16()
+    args = [t.requires_grad_(True) for t in ((x, w) if D else (x,))]
+    fn = linear_cross_entropy if D else softmax_cross_entropy
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = fn(*args, y)
+        grads = torch.autograd.grad(loss, args)
+    graph.replay()
+    torch.cuda.synchronize()
+    again = fn(*args, y)
+    assert torch.equal(loss, again), (loss, again)
+    for a, b in zip(grads, torch.autograd.grad(again, args)):
+        assert torch.equal(a, b)
+print("replayed")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                         timeout=300)
+    assert out.returncode == 0 and "replayed" in out.stdout, out.stderr[-2000:]
