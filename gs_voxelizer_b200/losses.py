@@ -25,7 +25,6 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import cuda as _C
 from ._lib import CeOptions, check, i3, lib
@@ -342,6 +341,20 @@ def _ce_call(fn, dev, *args):
         check(status)
 
 
+class _Once(Function):
+    """The identity on a gradient, whose own backward is refused: the class
+    losses are differentiable once. Only entered under create_graph (a
+    decorator that marks every backward costs each call a tenth)."""
+
+    @staticmethod
+    def forward(ctx, grad, *inputs):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the class losses are differentiable once")
+
+
 def _softmax_ce(scores, labels, opt):
     """(loss, stats): per row (maximum, log2 of the sum), then the number of
     labelled rows, then the call's workspace."""
@@ -370,7 +383,6 @@ class _SoftmaxCe(Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_loss):
         saved = ctx.saved_tensors
         if len(saved) == 1:
@@ -383,6 +395,8 @@ class _SoftmaxCe(Function):
         _ce_call(lib.gsv_softmax_ce_backward, dev, rows, V,
                  _CE_DTYPES[scores.dtype], scores.data_ptr(), labels.data_ptr(),
                  ctx.opt, p, p + 8 * rows, grad_loss.data_ptr(), g.data_ptr())
+        if torch.is_grad_enabled():
+            g = _Once.apply(g, scores, grad_loss)
         return g, None, None
 
 
@@ -455,7 +469,6 @@ class _LinearCe(Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_loss):
         need_x, need_w = ctx.needs_input_grad[:2]
         saved = ctx.saved_tensors
@@ -475,6 +488,9 @@ class _LinearCe(Function):
                  features.data_ptr(), weight.data_ptr(), labels.data_ptr(),
                  ctx.opt, state.data_ptr(), grad_loss.data_ptr(), _C._ptr(gx),
                  _C._ptr(gw), ws.data_ptr(), ws.numel())
+        if torch.is_grad_enabled():
+            gx, gw = (g if g is None else _Once.apply(g, features, weight, grad_loss)
+                      for g in (gx, gw))
         return gx, gw, None, None
 
 

@@ -430,10 +430,14 @@ def test_refusals():
             softmax_cross_entropy(s, y, **bad)
         with pytest.raises(ValueError):
             linear_cross_entropy(x, w, y, **bad)
-    s.requires_grad_(True)
-    (g,) = torch.autograd.grad(softmax_cross_entropy(s, y), s, create_graph=True)
-    with pytest.raises(RuntimeError):  # differentiable once
-        torch.autograd.grad(g.sum(), s)
+    for fn, leaves in ((softmax_cross_entropy, [s]), (linear_cross_entropy, [x, w])):
+        leaves = [t.clone().requires_grad_(True) for t in leaves]
+        plain = torch.autograd.grad(fn(*leaves, y), leaves)
+        kept = torch.autograd.grad(fn(*leaves, y), leaves, create_graph=True)
+        for a, b in zip(plain, kept):
+            assert torch.equal(a, b)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(kept[-1].sum(), leaves)
 
 
 @pytest.mark.parametrize("decode", [False, True])
@@ -469,7 +473,7 @@ def test_voxelize_then_class_loss(decode):
             loss = torch.nn.functional.cross_entropy(s.view(-1, V), labels.view(-1))
         results.append((loss.detach(), torch.autograd.grad(loss, leaves)))
     (a, ga), (b, gb) = results
-    assert float(a) == pytest.approx(float(b), rel=1e-5)
+    assert float(a) == pytest.approx(float(b.detach()), rel=1e-5)
     for x, y in zip(ga, gb):
         tol = 1e-4 * y.abs() + 1e-4 * y.abs().max()
         assert ((x - y).abs() <= tol).all()
