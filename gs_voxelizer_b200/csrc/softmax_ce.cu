@@ -10,6 +10,8 @@
 //    again, which costs less than the 16 bytes a row of keeping them;
 //  * longer rows: one block a row, 16-byte accesses from the first aligned
 //    element on, the running maximum and sum kept per thread and merged.
+#include <type_traits>
+
 #include "ce.cuh"
 
 namespace gsv {
@@ -310,40 +312,92 @@ __device__ __forceinline__ int head_of(const T *p, int V) {
     return mis ? min(V, (16 - mis) / (int)sizeof(T)) : 0;
 }
 
+// Eight (16 bits) or four scores of a 16-byte word, in pairs for the paired
+// FP32 instructions, before the cap.
+__device__ __forceinline__ void pairs_of(const Vec16<float> &q, float2 (&s)[2]) {
+    s[0] = make_float2(q.v[0], q.v[1]);
+    s[1] = make_float2(q.v[2], q.v[3]);
+}
+__device__ __forceinline__ void pairs_of(const Vec16<__nv_bfloat16> &q, float2 (&s)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        s[k] = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 *>(q.v)[k]);
+}
+__device__ __forceinline__ void pairs_of(const Vec16<__half> &q, float2 (&s)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] = __half22float2(reinterpret_cast<const __half2 *>(q.v)[k]);
+}
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kNT)
 row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict__ labels,
                CeOpt o, float *__restrict__ loss, float2 *__restrict__ lse_out,
                float *__restrict__ count, float2 *__restrict__ partials) {
-    constexpr int kN = Vec16<T>::kN;
+    constexpr int kN = Vec16<T>::kN, kP = kN / 2;
     const long long row = blockIdx.x;
     const T *p = scores + row * (long long)V;
-    const int head = head_of(p, V), nv = (V - head) / kN;
-    CeAcc a;
-    a.init();
+    const int y = ce_label(labels[row], o.ignore, V);
+    if (y == kCeIgnored) {  // nothing of the row is read, here or backward
+        if (threadIdx.x) return;
+        if (o.reduction == kCeNone) loss[row] = 0.f;
+        if (gridDim.x == 1)
+            ce_finish(0.0, 0.0, o.reduction, loss, count);
+        else
+            partials[row] = make_float2(0.f, 0.f);
+        return;
+    }
     auto score = [&](T v) {
         const float s = ce_to_float(v);
         return CAP ? o.cap * ce_tanh<sizeof(T) == 2>(s, o.cap) : s;
     };
+    const float zy = y >= 0 ? score(p[y]) : 0.f;
+    const int head = head_of(p, V), nv = (V - head) / kN;
+    const bool smooth = o.eps > 0.f;
+    CeAcc a;
+    a.init();
     auto one = [&](T v) {
         const float z = score(v);
         a.merge(z, 1.f, z);
     };
-    for (int i = threadIdx.x; i < nv; i += kNT) {
-        const Vec16<T> q = reinterpret_cast<const Vec16<T> *>(p + head)[i];
-        float z[kN], m = a.m;
+    float2 s2 = f2(0.f), sz2 = f2(0.f);
+    // two words at a time, both loads in flight
+    auto absorb = [&](const Vec16<T> *q, auto words) {
+        constexpr int kW = decltype(words)::value;
+        float2 z[kW][kP];
+        float m = a.m;
 #pragma unroll
-        for (int k = 0; k < kN; ++k) {
-            z[k] = score(q.v[k]);
-            m = fmaxf(m, z[k]);
-            a.sz += z[k];
+        for (int w = 0; w < kW; ++w) {
+            pairs_of(q[w], z[w]);
+#pragma unroll
+            for (int k = 0; k < kP; ++k) {
+                if (CAP)
+                    z[w][k] = make_float2(o.cap * ce_tanh<sizeof(T) == 2>(z[w][k].x, o.cap),
+                                          o.cap * ce_tanh<sizeof(T) == 2>(z[w][k].y, o.cap));
+                m = fmaxf(m, fmaxf(z[w][k].x, z[w][k].y));
+                if (smooth) sz2 = __fadd2_rn(sz2, z[w][k]);
+            }
         }
         const float b = CeAcc::base(m);
-        a.s *= ex2((a.m - b) * kLog2e);
+        s2 = __fmul2_rn(s2, f2(ex2((a.m - b) * kLog2e)));
         a.m = m;
 #pragma unroll
-        for (int k = 0; k < kN; ++k) a.s += ex2((z[k] - b) * kLog2e);
+        for (int w = 0; w < kW; ++w)
+#pragma unroll
+            for (int k = 0; k < kP; ++k) {
+                const float2 d = __fmul2_rn(__fadd2_rn(z[w][k], f2(-b)), f2(kLog2e));
+                s2 = __fadd2_rn(s2, make_float2(ex2(d.x), ex2(d.y)));
+            }
+    };
+    const Vec16<T> *words = reinterpret_cast<const Vec16<T> *>(p + head);
+    int i = threadIdx.x;
+    for (; i + kNT < nv; i += 2 * kNT) {
+        const Vec16<T> q[2] = {words[i], words[i + kNT]};
+        absorb(q, std::integral_constant<int, 2>{});
     }
+    if (i < nv) absorb(words + i, std::integral_constant<int, 1>{});
+    a.s = s2.x + s2.y;
+    a.sz = sz2.x + sz2.y;
     if ((int)threadIdx.x < head) one(p[threadIdx.x]);
     const int tail = head + nv * kN + (int)threadIdx.x;
     if (tail < V) one(p[tail]);
@@ -360,20 +414,18 @@ row_fwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict_
     __syncthreads();
     if (threadIdx.x) return;
     for (int w = 1; w < kNT / 32; ++w) a.merge(sm[w], ss[w], sz[w]);
-    const int y = ce_label(labels[row], o.ignore, V);
     float2 lse = a.lse();
-    float l = 0.f;
+    float l;
     if (y >= 0)
-        l = ce_row_loss(lse, score(p[y]), a.sz, V, o);
-    else if (y == kCeInvalid)
+        l = ce_row_loss(lse, zy, a.sz, V, o);
+    else
         l = lse.x = ce_nan();
     lse_out[row] = lse;
     if (o.reduction == kCeNone) loss[row] = l;
-    const float c = y == kCeIgnored ? 0.f : 1.f;
     if (gridDim.x == 1)
-        ce_finish(l, c, o.reduction, loss, count);
+        ce_finish(l, 1.0, o.reduction, loss, count);
     else
-        partials[row] = make_float2(l, c);
+        partials[row] = make_float2(l, 1.f);
 }
 
 template <typename T, bool CAP>
@@ -381,37 +433,54 @@ __global__ void __launch_bounds__(kNT)
 row_bwd_kernel(int V, const T *__restrict__ scores, const long long *__restrict__ labels,
                CeOpt o, const float2 *__restrict__ lse_in, const float *__restrict__ count,
                const float *__restrict__ grad_loss, T *__restrict__ grad, bool same_head) {
-    constexpr int kN = Vec16<T>::kN;
+    constexpr int kN = Vec16<T>::kN, kP = kN / 2;
     const long long row = blockIdx.x;
     const T *p = scores + row * (long long)V;
     T *out = grad + row * (long long)V;
     const int head = same_head ? head_of(p, V) : V;
-    const int nv = (V - head) / kN;
+    const int nv = (V - head) / kN, rest = head + nv * kN;
     const int y = ce_label(labels[row], o.ignore, V);
+    int4 *o16 = reinterpret_cast<int4 *>(out + head);
+    if (y == kCeIgnored) {
+        for (int i = threadIdx.x; i < nv; i += kNT) __stcs(o16 + i, make_int4(0, 0, 0, 0));
+        for (int j = threadIdx.x; j < head; j += kNT) out[j] = ce_from_float<T>(0.f);
+        for (int j = rest + (int)threadIdx.x; j < V; j += kNT) out[j] = ce_from_float<T>(0.f);
+        return;
+    }
     const float f = o.reduction == kCeNone ? grad_loss[row]
                     : o.reduction == kCeMean ? grad_loss[0] / count[0]
                                              : grad_loss[0];
     const RowGrad q = row_grad(lse_in[row], V, f, o);
-    auto one = [&](int j) {
-        const float d = grad_of<T, CAP>(p[j], j == y, q, o.cap);
-        out[j] = ce_from_float<T>(y == kCeIgnored ? 0.f : d);
-    };
-    int4 *o16 = reinterpret_cast<int4 *>(out + head);
-    if (y == kCeIgnored) {  // nothing of the row is read
-        for (int i = threadIdx.x; i < nv; i += kNT) __stcs(o16 + i, make_int4(0, 0, 0, 0));
-    } else {
+    const Vec16<T> *words = reinterpret_cast<const Vec16<T> *>(p + head);
 #pragma unroll 2
-        for (int i = threadIdx.x; i < nv; i += kNT) {
-            Vec16<T> v = reinterpret_cast<const Vec16<T> *>(p + head)[i];
-            const int at = y - (head + i * kN);
+    for (int i = threadIdx.x; i < nv; i += kNT) {
+        float2 z[kP];
+        pairs_of(words[i], z);
+        const int at = y - (head + i * kN);
+        Vec16<T> v;
 #pragma unroll
-            for (int t = 0; t < kN; ++t)
-                v.v[t] = ce_from_float<T>(grad_of<T, CAP>(v.v[t], t == at, q, o.cap));
-            __stcs(o16 + i, reinterpret_cast<const int4 &>(v));
+        for (int k = 0; k < kP; ++k) {
+            float2 t;
+            if (CAP) {
+                t = make_float2(ce_tanh<sizeof(T) == 2>(z[k].x, o.cap),
+                                ce_tanh<sizeof(T) == 2>(z[k].y, o.cap));
+                z[k] = __fmul2_rn(t, f2(o.cap));
+            }
+            float2 d = __ffma2_rn(__fadd2_rn(z[k], f2(-q.lse.x)), f2(kLog2e), f2(-q.lse.y));
+            d = __ffma2_rn(f2(q.kz), make_float2(ex2(d.x), ex2(d.y)), f2(-q.e));
+            if (at == 2 * k) d.x -= q.hit;
+            if (at == 2 * k + 1) d.y -= q.hit;
+            if (CAP) d = __fmul2_rn(d, __ffma2_rn(make_float2(-t.x, -t.y), t, f2(1.f)));
+            v.v[2 * k] = ce_from_float<T>(d.x);
+            v.v[2 * k + 1] = ce_from_float<T>(d.y);
         }
+        __stcs(o16 + i, reinterpret_cast<const int4 &>(v));
     }
+    auto one = [&](int j) {
+        out[j] = ce_from_float<T>(grad_of<T, CAP>(p[j], j == y, q, o.cap));
+    };
     for (int j = threadIdx.x; j < head; j += kNT) one(j);
-    for (int j = head + nv * kN + (int)threadIdx.x; j < V; j += kNT) one(j);
+    for (int j = rest + (int)threadIdx.x; j < V; j += kNT) one(j);
 }
 
 __global__ void __launch_bounds__(1024)
@@ -502,7 +571,8 @@ template <typename T, bool CAP, bool WORDS>
 cudaError_t staged_any(bool fwd, const Args &a) {
     switch (lanes_of(a.V)) {
         case 1:
-            return a.V <= 8    ? staged<T, 1, 8, CAP, WORDS>(fwd, a)
+            return a.V <= 4    ? staged<T, 1, (WORDS && sizeof(T) == 2 ? 8 : 4), CAP, WORDS>(fwd, a)
+                   : a.V <= 8  ? staged<T, 1, 8, CAP, WORDS>(fwd, a)
                    : a.V <= 16 ? staged<T, 1, 16, CAP, WORDS>(fwd, a)
                                : staged<T, 1, 32, CAP, WORDS>(fwd, a);
         case 2: return staged<T, 2, 32, CAP, WORDS>(fwd, a);
