@@ -5,7 +5,7 @@
 
 namespace gsv {
 
-constexpr int kFewRows = 4;  // rows at most
+constexpr int kFewRows = 8;  // rows at most (float32; 4 of 16 bits)
 
 struct FewArgs {
     int N, V, D;

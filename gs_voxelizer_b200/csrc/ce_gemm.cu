@@ -173,11 +173,9 @@ __device__ __forceinline__ void store8(void *p, const uint32_t *v) {
                  "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
-__device__ __forceinline__ void fetch8(const float *p, float *v) {
-    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]),
-                   "=f"(v[6]), "=f"(v[7])
-                 : "l"(p)
+__device__ __forceinline__ void store4(void *p, const uint32_t *v) {
+    asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3])
                  : "memory");
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
@@ -446,12 +444,12 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         uint32_t acc_phase = 0;
         bool ok = true;
         float scale = 1.f;
-        bool wide = true;  // output rows aligned to 32 bytes
+        bool wide = true;  // output rows aligned to 16 bytes
         float *stage_out = reinterpret_cast<float *>(
             smem_raw + (smem0 - smem_addr(smem_raw)) + kStages * kStageBytes);
         if (PRODUCT >= kCeGradX) {
-            wide = g.dst ? g.D % 16 == 0 && (reinterpret_cast<uintptr_t>(g.dst) & 31) == 0
-                         : g.D % 8 == 0;
+            wide = g.D % (g.dst && !F32 ? 8 : 4) == 0 &&
+                   (reinterpret_cast<uintptr_t>(g.dst) & 15) == 0;
             if (g.dst) scale = ce_grad_scale(g.up);
         }
         // a unit's row, read a unit ahead: units of few classes and channels
@@ -590,43 +588,44 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     } else {
                         const long long M = PRODUCT == kCeGradW ? g.nv : w.live;
                         const int cols = min(32, g.D - col0);
-                        const bool direct = !F32 && g.dst;
-                        const bool add = g.add || chunk > 0;
+                        const bool direct = g.dst != nullptr;
+                        const bool add = !direct && (g.add || chunk > 0);
                         long long to = r;  // row of the output
                         if (direct && PRODUCT == kCeGradX && r < M)
                             to = g.idx ? g.idx[g.row0 + r] : g.row0 + r;
                         if (direct && PRODUCT == kCeGradW) to += g.v0;
                         to *= g.D;
-                        float *acc_out = g.acc + t.split * g.acc_split;
-                        uint16_t *dst = static_cast<uint16_t *>(g.dst);
+                        // float32 sums, or float32 gradients; 16-bit gradients
+                        float *out32 = F32 && direct ? static_cast<float *>(g.dst)
+                                                     : g.acc + t.split * g.acc_split;
+                        uint16_t *out16 = static_cast<uint16_t *>(g.dst);
                         if (wide) {
                             if (r < M) {
 #pragma unroll
-                                for (int j = 0; j < 32; j += 16) {
-                                    if (direct) {
-                                        uint32_t out[8];
+                                for (int j = 0; j < 32; j += 8) {
+                                    if (j >= cols) continue;
+                                    if (!F32 && direct) {
+                                        uint32_t out[4];
 #pragma unroll
-                                        for (int i = 0; i < 8; ++i)
+                                        for (int i = 0; i < 4; ++i)
                                             out[i] = pack2(
                                                 __uint_as_float(v[j + 2 * i]) * scale,
                                                 __uint_as_float(v[j + 2 * i + 1]) * scale,
                                                 g.bf16);
-                                        if (j < cols) store8(dst + to + col0 + j, out);
+                                        store4(out16 + to + col0 + j, out);
                                         continue;
                                     }
 #pragma unroll
-                                    for (int q = j; q < j + 16; q += 8) {
+                                    for (int q = j; q < j + 8; q += 4) {
                                         if (q >= cols) continue;
-                                        float *p = acc_out + to + col0 + q;
-                                        if (add) {
-                                            float old[8];
-                                            fetch8(p, old);
-#pragma unroll
-                                            for (int i = 0; i < 8; ++i)
-                                                v[q + i] = __float_as_uint(
-                                                    __uint_as_float(v[q + i]) + old[i]);
-                                        }
-                                        store8(p, v + q);
+                                        float *p = out32 + to + col0 + q;
+                                        float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
+                                        if (add) old = *reinterpret_cast<const float4 *>(p);
+                                        *reinterpret_cast<float4 *>(p) = make_float4(
+                                            fmaf(__uint_as_float(v[q]), scale, old.x),
+                                            fmaf(__uint_as_float(v[q + 1]), scale, old.y),
+                                            fmaf(__uint_as_float(v[q + 2]), scale, old.z),
+                                            fmaf(__uint_as_float(v[q + 3]), scale, old.w));
                                     }
                                 }
                             }
@@ -644,10 +643,10 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                                 const long long at = __shfl_sync(0xffffffffu, to, i) + col0 + lane;
                                 const float x = turn[i * 33 + lane];
                                 if (lane < cols) {
-                                    if (direct)
-                                        dst[at] = (uint16_t)pack2(x, 0.f, g.bf16);
+                                    if (!F32 && direct)
+                                        out16[at] = (uint16_t)pack2(x, 0.f, g.bf16);
                                     else
-                                        acc_out[at] = (add ? acc_out[at] : 0.f) + x;
+                                        out32[at] = (add ? out32[at] : 0.f) + x;
                                 }
                             }
                             __syncwarp();
@@ -719,16 +718,35 @@ bool make_map(CUtensorMap *map, const CeMat &m, int planes, bool bf16, int box_r
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// columns of a tile: a multiple of 32 (K-major B) or of 128 (MN-major B)
-int tile_n(int cols, int unit) {
-    return std::min(kCeTileN, (int)(((long long)cols + unit - 1) / unit * unit));
+// columns of a gradient's tile (MN-major B: multiples of 128)
+int tile_n(int cols) { return cols <= 128 ? 128 : kCeTileN; }
+
+// Classes of a tile of scores: the width, in steps of 32, with which the pairs
+// are done first. A tile costs its width, below 64 no less (A's rows are read
+// all the same), and about 32 to turn around: 256 where there is much to do,
+// 160 for 1001 rows x 5003 classes (2 rounds instead of 2 wider ones), 64 for
+// 18 rows x 3021 (48 tiles instead of 24 at the same memory). float32 keeps a
+// tile's sums in registers, 64 a thread: 128 at most.
+int score_tile(long long rows, int nv, bool f32) {
+    const long long mt = (rows + kCeTileM - 1) / kCeTileM;
+    int best = 32;
+    long long cost = LLONG_MAX;
+    for (int nt = 32; nt <= (f32 ? 128 : kCeTileN); nt += 32) {
+        const long long units = mt * ((nv + nt - 1) / nt);
+        const long long c = (units + kCePairs - 1) / kCePairs * (std::max(nt, 64) + 32);
+        if (c <= cost) {
+            cost = c;
+            best = nt;
+        }
+        if (nt >= nv) break;
+    }
+    return best;
 }
 
 template <int PRODUCT, bool CAP, bool F32>
 cudaError_t launch(const CeGemm &g, cudaStream_t st) {
     constexpr bool kAMn = PRODUCT == kCeGradW, kBMn = PRODUCT >= kCeGradX;
-    // float32 scores keep a tile's sums in registers: 64 a thread
-    const int nt = kBMn ? tile_n(g.D, 128) : std::min(tile_n(g.nv, 32), F32 ? 128 : kCeTileN);
+    const int nt = kBMn ? tile_n(g.D) : score_tile(g.rows, g.nv, F32);
     CUtensorMap a, b;
     const CeMat &ma = PRODUCT >= kCeGradX ? g.P : g.X;
     const CeMat &mb = PRODUCT == kCeGradW ? g.X : g.W;
@@ -760,9 +778,9 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
 
 }  // namespace
 
-int ce_runs(long long rows, int V) {
+int ce_runs(long long rows, int V, bool f32) {
     const long long mt = (rows + kCeTileM - 1) / kCeTileM;
-    const int tiles = (V + kCeTileN - 1) / kCeTileN;
+    const int nt = score_tile(rows, V, f32), tiles = (V + nt - 1) / nt;
     // the longest pair's tiles, and about a third of a tile to begin a run
     int best = 1;
     double cost = 1e300;

@@ -68,8 +68,9 @@ struct CeGemm {
     float p_scale;
     const float *grow;  // upstream gradient by original row, or null
     const float *gmax;  // or null
-    // kCeGradX, kCeGradW: acc[split][m][D] (+)= product, or, with dst set (one
-    // plane), dst[row of m][D] = scale * product in the inputs' type
+    // kCeGradX, kCeGradW: acc[split][m][D] (+)= product, or, with dst set (of
+    // float32: K of at most 512), dst[row of m][D] = scale * product in the
+    // inputs' type
     float *acc;
     long long acc_split;  // elements between splits
     int splits;
@@ -83,7 +84,7 @@ constexpr int kCeTileN = 256;     // classes (or channels) a tile, at most
 constexpr int kCePairs = kSMs / 2;  // tiles in flight: a pair of SMs each
 
 // runs of class tiles for the forward: (rows of) partial sums and balance
-int ce_runs(long long rows, int V);
+int ce_runs(long long rows, int V, bool f32);
 
 cudaError_t launch_ce_gemm(const CeGemm &g, cudaStream_t stream);
 

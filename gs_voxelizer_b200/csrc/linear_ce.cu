@@ -452,7 +452,7 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     // `weight` null: the workspace query, which allows for any alignment
     p.pack_w = p.planes == 3 || D % 8 != 0 || weight == nullptr ||
                (reinterpret_cast<uintptr_t>(weight) & 15) != 0;
-    p.runs = ce_runs(N, V);
+    p.runs = ce_runs(N, V, p.planes == 3);
     size_t at = 0;
     auto take = [&](size_t b) {
         const size_t o = at;
@@ -495,8 +495,9 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     const long long tn = (D + kCeTileN - 1) / kCeTileN;
     p.split_x = splits_for(p.piece_rows / kCeTileM * tn, p.piece_classes);
     p.split_w = splits_for(up(p.piece_classes, kCeTileM) / kCeTileM * tn, p.piece_rows);
-    p.direct_x = p.planes == 1 && one_class_piece && p.split_x == 1;
-    p.direct_w = p.planes == 1 && p.one_row_piece && p.split_w == 1;
+    // (float32 sums of more than 512 terms are joined in memory)
+    p.direct_x = one_class_piece && p.split_x == 1 && (p.planes == 1 || V <= 512);
+    p.direct_w = p.one_row_piece && p.split_w == 1 && (p.planes == 1 || p.Np <= 512);
     p.dx = take(p.direct_x ? 0 : sizeof(float) * (size_t)p.split_x * p.piece_rows * D);
     p.dw = take(p.direct_w ? 0
                            : sizeof(float) * (size_t)p.split_w *
@@ -698,7 +699,7 @@ Path path_of(long long N, int V, int D, int type) {
                      : D <= kNarrowD ? (type == kCeF32 ? 256 : 64)
                                      : 0;
     if (V <= most) return kNarrow;
-    return N <= kFewRows ? kFew : kTiles;
+    return N <= (type == kCeF32 ? kFewRows : kFewRows / 2) ? kFew : kTiles;
 }
 
 // Rows that the forward's tiles read in place, 16 bits and aligned for TMA:

@@ -6,8 +6,10 @@
 // rows deep whatever the rows, and takes as long as the read. Here a warp
 // takes four classes at a time, its lanes 16 bytes of each, converts and
 // multiplies in float32 and keeps a running maximum and sum per row; at five
-// rows the multiply-adds would take longer than the read (22 of 45 bytes a
-// clock and SM at eight), so that more rows go to the tiles.
+// rows of 16 bits the multiply-adds would take longer than the read (22 of 45
+// bytes a clock and SM at eight), so that more rows go to the tiles. float32,
+// which the tiles would have to split into three planes first, comes here up
+// to eight rows.
 #include <type_traits>
 
 #include "ce_few.cuh"
@@ -18,7 +20,7 @@ namespace {
 constexpr int kNT = 256, kWarps = kNT / 32;
 constexpr int kClasses = 4;                 // classes a warp takes at once
 constexpr int kBlocks = 4 * kSMs;
-constexpr int kMergeNT = 256;
+constexpr int kMergeNT = 128;
 
 // kW elements from p as float32
 template <typename T, int kW>
@@ -35,7 +37,7 @@ __device__ __forceinline__ void fetch(const T *p, float (&v)[kW]) {
 
 // part[block][row] = (maximum, sum) of the block's classes, psum likewise
 template <typename T, int R, bool CAP, bool VEC>
-__global__ void __launch_bounds__(kNT, 4)
+__global__ void __launch_bounds__(kNT, R == 8 ? 2 : 4)
 few_fwd_kernel(int N, int V, int D, const T *__restrict__ features, const T *__restrict__ weight,
                const long long *__restrict__ labels, CeOpt o, float2 *__restrict__ part,
                float *__restrict__ psum, float *__restrict__ zt) {
@@ -115,7 +117,7 @@ few_fwd_kernel(int N, int V, int D, const T *__restrict__ features, const T *__r
     psum[blockIdx.x * N + r] = t.sz;
 }
 
-// All parts of all rows, 256 threads a row -> lse, loss, count.
+// All parts of all rows, 128 threads a row -> lse, loss, count.
 __global__ void __launch_bounds__(kMergeNT *kFewRows)
 few_merge_kernel(int N, int V, int parts, const float2 *__restrict__ part,
                  const float *__restrict__ psum, const float *__restrict__ zt,
@@ -196,8 +198,10 @@ cudaError_t few_forward(const FewArgs &a, float *loss, unsigned char *ws, cudaSt
         launch_rows<T, 1, CAP>(a, blocks, part, psum, zt, st);
     else if (a.N == 2)
         launch_rows<T, 2, CAP>(a, blocks, part, psum, zt, st);
-    else
+    else if (a.N <= 4 || sizeof(T) == 2)
         launch_rows<T, 4, CAP>(a, blocks, part, psum, zt, st);
+    else
+        launch_rows<T, 8, CAP>(a, blocks, part, psum, zt, st);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     few_merge_kernel<<<1, kMergeNT * a.N, 0, st>>>(a.N, a.V, blocks, part, psum, zt, a.labels,
