@@ -18,11 +18,12 @@ BUILD = HERE / "_build"
 LIB = HERE / "libgsvox.so"
 SOURCES = ["projection.cu", "binning.cu", "voxelize.cu", "bwd_tc.cu", "loss.cu",
            "ssim.cu", "noalloc.cu", "halo.cu", "softmax_ce.cu", "linear_ce.cu",
-           "linear_ce_narrow.cu", "linear_ce_few.cu", "ce_gemm.cu", "capi.cu"]
+           "linear_ce_narrow.cu", "linear_ce_wide.cu", "linear_ce_few.cu",
+           "ce_gemm.cu", "capi.cu"]
 # Sources compiled with IEEE arithmetic and math functions: their scores
 # reach the hundreds and their exponents may be infinite on purpose.
 PRECISE = {"softmax_ce.cu", "linear_ce.cu", "linear_ce_narrow.cu",
-           "linear_ce_few.cu", "ce_gemm.cu"}
+           "linear_ce_wide.cu", "linear_ce_few.cu", "ce_gemm.cu"}
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

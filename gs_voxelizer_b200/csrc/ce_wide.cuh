@@ -1,0 +1,27 @@
+// Linear class loss of few classes and many float32 channels
+// (linear_ce_wide.cu).
+#pragma once
+
+#include "ce_narrow.cuh"
+
+namespace gsv {
+
+constexpr int kWideV = 16;                  // classes at most
+constexpr size_t kWideTable = 96 << 10;     // bytes of the table at most
+
+struct WideShape {
+    int row_blocks;           // forward, dX: persistent blocks
+    int dw_chunks, dw_blocks; // dW: channel chunks x row blocks (parts)
+};
+WideShape wide_shape(long long N, int V, int D);
+inline size_t wide_p_bytes(long long N, int V) { return sizeof(float) * (size_t)N * ((V + 3) / 4 * 4); }
+
+// loss (one block) or per-block sums
+cudaError_t launch_wide_fwd(const NarrowArgs &a, float *loss, float2 *sums, cudaStream_t st);
+// grad (or null), and the derivatives P [N][V rounded up to 4]
+cudaError_t launch_wide_dx(const NarrowArgs &a, const CeUpstream &u, float *grad, float *p,
+                           cudaStream_t st);
+// acc [dw_blocks][V][D]
+cudaError_t launch_wide_dw(const NarrowArgs &a, const float *p, float *acc, cudaStream_t st);
+
+}  // namespace gsv

@@ -19,6 +19,7 @@
 #include "ce_few.cuh"
 #include "ce_gemm.cuh"
 #include "ce_narrow.cuh"
+#include "ce_wide.cuh"
 
 namespace gsv {
 namespace {
@@ -684,6 +685,44 @@ cudaError_t narrow_backward(const NarrowArgs &a, const float *grad_loss, void *g
 
 namespace {
 
+// Workspace of the wide path: per-block sums; or P, then parts of dW.
+struct WidePlan {
+    size_t dw, bytes;
+};
+WidePlan wide_plan(long long N, int V, int D, bool backward) {
+    const WideShape s = wide_shape(N, V, D);
+    WidePlan w{};
+    if (backward) {
+        w.dw = align256(wide_p_bytes(N, V));
+        w.bytes = w.dw + align256(sizeof(float) * (size_t)s.dw_blocks * V * D);
+    } else {
+        w.bytes = align256(sizeof(float2) * s.row_blocks);
+    }
+    return w;
+}
+
+cudaError_t wide_forward(const NarrowArgs &a, float *loss, unsigned char *ws, cudaStream_t st) {
+    float2 *sums = reinterpret_cast<float2 *>(ws);
+    GSV_CE_TRY(launch_wide_fwd(a, loss, sums, st));
+    const int blocks = wide_shape(a.N, a.V, a.D).row_blocks;
+    if (blocks > 1)
+        GSV_CE_TRY(launch_ce_finish(sums, blocks, a.opt.reduction, loss, a.count, st));
+    return cudaSuccess;
+}
+
+cudaError_t wide_backward(const NarrowArgs &a, const float *grad_loss, void *gx, void *gw,
+                          unsigned char *ws, cudaStream_t st) {
+    const WidePlan w = wide_plan(a.N, a.V, a.D, true);
+    const CeUpstream u{grad_loss, a.count, nullptr, 1.f, a.opt.reduction};
+    float *p = reinterpret_cast<float *>(ws), *dw = reinterpret_cast<float *>(ws + w.dw);
+    if (!gx && !gw) return cudaSuccess;
+    GSV_CE_TRY(launch_wide_dx(a, u, static_cast<float *>(gx), p, st));
+    if (!gw) return cudaSuccess;
+    GSV_CE_TRY(launch_wide_dw(a, p, dw, st));
+    return reduce_splits<float>((long long)a.V * a.D, dw, wide_shape(a.N, a.V, a.D).dw_blocks,
+                                gw, st);
+}
+
 // Which kernels serve a call. kNarrow (linear_ce_narrow.cu, the CUDA cores
 // without tiles): where it is the faster. Kernels' time of a training step,
 // narrow against tiles: 53000 rows x 203 classes, D = 16, 99 against 180 us of
@@ -691,14 +730,17 @@ namespace {
 // 10^6 rows x 20 classes, D = 16, 148 against 1311 and 134 against 530, D = 32,
 // 356 and 299 against 530 of bf16; 1000 rows x 50000 classes, D = 16, 267
 // against 472 and 250 against 160, D = 32, 584 against 480 of float32.
-// kFew: the forward alone; its backward takes tiles.
-enum Path { kNarrow, kFew, kTiles };
+// kWide: few classes, many float32 channels. kFew: the forward alone; its
+// backward takes tiles.
+enum Path { kNarrow, kWide, kFew, kTiles };
 Path path_of(long long N, int V, int D, int type) {
     const int most = D <= 8 ? INT_MAX
                      : D <= 16 ? (type == kCeF32 ? INT_MAX : 128)
                      : D <= kNarrowD ? (type == kCeF32 ? 256 : 64)
                                      : 0;
     if (V <= most) return kNarrow;
+    if (type == kCeF32 && V <= kWideV && sizeof(float) * (size_t)V * D <= kWideTable)
+        return kWide;
     return N <= (type == kCeF32 ? kFewRows : kFewRows / 2) ? kFew : kTiles;
 }
 
@@ -716,7 +758,8 @@ bool in_place(long long N, int V, int D, int type, const void *features) {
 
 size_t linear_ce_state_bytes(long long N, int V, int D, int type) {
     size_t b = (size_t)state_words(N) * 4;
-    if (path_of(N, V, D, type) == kNarrow) return b;
+    const Path path = path_of(N, V, D, type);
+    if (path == kNarrow || path == kWide) return b;
     const size_t xb = packed_bytes(up(N, kCeTileM), D, type), wb = packed_bytes(V, D, type);
     if (kept(xb)) b += align256(xb);
     if (kept(wb)) b += align256(wb);
@@ -731,6 +774,7 @@ size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backw
     const Path path = path_of(N, V, D, type);
     switch (backward && path == kFew ? kTiles : path) {
         case kNarrow: return own + narrow_plan(N, V, D, backward, o).bytes;
+        case kWide: return own + wide_plan(N, V, D, backward).bytes;
         case kFew: return own + few_workspace_bytes((int)N, V);
         default: return own + make_plan(N, V, D, type, nullptr, backward, o).bytes;
     }
@@ -753,6 +797,8 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
             default: return narrow_forward<__half>(a, loss, ws, st);
         }
     }
+    if (path == kWide)
+        return wide_forward({N, V, D, features, weight, labels, o, s.lse, s.count}, loss, ws, st);
     const Plan p = make_plan(N, V, D, type, weight, false, o);
     const bool direct = in_place(N, V, D, type, features);
     if (!forward_only || (path == kTiles && !direct)) {
@@ -818,6 +864,9 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
         }
 #undef GSV_CE_T
     }
+    if (path_of(N, V, D, type) == kWide)
+        return wide_backward({N, V, D, features, weight, labels, o, s.lse, s.count}, grad_loss,
+                             grad_features, grad_weight, ws, st);
     const Plan p = make_plan(N, V, D, type, weight, true, o);
     float *gmax = type == kCeF16 ? reinterpret_cast<float *>(ws + p.gmax) : nullptr;
     const bool none = o.reduction == kCeNone;

@@ -151,7 +151,8 @@ def test_scores(n, V, dtype):
 @pytest.mark.parametrize("n,V,D", [
     (1, 1, 1), (1, 20, 4), (2, 3, 2), (129, 20, 4), (1000, 5, 3), (300, 300, 8), (70, 33, 9),
     (128, 256, 64), (127, 255, 63), (129, 257, 65), (1, 5003, 128), (300, 1000, 40),
-    (40, 70, 1000), (513, 2, 16), (3, 20011, 24), (700, 1, 32)])
+    (40, 70, 1000), (513, 2, 16), (3, 20011, 24), (700, 1, 32),
+    (1, 3, 33), (1030, 9, 440), (333, 13, 325), (200, 16, 1536), (150, 17, 128), (90, 4, 5001)])
 def test_linear(n, V, D, dtype):
     for i, opt in enumerate(OPTS):
         run(n, V, D, dtype, opt, ignored=0.3 if i % 2 else 0.0)
@@ -163,6 +164,7 @@ def test_linear_many_rows(dtype):
     run(70001, 4097, 16, dtype, dict(), ignored=0.2)
     run(300001, 20, 4, dtype, dict(reduction="sum"), ignored=0.1)
     run(200003, 11, 24, dtype, dict(reduction="none"), ignored=0.1)
+    run(100003, 7, 100, dtype, dict(smoothing=0.1, z_loss=1e-3), ignored=0.1)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -264,7 +266,7 @@ def test_large_scores(D, dtype):
     check(data, labels, {}, up, loss, grads)
 
 
-@pytest.mark.parametrize("D,V", [(0, 37), (0, 2001), (4, 20), (64, 300), (40, 301)])
+@pytest.mark.parametrize("D,V", [(0, 37), (0, 2001), (4, 20), (64, 300), (40, 301), (64, 6)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_strides_and_alignment(D, V, dtype):
     """Views: transposed, strided rows, and a base that no wide access suits
@@ -311,7 +313,8 @@ def test_one_gradient_alone(D, which):
 
 
 @pytest.mark.parametrize("n,V,D,dtype", [(3000, 20, 4, F32), (20000, 37, 0, BF16),
-                                         (900, 5003, 64, BF16), (900, 503, 64, F32)])
+                                         (900, 5003, 64, BF16), (900, 503, 64, F32),
+                                         (9000, 9, 100, F32)])
 def test_same_result_every_time(n, V, D, dtype):
     data, labels = make(n, V, D, dtype, 11, ignored=0.2)
     first = call(data, labels, {}, torch.ones((), device="cuda"))
@@ -322,7 +325,8 @@ def test_same_result_every_time(n, V, D, dtype):
             assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("n,V,D", [(60, 30, 0), (40, 2000, 0), (60, 30, 4), (60, 300, 24)])
+@pytest.mark.parametrize("n,V,D", [(60, 30, 0), (40, 2000, 0), (60, 30, 4), (60, 300, 24),
+                                   (60, 9, 50), (60, 30, 50)])
 def test_gradient_against_differences(n, V, D):
     """The slope of the loss along the gradient's own direction is its
     norm squared; central differences of the float32 loss with a step that
@@ -343,7 +347,7 @@ def test_gradient_against_differences(n, V, D):
 
 @pytest.mark.parametrize("n,V,D,dtype", [(500, 20, 4, F32), (300, 37, 0, F32),
                                          (20, 3001, 0, BF16), (300, 1003, 72, BF16),
-                                         (300, 203, 32, F32)])
+                                         (300, 203, 32, F32), (300, 9, 100, F32)])
 def test_capture_and_replay(n, V, D, dtype):
     """Forward and backward captured once and replayed on new contents,
     a second graph in between."""
