@@ -739,8 +739,7 @@ Path path_of(long long N, int V, int D, int type) {
                      : D <= kNarrowD ? (type == kCeF32 ? 256 : 64)
                                      : 0;
     if (V <= most) return kNarrow;
-    if (type == kCeF32 && V <= kWideV && sizeof(float) * (size_t)V * D <= kWideTable)
-        return kWide;
+    if (type == kCeF32 && V <= kWideV && N >= kWideRows) return kWide;
     return N <= (type == kCeF32 ? kFewRows : kFewRows / 2) ? kFew : kTiles;
 }
 

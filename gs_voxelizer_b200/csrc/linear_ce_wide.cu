@@ -4,11 +4,14 @@
 // The features are all there is to move - read forward, for dX and for dW, dX
 // written: 4 passes of 4 N D bytes. The tensor cores' tiles would first split
 // them into three bf16 planes (10 bytes moved for 4, twice) and read those
-// three times. Here a warp takes four rows, its lanes four channels each, the
-// table in shared memory; the V sums of a row are joined by shuffles and the
-// softmax is formed by every lane. V multiply-adds a channel against the 11
-// floats a clock and SM that HBM delivers: bound by HBM up to about ten classes
-// and by the multiply-adds above. dW sums rows, the other axis: it reads the
+// three times: 3312 us of kernels at 603768 rows x 9 classes x 440 channels.
+// Here a block stages 32 channels of 256 rows (and of the table) at a time with
+// asynchronous copies, the next while one is used; a thread owns two rows, so
+// that the V sums of a row need no exchange, and every value of the table read
+// from shared memory serves both. (A warp a row, its sums joined by shuffles,
+// spent more on these and on the softmax in every lane: 2437 us.) V
+// multiply-adds a channel against the 11 floats a clock and SM that HBM
+// delivers: bound by HBM. dW sums rows, the other axis: it reads the
 // derivatives P (V floats a row, left by dX's kernel) beside the features, each
 // lane keeping V x 4 sums.
 #include <atomic>
@@ -18,87 +21,147 @@
 namespace gsv {
 namespace {
 
-constexpr int kNT = 256, kWarps = kNT / 32;
-constexpr int kR = 4;        // rows a warp takes at once
-constexpr int kChunk = 128;  // channels of a dW block
+constexpr int kNT = 128;                 // forward, dX
+constexpr int kR = 2;                    // rows a thread
+constexpr int kRows = kNT * kR;          // rows a tile
+constexpr int kDepth = 32;               // channels staged at once
+// floats of a staged row: rows 16-byte words apart by an odd number of them,
+// which reads of a word a lane take without bank conflicts
+constexpr int kPitch = kDepth + 4;
+constexpr int kDwNT = 256, kDwWarps = kDwNT / 32;
+constexpr int kDwRows = 64;              // rows a tile of dW, eight a warp
+constexpr int kChunk = 128;              // channels of a dW block
 
-template <bool VEC>
-__device__ __forceinline__ float4 load4(const float *p, int c, int D) {
-    if (VEC) return *reinterpret_cast<const float4 *>(p + c);
-    return make_float4(p[c], c + 1 < D ? p[c + 1] : 0.f, c + 2 < D ? p[c + 2] : 0.f,
-                       c + 3 < D ? p[c + 3] : 0.f);
+template <int VP>
+struct alignas(16) Stage {
+    float x[kRows][kPitch];
+    float w[VP][kDepth];
+};
+
+__device__ __forceinline__ void copy16(float *dst, const float *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src)
+                 : "memory");
 }
-
-// the table as [V][Dp], channels past D zero
+__device__ __forceinline__ void copy4(float *dst, const float *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src)
+                 : "memory");
+}
+// four floats of which `valid` exist, zeros after them; VEC: all or none, and
+// aligned to 16 bytes
 template <bool VEC>
-__device__ __forceinline__ void stage(float *sw, const float *w, int V, int D, int Dp) {
-    for (int i = threadIdx.x; i < V * (Dp / 4); i += kNT) {
-        const int j = i / (Dp / 4), c = i % (Dp / 4) * 4;
-        *reinterpret_cast<float4 *>(sw + j * Dp + c) = load4<VEC>(w + (long long)j * D, c, D);
+__device__ __forceinline__ void copy_word(float *dst, const float *src, int valid) {
+    if (VEC && valid > 0) {
+        copy16(dst, src);
+        return;
     }
-    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (k < valid)
+            copy4(dst + k, src + k);
+        else
+            dst[k] = 0.f;
+    }
+}
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
-// scores of rows r0 .. r0 + 3 (clamped to N - 1), in every lane
-template <int VP, bool VEC, bool CAP>
-__device__ __forceinline__ void scores_of(float (&z)[kR][VP], float (&t)[CAP ? kR : 1][VP],
-                                          const float *sw, const float *x, long long r0,
-                                          long long N, int V, int D, int Dp, float cap) {
-    const int lane = threadIdx.x & 31;
-    const float *row[kR];
-#pragma unroll
-    for (int k = 0; k < kR; ++k) row[k] = x + min(r0 + k, N - 1) * D;
+// channels [c0, c0 + 32) of the table, zeros past D
+template <int VP, bool VEC>
+__device__ __forceinline__ void stage_table(float (&dst)[VP][kDepth], const float *w, int V, int D,
+                                            int c0) {
+    for (int i = threadIdx.x; i < V * (kDepth / 4); i += kNT) {
+        const int j = i / (kDepth / 4), c = i % (kDepth / 4) * 4;
+        copy_word<VEC>(&dst[j][c], w + (long long)j * D + c0 + c, D - c0 - c);
+    }
+}
+
+// the same channels of rows [r0, r0 + 256), zeros past D and N
+template <bool VEC>
+__device__ __forceinline__ void stage_rows(float (&dst)[kRows][kPitch], const float *x,
+                                           long long r0, long long N, int D, int c0) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kRows * (kDepth / 4); i += kNT) {
+        const int r = i / (kDepth / 4), c = i % (kDepth / 4) * 4;
+        copy_word<VEC>(&dst[r][c], x + (r0 + r) * D + c0 + c, r0 + r < N ? D - c0 - c : 0);
+    }
+}
+
+// scores of the thread's rows r0 + threadIdx.x (+ 128)
+template <int VP, bool VEC>
+__device__ __forceinline__ void scores_of(float (&z)[kR][VP], Stage<VP> *st, const float *x,
+                                          const float *w, long long r0, long long N, int V,
+                                          int D) {
+    const int chunks = (D + kDepth - 1) / kDepth;
+    float2 s[kR][VP];
 #pragma unroll
     for (int k = 0; k < kR; ++k)
 #pragma unroll
-        for (int j = 0; j < VP; ++j) z[k][j] = 0.f;
-    for (int c = 4 * lane; c < D; c += 128) {
-        float4 v[kR];
-#pragma unroll
-        for (int k = 0; k < kR; ++k) v[k] = load4<VEC>(row[k], c, D);
-#pragma unroll
-        for (int j = 0; j < VP; ++j) {
-            if (j >= V) break;
-            const float4 w = *reinterpret_cast<const float4 *>(sw + j * Dp + c);
+        for (int j = 0; j < VP; ++j) s[k][j] = make_float2(0.f, 0.f);
+    __syncthreads();  // the stages are free
+    stage_rows<VEC>(st[0].x, x, r0, N, D, 0);
+    stage_table<VP, VEC>(st[0].w, w, V, D, 0);
+    copies_end_group();
+    for (int i = 0; i < chunks; ++i) {
+        if (i + 1 < chunks) {
+            Stage<VP> &next = st[(i + 1) & 1];
+            stage_rows<VEC>(next.x, x, r0, N, D, (i + 1) * kDepth);
+            stage_table<VP, VEC>(next.w, w, V, D, (i + 1) * kDepth);
+        }
+        copies_end_group();
+        copies_wait<1>();
+        __syncthreads();
+        const Stage<VP> &cur = st[i & 1];
+#pragma unroll 2
+        for (int c = 0; c < kDepth; c += 4) {
+            float4 v[kR];
 #pragma unroll
             for (int k = 0; k < kR; ++k)
-                z[k][j] = fmaf(v[k].x, w.x, fmaf(v[k].y, w.y, fmaf(v[k].z, w.z,
-                                                                  fmaf(v[k].w, w.w, z[k][j]))));
+                v[k] = *reinterpret_cast<const float4 *>(&cur.x[k * kNT + threadIdx.x][c]);
+#pragma unroll
+            for (int j = 0; j < VP; ++j) {
+                if (j >= V) break;
+                const float4 q = *reinterpret_cast<const float4 *>(&cur.w[j][c]);
+#pragma unroll
+                for (int k = 0; k < kR; ++k) {
+                    s[k][j] = __ffma2_rn(make_float2(v[k].x, v[k].y), make_float2(q.x, q.y),
+                                         s[k][j]);
+                    s[k][j] = __ffma2_rn(make_float2(v[k].z, v[k].w), make_float2(q.z, q.w),
+                                         s[k][j]);
+                }
+            }
         }
+        __syncthreads();
     }
 #pragma unroll
     for (int k = 0; k < kR; ++k)
 #pragma unroll
-        for (int j = 0; j < VP; ++j) {
-            if (j >= V) break;
-#pragma unroll
-            for (int s = 16; s; s >>= 1) z[k][j] += __shfl_xor_sync(0xffffffffu, z[k][j], s);
-            if (CAP) {
-                t[CAP ? k : 0][j] = ce_tanh<false>(z[k][j], cap);
-                z[k][j] = cap * t[CAP ? k : 0][j];
-            }
-        }
+        for (int j = 0; j < VP; ++j) z[k][j] = s[k][j].x + s[k][j].y;
 }
 
 template <int VP, bool VEC, bool CAP>
-__global__ void __launch_bounds__(kNT, 2)
-wide_fwd_kernel(long long N, int V, int D, int Dp, const float *__restrict__ features,
+__global__ void __launch_bounds__(kNT)
+wide_fwd_kernel(long long N, int V, int D, const float *__restrict__ features,
                 const float *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
                 float *__restrict__ loss, float2 *__restrict__ lse_out,
                 float *__restrict__ count, float2 *__restrict__ sums) {
-    extern __shared__ __align__(16) float wide_smem[];
-    __shared__ float2 sh[kWarps];
-    stage<VEC>(wide_smem, weight, V, D, Dp);
-    const int lane = threadIdx.x & 31;
+    extern __shared__ __align__(16) unsigned char wide_smem[];
+    __shared__ float2 sh[kNT / 32];
+    Stage<VP> *st = reinterpret_cast<Stage<VP> *>(wide_smem);
     float lsum = 0.f, cnt = 0.f;
-    const long long stride = (long long)gridDim.x * kWarps * kR;
-    for (long long r0 = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * kR; r0 < N;
-         r0 += stride) {
-        float z[kR][VP], t[CAP ? kR : 1][VP];
-        scores_of<VP, VEC, CAP>(z, t, wide_smem, features, r0, N, V, D, Dp, o.cap);
+    for (long long r0 = (long long)blockIdx.x * kRows; r0 < N;
+         r0 += (long long)gridDim.x * kRows) {
+        float z[kR][VP];
+        scores_of<VP, VEC>(z, st, features, weight, r0, N, V, D);
 #pragma unroll
         for (int k = 0; k < kR; ++k) {
-            const long long r = r0 + k;
+            const long long r = r0 + k * kNT + threadIdx.x;
             if (r >= N) break;
             const int y = ce_label(labels[r], o.ignore, V);
             CeAcc a;
@@ -106,16 +169,16 @@ wide_fwd_kernel(long long N, int V, int D, int Dp, const float *__restrict__ fea
             float zy = 0.f;
 #pragma unroll
             for (int j = 0; j < VP; ++j)
-                if (j < V) a.m = fmaxf(a.m, z[k][j]);
-            const float b = CeAcc::base(a.m);
-#pragma unroll
-            for (int j = 0; j < VP; ++j)
                 if (j < V) {
-                    a.s += ex2((z[k][j] - b) * kLog2e);
+                    if (CAP) z[k][j] = o.cap * ce_tanh<false>(z[k][j], o.cap);
+                    a.m = fmaxf(a.m, z[k][j]);
                     a.sz += z[k][j];
                     zy = y == j ? z[k][j] : zy;
                 }
-            if (lane != k) continue;
+            const float b = CeAcc::base(a.m);
+#pragma unroll
+            for (int j = 0; j < VP; ++j)
+                if (j < V) a.s += ex2((z[k][j] - b) * kLog2e);
             float2 lse = a.lse();
             float l = 0.f;
             if (y >= 0)
@@ -138,112 +201,165 @@ wide_fwd_kernel(long long N, int V, int D, int Dp, const float *__restrict__ fea
 }
 
 template <int VP, bool VEC, bool CAP>
-__global__ void __launch_bounds__(kNT, 2)
-wide_dx_kernel(long long N, int V, int D, int Dp, const float *__restrict__ features,
+__global__ void __launch_bounds__(kNT)
+wide_dx_kernel(long long N, int V, int D, const float *__restrict__ features,
                const float *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
                const float2 *__restrict__ lse, CeUpstream u, float *__restrict__ grad,
                float *__restrict__ p_out) {
-    extern __shared__ __align__(16) float wide_smem[];
-    stage<VEC>(wide_smem, weight, V, D, Dp);
-    const int lane = threadIdx.x & 31, ldp = (V + 3) / 4 * 4;
+    extern __shared__ __align__(16) unsigned char wide_smem[];
+    Stage<VP> *st = reinterpret_cast<Stage<VP> *>(wide_smem);
+    const int ldp = (V + 3) / 4 * 4, chunks = (D + kDepth - 1) / kDepth;
     const float common = common_grad(u), ev = o.eps / (float)V;
     const float *per_row = u.reduction == kCeNone ? u.g : nullptr;
-    const long long stride = (long long)gridDim.x * kWarps * kR;
-    for (long long r0 = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * kR; r0 < N;
-         r0 += stride) {
-        float z[kR][VP], t[CAP ? kR : 1][VP];
-        scores_of<VP, VEC, CAP>(z, t, wide_smem, features, r0, N, V, D, Dp, o.cap);
-        // scores to derivatives, the same in every lane
-        unsigned unlabelled = 0;
+    for (long long r0 = (long long)blockIdx.x * kRows; r0 < N;
+         r0 += (long long)gridDim.x * kRows) {
+        float z[kR][VP];
+        bool keep[kR];
+        scores_of<VP, VEC>(z, st, features, weight, r0, N, V, D);
 #pragma unroll
         for (int k = 0; k < kR; ++k) {
-            const long long r = r0 + k;
-            if (r >= N) break;
-            const int y = ce_label(labels[r], o.ignore, V);
-            if (y == kCeIgnored) unlabelled |= 1u << k;
-            const RowGrad q = row_grad<true>(r, y, lse[r], o, per_row, common, ev);
+            const long long r = r0 + k * kNT + threadIdx.x;
+            const int y = r < N ? ce_label(labels[r], o.ignore, V) : kCeIgnored;
+            keep[k] = y != kCeIgnored;
+            RowGrad q{};
+            if (keep[k]) q = row_grad<true>(r, y, lse[r], o, per_row, common, ev);
 #pragma unroll
             for (int j = 0; j < VP; ++j) {
-                if (j >= V) break;
-                float d = fmaf(q.kz, ce_prob(z[k][j], q.lse), -q.e);
-                if (y == j) d -= q.hit;
-                if (CAP) d *= fmaf(-t[CAP ? k : 0][j], t[CAP ? k : 0][j], 1.f);
-                z[k][j] = d = y == kCeIgnored ? 0.f : d;
-                if (lane == j) p_out[r * ldp + j] = d;
+                float d = 0.f;
+                if (j < V && keep[k]) {
+                    float t = 0.f;
+                    if (CAP) {
+                        t = ce_tanh<false>(z[k][j], o.cap);
+                        z[k][j] = o.cap * t;
+                    }
+                    d = fmaf(q.kz, ce_prob(z[k][j], q.lse), -q.e);
+                    if (y == j) d -= q.hit;
+                    if (CAP) d *= fmaf(-t, t, 1.f);
+                }
+                z[k][j] = d;
+            }
+            if (r < N) {
+#pragma unroll
+                for (int j = 0; j < VP; j += 4)
+                    if (j < V)
+                        *reinterpret_cast<float4 *>(p_out + r * ldp + j) = make_float4(
+                            z[k][j], z[k][j + 1], z[k][j + 2], z[k][j + 3]);
             }
         }
         if (!grad) continue;
-        for (int c = 4 * lane; c < D; c += 128) {
-            float4 out[kR];
+        // the table again, 32 channels at a time; the rows' gradients go out
+        // through the stage, a row's 128 bytes together
+        for (int i = 0; i < chunks; ++i) {
+            const int c0 = i * kDepth;
+            stage_table<VP, VEC>(st[0].w, weight, V, D, c0);
+            copies_end_group();
+            copies_wait<0>();
+            __syncthreads();
+#pragma unroll 2
+            for (int c = 0; c < kDepth; c += 4) {
+                float2 a[kR][2];
 #pragma unroll
-            for (int k = 0; k < kR; ++k) out[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < kR; ++k) a[k][0] = a[k][1] = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                if (j >= V) break;
-                const float4 w = *reinterpret_cast<const float4 *>(wide_smem + j * Dp + c);
+                for (int j = 0; j < VP; ++j) {
+                    if (j >= V) break;
+                    const float4 q = *reinterpret_cast<const float4 *>(&st[0].w[j][c]);
 #pragma unroll
-                for (int k = 0; k < kR; ++k) {
-                    out[k].x = fmaf(z[k][j], w.x, out[k].x);
-                    out[k].y = fmaf(z[k][j], w.y, out[k].y);
-                    out[k].z = fmaf(z[k][j], w.z, out[k].z);
-                    out[k].w = fmaf(z[k][j], w.w, out[k].w);
+                    for (int k = 0; k < kR; ++k) {
+                        a[k][0] = __ffma2_rn(f2(z[k][j]), make_float2(q.x, q.y), a[k][0]);
+                        a[k][1] = __ffma2_rn(f2(z[k][j]), make_float2(q.z, q.w), a[k][1]);
+                    }
                 }
-            }
-#pragma unroll
-            for (int k = 0; k < kR; ++k) {
-                if (r0 + k >= N) break;
                 // a row without a label is zero whatever the table holds
-                if (unlabelled >> k & 1) out[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                float *g = grad + (r0 + k) * D + c;
+#pragma unroll
+                for (int k = 0; k < kR; ++k)
+                    *reinterpret_cast<float4 *>(&st[0].x[k * kNT + threadIdx.x][c]) =
+                        keep[k] ? make_float4(a[k][0].x, a[k][0].y, a[k][1].x, a[k][1].y)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < kRows * (kDepth / 4); e += kNT) {
+                const int r = e / (kDepth / 4), c = e % (kDepth / 4) * 4;
+                if (r0 + r >= N || c0 + c >= D) continue;
+                const float4 v = *reinterpret_cast<const float4 *>(&st[0].x[r][c]);
+                float *to = grad + (r0 + r) * D + c0 + c;
                 if (VEC) {
-                    __stcs(reinterpret_cast<float4 *>(g), out[k]);
+                    __stcs(reinterpret_cast<float4 *>(to), v);
                 } else {
-                    g[0] = out[k].x;
-                    if (c + 1 < D) g[1] = out[k].y;
-                    if (c + 2 < D) g[2] = out[k].z;
-                    if (c + 3 < D) g[3] = out[k].w;
+                    to[0] = v.x;
+                    if (c0 + c + 1 < D) to[1] = v.y;
+                    if (c0 + c + 2 < D) to[2] = v.z;
+                    if (c0 + c + 3 < D) to[3] = v.w;
                 }
             }
+            __syncthreads();
         }
     }
 }
 
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float *p, int c, int D) {
+    if (VEC) return *reinterpret_cast<const float4 *>(p + c);
+    return make_float4(p[c], c + 1 < D ? p[c + 1] : 0.f, c + 2 < D ? p[c + 2] : 0.f,
+                       c + 3 < D ? p[c + 3] : 0.f);
+}
+
 template <int VP, bool VEC>
-__global__ void __launch_bounds__(kNT, 2)
+__global__ void __launch_bounds__(kDwNT, 2)
 wide_dw_kernel(long long N, int V, int D, const float *__restrict__ features,
                const long long *__restrict__ labels, long long ignore,
                const float *__restrict__ p, float *__restrict__ acc) {
+    constexpr int kPer = kDwRows / kDwWarps;
     __shared__ float4 sum[VP][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ldp = (V + 3) / 4 * 4;
+    __shared__ float4 ps[2][kDwRows][VP / 4];
+    __shared__ int keep[2][kDwRows];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, words = (V + 3) / 4;
     const int c = blockIdx.y * kChunk + 4 * lane;
     float4 a[VP];
 #pragma unroll
     for (int j = 0; j < VP; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-    // contiguous rows a warp, so that its derivatives are too
-    const long long warps = (long long)gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
-    const long long first = N * w / warps, last = N * (w + 1) / warps;
-#pragma unroll 2
-    for (long long r = first; r < last; ++r) {
-        const bool keep = labels[r] != ignore;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (keep && c < D) x = load4<VEC>(features + r * D, c, D);
-        const float4 *q = reinterpret_cast<const float4 *>(p + r * ldp);
+    int b = 0;
+    for (long long r0 = (long long)blockIdx.x * kDwRows; r0 < N;
+         r0 += (long long)gridDim.x * kDwRows, b ^= 1) {
+        // the tile's derivatives and which rows have a label; eight rows of
+        // features a warp on their way meanwhile
+        for (int i = threadIdx.x; i < kDwRows * words; i += kDwNT) {
+            const int r = i / words;
+            ps[b][r][i % words] =
+                r0 + r < N ? reinterpret_cast<const float4 *>(p)[(r0 + r) * words + i % words]
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (threadIdx.x < kDwRows)
+            keep[b][threadIdx.x] =
+                r0 + threadIdx.x < N && labels[r0 + threadIdx.x] != ignore;
+        float4 x[kPer];
 #pragma unroll
-        for (int j = 0; j < VP; j += 4) {
-            if (j >= V) break;
-            const float4 d = q[j / 4];
-            const float dv[4] = {d.x, d.y, d.z, d.w};
+        for (int k = 0; k < kPer; ++k) {
+            const long long r = r0 + warp * kPer + k;
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < N && c < D) x[k] = load4<VEC>(features + r * D, c, D);
+        }
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (j + i >= V) break;
-                a[j + i].x = fmaf(dv[i], x.x, a[j + i].x);
-                a[j + i].y = fmaf(dv[i], x.y, a[j + i].y);
-                a[j + i].z = fmaf(dv[i], x.z, a[j + i].z);
-                a[j + i].w = fmaf(dv[i], x.w, a[j + i].w);
+        for (int k = 0; k < kPer; ++k) {
+            const int r = warp * kPer + k;
+            if (!keep[b][r]) continue;  // the whole warp alike
+#pragma unroll
+            for (int j = 0; j < VP; j += 4) {
+                if (j >= V) break;
+                const float4 d = ps[b][r][j / 4];
+                const float dv[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    a[j + i].x = fmaf(dv[i], x[k].x, a[j + i].x);
+                    a[j + i].y = fmaf(dv[i], x[k].y, a[j + i].y);
+                    a[j + i].z = fmaf(dv[i], x[k].z, a[j + i].z);
+                    a[j + i].w = fmaf(dv[i], x[k].w, a[j + i].w);
+                }
             }
         }
     }
-    for (int k = 0; k < kWarps; ++k) {
+    for (int k = 0; k < kDwWarps; ++k) {
         if (warp == k) {
 #pragma unroll
             for (int j = 0; j < VP; ++j) {
@@ -257,7 +373,7 @@ wide_dw_kernel(long long N, int V, int D, const float *__restrict__ features,
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < V * kChunk; i += kNT) {
+    for (int i = threadIdx.x; i < V * kChunk; i += kDwNT) {
         const int j = i / kChunk, d = blockIdx.y * kChunk + i % kChunk;
         if (d < D)
             acc[((long long)blockIdx.x * V + j) * D + d] =
@@ -285,14 +401,14 @@ bool wide_rows(const NarrowArgs &a, const void *grad) {
                              reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
 }
 
-// the table's shared memory, allowed once a kernel and device
-template <typename K>
-cudaError_t allow_table(K kernel, std::atomic<unsigned long long> &ready) {
+// two stages of shared memory, allowed once a kernel and device
+template <int VP, typename K>
+cudaError_t allow_stages(K kernel, std::atomic<unsigned long long> &ready) {
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess || (ready.load() >> (dev & 63) & 1)) return err;
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)(kWideTable + 16 * kWideV));
+                               (int)(2 * sizeof(Stage<VP>)));
     if (err == cudaSuccess) ready.fetch_or(1ull << (dev & 63));
     return err;
 }
@@ -301,24 +417,23 @@ cudaError_t allow_table(K kernel, std::atomic<unsigned long long> &ready) {
 
 WideShape wide_shape(long long N, int V, int D) {
     WideShape s;
-    s.row_blocks = (int)std::min(ceil_div(N, kWarps * kR), 2LL * kSMs);
+    // three blocks an SM (two stages of 37 KB each)
+    s.row_blocks = (int)std::min(ceil_div(N, kRows), 3LL * kSMs);
     s.dw_chunks = (int)ceil_div(D, kChunk);
-    // parts of 64 rows a warp at least
     s.dw_blocks = (int)std::max(
-        1LL, std::min(ceil_div(N, kWarps * 64), std::max(1LL, 4LL * kSMs / s.dw_chunks)));
+        1LL, std::min(ceil_div(N, 4 * kDwRows), std::max(1LL, 2LL * kSMs / s.dw_chunks)));
     return s;
 }
 
 cudaError_t launch_wide_fwd(const NarrowArgs &a, float *loss, float2 *sums, cudaStream_t st) {
     return by_form(a.V, wide_rows(a, nullptr), a.opt.cap > 0.f, [&](auto vp, auto vec, auto cap) {
-        auto kernel =
-            wide_fwd_kernel<decltype(vp)::value, decltype(vec)::value, decltype(cap)::value>;
+        constexpr int VP = decltype(vp)::value;
+        auto kernel = wide_fwd_kernel<VP, decltype(vec)::value, decltype(cap)::value>;
         static std::atomic<unsigned long long> ready{0};
-        const cudaError_t err = allow_table(kernel, ready);
+        const cudaError_t err = allow_stages<VP>(kernel, ready);
         if (err != cudaSuccess) return err;
-        const int Dp = (a.D + 3) / 4 * 4;
-        kernel<<<wide_shape(a.N, a.V, a.D).row_blocks, kNT, sizeof(float) * a.V * Dp, st>>>(
-            a.N, a.V, a.D, Dp, static_cast<const float *>(a.features),
+        kernel<<<wide_shape(a.N, a.V, a.D).row_blocks, kNT, 2 * sizeof(Stage<VP>), st>>>(
+            a.N, a.V, a.D, static_cast<const float *>(a.features),
             static_cast<const float *>(a.weight), a.labels, a.opt, loss, a.lse, a.count, sums);
         count_launches(1);
         return cudaGetLastError();
@@ -328,14 +443,13 @@ cudaError_t launch_wide_fwd(const NarrowArgs &a, float *loss, float2 *sums, cuda
 cudaError_t launch_wide_dx(const NarrowArgs &a, const CeUpstream &u, float *grad, float *p,
                            cudaStream_t st) {
     return by_form(a.V, wide_rows(a, grad), a.opt.cap > 0.f, [&](auto vp, auto vec, auto cap) {
-        auto kernel =
-            wide_dx_kernel<decltype(vp)::value, decltype(vec)::value, decltype(cap)::value>;
+        constexpr int VP = decltype(vp)::value;
+        auto kernel = wide_dx_kernel<VP, decltype(vec)::value, decltype(cap)::value>;
         static std::atomic<unsigned long long> ready{0};
-        const cudaError_t err = allow_table(kernel, ready);
+        const cudaError_t err = allow_stages<VP>(kernel, ready);
         if (err != cudaSuccess) return err;
-        const int Dp = (a.D + 3) / 4 * 4;
-        kernel<<<wide_shape(a.N, a.V, a.D).row_blocks, kNT, sizeof(float) * a.V * Dp, st>>>(
-            a.N, a.V, a.D, Dp, static_cast<const float *>(a.features),
+        kernel<<<wide_shape(a.N, a.V, a.D).row_blocks, kNT, 2 * sizeof(Stage<VP>), st>>>(
+            a.N, a.V, a.D, static_cast<const float *>(a.features),
             static_cast<const float *>(a.weight), a.labels, a.opt, a.lse, u, grad, p);
         count_launches(1);
         return cudaGetLastError();
@@ -346,7 +460,7 @@ cudaError_t launch_wide_dw(const NarrowArgs &a, const float *p, float *acc, cuda
     return by_form(a.V, wide_rows(a, nullptr), false, [&](auto vp, auto vec, auto) {
         const WideShape s = wide_shape(a.N, a.V, a.D);
         wide_dw_kernel<decltype(vp)::value, decltype(vec)::value>
-            <<<dim3(s.dw_blocks, s.dw_chunks), kNT, 0, st>>>(
+            <<<dim3(s.dw_blocks, s.dw_chunks), kDwNT, 0, st>>>(
                 a.N, a.V, a.D, static_cast<const float *>(a.features), a.labels, a.opt.ignore, p,
                 acc);
         count_launches(1);

@@ -164,7 +164,8 @@ def test_linear_many_rows(dtype):
     run(70001, 4097, 16, dtype, dict(), ignored=0.2)
     run(300001, 20, 4, dtype, dict(reduction="sum"), ignored=0.1)
     run(200003, 11, 24, dtype, dict(reduction="none"), ignored=0.1)
-    run(100003, 7, 100, dtype, dict(smoothing=0.1, z_loss=1e-3), ignored=0.1)
+    for i, opt in enumerate(OPTS):
+        run(16384 + 129 * i, 3 * i + 1, [33, 100, 325, 64, 131, 440][i], dtype, opt, ignored=0.1)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -314,7 +315,7 @@ def test_one_gradient_alone(D, which):
 
 @pytest.mark.parametrize("n,V,D,dtype", [(3000, 20, 4, F32), (20000, 37, 0, BF16),
                                          (900, 5003, 64, BF16), (900, 503, 64, F32),
-                                         (9000, 9, 100, F32)])
+                                         (17000, 9, 100, F32)])
 def test_same_result_every_time(n, V, D, dtype):
     data, labels = make(n, V, D, dtype, 11, ignored=0.2)
     first = call(data, labels, {}, torch.ones((), device="cuda"))
@@ -347,7 +348,7 @@ def test_gradient_against_differences(n, V, D):
 
 @pytest.mark.parametrize("n,V,D,dtype", [(500, 20, 4, F32), (300, 37, 0, F32),
                                          (20, 3001, 0, BF16), (300, 1003, 72, BF16),
-                                         (300, 203, 32, F32), (300, 9, 100, F32)])
+                                         (300, 203, 32, F32), (17000, 9, 100, F32)])
 def test_capture_and_replay(n, V, D, dtype):
     """Forward and backward captured once and replayed on new contents,
     a second graph in between."""
