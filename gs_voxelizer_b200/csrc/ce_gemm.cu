@@ -14,8 +14,15 @@
 // (K-major); the gradients sum over rows or classes, the strided axis, and
 // read P, W and X in place as MN-major tiles. No operand is transposed.
 //
+// What bounds it: the power limit. The MMAs take 99.5 % of the cycles (8192 x
+// 32768 x 4096: 1.845 of 1.835 million ideal ones), the clock falls to what
+// 1000 W allow; 8192 x 131072 x 4096 takes 6.6 to 6.7 ms a product, 1.32
+// PFLOP/s, against 1.39 of a plain library product sustained. Small products
+// are bound by their turn-around, about 6 us a launch.
+//
 // Waits are bounded: on a timeout a role sets g_ce_error, leaves its loop and
-// the kernel ends, its tensor memory freed; the result is invalid.
+// the kernel ends, its copies done and its tensor memory freed; the result is
+// invalid.
 #include <cuda.h>
 
 #include <atomic>
@@ -372,6 +379,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 }
             }
         }
+        // After a timeout (seconds) a millisecond more for copies in flight.
+        for (int i = 0; !ok && i < 1000; ++i) __nanosleep(1000);
         // Every load is consumed, and every arrival at this CTA's barriers
         // has come, before the CTA may end.
         for (int i = 0; ok && i < kStages; ++i) {

@@ -10,12 +10,14 @@
 // multiplied into both gradients: dX += P W, dW += P^T X, accumulated in
 // float32 and rounded once.
 //
-// Rounding P to 16 bits costs at most half a unit of its last place
-// (2^-9 of the value in bf16, 2^-12 in fp16), which is below the rounding of
-// the gradients themselves to the same type. fp16 keeps P times a power of
-// two (see p_scale_of) so that small probabilities stay normal numbers.
-// float32 inputs keep three bf16 planes of every operand, which hold all 24
-// bits.
+// Rounding P to 16 bits costs at most half a step (2^-8 of the value in bf16,
+// 2^-11 in fp16), no more than rounding the gradients themselves to the same
+// type. fp16 keeps P times a power of two (see p_scale_of) so that small
+// probabilities stay normal numbers. float32 inputs keep three bf16 planes of
+// every operand, which hold all 24 bits.
+//
+// Few channels, few classes of many float32 channels, and few rows have
+// kernels of their own (see path_of).
 #include "ce_few.cuh"
 #include "ce_gemm.cuh"
 #include "ce_narrow.cuh"
@@ -91,7 +93,10 @@ index_kernel(long long n, long long padded, int V, const long long *__restrict__
         lab[r] = ce_label(y, ignore, V);
     }
     if (i >= all && i < padded) lab[i] = kCeIgnored;
-    if (i == 0) total[0] = (int)all;
+    if (i == 0) {
+        total[0] = (int)all;
+        total[1] = 0;  // the merge's ticket
+    }
 }
 
 // Splits a float into bf16 planes whose sum it is. Infinities and NaN live
@@ -178,10 +183,10 @@ pack_kernel(long long rows, int D, long long ld, long long plane, int cx,
 constexpr int kMergeNT = 256;
 
 // One row's (maximum, sum) pairs of all class runs -> lse and loss. SLICES
-// parts of the pairs run side by side for 256 / SLICES rows (a warp's, so
-// that one warp ends each row). LOG2: the maxima are exponents of two, and
-// stay so in lse. Rows are packed ones where idx is given: lse is kept as
-// they are, loss by original row, and the pairs are found by either (PACKED).
+// parts of the pairs run side by side for 256 / SLICES rows. LOG2: the maxima
+// are exponents of two, and stay so in lse. With idx the rows are packed ones:
+// lse is kept in their order, the loss goes to the original row, and the pairs
+// lie in either order (`packed`).
 template <bool LOG2, int SLICES>
 __global__ void __launch_bounds__(kMergeNT)
 merge_kernel(long long rows, int tiles, int V, bool packed, const float2 *__restrict__ part,
@@ -189,7 +194,8 @@ merge_kernel(long long rows, int tiles, int V, bool packed, const float2 *__rest
              const int *__restrict__ total, const int *__restrict__ idx,
              const int *__restrict__ lab, const long long *__restrict__ labels, CeOpt o,
              float *__restrict__ loss, float2 *__restrict__ lse_out,
-             float *__restrict__ count, float2 *__restrict__ block_sums) {
+             float *__restrict__ count, float2 *__restrict__ block_sums,
+             int *__restrict__ ticket) {
     constexpr int kRows = kMergeNT / SLICES;
     __shared__ float sm[SLICES][kRows], ss[SLICES][kRows], sz[SLICES][kRows];
     __shared__ float2 sh[kMergeNT / 32];
@@ -226,12 +232,45 @@ merge_kernel(long long rows, int tiles, int V, bool packed, const float2 *__rest
         if (o.reduction == kCeNone) loss[idx ? idx[r] : r] = l;
     }
     const float2 t = ce_block_sum<kMergeNT>(l, c, sh);
-    if (threadIdx.x == 0) {
-        if (gridDim.x == 1)
-            ce_finish(t.x, t.y, o.reduction, loss, count);
-        else
-            block_sums[blockIdx.x] = t;
+    if (gridDim.x == 1) {
+        if (threadIdx.x == 0) ce_finish(t.x, t.y, o.reduction, loss, count);
+        return;
     }
+    if (threadIdx.x == 0) block_sums[blockIdx.x] = t;
+    if (!ticket) return;
+    // the block that ends last sums all of them, in an order of its own that
+    // is the same whichever it is
+    __shared__ bool last;
+    __shared__ double sl[kMergeNT / 32], sc[kMergeNT / 32];
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(ticket, 1) == (int)gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double ls = 0.0, cs = 0.0;
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += kMergeNT) {
+        const float2 q = __ldcg(block_sums + i);
+        ls += q.x;
+        cs += q.y;
+    }
+#pragma unroll
+    for (int k = 16; k; k >>= 1) {
+        ls += __shfl_xor_sync(0xffffffffu, ls, k);
+        cs += __shfl_xor_sync(0xffffffffu, cs, k);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        sl[threadIdx.x >> 5] = ls;
+        sc[threadIdx.x >> 5] = cs;
+    }
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int k = 1; k < kMergeNT / 32; ++k) {
+        ls += sl[k];
+        cs += sc[k];
+    }
+    ce_finish(ls, cs, o.reduction, loss, count);
 }
 
 // few pairs a row: a thread a row; many: eight threads
@@ -242,12 +281,12 @@ void launch_merge(long long rows, long long grid_rows, int parts, int V, bool pa
                   const float2 *part,
                   const float *psum, const float *zt, const int *total, const int *idx,
                   const int *lab, const long long *labels, const CeOpt &o, float *loss,
-                  float2 *lse, float *count, float2 *sums, cudaStream_t st) {
+                  float2 *lse, float *count, float2 *sums, int *ticket, cudaStream_t st) {
     const int per = merge_rows(parts);
     const unsigned blocks = (unsigned)((grid_rows + per - 1) / per);
     const auto kernel = per == kMergeNT ? merge_kernel<LOG2, 1> : merge_kernel<LOG2, 8>;
     kernel<<<blocks, kMergeNT, 0, st>>>(rows, parts, V, packed, part, psum, zt, total, idx, lab, labels,
-                                        o, loss, lse, count, sums);
+                                        o, loss, lse, count, sums, ticket);
     count_launches(1);
 }
 
@@ -268,29 +307,40 @@ max_abs_kernel(const float *__restrict__ g, const int *__restrict__ idx,
         atomicMax(reinterpret_cast<int *>(out), __float_as_int(m));
 }
 
-// dst[idx[r]] = scale * sum over splits of acc[s][r], four columns a thread.
-// The rows are those of a piece: packed rows row0 .. row0 + rows. VEC: D is a
-// multiple of four and dst aligned to four elements.
-template <typename T, bool ROWS, bool VEC>
-__global__ void __launch_bounds__(256)
-finish_grad_kernel(long long row0, long long rows, int D, int cx, const float *__restrict__ acc,
-                   long long split, int splits, const int *__restrict__ idx,
-                   const int *__restrict__ total, CeUpstream upstream, T *__restrict__ dst) {
-    const long long r = (long long)blockIdx.x * (256 / cx) + threadIdx.x / cx;
-    if (r >= rows) return;
+// A gradient to be finished: dst[row of r] = scale * sum over splits of
+// acc[s][r], rows [0, rows) of a piece that begins at row0. Blocks of 256
+// threads, cx side by side in a row, four columns each. wide: D is a multiple
+// of four and dst aligned to four elements.
+struct FinishJob {
+    unsigned blocks;
+    int cx;
+    bool wide;
+    long long row0, rows;
+    const float *acc;
+    long long split;
+    int splits;
+    void *dst;
+};
+
+// ROWS: r is a packed row, and its place idx[row0 + r]
+template <typename T, bool ROWS>
+__device__ __forceinline__ void finish_block(const FinishJob &f, unsigned block, int D,
+                                             const int *idx, const int *total, float scale) {
+    const long long r = (long long)block * (256 / f.cx) + threadIdx.x / f.cx;
+    if (r >= f.rows) return;
     long long to = r;
     if (ROWS) {
-        if (row0 + r >= *total) return;
-        to = idx[row0 + r];
+        if (f.row0 + r >= *total) return;
+        to = idx[f.row0 + r];
     }
-    const float k = ce_grad_scale(upstream);
-    for (long long c = 4 * (threadIdx.x % cx); c < D; c += 4 * cx) {
-        const float *p = acc + r * D + c;
+    T *dst = static_cast<T *>(f.dst) + to * D;
+    for (long long c = 4 * (threadIdx.x % f.cx); c < D; c += 4 * f.cx) {
+        const float *p = f.acc + r * D + c;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (VEC) {
+        if (f.wide) {
 #pragma unroll 4
-            for (int s = 0; s < splits; ++s) {
-                const float4 q = *reinterpret_cast<const float4 *>(p + s * split);
+            for (int s = 0; s < f.splits; ++s) {
+                const float4 q = *reinterpret_cast<const float4 *>(p + s * f.split);
                 v[0] += q.x;
                 v[1] += q.y;
                 v[2] += q.z;
@@ -299,17 +349,61 @@ finish_grad_kernel(long long row0, long long rows, int D, int cx, const float *_
             struct alignas(4 * sizeof(T)) Out { T t[4]; };
             Out out;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out.t[i] = ce_from_float<T>(v[i] * k);
-            *reinterpret_cast<Out *>(dst + to * D + c) = out;
+            for (int i = 0; i < 4; ++i) out.t[i] = ce_from_float<T>(v[i] * scale);
+            *reinterpret_cast<Out *>(dst + c) = out;
         } else {
-            for (int s = 0; s < splits; ++s)
+            for (int s = 0; s < f.splits; ++s)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] += c + i < D ? p[s * split + i] : 0.f;
+                for (int i = 0; i < 4; ++i) v[i] += c + i < D ? p[s * f.split + i] : 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (c + i < D) dst[to * D + c + i] = ce_from_float<T>(v[i] * k);
+                if (c + i < D) dst[c + i] = ce_from_float<T>(v[i] * scale);
         }
     }
+}
+
+// Rows without a label: zero gradient, `bytes` a row. A warp reads 32 labels
+// and writes the rows among them.
+__device__ __forceinline__ void zero_block(unsigned block, long long n, long long bytes,
+                                           const long long *labels, long long ignore,
+                                           unsigned char *dst) {
+    const long long r = block * 256LL + threadIdx.x;
+    const int lane = threadIdx.x & 31;
+    unsigned rows = __ballot_sync(0xffffffffu, r < n && labels[r] == ignore);
+    while (rows) {
+        unsigned char *p = dst + (r - lane + __ffs(rows) - 1) * bytes;
+        rows &= rows - 1;
+        // whole words from the first aligned byte on (rows are of 2-byte
+        // elements at least)
+        const int head = (int)min((long long)(-reinterpret_cast<uintptr_t>(p) & 15), bytes);
+        for (int i = 2 * lane; i < head; i += 64) *reinterpret_cast<uint16_t *>(p + i) = 0;
+        const long long words = (bytes - head) / 16;
+        for (long long i = lane; i < words; i += 32)
+            reinterpret_cast<int4 *>(p + head)[i] = make_int4(0, 0, 0, 0);
+        for (long long i = head + 16 * words + 2 * lane; i < bytes; i += 64)
+            *reinterpret_cast<uint16_t *>(p + i) = 0;
+    }
+}
+
+// What is left of the gradients, in one launch: zero_blocks blocks for the
+// rows without a label, x.blocks for the features, w.blocks for the table.
+template <typename T>
+__global__ void __launch_bounds__(256)
+finish_kernel(long long n, int D, const long long *__restrict__ labels, long long ignore,
+              T *grad_features, unsigned zero_blocks, const int *__restrict__ idx,
+              const int *__restrict__ total, FinishJob x, FinishJob w, CeUpstream upstream) {
+    unsigned b = blockIdx.x;
+    if (b < zero_blocks) {
+        zero_block(b, n, (long long)D * sizeof(T), labels, ignore,
+                   reinterpret_cast<unsigned char *>(grad_features));
+        return;
+    }
+    b -= zero_blocks;
+    const float scale = ce_grad_scale(upstream);
+    if (b < x.blocks)
+        finish_block<T, true>(x, b, D, idx, total, scale);
+    else
+        finish_block<T, false>(w, b - x.blocks, D, idx, total, scale);
 }
 
 // dst[i] = sum over splits of acc[s][i], a thread each
@@ -341,29 +435,6 @@ reduce_splits_kernel(long long n, const float *__restrict__ acc, int splits,
     if (slice || i >= n) return;
     for (int s = 1; s < 32; ++s) v += sh[s][lane];
     dst[i] = ce_from_float<T>(v);
-}
-
-// Rows without a label: zero gradient. A warp reads 32 labels and writes the
-// rows among them, `bytes` each.
-__global__ void __launch_bounds__(256)
-zero_ignored_kernel(long long n, long long bytes, const long long *__restrict__ labels,
-                    long long ignore, unsigned char *__restrict__ dst) {
-    const long long r = blockIdx.x * 256LL + threadIdx.x;
-    const int lane = threadIdx.x & 31;
-    unsigned rows = __ballot_sync(0xffffffffu, r < n && labels[r] == ignore);
-    while (rows) {
-        unsigned char *p = dst + (r - lane + __ffs(rows) - 1) * bytes;
-        rows &= rows - 1;
-        // whole words from the first aligned byte on (rows are of 2-byte
-        // elements at least)
-        const int head = (int)min((long long)(-reinterpret_cast<uintptr_t>(p) & 15), bytes);
-        for (int i = 2 * lane; i < head; i += 64) *reinterpret_cast<uint16_t *>(p + i) = 0;
-        const long long words = (bytes - head) / 16;
-        for (long long i = lane; i < words; i += 32)
-            reinterpret_cast<int4 *>(p + head)[i] = make_int4(0, 0, 0, 0);
-        for (long long i = head + 16 * words + 2 * lane; i < bytes; i += 64)
-            *reinterpret_cast<uint16_t *>(p + i) = 0;
-    }
 }
 
 // ------------------------------------------------------------------- plan
@@ -530,33 +601,36 @@ cudaError_t pack_any(const Plan &p, bool rows, const void *src, const State &s, 
     }
 }
 
+FinishJob finish_job(const Plan &p, long long row0, long long rows, const float *acc,
+                     long long split, int splits, void *dst) {
+    const int size = p.type == kCeF32 ? 4 : 2;
+    const RowShape g = row_shape(rows, (p.D + 3) / 4);
+    const bool wide =
+        p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & (4 * size - 1)) == 0;
+    return {g.blocks, g.cx, wide, row0, rows, acc, split, splits, dst};
+}
+
 template <typename T>
-cudaError_t finish_grad(const Plan &p, bool rows, long long row0, long long n,
-                        const float *acc, long long split, int splits, const State &s,
-                        const CeUpstream &u, void *dst, cudaStream_t st) {
-    const bool vec = p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & (4 * sizeof(T) - 1)) == 0;
-    const RowShape g = row_shape(n, (p.D + 3) / 4);
-    const auto kernel =
-        rows ? (vec ? finish_grad_kernel<T, true, true> : finish_grad_kernel<T, true, false>)
-             : (vec ? finish_grad_kernel<T, false, true> : finish_grad_kernel<T, false, false>);
-    T *out = static_cast<T *>(dst) + (rows ? 0 : row0 * p.D);
-    kernel<<<g.blocks, 256, 0, st>>>(rows ? row0 : 0, n, p.D, g.cx, acc, split, splits, s.idx,
-                                     s.total, u, out);
+cudaError_t finish(const Plan &p, const State &s, const long long *labels, long long ignore,
+                   void *zero, const FinishJob &x, const FinishJob &w, const CeUpstream &u,
+                   cudaStream_t st) {
+    const unsigned zeros = zero ? (unsigned)((p.N + 255) / 256) : 0;
+    const unsigned blocks = zeros + x.blocks + w.blocks;
+    if (!blocks) return cudaSuccess;
+    finish_kernel<T><<<blocks, 256, 0, st>>>(p.N, p.D, labels, ignore, static_cast<T *>(zero),
+                                             zeros, s.idx, s.total, x, w, u);
     count_launches(1);
     return cudaGetLastError();
 }
 
-cudaError_t finish_any(const Plan &p, bool rows, long long row0, long long n,
-                       const float *acc, long long split, int splits, const State &s,
-                       const CeUpstream &u, void *dst, cudaStream_t st) {
-#define GSV_CE_T(T) \
-    finish_grad<T>(p, rows, row0, n, acc, split, splits, s, u, dst, st)
+cudaError_t finish_any(const Plan &p, const State &s, const long long *labels, long long ignore,
+                       void *zero, const FinishJob &x, const FinishJob &w, const CeUpstream &u,
+                       cudaStream_t st) {
     switch (p.type) {
-        case kCeF32: return GSV_CE_T(float);
-        case kCeBf16: return GSV_CE_T(__nv_bfloat16);
-        default: return GSV_CE_T(__half);
+        case kCeF32: return finish<float>(p, s, labels, ignore, zero, x, w, u, st);
+        case kCeBf16: return finish<__nv_bfloat16>(p, s, labels, ignore, zero, x, w, u, st);
+        default: return finish<__half>(p, s, labels, ignore, zero, x, w, u, st);
     }
-#undef GSV_CE_T
 }
 
 #define GSV_CE_TRY(expr)                              \
@@ -589,11 +663,6 @@ CeGemm gemm_of(const Plan &p, const State &s, const void *weight, unsigned char 
     g.idx = s.idx;
     return g;
 }
-
-}  // namespace
-
-
-namespace {
 
 // Workspace of the narrow path: per-block sums, parts of the class splits,
 // parts of dX, parts of dW.
@@ -643,7 +712,7 @@ cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
         blocks = (a.N + merge_rows(p.splits) - 1) / merge_rows(p.splits);
         const auto merge = a.opt.cap > 0.f ? launch_merge<false> : launch_merge<true>;
         merge(a.N, a.N, p.splits, a.V, false, part, psum, zt, nullptr, nullptr, nullptr, a.labels,
-              a.opt, loss, a.lse, a.count, sums, st);
+              a.opt, loss, a.lse, a.count, sums, nullptr, st);
         GSV_CE_TRY(cudaGetLastError());
     }
     if (blocks > 1)
@@ -681,10 +750,6 @@ cudaError_t narrow_backward(const NarrowArgs &a, const float *grad_loss, void *g
     return cudaSuccess;
 }
 
-}  // namespace
-
-namespace {
-
 // Workspace of the wide path: per-block sums; or P, then parts of dW.
 struct WidePlan {
     size_t dw, bytes;
@@ -715,7 +780,6 @@ cudaError_t wide_backward(const NarrowArgs &a, const float *grad_loss, void *gx,
     const WidePlan w = wide_plan(a.N, a.V, a.D, true);
     const CeUpstream u{grad_loss, a.count, nullptr, 1.f, a.opt.reduction};
     float *p = reinterpret_cast<float *>(ws), *dw = reinterpret_cast<float *>(ws + w.dw);
-    if (!gx && !gw) return cudaSuccess;
     GSV_CE_TRY(launch_wide_dx(a, u, static_cast<float *>(gx), p, st));
     if (!gw) return cudaSuccess;
     GSV_CE_TRY(launch_wide_dw(a, p, dw, st));
@@ -730,8 +794,8 @@ cudaError_t wide_backward(const NarrowArgs &a, const float *grad_loss, void *gx,
 // 10^6 rows x 20 classes, D = 16, 148 against 1311 and 134 against 530, D = 32,
 // 356 and 299 against 530 of bf16; 1000 rows x 50000 classes, D = 16, 267
 // against 472 and 250 against 160, D = 32, 584 against 480 of float32.
-// kWide: few classes, many float32 channels. kFew: the forward alone; its
-// backward takes tiles.
+// kWide: few classes, many float32 channels (linear_ce_wide.cu). kFew
+// (linear_ce_few.cu): the forward alone; its backward takes tiles.
 enum Path { kNarrow, kWide, kFew, kTiles };
 Path path_of(long long N, int V, int D, int type) {
     const int most = D <= 8 ? INT_MAX
@@ -840,9 +904,11 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     const bool indexed = !forward_only || !direct;
     launch_merge<false>(g.rows, N, 2 * p.runs, V, !direct, g.part, g.psum, g.zt,
                         indexed ? s.total : nullptr, indexed ? s.idx : nullptr,
-                        indexed ? s.lab : nullptr, labels, o, loss, s.lse, s.count, sums, st);
+                        indexed ? s.lab : nullptr, labels, o, loss, s.lse, s.count, sums,
+                        indexed ? s.total + 1 : nullptr, st);
     GSV_CE_TRY(cudaGetLastError());
-    if (mb > 1) GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));
+    if (mb > 1 && !indexed)
+        GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));
     return cudaSuccess;
 }
 
@@ -851,6 +917,7 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
                                       const long long *labels, const CeOpt &o, void *state,
                                       const float *grad_loss, void *grad_features,
                                       void *grad_weight, void *workspace, cudaStream_t st) {
+    if (!grad_features && !grad_weight) return cudaSuccess;
     const State s = state_of(state, N);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     if (path_of(N, V, D, type) == kNarrow) {
@@ -879,13 +946,6 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
         GSV_CE_TRY(cudaMemsetAsync(gmax, 0, sizeof(float), st));
         const int nb = (int)std::min<long long>(kSMs, (N + 1023) / 1024);
         max_abs_kernel<<<nb, 256, 0, st>>>(grad_loss, s.idx, s.total, gmax);
-        count_launches(1);
-        GSV_CE_TRY(cudaGetLastError());
-    }
-    if (grad_features) {
-        zero_ignored_kernel<<<(unsigned)((N + 255) / 256), 256, 0, st>>>(
-            N, (long long)D * (type == kCeF32 ? 4 : 2), labels, o.ignore,
-            static_cast<unsigned char *>(grad_features));
         count_launches(1);
         GSV_CE_TRY(cudaGetLastError());
     }
@@ -928,18 +988,28 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
                 w.add = r0 > 0;
                 w.dst = p.direct_w ? grad_weight : nullptr;
                 GSV_CE_TRY(launch_ce_gemm(w, st));
-                if (p.one_row_piece && !p.direct_w)
-                    GSV_CE_TRY(finish_any(p, false, v0, g.nv, dw, w_split, p.split_w, s, g.up,
-                                          grad_weight, st));
+                // one class piece of several: the buffer is the next one's
+                if (p.one_row_piece && !p.direct_w && p.piece_classes < V)
+                    GSV_CE_TRY(finish_any(
+                        p, s, labels, o.ignore, nullptr, FinishJob{},
+                        finish_job(p, 0, g.nv, dw, w_split, p.split_w,
+                                   static_cast<unsigned char *>(grad_weight) +
+                                       (size_t)v0 * D * (type == kCeF32 ? 4 : 2)),
+                        g.up, st));
             }
         }
-        if (grad_features && !p.direct_x)
-            GSV_CE_TRY(finish_any(p, true, r0, g.rows, dx, x_split, p.split_x, s, g.up,
-                                  grad_features, st));
+        if (grad_features && !p.direct_x && !p.one_row_piece)
+            GSV_CE_TRY(finish_any(
+                p, s, labels, o.ignore, nullptr,
+                finish_job(p, r0, g.rows, dx, x_split, p.split_x, grad_features), FinishJob{},
+                g.up, st));
     }
-    if (grad_weight && !p.one_row_piece)
-        GSV_CE_TRY(finish_any(p, false, 0, V, dw, w_split, p.split_w, s, g.up, grad_weight, st));
-    return cudaSuccess;
+    FinishJob x{}, w{};
+    if (grad_features && !p.direct_x && p.one_row_piece)
+        x = finish_job(p, 0, p.Np, dx, x_split, p.split_x, grad_features);
+    if (grad_weight && !p.direct_w && (!p.one_row_piece || p.piece_classes >= V))
+        w = finish_job(p, 0, V, dw, w_split, p.split_w, grad_weight);
+    return finish_any(p, s, labels, o.ignore, grad_features, x, w, g.up, st);
 }
 
 }  // namespace gsv
