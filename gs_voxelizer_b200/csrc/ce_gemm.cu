@@ -225,7 +225,7 @@ struct Unit {
 };
 
 // float32 products are accumulated in tensor memory over 512 of K at most
-// and summed in registers or memory from there: the tensor cores truncate
+// and summed in registers from there: the tensor cores truncate
 // each addition, which over 4000 of K cost 4e-6 of the result (16 at a time;
 // 5e-7 over 512). 16-bit results do not see it.
 constexpr int kChunk = 512 / kDepth;
@@ -457,8 +457,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         float *stage_out = reinterpret_cast<float *>(
             smem_raw + (smem0 - smem_addr(smem_raw)) + kStages * kStageBytes);
         if (PRODUCT >= kCeGradX) {
-            wide = g.D % (g.dst && !F32 ? 8 : 4) == 0 &&
-                   (reinterpret_cast<uintptr_t>(g.dst) & 15) == 0;
+            wide = !g.dst || (g.D % (F32 ? 4 : 8) == 0 &&
+                              (reinterpret_cast<uintptr_t>(g.dst) & 15) == 0);
             if (g.dst) scale = ce_grad_scale(g.up);
         }
         // a unit's row, read a unit ahead: units of few classes and channels
@@ -494,7 +494,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 e = o.eps / (float)g.V * f;
                 hit = (1.f - o.eps) * f;
             }
-            float sum[F32 && PRODUCT <= kCeProbs ? 2 : 1][32];
+            float sum[F32 ? 2 : 1][32];
             for (int i = 0; ok && i < t.steps(); ++i) {
                 const int n = t.n0 + i / t.chunks, chunk = i % t.chunks;
                 const bool last = chunk == t.chunks - 1;
@@ -505,8 +505,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     fence_after();
                 }
                 uint32_t v[32];
-#pragma unroll(F32 && PRODUCT <= kCeProbs ? 2 : 1)
-                for (int h = 0; h < (F32 && PRODUCT <= kCeProbs ? 2 : 4); ++h) {
+#pragma unroll(F32 ? 2 : 1)
+                for (int h = 0; h < (F32 ? 2 : 4); ++h) {
                     const int c = 2 * h + half;
                     if (c >= chunks) continue;
                     const int col0 = n * nt + c * 32;  // within the piece
@@ -517,7 +517,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         load32(tlane + acc * kCeTileN + c * 32, v);
                         load_wait(v);
                     }
-                    if constexpr (F32 && PRODUCT <= kCeProbs) {
+                    if constexpr (F32) {
                         if (t.chunks > 1) {
                             // the chunks of K, summed in float32
 #pragma unroll
@@ -598,49 +598,51 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         const long long M = PRODUCT == kCeGradW ? g.nv : w.live;
                         const int cols = min(32, g.D - col0);
                         const bool direct = g.dst != nullptr;
-                        const bool add = !direct && (g.add || chunk > 0);
+                        const bool add = !direct && g.add;
                         long long to = r;  // row of the output
                         if (direct && PRODUCT == kCeGradX && r < M)
                             to = g.idx ? g.idx[g.row0 + r] : g.row0 + r;
                         if (direct && PRODUCT == kCeGradW) to += g.v0;
-                        to *= g.D;
+                        to *= direct ? g.D : g.acc_ld;
                         // float32 sums, or float32 gradients; 16-bit gradients
                         float *out32 = F32 && direct ? static_cast<float *>(g.dst)
                                                      : g.acc + t.split * g.acc_split;
                         uint16_t *out16 = static_cast<uint16_t *>(g.dst);
                         if (wide) {
-                            if (r < M) {
+                            if (r < M && !F32 && direct) {
 #pragma unroll
                                 for (int j = 0; j < 32; j += 8) {
                                     if (j >= cols) continue;
-                                    if (!F32 && direct) {
-                                        uint32_t out[4];
+                                    uint32_t out[4];
 #pragma unroll
-                                        for (int i = 0; i < 4; ++i)
-                                            out[i] = pack2(
-                                                __uint_as_float(v[j + 2 * i]) * scale,
-                                                __uint_as_float(v[j + 2 * i + 1]) * scale,
-                                                g.bf16);
-                                        store4(out16 + to + col0 + j, out);
-                                        continue;
-                                    }
+                                    for (int i = 0; i < 4; ++i)
+                                        out[i] = pack2(__uint_as_float(v[j + 2 * i]) * scale,
+                                                       __uint_as_float(v[j + 2 * i + 1]) * scale,
+                                                       g.bf16);
+                                    store4(out16 + to + col0 + j, out);
+                                }
+                            } else if (r < M) {
+                                float4 *p = reinterpret_cast<float4 *>(out32 + to + col0);
+                                // all reads before the first write: one latency
+                                float4 old[8];
 #pragma unroll
-                                    for (int q = j; q < j + 8; q += 4) {
-                                        if (q >= cols) continue;
-                                        float *p = out32 + to + col0 + q;
-                                        float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
-                                        if (add) old = *reinterpret_cast<const float4 *>(p);
-                                        *reinterpret_cast<float4 *>(p) = make_float4(
-                                            fmaf(__uint_as_float(v[q]), scale, old.x),
-                                            fmaf(__uint_as_float(v[q + 1]), scale, old.y),
-                                            fmaf(__uint_as_float(v[q + 2]), scale, old.z),
-                                            fmaf(__uint_as_float(v[q + 3]), scale, old.w));
-                                    }
+                                for (int j = 0; j < 8; ++j) {
+                                    old[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                    if (add && 4 * j < cols) old[j] = p[j];
+                                }
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    if (4 * j >= cols) continue;
+                                    p[j] = make_float4(
+                                        fmaf(__uint_as_float(v[4 * j]), scale, old[j].x),
+                                        fmaf(__uint_as_float(v[4 * j + 1]), scale, old[j].y),
+                                        fmaf(__uint_as_float(v[4 * j + 2]), scale, old[j].z),
+                                        fmaf(__uint_as_float(v[4 * j + 3]), scale, old[j].w));
                                 }
                             }
                         } else if (cols > 0) {
-                            // rows of no alignment: the warp turns its 32 x 32
-                            // and writes row by row
+                            // gradients of no alignment: the warp turns its 32
+                            // x 32 and writes row by row
                             float *turn = stage_out + (warp - 4) * 32 * 33;
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
@@ -652,10 +654,10 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                                 const long long at = __shfl_sync(0xffffffffu, to, i) + col0 + lane;
                                 const float x = turn[i * 33 + lane];
                                 if (lane < cols) {
-                                    if (!F32 && direct)
-                                        out16[at] = (uint16_t)pack2(x, 0.f, g.bf16);
+                                    if (F32)
+                                        out32[at] = x;
                                     else
-                                        out32[at] = (add ? out32[at] : 0.f) + x;
+                                        out16[at] = (uint16_t)pack2(x, 0.f, g.bf16);
                                 }
                             }
                             __syncwarp();
@@ -727,15 +729,12 @@ bool make_map(CUtensorMap *map, const CeMat &m, int planes, bool bf16, int box_r
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// columns of a gradient's tile (MN-major B: multiples of 128)
-int tile_n(int cols) { return cols <= 128 ? 128 : kCeTileN; }
-
 // Classes of a tile of scores: the width, in steps of 32, with which the pairs
 // are done first. A tile costs its width, below 64 no less (A's rows are read
 // all the same), and about 32 to turn around: 256 where there is much to do,
 // 160 for 1001 rows x 5003 classes (2 rounds instead of 2 wider ones), 64 for
-// 18 rows x 3021 (48 tiles instead of 24 at the same memory). float32 keeps a
-// tile's sums in registers, 64 a thread: 128 at most.
+// 18 rows x 3021 (48 tiles instead of 24 at the same memory). float32: 128
+// at most, as for the gradients.
 int score_tile(long long rows, int nv, bool f32) {
     const long long mt = (rows + kCeTileM - 1) / kCeTileM;
     int best = 32;
@@ -755,7 +754,7 @@ int score_tile(long long rows, int nv, bool f32) {
 template <int PRODUCT, bool CAP, bool F32>
 cudaError_t launch(const CeGemm &g, cudaStream_t st) {
     constexpr bool kAMn = PRODUCT == kCeGradW, kBMn = PRODUCT >= kCeGradX;
-    const int nt = kBMn ? tile_n(g.D) : score_tile(g.rows, g.nv, F32);
+    const int nt = kBMn ? ce_grad_tile(g.D, F32) : score_tile(g.rows, g.nv, F32);
     CUtensorMap a, b;
     const CeMat &ma = PRODUCT >= kCeGradX ? g.P : g.X;
     const CeMat &mb = PRODUCT == kCeGradW ? g.X : g.W;
@@ -786,6 +785,11 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
 }
 
 }  // namespace
+
+// Columns of a gradient's tile (MN-major B: multiples of 128). float32 keeps
+// a tile's sums in registers, 64 a thread: 128 at most. (256 wide, summed in
+// memory a chunk at a time: 42765 x 26421 x 621, 16 + 20 ms a step, now 11 + 11.)
+int ce_grad_tile(int cols, bool f32) { return f32 || cols <= 128 ? 128 : kCeTileN; }
 
 int ce_runs(long long rows, int V, bool f32) {
     const long long mt = (rows + kCeTileM - 1) / kCeTileM;

@@ -68,10 +68,10 @@ struct CeGemm {
     float p_scale;
     const float *grow;  // upstream gradient by original row, or null
     const float *gmax;  // or null
-    // kCeGradX, kCeGradW: acc[split][m][D] (+)= product, or, with dst set (of
-    // float32: K of at most 512), dst[row of m][D] = scale * product in the
-    // inputs' type
+    // kCeGradX, kCeGradW: acc[split][m][acc_ld] (+)= product, or, with dst set,
+    // dst[row of m][D] = scale * product in the inputs' type
     float *acc;
+    long long acc_ld;     // elements between rows: D in whole 16-byte words
     long long acc_split;  // elements between splits
     int splits;
     bool add;
@@ -85,6 +85,8 @@ constexpr int kCePairs = kSMs / 2;  // tiles in flight: a pair of SMs each
 
 // runs of class tiles for the forward: (rows of) partial sums and balance
 int ce_runs(long long rows, int V, bool f32);
+// columns of a gradient's tile
+int ce_grad_tile(int cols, bool f32);
 
 cudaError_t launch_ce_gemm(const CeGemm &g, cudaStream_t stream);
 

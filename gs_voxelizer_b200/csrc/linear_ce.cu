@@ -308,16 +308,16 @@ max_abs_kernel(const float *__restrict__ g, const int *__restrict__ idx,
 }
 
 // A gradient to be finished: dst[row of r] = scale * sum over splits of
-// acc[s][r], rows [0, rows) of a piece that begins at row0. Blocks of 256
-// threads, cx side by side in a row, four columns each. wide: D is a multiple
-// of four and dst aligned to four elements.
+// acc[s][r], rows [0, rows) of a piece that begins at row0, acc's of ld floats
+// (a multiple of four). Blocks of 256 threads, cx side by side in a row, four
+// columns each. wide: D is a multiple of four and dst aligned to four elements.
 struct FinishJob {
     unsigned blocks;
     int cx;
     bool wide;
     long long row0, rows;
     const float *acc;
-    long long split;
+    long long ld, split;
     int splits;
     void *dst;
 };
@@ -335,26 +335,23 @@ __device__ __forceinline__ void finish_block(const FinishJob &f, unsigned block,
     }
     T *dst = static_cast<T *>(f.dst) + to * D;
     for (long long c = 4 * (threadIdx.x % f.cx); c < D; c += 4 * f.cx) {
-        const float *p = f.acc + r * D + c;
+        const float *p = f.acc + r * f.ld + c;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (f.wide) {
 #pragma unroll 4
-            for (int s = 0; s < f.splits; ++s) {
-                const float4 q = *reinterpret_cast<const float4 *>(p + s * f.split);
-                v[0] += q.x;
-                v[1] += q.y;
-                v[2] += q.z;
-                v[3] += q.w;
-            }
+        for (int k = 0; k < f.splits; ++k) {
+            const float4 q = *reinterpret_cast<const float4 *>(p + k * f.split);
+            v[0] += q.x;
+            v[1] += q.y;
+            v[2] += q.z;
+            v[3] += q.w;
+        }
+        if (f.wide) {
             struct alignas(4 * sizeof(T)) Out { T t[4]; };
             Out out;
 #pragma unroll
             for (int i = 0; i < 4; ++i) out.t[i] = ce_from_float<T>(v[i] * scale);
             *reinterpret_cast<Out *>(dst + c) = out;
         } else {
-            for (int s = 0; s < f.splits; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] += c + i < D ? p[s * f.split + i] : 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (c + i < D) dst[c + i] = ce_from_float<T>(v[i] * scale);
@@ -564,16 +561,17 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     const bool one_class_piece = p.piece_classes >= V;
     p.piece_rows = std::min(p.piece_rows, p.Np);
     p.p = take((size_t)p.planes * p.piece_rows * p.ldp * 2);
-    const long long tn = (D + kCeTileN - 1) / kCeTileN;
+    const int nt = ce_grad_tile(D, p.planes == 3);
+    const long long tn = (D + nt - 1) / nt;
     p.split_x = splits_for(p.piece_rows / kCeTileM * tn, p.piece_classes);
     p.split_w = splits_for(up(p.piece_classes, kCeTileM) / kCeTileM * tn, p.piece_rows);
-    // (float32 sums of more than 512 terms are joined in memory)
-    p.direct_x = one_class_piece && p.split_x == 1 && (p.planes == 1 || V <= 512);
-    p.direct_w = p.one_row_piece && p.split_w == 1 && (p.planes == 1 || p.Np <= 512);
-    p.dx = take(p.direct_x ? 0 : sizeof(float) * (size_t)p.split_x * p.piece_rows * D);
+    p.direct_x = one_class_piece && p.split_x == 1;
+    p.direct_w = p.one_row_piece && p.split_w == 1;
+    const size_t lda = (size_t)up(D, 4);  // of the float32 sums
+    p.dx = take(p.direct_x ? 0 : sizeof(float) * (size_t)p.split_x * p.piece_rows * lda);
     p.dw = take(p.direct_w ? 0
                            : sizeof(float) * (size_t)p.split_w *
-                                 (p.one_row_piece ? p.piece_classes : V) * D);
+                                 (p.one_row_piece ? p.piece_classes : V) * lda);
     p.bytes = at;
     return p;
 }
@@ -607,7 +605,7 @@ FinishJob finish_job(const Plan &p, long long row0, long long rows, const float 
     const RowShape g = row_shape(rows, (p.D + 3) / 4);
     const bool wide =
         p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & (4 * size - 1)) == 0;
-    return {g.blocks, g.cx, wide, row0, rows, acc, split, splits, dst};
+    return {g.blocks, g.cx, wide, row0, rows, acc, up(p.D, 4), split, splits, dst};
 }
 
 template <typename T>
@@ -958,8 +956,9 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
     g.up = {grad_loss, s.count, gmax, 1.f / g.p_scale, o.reduction};
     float *dx = reinterpret_cast<float *>(ws + p.dx);
     float *dw = reinterpret_cast<float *>(ws + p.dw);
-    const long long x_split = p.piece_rows * D;
-    const long long w_split = (long long)(p.one_row_piece ? p.piece_classes : V) * D;
+    g.acc_ld = up(D, 4);
+    const long long x_split = p.piece_rows * g.acc_ld;
+    const long long w_split = (long long)(p.one_row_piece ? p.piece_classes : V) * g.acc_ld;
     for (long long r0 = 0; r0 < p.Np; r0 += p.piece_rows) {
         g.row0 = r0;
         g.rows = std::min(p.piece_rows, p.Np - r0);
@@ -983,7 +982,7 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
                 CeGemm w = g;
                 w.product = kCeGradW;
                 w.splits = p.split_w;
-                w.acc = p.one_row_piece ? dw : dw + (long long)v0 * D;
+                w.acc = p.one_row_piece ? dw : dw + (long long)v0 * g.acc_ld;
                 w.acc_split = w_split;
                 w.add = r0 > 0;
                 w.dst = p.direct_w ? grad_weight : nullptr;
