@@ -7,7 +7,8 @@
 // a stage; the leader's MMA thread multiplies both halves. 256 x 256 tiles
 // need 32 KB of operands a stage and SM for 2 x 256 x 256 x 64 products, two
 // thirds of what 128 x 256 tiles of a single SM load: the L2 could not feed
-// those at the tensor cores' rate. Two accumulators alternate, so that the
+// those at the tensor cores' rate. (float32: 256 x 128 tiles of three planes,
+// 72 KB of operands for six products.) Two accumulators alternate, so that the
 // epilogue of a tile (eight warps) runs under the next tile's products.
 //
 // Operand layouts: X W^T reads both operands along the contiguous axis
@@ -17,7 +18,8 @@
 // What bounds it: the power limit. The MMAs take 99.5 % of the cycles (8192 x
 // 32768 x 4096: 1.845 of 1.835 million ideal ones), the clock falls to what
 // 1000 W allow; 8192 x 131072 x 4096 takes 6.6 to 6.7 ms a product, 1.32
-// PFLOP/s, against 1.39 of a plain library product sustained. Small products
+// PFLOP/s, against 1.39 of a plain library product sustained (42765 x 26421 x
+// 621 in float32, six products each: 5.6 to 8.0 ms, 1.50 to 1.06 PFLOP/s). Small products
 // are bound by their turn-around, about 6 us a launch.
 //
 // Waits are bounded: on a timeout a role sets g_ce_error, leaves its loop and
@@ -37,19 +39,31 @@ __device__ int g_ce_error = 0;
 
 namespace {
 
-constexpr int kStages = 6;
 constexpr int kDepth = 64;                       // K a stage
-constexpr int kABytes = 128 * kDepth * 2;        // per CTA
-constexpr int kStageBytes = 2 * kABytes;         // A and B halves
+constexpr int kABytes = 128 * kDepth * 2;        // per CTA and plane
 constexpr int kEpiWarps = 8;
-// stages, their alignment, and a 32 x 32 turn a warp for the gradients
-constexpr int kSmemBytes = kStages * kStageBytes + 1024 + kEpiWarps * 32 * 33 * 4;
+// A stage holds all planes of its A and B halves: six plane pairs are
+// multiplied out of one float32 stage, which is half the loads of a stage a
+// pair (those bound the tiles of 128 columns at 1.09 PFLOP/s).
+template <bool F32>
+struct Shape {
+    static constexpr int kPlanes = F32 ? 3 : 1;
+    static constexpr int kStages = F32 ? 3 : 6;
+    static constexpr int kTile = F32 ? 128 : kCeTileN;  // columns, at most
+    static constexpr int kBBytes = kTile / 2 * kDepth * 2;
+    static constexpr int kStageBytes = kPlanes * (kABytes + kBBytes);
+    // rows of 32 that a warp turns at a time
+    static constexpr int kTurn = F32 ? 8 : 32;
+    static constexpr int kSmemBytes =
+        kStages * kStageBytes + 1024 + kEpiWarps * kTurn * 33 * 4;
+};
+constexpr int kMaxStages = 6;
 constexpr int kThreads = (4 + kEpiWarps) * 32;
 constexpr int kCols = 512;
 constexpr int kSpinLimit = 1 << 24;
 
 struct Barriers {
-    uint64_t full[kStages], empty[kStages], tfull[2], tempty[2];
+    uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2];
     uint32_t tmem;
 };
 
@@ -276,16 +290,13 @@ struct RowInfo {
     float g;
 };
 
-// Plane pairs of a float32 product, least first: (2,0) (0,2) (1,1) (1,0)
-// (0,1) (0,0). The pairs left out are below 2^-26 of the whole.
-template <bool F32>
-__device__ __forceinline__ int plane_a(int p) {
-    return F32 ? (0x001102 >> (4 * p)) & 3 : 0;
-}
-template <bool F32>
-__device__ __forceinline__ int plane_b(int p) {
-    return F32 ? (0x010120 >> (4 * p)) & 3 : 0;
-}
+// Plane pairs of a float32 product: (2,0) (0,2) (1,1) (1,0) (0,1), summed in
+// an accumulator of their own beside the first, and (0,0): what the tensor
+// cores truncate is relative to the sum at hand. The pairs left out are below
+// 2^-26 of the whole.
+constexpr int kPairs32 = 6;
+__device__ __forceinline__ constexpr int plane_a(int p) { return (0x001102 >> (4 * p)) & 3; }
+__device__ __forceinline__ constexpr int plane_b(int p) { return (0x010120 >> (4 * p)) & 3; }
 
 // F32: three planes
 template <int PRODUCT, bool CAP, bool F32>
@@ -294,6 +305,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                const CeGemm g, const int nt) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ Barriers S;
+    using Sh = Shape<F32>;
+    constexpr int kStages = Sh::kStages, kStageBytes = Sh::kStageBytes;
     // the same offset in both CTAs: the MMA reads both through one descriptor
     const uint32_t smem0 = (smem_addr(smem_raw) + 1023) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -326,14 +339,13 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     fence_after();
     const uint32_t tmem = S.tmem;
     const Work w = work_of<PRODUCT>(g, nt);
-    const int pairs = F32 ? 6 : 1;
 
     if (warp == 0 && elect_one()) {
         // ------------------------------------------------------ producer
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        const uint32_t bytes = 2 * (kABytes + nt / 2 * kDepth * 2);
+        const uint32_t bytes = 2 * Sh::kPlanes * (kABytes + nt / 2 * kDepth * 2);
         for (int u = first; ok && u < w.units; u += step) {
             const Unit t = unit_of<PRODUCT, F32>(g, w, u);
             const int m_at = t.m * kCeTileM + (int)rank * 128;
@@ -341,40 +353,42 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const int n_at = (t.n0 + i / t.chunks) * nt + (int)rank * (nt / 2);
                 const int k0 = t.k0 + (F32 ? i % t.chunks * kChunk : 0);
                 const int k1 = F32 ? min(t.k1, k0 + kChunk) : t.k1;
-                for (int p = 0; ok && p < pairs; ++p) {
-                    const int pa = plane_a<F32>(p), pb = plane_b<F32>(p);
-                    for (int k = k0; k < k1; ++k) {
-                        if (!bar_wait(&S.empty[stage], phase ^ 1)) {
-                            ok = false;
-                            break;
-                        }
-                        const uint32_t bar = in_leader(smem_addr(&S.full[stage]));
-                        const uint32_t a = smem0 + stage * kStageBytes, b = a + kABytes;
-                        if (rank == 0)
-                            asm volatile(
-                                "mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
-                                    smem_addr(&S.full[stage])),
-                                "r"(bytes)
-                                : "memory");
-                        const int kk = k * kDepth;
+                for (int k = k0; k < k1; ++k) {
+                    if (!bar_wait(&S.empty[stage], phase ^ 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = in_leader(smem_addr(&S.full[stage]));
+                    if (rank == 0)
+                        asm volatile(
+                            "mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                                smem_addr(&S.full[stage])),
+                            "r"(bytes)
+                            : "memory");
+                    const int kk = k * kDepth;
+#pragma unroll
+                    for (int p = 0; p < Sh::kPlanes; ++p) {
+                        const uint32_t a = smem0 + stage * kStageBytes + p * kABytes;
+                        const uint32_t b = smem0 + stage * kStageBytes +
+                                           Sh::kPlanes * kABytes + p * Sh::kBBytes;
                         if (kAMn) {
-                            tma_load(&map_a, a, bar, m_at, kk, pa);
-                            tma_load(&map_a, a + 8192, bar, m_at + 64, kk, pa);
+                            tma_load(&map_a, a, bar, m_at, kk, p);
+                            tma_load(&map_a, a + 8192, bar, m_at + 64, kk, p);
                         } else {
                             const long long r0 = PRODUCT == kCeGradX ? 0 : g.row0;
-                            tma_load(&map_a, a, bar, kk, (int)(r0 + m_at), pa);
+                            tma_load(&map_a, a, bar, kk, (int)(r0 + m_at), p);
                         }
                         if (kBMn) {
                             const int r0 = PRODUCT == kCeGradX ? g.v0 : (int)g.row0;
                             for (int h = 0; h < nt / 2; h += 64)
-                                tma_load(&map_b, b + h * 128, bar, n_at + h, r0 + kk, pb);
+                                tma_load(&map_b, b + h * 128, bar, n_at + h, r0 + kk, p);
                         } else {
-                            tma_load(&map_b, b, bar, kk, g.v0 + n_at, pb);
+                            tma_load(&map_b, b, bar, kk, g.v0 + n_at, p);
                         }
-                        if (++stage == kStages) {
-                            stage = 0;
-                            phase ^= 1;
-                        }
+                    }
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
                     }
                 }
             }
@@ -411,31 +425,38 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     break;
                 }
                 fence_after();
-                uint32_t accumulate = 0;
-                for (int p = 0; ok && p < pairs; ++p)
-                    for (int k = k0; k < k1; ++k) {
-                        if (!bar_wait(&S.full[stage], phase)) {
-                            ok = false;
-                            break;
-                        }
-                        fence_after();
-                        const uint32_t a = smem0 + stage * kStageBytes;
-                        uint64_t da = tile_desc(a, kAMn), db = tile_desc(a + kABytes, kBMn);
-                        // the last block may end early (its rest is zeros)
-                        const long long left = w.K - (long long)k * kDepth;
-                        const int steps = left >= kDepth ? 4 : (int)((left + 15) / 16);
+                const uint32_t d = tmem + acc * kCeTileN;
+                for (int k = k0; k < k1; ++k) {
+                    if (!bar_wait(&S.full[stage], phase)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_after();
+                    const uint32_t a = smem0 + stage * kStageBytes;
+                    const uint32_t b = a + Sh::kPlanes * kABytes;
+                    // the last block may end early (its rest is zeros)
+                    const long long left = w.K - (long long)k * kDepth;
+                    const int steps = left >= kDepth ? 4 : (int)((left + 15) / 16);
+#pragma unroll
+                    for (int p = 0; p < (F32 ? kPairs32 : 1); ++p) {
+                        const int pa = F32 ? plane_a(p) : 0, pb = F32 ? plane_b(p) : 0;
+                        uint64_t da = tile_desc(a + pa * kABytes, kAMn);
+                        uint64_t db = tile_desc(b + pb * Sh::kBBytes, kBMn);
+                        const bool small = F32 && p < kPairs32 - 1;
+                        uint32_t accumulate = k > k0 || (small && p > 0);
                         for (int j = 0; j < steps; ++j) {
-                            mma(tmem + acc * kCeTileN, da, db, idesc, accumulate);
+                            mma(d + (small ? Sh::kTile : 0), da, db, idesc, accumulate);
                             accumulate = 1;
                             da += k_step(kAMn);
                             db += k_step(kBMn);
                         }
-                        commit(&S.empty[stage]);
-                        if (++stage == kStages) {
-                            stage = 0;
-                            phase ^= 1;
-                        }
                     }
+                    commit(&S.empty[stage]);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
                 commit(&S.tfull[acc]);
                 if (++acc == 2) {
                     acc = 0;
@@ -518,16 +539,22 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         load_wait(v);
                     }
                     if constexpr (F32) {
-                        if (t.chunks > 1) {
-                            // the chunks of K, summed in float32
+                        // both accumulators and the chunks of K, in float32
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const float a = __uint_as_float(v[j]);
-                                sum[h][j] = chunk ? sum[h][j] + a : a;
-                                v[j] = __float_as_uint(sum[h][j]);
-                            }
-                            if (!last) continue;
+                        for (int j = 0; j < 32; ++j) {
+                            const float a = __uint_as_float(v[j]);
+                            sum[h][j] = chunk ? sum[h][j] + a : a;
                         }
+                        if (!empty) {
+                            load32(tlane + acc * kCeTileN + Sh::kTile + c * 32, v);
+                            load_wait(v);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            sum[h][j] += __uint_as_float(v[j]);
+                            v[j] = __float_as_uint(sum[h][j]);
+                        }
+                        if (!last) continue;
                     }
                     if constexpr (PRODUCT == kCeScores) {
                         const int valid = g.nv - col0;
@@ -643,24 +670,30 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         } else if (cols > 0) {
                             // gradients of no alignment: the warp turns its 32
                             // x 32 and writes row by row
-                            float *turn = stage_out + (warp - 4) * 32 * 33;
+                            float *turn = stage_out + (warp - 4) * Sh::kTurn * 33;
+                            const int n_rows = (int)max(0LL, min(32LL, M - (r - lane)));
+#pragma unroll 1
+                            for (int i0 = 0; i0 < n_rows; i0 += Sh::kTurn) {
+                                if (lane / Sh::kTurn == i0 / Sh::kTurn) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                turn[lane * 33 + j] = __uint_as_float(v[j]) * scale;
-                            __syncwarp();
-                            const long long first_row = r - lane;
-                            const int n_rows = (int)max(0LL, min(32LL, M - first_row));
-                            for (int i = 0; i < n_rows; ++i) {
-                                const long long at = __shfl_sync(0xffffffffu, to, i) + col0 + lane;
-                                const float x = turn[i * 33 + lane];
-                                if (lane < cols) {
-                                    if (F32)
-                                        out32[at] = x;
-                                    else
-                                        out16[at] = (uint16_t)pack2(x, 0.f, g.bf16);
+                                    for (int j = 0; j < 32; ++j)
+                                        turn[lane % Sh::kTurn * 33 + j] =
+                                            __uint_as_float(v[j]) * scale;
                                 }
+                                __syncwarp();
+                                for (int i = i0; i < min(n_rows, i0 + Sh::kTurn); ++i) {
+                                    const long long at =
+                                        __shfl_sync(0xffffffffu, to, i) + col0 + lane;
+                                    const float x = turn[(i - i0) * 33 + lane];
+                                    if (lane < cols) {
+                                        if (F32)
+                                            out32[at] = x;
+                                        else
+                                            out16[at] = (uint16_t)pack2(x, 0.f, g.bf16);
+                                    }
+                                }
+                                __syncwarp();
                             }
-                            __syncwarp();
                         }
                     }
                 }
@@ -769,7 +802,7 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
     if (err != cudaSuccess) return err;
     if (!(ready.load() >> (dev & 63) & 1)) {
         err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   kSmemBytes);
+                                   Shape<F32>::kSmemBytes);
         if (err != cudaSuccess) return err;
         ready.fetch_or(1ull << (dev & 63));
     }
@@ -779,7 +812,7 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
     const long long units =
         mt * (PRODUCT == kCeScores ? g.runs : (n + nt - 1) / nt * g.splits);
     const int grid = 2 * (int)std::min<long long>(kCePairs, units);
-    kernel<<<grid, kThreads, kSmemBytes, st>>>(a, b, g, nt);
+    kernel<<<grid, kThreads, Shape<F32>::kSmemBytes, st>>>(a, b, g, nt);
     count_launches(1);
     return cudaGetLastError();
 }
@@ -788,7 +821,8 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
 
 // Columns of a gradient's tile (MN-major B: multiples of 128). float32 keeps
 // a tile's sums in registers, 64 a thread: 128 at most. (256 wide, summed in
-// memory a chunk at a time: 42765 x 26421 x 621, 16 + 20 ms a step, now 11 + 11.)
+// memory a chunk at a time, the two gradients of 42765 x 26421 x 621 took 36
+// ms, with the planes loaded once a stage 16.)
 int ce_grad_tile(int cols, bool f32) { return f32 || cols <= 128 ? 128 : kCeTileN; }
 
 int ce_runs(long long rows, int V, bool f32) {
