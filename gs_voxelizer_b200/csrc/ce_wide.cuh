@@ -12,17 +12,22 @@ constexpr int kWideV = 16;  // classes at most
 constexpr long long kWideRows = 16384;
 
 struct WideShape {
-    int row_blocks;           // forward, dX: persistent blocks
-    int dw_chunks, dw_blocks; // dW: channel chunks x row blocks (parts)
+    int row_blocks;            // forward: persistent blocks
+    int dw_chunks, dx_blocks;  // channel chunks x row blocks
+    int dw_blocks;             // those of dW: parts
 };
 WideShape wide_shape(long long N, int V, int D);
-inline size_t wide_p_bytes(long long N, int V) { return sizeof(float) * (size_t)N * ((V + 3) / 4 * 4); }
+// of scores and of derivatives: [N][V rounded up to 4]
+inline size_t wide_p_bytes(long long N, int V) {
+    return sizeof(float) * (size_t)N * ((V + 3) / 4 * 4);
+}
 
-// loss (one block) or per-block sums
-cudaError_t launch_wide_fwd(const NarrowArgs &a, float *loss, float2 *sums, cudaStream_t st);
-// grad (or null), and the derivatives P [N][V rounded up to 4]
-cudaError_t launch_wide_dx(const NarrowArgs &a, const CeUpstream &u, float *grad, float *p,
-                           cudaStream_t st);
+// loss (one block) or per-block sums; the (capped) scores, if z is not null
+cudaError_t launch_wide_fwd(const NarrowArgs &a, float *z, float *loss, float2 *sums,
+                            cudaStream_t st);
+cudaError_t launch_wide_probs(const NarrowArgs &a, const CeUpstream &u, const float *z, float *p,
+                              cudaStream_t st);
+cudaError_t launch_wide_dx(const NarrowArgs &a, const float *p, float *grad, cudaStream_t st);
 // acc [dw_blocks][V][D]
 cudaError_t launch_wide_dw(const NarrowArgs &a, const float *p, float *acc, cudaStream_t st);
 

@@ -457,7 +457,8 @@ struct Plan {
 // lse [N] (two floats; of packed rows but on the narrow path), packed total
 // (int, padded to 4 words), idx [Np], lab [Np], block counts; then the packed
 // features and the packed table where they are small: their kernels' launches
-// cost more than their memory, and the backward need not repeat them.
+// cost more than their memory, and the backward need not repeat them. On the
+// wide path the scores instead.
 struct State {
     float *count;
     float2 *lse;
@@ -764,21 +765,23 @@ WidePlan wide_plan(long long N, int V, int D, bool backward) {
     return w;
 }
 
-cudaError_t wide_forward(const NarrowArgs &a, float *loss, unsigned char *ws, cudaStream_t st) {
+cudaError_t wide_forward(const NarrowArgs &a, float *z, float *loss, unsigned char *ws,
+                         cudaStream_t st) {
     float2 *sums = reinterpret_cast<float2 *>(ws);
-    GSV_CE_TRY(launch_wide_fwd(a, loss, sums, st));
+    GSV_CE_TRY(launch_wide_fwd(a, z, loss, sums, st));
     const int blocks = wide_shape(a.N, a.V, a.D).row_blocks;
     if (blocks > 1)
         GSV_CE_TRY(launch_ce_finish(sums, blocks, a.opt.reduction, loss, a.count, st));
     return cudaSuccess;
 }
 
-cudaError_t wide_backward(const NarrowArgs &a, const float *grad_loss, void *gx, void *gw,
-                          unsigned char *ws, cudaStream_t st) {
+cudaError_t wide_backward(const NarrowArgs &a, const float *z, const float *grad_loss, void *gx,
+                          void *gw, unsigned char *ws, cudaStream_t st) {
     const WidePlan w = wide_plan(a.N, a.V, a.D, true);
     const CeUpstream u{grad_loss, a.count, nullptr, 1.f, a.opt.reduction};
     float *p = reinterpret_cast<float *>(ws), *dw = reinterpret_cast<float *>(ws + w.dw);
-    GSV_CE_TRY(launch_wide_dx(a, u, static_cast<float *>(gx), p, st));
+    GSV_CE_TRY(launch_wide_probs(a, u, z, p, st));
+    if (gx) GSV_CE_TRY(launch_wide_dx(a, p, static_cast<float *>(gx), st));
     if (!gw) return cudaSuccess;
     GSV_CE_TRY(launch_wide_dw(a, p, dw, st));
     return reduce_splits<float>((long long)a.V * a.D, dw, wide_shape(a.N, a.V, a.D).dw_blocks,
@@ -820,7 +823,8 @@ bool in_place(long long N, int V, int D, int type, const void *features) {
 size_t linear_ce_state_bytes(long long N, int V, int D, int type) {
     size_t b = (size_t)state_words(N) * 4;
     const Path path = path_of(N, V, D, type);
-    if (path == kNarrow || path == kWide) return b;
+    if (path == kNarrow) return b;
+    if (path == kWide) return b + wide_p_bytes(N, V);
     const size_t xb = packed_bytes(up(N, kCeTileM), D, type), wb = packed_bytes(V, D, type);
     if (kept(xb)) b += align256(xb);
     if (kept(wb)) b += align256(wb);
@@ -859,7 +863,9 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         }
     }
     if (path == kWide)
-        return wide_forward({N, V, D, features, weight, labels, o, s.lse, s.count}, loss, ws, st);
+        return wide_forward({N, V, D, features, weight, labels, o, s.lse, s.count},
+                            forward_only ? nullptr : reinterpret_cast<float *>(s.packed), loss,
+                            ws, st);
     const Plan p = make_plan(N, V, D, type, weight, false, o);
     const bool direct = in_place(N, V, D, type, features);
     if (!forward_only || (path == kTiles && !direct)) {
@@ -929,8 +935,9 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
 #undef GSV_CE_T
     }
     if (path_of(N, V, D, type) == kWide)
-        return wide_backward({N, V, D, features, weight, labels, o, s.lse, s.count}, grad_loss,
-                             grad_features, grad_weight, ws, st);
+        return wide_backward({N, V, D, features, weight, labels, o, s.lse, s.count},
+                             reinterpret_cast<const float *>(s.packed), grad_loss, grad_features,
+                             grad_weight, ws, st);
     const Plan p = make_plan(N, V, D, type, weight, true, o);
     float *gmax = type == kCeF16 ? reinterpret_cast<float *>(ws + p.gmax) : nullptr;
     const bool none = o.reduction == kCeNone;

@@ -1,19 +1,22 @@
 // Linear class loss of at most 16 classes and more than 32 float32 channels,
 // on the CUDA cores: a feature volume against a handful of classes.
 //
-// The features are all there is to move - read forward, for dX and for dW, dX
-// written: 4 passes of 4 N D bytes. The tensor cores' tiles would first split
-// them into three bf16 planes (10 bytes moved for 4, twice) and read those
-// three times: 3312 us of kernels at 603768 rows x 9 classes x 440 channels.
-// Here a block stages 32 channels of 256 rows (and of the table) at a time with
+// The features are all there is to move - read forward and for dW, dX written:
+// 3 passes of 4 N D bytes. The tensor cores' tiles would first split them into
+// three bf16 planes (10 bytes moved for 4, twice) and read those three times:
+// 3312 us of kernels at 603768 rows x 9 classes x 440 channels. Here the
+// forward stages 32 channels of 256 rows (and of the table) at a time with
 // asynchronous copies, the next while one is used; a thread owns two rows, so
 // that the V sums of a row need no exchange, and every value of the table read
-// from shared memory serves both. (A warp a row, its sums joined by shuffles,
-// spent more on these and on the softmax in every lane: 2437 us.) V
+// from shared memory serves both. It keeps the scores (V floats a row, less
+// than half of the features), and the backward need not form them again:
+// derivatives P from them, then dX with a lane's four columns of the table in
+// registers and whole rows written, and dW with V x 4 sums a lane. V
 // multiply-adds a channel against the 11 floats a clock and SM that HBM
-// delivers: bound by HBM. dW sums rows, the other axis: it reads the
-// derivatives P (V floats a row, left by dX's kernel) beside the features, each
-// lane keeping V x 4 sums.
+// delivers; it reaches 2.4 to 3 TB/s a pass, the loads in flight limit it. 603768 x
+// 9 x 440: 1242 us of kernels (scores formed again and dX written by their
+// threads: 1518; a warp a row with sums by shuffles: 2437); 147949 x 6 x 1578:
+// 1063 (1906).
 #include <atomic>
 
 #include "ce_wide.cuh"
@@ -21,7 +24,7 @@
 namespace gsv {
 namespace {
 
-constexpr int kNT = 128;                 // forward, dX
+constexpr int kNT = 128;                 // forward
 constexpr int kR = 2;                    // rows a thread
 constexpr int kRows = kNT * kR;          // rows a tile
 constexpr int kDepth = 32;               // channels staged at once
@@ -86,6 +89,18 @@ __device__ __forceinline__ void stage_table(float (&dst)[VP][kDepth], const floa
 template <bool VEC>
 __device__ __forceinline__ void stage_rows(float (&dst)[kRows][kPitch], const float *x,
                                            long long r0, long long N, int D, int c0) {
+    if (!VEC) {
+        // a warp copies a row's 128 bytes, a word a lane
+#pragma unroll 8
+        for (int i = threadIdx.x; i < kRows * kDepth; i += kNT) {
+            const int r = i / kDepth, c = i % kDepth;
+            if (r0 + r < N && c0 + c < D)
+                copy4(&dst[r][c], x + (r0 + r) * D + c0 + c);
+            else
+                dst[r][c] = 0.f;
+        }
+        return;
+    }
 #pragma unroll 4
     for (int i = threadIdx.x; i < kRows * (kDepth / 4); i += kNT) {
         const int r = i / (kDepth / 4), c = i % (kDepth / 4) * 4;
@@ -149,7 +164,7 @@ template <int VP, bool VEC, bool CAP>
 __global__ void __launch_bounds__(kNT)
 wide_fwd_kernel(long long N, int V, int D, const float *__restrict__ features,
                 const float *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
-                float *__restrict__ loss, float2 *__restrict__ lse_out,
+                float *__restrict__ loss, float2 *__restrict__ lse_out, float *__restrict__ z_out,
                 float *__restrict__ count, float2 *__restrict__ sums) {
     extern __shared__ __align__(16) unsigned char wide_smem[];
     __shared__ float2 sh[kNT / 32];
@@ -186,6 +201,13 @@ wide_fwd_kernel(long long N, int V, int D, const float *__restrict__ features,
             else if (y == kCeInvalid)
                 l = lse.x = ce_nan();
             lse_out[r] = lse;
+            if (z_out) {
+                float4 *to = reinterpret_cast<float4 *>(z_out) + r * ((V + 3) / 4);
+#pragma unroll
+                for (int j = 0; j < VP; j += 4)
+                    if (j < V)
+                        to[j / 4] = make_float4(z[k][j], z[k][j + 1], z[k][j + 2], z[k][j + 3]);
+            }
             if (o.reduction == kCeNone) loss[r] = l;
             lsum += l;
             cnt += y == kCeIgnored ? 0.f : 1.f;
@@ -200,99 +222,122 @@ wide_fwd_kernel(long long N, int V, int D, const float *__restrict__ features,
     }
 }
 
-template <int VP, bool VEC, bool CAP>
-__global__ void __launch_bounds__(kNT)
-wide_dx_kernel(long long N, int V, int D, const float *__restrict__ features,
-               const float *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
-               const float2 *__restrict__ lse, CeUpstream u, float *__restrict__ grad,
-               float *__restrict__ p_out) {
-    extern __shared__ __align__(16) unsigned char wide_smem[];
-    Stage<VP> *st = reinterpret_cast<Stage<VP> *>(wide_smem);
-    const int ldp = (V + 3) / 4 * 4, chunks = (D + kDepth - 1) / kDepth;
-    const float common = common_grad(u), ev = o.eps / (float)V;
+// the loss's derivative in the scores; rows of V floats, rounded up to four
+// and zeros there, in both
+template <int VP, bool CAP>
+__global__ void __launch_bounds__(kDwNT)
+wide_probs_kernel(long long N, int V, const long long *__restrict__ labels, CeOpt o,
+                  const float2 *__restrict__ lse, CeUpstream u, const float4 *__restrict__ z_in,
+                  float4 *__restrict__ p_out) {
+    const long long r = (long long)blockIdx.x * kDwNT + threadIdx.x;
+    if (r >= N) return;
+    const int words = (V + 3) / 4;
     const float *per_row = u.reduction == kCeNone ? u.g : nullptr;
-    for (long long r0 = (long long)blockIdx.x * kRows; r0 < N;
-         r0 += (long long)gridDim.x * kRows) {
-        float z[kR][VP];
-        bool keep[kR];
-        scores_of<VP, VEC>(z, st, features, weight, r0, N, V, D);
+    const int y = ce_label(labels[r], o.ignore, V);
+    const bool keep = y != kCeIgnored;
+    RowGrad q{};
+    if (keep) q = row_grad<true>(r, y, lse[r], o, per_row, common_grad(u), o.eps / (float)V);
 #pragma unroll
-        for (int k = 0; k < kR; ++k) {
-            const long long r = r0 + k * kNT + threadIdx.x;
-            const int y = r < N ? ce_label(labels[r], o.ignore, V) : kCeIgnored;
-            keep[k] = y != kCeIgnored;
-            RowGrad q{};
-            if (keep[k]) q = row_grad<true>(r, y, lse[r], o, per_row, common, ev);
+    for (int w = 0; w < VP / 4; ++w) {
+        if (w >= words) break;
+        const float4 in = z_in[r * words + w];
+        const float z[4] = {in.x, in.y, in.z, in.w};
+        float d[4];
 #pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                float d = 0.f;
-                if (j < V && keep[k]) {
-                    float t = 0.f;
-                    if (CAP) {
-                        t = ce_tanh<false>(z[k][j], o.cap);
-                        z[k][j] = o.cap * t;
-                    }
-                    d = fmaf(q.kz, ce_prob(z[k][j], q.lse), -q.e);
-                    if (y == j) d -= q.hit;
-                    if (CAP) d *= fmaf(-t, t, 1.f);
+        for (int i = 0; i < 4; ++i) {
+            const int j = 4 * w + i;
+            d[i] = 0.f;
+            if (j < V && keep) {
+                d[i] = fmaf(q.kz, ce_prob(z[i], q.lse), -q.e);
+                if (y == j) d[i] -= q.hit;
+                if (CAP) {
+                    const float t = z[i] / o.cap;
+                    d[i] *= fmaf(-t, t, 1.f);
                 }
-                z[k][j] = d;
-            }
-            if (r < N) {
-#pragma unroll
-                for (int j = 0; j < VP; j += 4)
-                    if (j < V)
-                        *reinterpret_cast<float4 *>(p_out + r * ldp + j) = make_float4(
-                            z[k][j], z[k][j + 1], z[k][j + 2], z[k][j + 3]);
             }
         }
-        if (!grad) continue;
-        // the table again, 32 channels at a time; the rows' gradients go out
-        // through the stage, a row's 128 bytes together
-        for (int i = 0; i < chunks; ++i) {
-            const int c0 = i * kDepth;
-            stage_table<VP, VEC>(st[0].w, weight, V, D, c0);
-            copies_end_group();
-            copies_wait<0>();
-            __syncthreads();
-#pragma unroll 2
-            for (int c = 0; c < kDepth; c += 4) {
-                float2 a[kR][2];
+        p_out[r * words + w] = make_float4(d[0], d[1], d[2], d[3]);
+    }
+}
+
+// a tile's derivatives and which rows have a label
+template <int VP>
+struct Derivatives {
+    float4 p[2][kDwRows][VP / 4];
+    int keep[2][kDwRows];
+
+    __device__ __forceinline__ void load(int b, const float4 *src, const long long *labels,
+                                         long long ignore, long long r0, long long N,
+                                         int words) {
+        for (int i = threadIdx.x; i < kDwRows * words; i += kDwNT) {
+            const int r = i / words;
+            p[b][r][i % words] = r0 + r < N ? src[(r0 + r) * words + i % words]
+                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (threadIdx.x < kDwRows)
+            keep[b][threadIdx.x] =
+                r0 + threadIdx.x < N && labels[r0 + threadIdx.x] != ignore;
+    }
+};
+
+// A lane's columns of a block's 128: four side by side (VEC), else every 32nd,
+// so that a warp's accesses stay side by side.
+template <int VP, bool VEC>
+__global__ void __launch_bounds__(kDwNT, 2)
+wide_dx_kernel(long long N, int V, int D, const float *__restrict__ weight,
+               const long long *__restrict__ labels, long long ignore,
+               const float4 *__restrict__ p, float *__restrict__ grad) {
+    constexpr int kPer = kDwRows / kDwWarps;
+    __shared__ Derivatives<VP> ds;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, words = (V + 3) / 4;
+    const int c = blockIdx.y * kChunk + (VEC ? 4 * lane : lane);
+    float2 w[VP][2];
 #pragma unroll
-                for (int k = 0; k < kR; ++k) a[k][0] = a[k][1] = make_float2(0.f, 0.f);
+    for (int j = 0; j < VP; ++j) {
+        float q[4];
 #pragma unroll
-                for (int j = 0; j < VP; ++j) {
+        for (int i = 0; i < 4; ++i) {
+            const int col = c + (VEC ? i : 32 * i);
+            q[i] = j < V && col < D ? weight[(long long)j * D + col] : 0.f;
+        }
+        w[j][0] = make_float2(q[0], q[1]);
+        w[j][1] = make_float2(q[2], q[3]);
+    }
+    int b = 0;
+    for (long long r0 = (long long)blockIdx.x * kDwRows; r0 < N;
+         r0 += (long long)gridDim.x * kDwRows, b ^= 1) {
+        ds.load(b, p, labels, ignore, r0, N, words);
+        __syncthreads();
+#pragma unroll 4
+        for (int k = 0; k < kPer; ++k) {
+            const int r = warp * kPer + k;
+            if (r0 + r >= N) break;
+            float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            // a row without a label is zero whatever the table holds
+            if (ds.keep[b][r]) {
+#pragma unroll
+                for (int j = 0; j < VP; j += 4) {
                     if (j >= V) break;
-                    const float4 q = *reinterpret_cast<const float4 *>(&st[0].w[j][c]);
+                    const float4 d = ds.p[b][r][j / 4];
+                    const float dv[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-                    for (int k = 0; k < kR; ++k) {
-                        a[k][0] = __ffma2_rn(f2(z[k][j]), make_float2(q.x, q.y), a[k][0]);
-                        a[k][1] = __ffma2_rn(f2(z[k][j]), make_float2(q.z, q.w), a[k][1]);
+                    for (int i = 0; i < 4; ++i) {
+                        a[0] = __ffma2_rn(f2(dv[i]), w[j + i][0], a[0]);
+                        a[1] = __ffma2_rn(f2(dv[i]), w[j + i][1], a[1]);
                     }
                 }
-                // a row without a label is zero whatever the table holds
-#pragma unroll
-                for (int k = 0; k < kR; ++k)
-                    *reinterpret_cast<float4 *>(&st[0].x[k * kNT + threadIdx.x][c]) =
-                        keep[k] ? make_float4(a[k][0].x, a[k][0].y, a[k][1].x, a[k][1].y)
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            __syncthreads();
-            for (int e = threadIdx.x; e < kRows * (kDepth / 4); e += kNT) {
-                const int r = e / (kDepth / 4), c = e % (kDepth / 4) * 4;
-                if (r0 + r >= N || c0 + c >= D) continue;
-                const float4 v = *reinterpret_cast<const float4 *>(&st[0].x[r][c]);
-                float *to = grad + (r0 + r) * D + c0 + c;
-                if (VEC) {
-                    __stcs(reinterpret_cast<float4 *>(to), v);
-                } else {
-                    to[0] = v.x;
-                    if (c0 + c + 1 < D) to[1] = v.y;
-                    if (c0 + c + 2 < D) to[2] = v.z;
-                    if (c0 + c + 3 < D) to[3] = v.w;
-                }
+            float *to = grad + (r0 + r) * D + c;
+            if (VEC) {
+                if (c < D)
+                    __stcs(reinterpret_cast<float4 *>(to),
+                           make_float4(a[0].x, a[0].y, a[1].x, a[1].y));
+            } else {
+                if (c < D) to[0] = a[0].x;
+                if (c + 32 < D) to[32] = a[0].y;
+                if (c + 64 < D) to[64] = a[1].x;
+                if (c + 96 < D) to[96] = a[1].y;
             }
-            __syncthreads();
         }
     }
 }
@@ -300,38 +345,28 @@ wide_dx_kernel(long long N, int V, int D, const float *__restrict__ features,
 template <bool VEC>
 __device__ __forceinline__ float4 load4(const float *p, int c, int D) {
     if (VEC) return *reinterpret_cast<const float4 *>(p + c);
-    return make_float4(p[c], c + 1 < D ? p[c + 1] : 0.f, c + 2 < D ? p[c + 2] : 0.f,
-                       c + 3 < D ? p[c + 3] : 0.f);
+    return make_float4(p[c], c + 32 < D ? p[c + 32] : 0.f, c + 64 < D ? p[c + 64] : 0.f,
+                       c + 96 < D ? p[c + 96] : 0.f);
 }
 
 template <int VP, bool VEC>
 __global__ void __launch_bounds__(kDwNT, 2)
 wide_dw_kernel(long long N, int V, int D, const float *__restrict__ features,
                const long long *__restrict__ labels, long long ignore,
-               const float *__restrict__ p, float *__restrict__ acc) {
+               const float4 *__restrict__ p, float *__restrict__ acc) {
     constexpr int kPer = kDwRows / kDwWarps;
     __shared__ float4 sum[VP][32];
-    __shared__ float4 ps[2][kDwRows][VP / 4];
-    __shared__ int keep[2][kDwRows];
+    __shared__ Derivatives<VP> ds;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, words = (V + 3) / 4;
-    const int c = blockIdx.y * kChunk + 4 * lane;
+    const int c = blockIdx.y * kChunk + (VEC ? 4 * lane : lane);
     float4 a[VP];
 #pragma unroll
     for (int j = 0; j < VP; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     int b = 0;
     for (long long r0 = (long long)blockIdx.x * kDwRows; r0 < N;
          r0 += (long long)gridDim.x * kDwRows, b ^= 1) {
-        // the tile's derivatives and which rows have a label; eight rows of
-        // features a warp on their way meanwhile
-        for (int i = threadIdx.x; i < kDwRows * words; i += kDwNT) {
-            const int r = i / words;
-            ps[b][r][i % words] =
-                r0 + r < N ? reinterpret_cast<const float4 *>(p)[(r0 + r) * words + i % words]
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        if (threadIdx.x < kDwRows)
-            keep[b][threadIdx.x] =
-                r0 + threadIdx.x < N && labels[r0 + threadIdx.x] != ignore;
+        // eight rows of features a warp on their way with the derivatives
+        ds.load(b, p, labels, ignore, r0, N, words);
         float4 x[kPer];
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
@@ -343,11 +378,11 @@ wide_dw_kernel(long long N, int V, int D, const float *__restrict__ features,
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             const int r = warp * kPer + k;
-            if (!keep[b][r]) continue;  // the whole warp alike
+            if (!ds.keep[b][r]) continue;  // the whole warp alike
 #pragma unroll
             for (int j = 0; j < VP; j += 4) {
                 if (j >= V) break;
-                const float4 d = ps[b][r][j / 4];
+                const float4 d = ds.p[b][r][j / 4];
                 const float dv[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -374,10 +409,12 @@ wide_dw_kernel(long long N, int V, int D, const float *__restrict__ features,
         __syncthreads();
     }
     for (int i = threadIdx.x; i < V * kChunk; i += kDwNT) {
-        const int j = i / kChunk, d = blockIdx.y * kChunk + i % kChunk;
+        const int j = i / kChunk, k = i % kChunk, d = blockIdx.y * kChunk + k;
+        // column k: lane and component
+        const int at = VEC ? k : k % 32 * 4 + k / 32;
         if (d < D)
             acc[((long long)blockIdx.x * V + j) * D + d] =
-                reinterpret_cast<const float *>(&sum[j][0])[i % kChunk];
+                reinterpret_cast<const float *>(&sum[j][0])[at];
     }
 }
 
@@ -420,12 +457,14 @@ WideShape wide_shape(long long N, int V, int D) {
     // three blocks an SM (two stages of 37 KB each)
     s.row_blocks = (int)std::min(ceil_div(N, kRows), 3LL * kSMs);
     s.dw_chunks = (int)ceil_div(D, kChunk);
+    s.dx_blocks = (int)std::min(ceil_div(N, kDwRows), std::max(1LL, 4LL * kSMs / s.dw_chunks));
     s.dw_blocks = (int)std::max(
         1LL, std::min(ceil_div(N, 4 * kDwRows), std::max(1LL, 2LL * kSMs / s.dw_chunks)));
     return s;
 }
 
-cudaError_t launch_wide_fwd(const NarrowArgs &a, float *loss, float2 *sums, cudaStream_t st) {
+cudaError_t launch_wide_fwd(const NarrowArgs &a, float *z, float *loss, float2 *sums,
+                            cudaStream_t st) {
     return by_form(a.V, wide_rows(a, nullptr), a.opt.cap > 0.f, [&](auto vp, auto vec, auto cap) {
         constexpr int VP = decltype(vp)::value;
         auto kernel = wide_fwd_kernel<VP, decltype(vec)::value, decltype(cap)::value>;
@@ -434,23 +473,32 @@ cudaError_t launch_wide_fwd(const NarrowArgs &a, float *loss, float2 *sums, cuda
         if (err != cudaSuccess) return err;
         kernel<<<wide_shape(a.N, a.V, a.D).row_blocks, kNT, 2 * sizeof(Stage<VP>), st>>>(
             a.N, a.V, a.D, static_cast<const float *>(a.features),
-            static_cast<const float *>(a.weight), a.labels, a.opt, loss, a.lse, a.count, sums);
+            static_cast<const float *>(a.weight), a.labels, a.opt, loss, a.lse, z, a.count,
+            sums);
         count_launches(1);
         return cudaGetLastError();
     });
 }
 
-cudaError_t launch_wide_dx(const NarrowArgs &a, const CeUpstream &u, float *grad, float *p,
-                           cudaStream_t st) {
-    return by_form(a.V, wide_rows(a, grad), a.opt.cap > 0.f, [&](auto vp, auto vec, auto cap) {
-        constexpr int VP = decltype(vp)::value;
-        auto kernel = wide_dx_kernel<VP, decltype(vec)::value, decltype(cap)::value>;
-        static std::atomic<unsigned long long> ready{0};
-        const cudaError_t err = allow_stages<VP>(kernel, ready);
-        if (err != cudaSuccess) return err;
-        kernel<<<wide_shape(a.N, a.V, a.D).row_blocks, kNT, 2 * sizeof(Stage<VP>), st>>>(
-            a.N, a.V, a.D, static_cast<const float *>(a.features),
-            static_cast<const float *>(a.weight), a.labels, a.opt, a.lse, u, grad, p);
+cudaError_t launch_wide_probs(const NarrowArgs &a, const CeUpstream &u, const float *z, float *p,
+                              cudaStream_t st) {
+    return by_form(a.V, true, a.opt.cap > 0.f, [&](auto vp, auto, auto cap) {
+        wide_probs_kernel<decltype(vp)::value, decltype(cap)::value>
+            <<<(unsigned)ceil_div(a.N, kDwNT), kDwNT, 0, st>>>(
+                a.N, a.V, a.labels, a.opt, a.lse, u, reinterpret_cast<const float4 *>(z),
+                reinterpret_cast<float4 *>(p));
+        count_launches(1);
+        return cudaGetLastError();
+    });
+}
+
+cudaError_t launch_wide_dx(const NarrowArgs &a, const float *p, float *grad, cudaStream_t st) {
+    return by_form(a.V, wide_rows(a, grad), false, [&](auto vp, auto vec, auto) {
+        const WideShape s = wide_shape(a.N, a.V, a.D);
+        wide_dx_kernel<decltype(vp)::value, decltype(vec)::value>
+            <<<dim3(s.dx_blocks, s.dw_chunks), kDwNT, 0, st>>>(
+                a.N, a.V, a.D, static_cast<const float *>(a.weight), a.labels, a.opt.ignore,
+                reinterpret_cast<const float4 *>(p), grad);
         count_launches(1);
         return cudaGetLastError();
     });
@@ -461,8 +509,8 @@ cudaError_t launch_wide_dw(const NarrowArgs &a, const float *p, float *acc, cuda
         const WideShape s = wide_shape(a.N, a.V, a.D);
         wide_dw_kernel<decltype(vp)::value, decltype(vec)::value>
             <<<dim3(s.dw_blocks, s.dw_chunks), kDwNT, 0, st>>>(
-                a.N, a.V, a.D, static_cast<const float *>(a.features), a.labels, a.opt.ignore, p,
-                acc);
+                a.N, a.V, a.D, static_cast<const float *>(a.features), a.labels, a.opt.ignore,
+                reinterpret_cast<const float4 *>(p), acc);
         count_launches(1);
         return cudaGetLastError();
     });
