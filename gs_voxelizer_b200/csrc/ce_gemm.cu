@@ -681,15 +681,21 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                                             __uint_as_float(v[j]) * scale;
                                 }
                                 __syncwarp();
-                                for (int i = i0; i < min(n_rows, i0 + Sh::kTurn); ++i) {
-                                    const long long at =
-                                        __shfl_sync(0xffffffffu, to, i) + col0 + lane;
-                                    const float x = turn[(i - i0) * 33 + lane];
-                                    if (lane < cols) {
+                                // eight rows together: one latency
+                                for (int i = i0; i < min(n_rows, i0 + Sh::kTurn); i += 8) {
+                                    float x[8];
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k)
+                                        x[k] = turn[(i - i0 + k) * 33 + lane];
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) {
+                                        const long long at =
+                                            __shfl_sync(0xffffffffu, to, i + k) + col0 + lane;
+                                        if (lane >= cols || i + k >= n_rows) continue;
                                         if (F32)
-                                            out32[at] = x;
+                                            out32[at] = x[k];
                                         else
-                                            out16[at] = (uint16_t)pack2(x, 0.f, g.bf16);
+                                            out16[at] = (uint16_t)pack2(x[k], 0.f, g.bf16);
                                     }
                                 }
                                 __syncwarp();

@@ -512,7 +512,10 @@ def linear_cross_entropy(
     rounded to the inputs' type. The forward keeps 16 bytes a row and, up to
     16 MB each, its packed operands; the backward computes the scores again in
     pieces, with a workspace of a few hundred MB beside packed copies of the
-    operands and float32 copies of what it accumulates over several pieces. With ``reduction="none"`` and no gradient it is minus the
+    operands and float32 copies of what it accumulates over several pieces.
+    (Scores of at most 16 classes over more than 32 float32 channels, less than
+    half of the features' size, are kept instead, from 16384 rows on.) With
+    ``reduction="none"`` and no gradient it is minus the
     log-probability of each row's label.
 
     Args:

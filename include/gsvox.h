@@ -500,8 +500,9 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
 
 /*
  * Class losses: softmax cross entropy of scores in memory (gsv_softmax_ce_*)
- * and of the scores features . weight^T, which are never in memory
- * (gsv_linear_ce_*), each with its gradient. No reference counterpart.
+ * and of the scores features . weight^T, which are not written to memory
+ * (gsv_linear_ce_*; at most 16 float32 classes of more than 32 channels are,
+ * to `state`), each with its gradient. No reference counterpart.
  *
  * Of row i with scores s_ij (capped to z = cap tanh(s / cap) when softcap =
  * cap > 0, else z = s), label y and lse_i = log sum_j exp z_ij:
