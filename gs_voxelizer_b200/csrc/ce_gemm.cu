@@ -19,7 +19,7 @@
 // 32768 x 4096: 1.845 of 1.835 million ideal ones), the clock falls to what
 // 1000 W allow; 8192 x 131072 x 4096 takes 6.6 to 6.7 ms a product, 1.32
 // PFLOP/s, against 1.39 of a plain library product sustained (42765 x 26421 x
-// 621 in float32, six products each: 5.6 to 8.0 ms, 1.50 to 1.06 PFLOP/s). Small products
+// 621 in float32, six products each: 5.6 to 8.1 ms, 1.50 to 1.04 PFLOP/s). Small products
 // are bound by their turn-around, about 6 us a launch.
 //
 // Waits are bounded: on a timeout a role sets g_ce_error, leaves its loop and
@@ -828,7 +828,7 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
 // Columns of a gradient's tile (MN-major B: multiples of 128). float32 keeps
 // a tile's sums in registers, 64 a thread: 128 at most. (256 wide, summed in
 // memory a chunk at a time, the two gradients of 42765 x 26421 x 621 took 36
-// ms, with the planes loaded once a stage 16.)
+// ms, with the planes loaded once a stage 14.)
 int ce_grad_tile(int cols, bool f32) { return f32 || cols <= 128 ? 128 : kCeTileN; }
 
 int ce_runs(long long rows, int V, bool f32) {
