@@ -794,6 +794,13 @@ template <int PRODUCT, bool CAP, bool F32>
 cudaError_t launch(const CeGemm &g, cudaStream_t st) {
     constexpr bool kAMn = PRODUCT == kCeGradW, kBMn = PRODUCT >= kCeGradX;
     const int nt = kBMn ? ce_grad_tile(g.D, F32) : score_tile(g.rows, g.nv, F32);
+    // The driver encodes tensor maps only where a context is current, and this
+    // may be the calling thread's first work (autograd's): setting the device
+    // makes its context current.
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err == cudaSuccess) err = cudaSetDevice(dev);
+    if (err != cudaSuccess) return err;
     CUtensorMap a, b;
     const CeMat &ma = PRODUCT >= kCeGradX ? g.P : g.X;
     const CeMat &mb = PRODUCT == kCeGradW ? g.X : g.W;
@@ -803,9 +810,6 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
     auto kernel = ce_gemm_kernel<PRODUCT, CAP, F32>;
     // once a device (a repeated call is harmless)
     static std::atomic<unsigned long long> ready{0};
-    int dev = 0;
-    cudaError_t err = cudaGetDevice(&dev);
-    if (err != cudaSuccess) return err;
     if (!(ready.load() >> (dev & 63) & 1)) {
         err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    Shape<F32>::kSmemBytes);

@@ -175,6 +175,62 @@ def test_linear_many_classes(dtype):
     run(130, 40013, 72, dtype, dict(reduction="none"), ignored=0.2)
 
 
+@pytest.mark.parametrize("n,V,D", [(1300, 700, 131), (2100, 515, 1030), (600, 9001, 77),
+                                   (5000, 300, 514), (3, 6000, 1301)])
+def test_linear_float32(n, V, D):
+    """Sums of more than one accumulator's length, split or not, and results
+    of no alignment."""
+    for i, opt in enumerate(OPTS):
+        run(n, V, D, F32, opt, ignored=0.3 if i % 2 else 0.0)
+
+
+@pytest.mark.parametrize("D", [35, 72])
+def test_linear_float32_pieces(D):
+    """Rows and classes that no piece of the backward holds at once."""
+    run(12001, 8201, D, F32, dict(z_loss=1e-4), ignored=0.05)
+    run(12001, 8201, D, F32, dict(reduction="none"), ignored=0.05)
+
+
+@pytest.mark.parametrize("V,D", [(6, 44), (13, 41)])
+def test_linear_few_classes_float32(V, D):
+    """Kept scores: rows without a label, labels out of range, unaligned
+    views, one gradient alone, caps."""
+    from gs_voxelizer_b200.losses import linear_cross_entropy
+    n = 16500
+    data, labels = make(n, V, D, F32, V, ignored=0.3)
+    data[0][labels == -100] = float("nan")
+    up = torch.ones((), device="cuda")
+    for opt in (*OPTS, dict(softcap=0.5), dict(softcap=1e8)):
+        if opt.get("reduction") == "none":
+            continue
+        loss, both = call(data, labels, opt, up)
+        check(data, labels, opt, up, loss, both)
+        assert (both[0][labels == -100] == 0).all()
+    _, both = call(data, labels, {}, up)
+    for which in (0, 1):
+        leaves = list(data)
+        leaves[which] = leaves[which].clone().requires_grad_(True)
+        (g,) = torch.autograd.grad(linear_cross_entropy(*leaves, labels), leaves[which])
+        assert torch.equal(g, both[which])
+    flat = torch.empty(n * D + 1, device="cuda")
+    flat[1:] = data[0].reshape(-1)
+    leaves = [flat[1:].view(n, D).requires_grad_(True), data[1].clone().requires_grad_(True)]
+    loss = linear_cross_entropy(*leaves, labels)
+    check(data, labels, {}, up, loss.detach(), torch.autograd.grad(loss, leaves))
+    leaves = [t.clone().requires_grad_(True) for t in data]
+    loss = linear_cross_entropy(*leaves, labels)
+    first = torch.autograd.grad(loss, leaves, retain_graph=True)
+    again = torch.autograd.grad(loss, leaves)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    labels[16390] = V
+    loss, grads = call(data, labels, dict(reduction="none"), torch.ones(n, device="cuda"))
+    assert loss[16390].isnan() and loss.isnan().sum() == 1
+    assert grads[0].isnan().any(1).sum() == 1 and grads[1].isnan().all()
+    labels[:] = -100
+    loss, grads = call(data, labels, {}, up)
+    assert loss == 0 and all((g == 0).all() for g in grads)
+
+
 @pytest.mark.parametrize("D", [0, 4, 24])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_volume_shapes(D, dtype):
@@ -613,3 +669,30 @@ print("replayed")
     out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
                          timeout=300)
     assert out.returncode == 0 and "replayed" in out.stdout, out.stderr[-2000:]
+
+
+def test_backward_as_first_call_of_its_thread():
+    """Autograd runs backwards in a thread of its own. Where that finds its
+    memory cached and the operands packed, the products are its first work."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from gs_voxelizer_b200.losses import linear_cross_entropy
+cached = [torch.empty(1 << 18, device="cuda") for _ in range(16)]
+x = torch.randn(9, 4050, device="cuda", requires_grad=True)
+w = torch.randn(3, 4050, device="cuda", requires_grad=True)
+y = torch.zeros(9, dtype=torch.int64, device="cuda")
+up = torch.ones((), device="cuda")
+cached += [torch.empty(1 << 22, dtype=torch.uint8, device="cuda") for _ in range(8)]
+del cached
+loss = linear_cross_entropy(x, w, y)
+torch.autograd.grad(loss, (x, w), up)
+torch.cuda.synchronize()
+print("done")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                         timeout=300)
+    assert out.returncode == 0 and "done" in out.stdout, out.stderr[-2000:]
