@@ -511,7 +511,7 @@ float p_scale_of(int type, const CeOpt &o) {
 int splits_for(long long tiles, long long depth, bool f32, long long elements) {
     int best = 1;
     double cost = 0;
-    for (int s = 1; s <= 32 && (s == 1 || (depth / s >= 512 &&
+    for (int s = 1; s <= kCePairs && (s == 1 || (depth / s >= 512 &&
                                            s * elements * 4 <= (long long)kPieceBytes)); ++s) {
         const double c = (f32 ? 6. : 1.) * depth / s * ((tiles * s + kCePairs - 1) / kCePairs) +
                          (s > 1 ? 1000. * s * tiles / kCePairs : 0.);
