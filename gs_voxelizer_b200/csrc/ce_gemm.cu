@@ -836,12 +836,14 @@ cudaError_t launch(const CeGemm &g, cudaStream_t st) {
 int ce_grad_tile(int cols, bool f32) { return f32 || cols <= 128 ? 128 : kCeTileN; }
 
 int ce_runs(long long rows, int V, bool f32) {
-    const long long mt = (rows + kCeTileM - 1) / kCeTileM;
-    const int nt = score_tile(rows, V, f32), tiles = (V + nt - 1) / nt;
+    // (rows below 2^31: 2^23 tiles, 2^31 units at most)
+    const unsigned mt = (unsigned)((rows + kCeTileM - 1) / kCeTileM);
+    const int nt = score_tile(rows, V, f32);
+    const unsigned tiles = (unsigned)((V + nt - 1) / nt);
     // the longest pair's tiles, and about a third of a tile to begin a run
     int best = 1;
     double cost = 1e300;
-    for (int r = 1; r <= std::min(tiles, 2 * kCePairs); ++r) {
+    for (unsigned r = 1; r <= std::min(tiles, 2u * kCePairs); ++r) {
         const double c = (double)((mt * r + kCePairs - 1) / kCePairs) *
                          ((tiles + r - 1) / r + 0.33);
         if (c < cost - 1e-9) {

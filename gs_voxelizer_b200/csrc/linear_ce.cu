@@ -536,7 +536,6 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     // `weight` null: the workspace query, which allows for any alignment
     p.pack_w = p.planes == 3 || D % 8 != 0 || weight == nullptr ||
                (reinterpret_cast<uintptr_t>(weight) & 15) != 0;
-    p.runs = ce_runs(N, V, p.planes == 3);
     size_t at = 0;
     auto take = [&](size_t b) {
         const size_t o = at;
@@ -551,6 +550,7 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     p.xp = p.keep_x ? 0 : take(xb);
     p.wp = p.keep_w ? (p.keep_x ? align256(xb) : 0) : take(p.pack_w ? wb : 0);
     if (!backward) {
+        p.runs = ce_runs(N, V, p.planes == 3);
         p.part = take(sizeof(float2) * 2 * (size_t)p.runs * p.Np);
         p.psum = take(o.eps > 0.f ? sizeof(float) * 2 * (size_t)p.runs * p.Np : 0);
         p.zt = take(sizeof(float) * (size_t)p.Np);
