@@ -5,6 +5,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/gsvox.h"
@@ -1105,6 +1106,15 @@ gsv::CeOpt ce_opt(const gsv_ce_options *o) {
 
 const long long *as_ll(const int64_t *p) { return reinterpret_cast<const long long *>(p); }
 
+// Whether all of these are multiples of `bytes`: a kernel's access to anything
+// else is a fault.
+bool aligned(size_t bytes, std::initializer_list<const void *> pointers) {
+    uintptr_t bits = 0;
+    for (const void *p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
+    return (bits & (bytes - 1)) == 0;
+}
+size_t ce_size(int32_t dtype) { return dtype == GSV_F32 ? 4 : 2; }
+
 }  // namespace
 
 extern "C" {
@@ -1125,8 +1135,9 @@ int gsv_softmax_ce_forward(int64_t rows, int32_t classes, int32_t dtype, const v
     const size_t need = gsv_softmax_ce_workspace_bytes(rows, classes);
     GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
                 "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
-    GSV_REQUIRE((reinterpret_cast<uintptr_t>(lse) & 7) == 0, GSV_ERR_INVALID_ARGUMENT,
-                "%s: lse not aligned", fn);
+    GSV_REQUIRE(aligned(ce_size(dtype), {scores}) && aligned(8, {labels, lse, ws}) &&
+                    aligned(4, {loss, count}),
+                GSV_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned", fn);
     return cuda_status(gsv::launch_softmax_ce(true, dtype, rows, classes, scores,
                                               as_ll(labels), ce_opt(options), loss,
                                               reinterpret_cast<float2 *>(lse), count, nullptr, nullptr, ws, as_stream(stream)),
@@ -1141,6 +1152,9 @@ int gsv_softmax_ce_backward(int64_t rows, int32_t classes, int32_t dtype, const 
     if (const int st = check_ce(fn, rows, classes, 1, dtype, options)) return st;
     GSV_REQUIRE(scores && labels && lse && count && grad_loss && grad_scores,
                 GSV_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+    GSV_REQUIRE(aligned(ce_size(dtype), {scores, grad_scores}) && aligned(8, {labels, lse}) &&
+                    aligned(4, {count, grad_loss}),
+                GSV_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned", fn);
     return cuda_status(gsv::launch_softmax_ce(
                            false, dtype, rows, classes, scores, as_ll(labels),
                            ce_opt(options), nullptr,
@@ -1178,9 +1192,11 @@ int gsv_linear_ce_forward(int64_t rows, int32_t classes, int32_t channels, int32
         gsv_linear_ce_workspace_bytes(rows, classes, channels, dtype, options, 0);
     GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
                 "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
-    GSV_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0 &&
-                    (reinterpret_cast<uintptr_t>(state) & 15) == 0,
-                GSV_ERR_INVALID_ARGUMENT, "%s: workspace or state not aligned", fn);
+    GSV_REQUIRE(aligned(256, {ws}) && aligned(16, {state}), GSV_ERR_INVALID_ARGUMENT,
+                "%s: workspace or state not aligned", fn);
+    GSV_REQUIRE(aligned(ce_size(dtype), {features, weight}) && aligned(8, {labels}) &&
+                    aligned(4, {loss}),
+                GSV_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned", fn);
     return cuda_status(gsv::launch_linear_ce_forward(rows, classes, channels, dtype, features,
                                                      weight, as_ll(labels), ce_opt(options),
                                                      loss, state, ws, as_stream(stream)),
@@ -1200,9 +1216,11 @@ int gsv_linear_ce_backward(int64_t rows, int32_t classes, int32_t channels, int3
         gsv_linear_ce_workspace_bytes(rows, classes, channels, dtype, options, 1);
     GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
                 "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
-    GSV_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0 &&
-                    (reinterpret_cast<uintptr_t>(state) & 15) == 0,
-                GSV_ERR_INVALID_ARGUMENT, "%s: workspace or state not aligned", fn);
+    GSV_REQUIRE(aligned(256, {ws}) && aligned(16, {state}), GSV_ERR_INVALID_ARGUMENT,
+                "%s: workspace or state not aligned", fn);
+    GSV_REQUIRE(aligned(ce_size(dtype), {features, weight, grad_features, grad_weight}) &&
+                    aligned(8, {labels}) && aligned(4, {grad_loss}),
+                GSV_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned", fn);
     return cuda_status(gsv::launch_linear_ce_backward(
                            rows, classes, channels, dtype, features, weight, as_ll(labels),
                            ce_opt(options), state, grad_loss, grad_features, grad_weight, ws,

@@ -525,8 +525,9 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
  * float32 [rows][2], 8-byte aligned, and [1]) or in `state` (gsv_linear_ce_state_bytes, 16-byte
  * aligned); the backward is called with the same sizes, inputs and options.
  * A null state: no backward follows.
- * Workspaces are scratch of one call, 256-byte aligned. A null gradient output
- * of gsv_linear_ce_backward is not computed.
+ * Workspaces are scratch of one call, 256-byte aligned (gsv_softmax_ce_forward:
+ * 8-byte). Everything else is aligned to its elements; a pointer that is not is
+ * refused. A null gradient output of gsv_linear_ce_backward is not computed.
  */
 enum gsv_dtype { GSV_F32 = 0, GSV_BF16 = 1, GSV_F16 = 2 };
 enum gsv_reduction { GSV_REDUCE_NONE = 0, GSV_REDUCE_SUM = 1, GSV_REDUCE_MEAN = 2 };

@@ -1,0 +1,68 @@
+"""CPU tests of what the C entries of the class losses refuse before any device
+work, beyond sizes and options: pointers that the kernels' accesses would fault
+on."""
+import ctypes
+
+import pytest
+
+from gs_voxelizer_b200._lib import CeOptions, lib
+
+P = 4096
+
+
+def options():
+    return CeOptions(-100, 0.0, 0.0, 0.0, 2)
+
+
+def refused(status):
+    return status == 1 and b"aligned" in lib.gsv_last_error()
+
+
+def call(fn, head, pointers, dtype, tail):
+    """fn with `pointers` = {name: address} in the entry's order, options where
+    the name is `opt`."""
+    args = [options() if k == "opt" else ctypes.c_void_p(v) for k, v in pointers.items()]
+    return fn(*head, dtype, *args, *tail)
+
+
+@pytest.mark.parametrize("dtype,size", [(0, 4), (1, 2), (2, 2)])
+@pytest.mark.parametrize("classes", [5, 5000])
+def test_softmax_entries_refuse_misaligned_pointers(dtype, size, classes):
+    names = dict(scores=size, labels=8, opt=0, loss=4, lse=8, count=4, ws=8)
+    for name, size_of in names.items():
+        if name == "opt":
+            continue
+        ptr = {k: P for k in names}
+        ptr[name] += size_of // 2
+        assert refused(call(lib.gsv_softmax_ce_forward, (7, classes), ptr, dtype,
+                            (1 << 20, None))), name
+    names = dict(scores=size, labels=8, opt=0, lse=8, count=4, grad_loss=4, grad_scores=size)
+    for name, size_of in names.items():
+        if name == "opt":
+            continue
+        ptr = {k: P for k in names}
+        ptr[name] += size_of // 2
+        assert refused(call(lib.gsv_softmax_ce_backward, (7, classes), ptr, dtype,
+                            (None,))), name
+
+
+@pytest.mark.parametrize("dtype,size", [(0, 4), (1, 2), (2, 2)])
+@pytest.mark.parametrize("sizes", [(7, 20, 4), (20000, 9, 64), (3, 500, 64), (700, 500, 64)])
+def test_linear_entries_refuse_misaligned_pointers(dtype, size, sizes):
+    names = dict(features=size, weight=size, labels=8, opt=0, loss=4, state=16, ws=256)
+    for name, size_of in names.items():
+        if name == "opt":
+            continue
+        ptr = {k: P for k in names}
+        ptr[name] += size_of // 2
+        assert refused(call(lib.gsv_linear_ce_forward, sizes, ptr, dtype,
+                            (1 << 40, None))), name
+    names = dict(features=size, weight=size, labels=8, opt=0, state=16, grad_loss=4,
+                 grad_features=size, grad_weight=size, ws=256)
+    for name, size_of in names.items():
+        if name == "opt":
+            continue
+        ptr = {k: P for k in names}
+        ptr[name] += size_of // 2
+        assert refused(call(lib.gsv_linear_ce_backward, sizes, ptr, dtype,
+                            (1 << 40, None))), name
