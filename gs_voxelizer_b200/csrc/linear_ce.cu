@@ -829,9 +829,23 @@ Path path_of(long long N, int V, int D, int type) {
 // saves. Packing moves 4 N D bytes, a share f of unlabelled rows takes
 // 2 f N V D operations: at 5 TB/s and 1.4 PFLOP/s they meet at f V = 570.
 // One tile of rows cannot become fewer.
+bool in_place_sizes(long long N, int V, int D, int type) {
+    return (N <= kCeTileM || V <= 1024) && type != kCeF32 && D % 8 == 0;
+}
 bool in_place(long long N, int V, int D, int type, const void *features) {
-    return (N <= kCeTileM || V <= 1024) && type != kCeF32 && D % 8 == 0 &&
-           (reinterpret_cast<uintptr_t>(features) & 15) == 0;
+    return in_place_sizes(N, V, D, type) && (reinterpret_cast<uintptr_t>(features) & 15) == 0;
+}
+
+// What a forward with a state has packed and kept whatever its pointers were:
+// the backward's may be others (of the same contents), and what the forward
+// packed only for its pointers' alignment is packed again.
+bool x_is_kept(const Plan &p) {
+    return path_of(p.N, p.V, p.D, p.type) == kTiles && p.keep_x &&
+           !in_place_sizes(p.N, p.V, p.D, p.type);
+}
+bool w_is_kept(const Plan &p) {
+    return path_of(p.N, p.V, p.D, p.type) == kTiles && p.keep_w &&
+           (p.planes == 3 || p.D % 8 != 0);
 }
 
 }  // namespace
@@ -957,11 +971,8 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
     const Plan p = make_plan(N, V, D, type, weight, true, o);
     float *gmax = type == kCeF16 ? reinterpret_cast<float *>(ws + p.gmax) : nullptr;
     const bool none = o.reduction == kCeNone;
-    // what the forward packed and kept is there (kFew packed nothing)
-    const bool tiled = path_of(N, V, D, type) == kTiles;
-    if (!(tiled && p.keep_x && !in_place(N, V, D, type, features)))
-        GSV_CE_TRY(pack_any(p, true, features, s, x_of(p, s, ws), st));
-    if (p.pack_w && !(tiled && p.keep_w))
+    if (!x_is_kept(p)) GSV_CE_TRY(pack_any(p, true, features, s, x_of(p, s, ws), st));
+    if (p.pack_w && !w_is_kept(p))
         GSV_CE_TRY(pack_any(p, false, weight, s, w_of(p, s, ws), st));
     if (none && gmax) {
         GSV_CE_TRY(cudaMemsetAsync(gmax, 0, sizeof(float), st));

@@ -355,6 +355,13 @@ class _Once(Function):
         raise RuntimeError("the class losses are differentiable once")
 
 
+def _saved(t):
+    """A saved tensor as the kernels take it: a hook may have brought it back
+    with other strides, or (raw bytes) off the alignment of what it holds."""
+    t = t.contiguous()
+    return t.clone() if t.dtype == torch.uint8 and t.data_ptr() & 15 else t
+
+
 def _softmax_ce(scores, labels, opt):
     """(loss, stats): per row (maximum, log2 of the sum), then the number of
     labelled rows, then the call's workspace."""
@@ -387,7 +394,7 @@ class _SoftmaxCe(Function):
         saved = ctx.saved_tensors
         if len(saved) == 1:
             return torch.zeros_like(saved[0]), None, None
-        scores, labels, stats = saved
+        scores, labels, stats = map(_saved, saved)
         dev, rows, V = scores.device, labels.numel(), scores.size(-1)
         grad_loss = grad_loss.contiguous()  # float32, as the loss is
         g = torch.empty_like(scores)
@@ -475,7 +482,7 @@ class _LinearCe(Function):
         if len(saved) == 2:
             return (*(torch.zeros_like(t) if need else None for t, need in
                       zip(saved, (need_x, need_w))), None, None)
-        features, weight, labels, state = saved
+        features, weight, labels, state = map(_saved, saved)
         dev = features.device
         rows, (V, D) = labels.numel(), weight.shape
         dtype = _CE_DTYPES[features.dtype]

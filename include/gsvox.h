@@ -523,7 +523,8 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
  *
  * The forward leaves what the backward needs in `lse` / `count` (device
  * float32 [rows][2], 8-byte aligned, and [1]) or in `state` (gsv_linear_ce_state_bytes, 16-byte
- * aligned); the backward is called with the same sizes, inputs and options.
+ * aligned); the backward is called with the same sizes, contents and options
+ * (the inputs may lie elsewhere by then).
  * A null state: no backward follows.
  * Workspaces are scratch of one call, 256-byte aligned (gsv_softmax_ce_forward:
  * 8-byte). Everything else is aligned to its elements; a pointer that is not is
