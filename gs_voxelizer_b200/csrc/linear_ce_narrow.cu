@@ -24,6 +24,8 @@
 // sum of all scores (x . sum of the table) and the smoothing's share of dX.
 // Few rows or many classes: the classes (for dW the rows) are split over
 // blocks and the parts are joined in a fixed order.
+#include <cfloat>
+
 #include "ce_narrow.cuh"
 
 namespace gsv {
@@ -46,12 +48,26 @@ struct alignas(16) Pairs {
 };
 
 template <int DP>
-__device__ __forceinline__ Pairs<DP> to_pairs(const Row<DP> &r, float scale) {
+__device__ __forceinline__ Pairs<DP> to_pairs(const Row<DP> &r) {
     Pairs<DP> p;
 #pragma unroll
-    for (int d = 0; d < DP / 2; ++d)
-        p.v[d] = make_float2(r.v[2 * d] * scale, r.v[2 * d + 1] * scale);
+    for (int d = 0; d < DP / 2; ++d) p.v[d] = make_float2(r.v[2 * d], r.v[2 * d + 1]);
     return p;
+}
+
+// A row of the table times unit<CAP>(). What was finite stays so: rows at the
+// type's lowest value mask classes, and 0 times infinity would be NaN.
+template <int DP, bool CAP>
+__device__ __forceinline__ Pairs<DP> table_pairs(Row<DP> r) {
+    if (!CAP) {
+#pragma unroll
+        for (int d = 0; d < DP; ++d) {
+            const float v = r.v[d];
+            r.v[d] = isinf(v) ? v : fminf(fmaxf(v * unit<CAP>(), -FLT_MAX), FLT_MAX);
+            if (isnan(v)) r.v[d] = v;  // (the bounds above would replace it)
+        }
+    }
+    return to_pairs<DP>(r);
 }
 
 // four chains of multiply-adds, two to a register pair
@@ -67,11 +83,10 @@ __device__ __forceinline__ float dot_pairs(const Pairs<DP> &a, const Pairs<DP> &
     return s.x + s.y;
 }
 
-template <typename T, int DP, bool VEC>
-__device__ __forceinline__ void stage_pairs(Pairs<DP> *sw, const T *w, long long v0, int n, int D,
-                                            float scale) {
+template <typename T, int DP, bool CAP, bool VEC>
+__device__ __forceinline__ void stage_pairs(Pairs<DP> *sw, const T *w, long long v0, int n, int D) {
     for (int j = threadIdx.x; j < n; j += kNT)
-        sw[j] = to_pairs<DP>(load_row<T, DP, VEC>(w, v0 + j, D), scale);
+        sw[j] = table_pairs<DP, CAP>(load_row<T, DP, VEC>(w, v0 + j, D));
 }
 
 // What a thread reads of its rows, one tile ahead of their use: the loads of a
@@ -133,9 +148,10 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
         int y[R];
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-            x[k] = to_pairs<DP>(next.x[k], 1.f);
+            x[k] = to_pairs<DP>(next.x[k]);
             y[k] = ce_label(next.label[k], o.ignore, V);
-            m[k] = ce_neg_inf();
+            // finite, so that classes at -inf add e^-inf = 0 wherever they come
+            m[k] = -FLT_MAX;
             s[k] = sz[k] = 0.f;
         }
         // (of more channels there are no registers to read ahead into)
@@ -146,7 +162,7 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
             const int n = min(kChunk, span.v1 - v0);
             if (!staged) {
                 __syncthreads();
-                stage_pairs<T, DP, VEC>(sw, weight, v0, n, D, unit<CAP>());
+                stage_pairs<T, DP, CAP, VEC>(sw, weight, v0, n, D);
                 __syncthreads();
                 staged = span.v1 - span.v0 <= kChunk;
             }
@@ -170,7 +186,6 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
                     float top = m[k];
 #pragma unroll
                     for (int j = 0; j < kG; ++j) top = fmaxf(top, z[k][j]);
-                    // (all scores at -inf: no distribution, NaN like theirs)
                     s[k] *= exp_of<CAP>(m[k] - top);
                     m[k] = top;
                     float e = 0.f;
@@ -191,11 +206,11 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
         for (int k = 0; k < R; ++k) {
             const long long r = t0 + k * kNT + threadIdx.x;
             if (r >= N) continue;
-            if (smooth && !CAP) sz[k] = dot_pairs<DP>(x[k], to_pairs<DP>(s_wsum, 1.f));
+            if (smooth && !CAP) sz[k] = dot_pairs<DP>(x[k], to_pairs<DP>(s_wsum));
             float zy = 0.f;
             if (y[k] >= 0) {
                 zy = dot_pairs<DP>(x[k],
-                                   to_pairs<DP>(load_row<T, DP, VEC>(weight, y[k], D), 1.f));
+                                   to_pairs<DP>(load_row<T, DP, VEC>(weight, y[k], D)));
                 if (CAP) zy = o.cap * ce_tanh<sizeof(T) == 2>(zy, o.cap);
             }
             if (gridDim.y > 1) {
@@ -205,7 +220,7 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
                 continue;
             }
             float l = 0.f;
-            float2 lse = make_float2(CeAcc::base(m[k]), __log2f(s[k]));
+            float2 lse = make_float2(m[k], __log2f(s[k]));
             if (y[k] >= 0)
                 l = ce_row_loss(make_float2(CAP ? lse.x : lse.x * kCeLn2, lse.y), zy, sz[k], V,
                                 o);
@@ -274,7 +289,7 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
             const long long r = t0 + k * kNT + threadIdx.x;
             y[k] = ce_label(next.label[k], o.ignore, V);
             q[k] = row_grad<CAP>(r, y[k], next.lse[k], o, per_row, common, ev);
-            x[k] = to_pairs<DP>(next.x[k], 1.f);
+            x[k] = to_pairs<DP>(next.x[k]);
 #pragma unroll
             for (int d = 0; d < DP / 2; ++d) dx[k].v[d] = f2(0.f);
         }
@@ -285,7 +300,7 @@ narrow_dx_kernel(long long N, int V, int D, const T *__restrict__ features,
             const int n = min(kChunk, span.v1 - v0);
             if (!staged) {
                 __syncthreads();
-                stage_pairs<T, DP, VEC>(sw, weight, v0, n, D, unit<CAP>());
+                stage_pairs<T, DP, CAP, VEC>(sw, weight, v0, n, D);
                 __syncthreads();
                 staged = span.v1 - span.v0 <= kChunk;
             }
@@ -382,8 +397,17 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
 #pragma unroll
         for (int d = 0; d < DP / 2; ++d) w[c].v[d] = dw[c].v[d] = f2(0.f);
         if (active && j0 + c * lanes < V)
-            w[c] = to_pairs<DP>(load_row<T, DP, VEC>(weight, j0 + c * lanes, D), unit<CAP>());
+            w[c] = table_pairs<DP, CAP>(load_row<T, DP, VEC>(weight, j0 + c * lanes, D));
     }
+    // The zeros of a row without a label are NaN times an infinite entry. Only
+    // then are such rows passed over: the branch in the loop costs 6 to 12 %.
+    bool infinite = false;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int d = 0; d < DP / 2; ++d)
+            infinite = infinite || !isfinite(w[c].v[d].x) || !isfinite(w[c].v[d].y);
+    infinite = __syncthreads_or(infinite);
     const bool plain = o.eps == 0.f && o.zeta == 0.f;
     const float common = common_grad(u), ev = o.eps / (float)V;
     const float *per_row = u.reduction == kCeNone ? u.g : nullptr;
@@ -404,7 +428,7 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
             if (s.y != kCeIgnored) {
                 const RowGrad q = row_grad<CAP>(t0 + threadIdx.x, s.y, next.lse[0], o, per_row,
                                                 common, ev);
-                s.x = to_pairs<DP>(next.x[0], 1.f);
+                s.x = to_pairs<DP>(next.x[0]);
                 s.lse = q.lse;
                 s.kz = q.kz;
                 s.e = q.e;
@@ -416,30 +440,37 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
         }
         __syncthreads();
         if (!active) continue;
+        auto add_rows = [&](auto pass_over) {
 #pragma unroll(DP == 8 || DP == 32 ? 2 : 1)
-        for (int i = slice; i < kDwRows; i += slices) {
-            const Pairs<DP> x = rows[i].x;
-            const float2 l = rows[i].lse;
-            const float kz = rows[i].kz;
-            const int y = rows[i].y;
-            float hit = kz, e = 0.f;
-            if (!plain) {
-                hit = rows[i].hit;
-                e = rows[i].e;
-            }
+            for (int i = slice; i < kDwRows; i += slices) {
+                const Pairs<DP> x = rows[i].x;
+                const float2 l = rows[i].lse;
+                const float kz = rows[i].kz;
+                const int y = rows[i].y;
+                if (decltype(pass_over)::value && y == kCeIgnored) continue;
+                float hit = kz, e = 0.f;
+                if (!plain) {
+                    hit = rows[i].hit;
+                    e = rows[i].e;
+                }
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float slope = 1.f;
-                const float p =
-                    prob<CAP, sizeof(T) == 2>(dot_pairs<DP>(x, w[c]), l, o.cap, slope);
-                float d = fmaf(kz, p, -e);
-                if (y == j0 + c * lanes) d -= hit;
-                if (CAP) d *= slope;
+                for (int c = 0; c < C; ++c) {
+                    float slope = 1.f;
+                    const float p =
+                        prob<CAP, sizeof(T) == 2>(dot_pairs<DP>(x, w[c]), l, o.cap, slope);
+                    float d = fmaf(kz, p, -e);
+                    if (y == j0 + c * lanes) d -= hit;
+                    if (CAP) d *= slope;
 #pragma unroll
-                for (int k = 0; k < DP / 2; ++k)
-                    dw[c].v[k] = __ffma2_rn(f2(d), x.v[k], dw[c].v[k]);
+                    for (int k = 0; k < DP / 2; ++k)
+                        dw[c].v[k] = __ffma2_rn(f2(d), x.v[k], dw[c].v[k]);
+                }
             }
-        }
+        };
+        if (infinite)
+            add_rows(std::true_type{});
+        else
+            add_rows(std::false_type{});
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {

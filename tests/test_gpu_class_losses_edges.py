@@ -5,7 +5,7 @@ rounding (test_gpu_class_losses.py has the definition over all shapes)."""
 import pytest
 import torch
 
-from tests.test_gpu_class_losses import BF16, DTYPES, F16, F32, make
+from tests.test_gpu_class_losses import BF16, DTYPES, F16, F32, call, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,47 @@ def test_saved_tensor_hooks(n, V, D, dtype, form):
         # (where a row's words begin decides the order of its sums)
         tol = 2.0 ** {F32: -20, BF16: -7, F16: -10}[dtype]
         assert torch.allclose(a.float(), c.float(), rtol=tol, atol=tol * float(c.abs().max()))
+
+
+def masked_table(n, V, D, dtype, lead, low):
+    """A table whose first `lead` rows are at `low`, with positive features:
+    those classes score -inf, or lower than any other, and have probability 0."""
+    g = torch.Generator("cuda").manual_seed(n + V + D + lead)
+    x = (0.5 + torch.rand(n, D, generator=g, device="cuda")).to(dtype)
+    w = (torch.randn(V, D, generator=g, device="cuda") / D).to(dtype)
+    w[:lead] = low
+    labels = torch.randint(lead, V, (n,), generator=g, device="cuda")
+    labels[::4] = -100
+    return x, w, labels
+
+
+def check_masked(n, V, D, dtype, lead, low):
+    x, w, labels = masked_table(n, V, D, dtype, lead, low)
+    if low != float("-inf") and D > 1:
+        x[:, 0] = 0  # (0 * -inf would be NaN by definition)
+    for opt in (dict(), dict(z_loss=1e-3, reduction="sum")):
+        up = torch.tensor(16.0, device="cuda")
+        loss, grads = call((x, w), labels, opt, up)
+        # as if those classes were not there; their own gradient is 0 . x
+        rest = torch.where(labels == -100, -100, labels - lead)
+        dx = grads[0]
+        if low == float("-inf"):  # 0 * -inf again: held to the table without them
+            dx = call((x, w[lead:]), rest, opt, up)[1][0]
+        check((x, w[lead:].contiguous()), rest, opt, up, loss, [dx, grads[1][lead:]])
+        assert (grads[1][:lead] == 0).all()
+        assert (grads[0][labels == -100] == 0).all()
+        alone, _ = call((x, w), labels, opt)
+        check((x, w[lead:].contiguous()), rest, opt, None, alone, [])
+
+
+NARROW = [(300, 3, 1, 1), (300, 5, 4, 3), (300, 20, 4, 9), (60, 300, 4, 130), (300, 20, 7, 12),
+          (2000, 64, 16, 8), (300, 20, 24, 9), (5, 700, 3, 600)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,D,lead", NARROW)
+def test_masked_classes_few_channels(n, V, D, lead, dtype):
+    """Classes masked by their table rows, whole groups and whole splits of
+    them first."""
+    for low in (float("-inf"), torch.finfo(dtype).min):
+        check_masked(n, V, D, dtype, lead, low)
