@@ -100,8 +100,9 @@ index_kernel(long long n, long long padded, int V, const long long *__restrict__
 }
 
 // Splits a float into bf16 planes whose sum it is. Infinities and NaN live
-// in the first plane alone; a finite value that would round to infinity is
-// held at the largest bf16 and the remainder follows.
+// in the first plane alone, of which the products' sums take them (ce_gemm.cu);
+// a finite value that would round to infinity is held at the largest bf16 and
+// the remainder follows.
 __device__ __forceinline__ void split3(float v, __nv_bfloat16 (&h)[3]) {
 #pragma unroll
     for (int p = 0; p < 3; ++p) {

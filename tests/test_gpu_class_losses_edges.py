@@ -83,3 +83,38 @@ def test_masked_classes_few_channels(n, V, D, lead, dtype):
     them first."""
     for low in (float("-inf"), torch.finfo(dtype).min):
         check_masked(n, V, D, dtype, lead, low)
+
+
+TILES = [(300, 37, 40, 20), (300, 300, 64, 129), (2, 37, 40, 11), (3, 500, 33, 400),
+         (16500, 9, 40, 5), (700, 20, 1030, 7)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,D,lead", TILES)
+def test_masked_classes_many_channels(n, V, D, lead, dtype):
+    for low in (float("-inf"), torch.finfo(dtype).min):
+        check_masked(n, V, D, dtype, lead, low)
+
+
+@pytest.mark.parametrize("D", [4, 40, 64])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_label_at_a_masked_class(D, dtype):
+    """The loss is infinite there, and in no other row."""
+    x, w, labels = masked_table(300, 37, D, dtype, 5, float("-inf"))
+    labels[9] = 2
+    loss, _ = call((x, w), labels, dict(reduction="none"))
+    assert loss[9] == float("inf") and loss.isfinite().sum() == 299
+
+
+@pytest.mark.parametrize("D", [4, 24, 40, 64])
+@pytest.mark.parametrize("n,V", [(300, 37), (16500, 9)])
+def test_infinite_upstream_stays_in_its_row_float32(n, V, D):
+    (x, w), labels = make(n, V, D, F32, 51, ignored=0.2, garbage=False)
+    labels[7] = 3
+    up = torch.ones(n, device="cuda")
+    want = call((x, w), labels, dict(reduction="none"), up)[1][0]
+    up[7] = float("inf")
+    got = call((x, w), labels, dict(reduction="none"), up)[1][0]
+    assert not got[7].isfinite().any()
+    got[7] = want[7]
+    assert torch.equal(got, want)
