@@ -482,6 +482,9 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                               (reinterpret_cast<uintptr_t>(g.dst) & 15) == 0);
             if (g.dst) scale = ce_grad_scale(g.up);
         }
+        // (the ratio is formed first: 2^14 over a vanishing gmax is infinite)
+        float gmax = 1.f;
+        if (PRODUCT == kCeProbs && g.grow && g.gmax && *g.gmax > 0.f) gmax = *g.gmax;
         // a unit's row, read a unit ahead: units of few classes and channels
         // take no longer than these loads
         auto row_of = [&](int u) {
@@ -493,12 +496,10 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             x.y = g.lab ? g.lab[g.row0 + r] : ce_label(g.labels[g.row0 + r], o.ignore, g.V);
             if (PRODUCT == kCeProbs) {
                 x.lse = g.lse[g.row0 + r];
-                if (g.grow) x.g = g.grow[g.idx[g.row0 + r]];
+                if (g.grow) x.g = g.grow[g.idx[g.row0 + r]] / gmax;
             }
             return x;
         };
-        float unit_scale = g.p_scale;
-        if (PRODUCT == kCeProbs && g.grow && g.gmax && *g.gmax > 0.f) unit_scale /= *g.gmax;
         RowInfo next = row_of(first);
         for (int u = first; ok && u < w.units; u += step) {
             const Unit t = unit_of<PRODUCT, F32>(g, w, u);
@@ -510,7 +511,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             float top = ce_neg_inf(), s = 0.f, sz = 0.f;
             float kz = 1.f, e = 0.f, hit = 0.f;
             if (PRODUCT == kCeProbs) {
-                const float f = unit_scale * row.g;
+                const float f = g.p_scale * row.g;
                 kz = (1.f + 2.f * o.zeta * ce_lse(lse)) * f;
                 e = o.eps / (float)g.V * f;
                 hit = (1.f - o.eps) * f;

@@ -23,7 +23,7 @@ struct CeMat {
 };
 
 // Factor of the summed gradients. With reduction "none" each row's upstream
-// gradient is in P already, over the largest one (gmax) in fp16.
+// gradient is in P already, over the largest finite one (gmax) in fp16.
 struct CeUpstream {
     const float *g;      // [1]
     const float *count;  // labelled rows, at least 1

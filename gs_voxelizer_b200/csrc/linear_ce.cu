@@ -293,15 +293,18 @@ void launch_merge(long long rows, long long grid_rows, int parts, int V, bool pa
 
 // -------------------------------------------------------------- gradients
 
-// out[0] (zero before) = largest |g| of the labelled rows; the bits of
+// out[0] (zero before) = largest finite |g| of the labelled rows (an infinite
+// one is its own row's, and its factor is infinite over any other); the bits of
 // non-negative floats order as integers, and a maximum has no order
 __global__ void __launch_bounds__(256)
 max_abs_kernel(const float *__restrict__ g, const int *__restrict__ idx,
                const int *__restrict__ total, float *__restrict__ out) {
     float m = 0.f;
     const long long n = *total;
-    for (long long r = blockIdx.x * 256LL + threadIdx.x; r < n; r += gridDim.x * 256LL)
-        m = fmaxf(m, fabsf(g[idx[r]]));
+    for (long long r = blockIdx.x * 256LL + threadIdx.x; r < n; r += gridDim.x * 256LL) {
+        const float a = fabsf(g[idx[r]]);
+        if (isfinite(a)) m = fmaxf(m, a);
+    }
 #pragma unroll
     for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
     if ((threadIdx.x & 31) == 0 && m > 0.f)

@@ -118,3 +118,28 @@ def test_infinite_upstream_stays_in_its_row_float32(n, V, D):
     assert not got[7].isfinite().any()
     got[7] = want[7]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("D", [4, 40, 64])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_infinite_upstream_stays_in_its_row(bad, dtype, D):
+    (x, w), labels = make(300, 137, D, dtype, 52, ignored=0.2, garbage=False)
+    labels[7] = 3
+    up = torch.ones(300, device="cuda")
+    want = call((x, w), labels, dict(reduction="none"), up)[1][0]
+    up[7] = bad
+    got = call((x, w), labels, dict(reduction="none"), up)[1][0]
+    assert not got[7].isfinite().any()
+    got[7] = want[7]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tiny", [1e-30, 1e-36, 1e-44])
+@pytest.mark.parametrize("D", [4, 40, 64])
+def test_vanishing_upstream_fp16(D, tiny):
+    """Gradients far below fp16's least step are 0, whatever their factor."""
+    data, labels = make(300, 137, D, F16, 53, ignored=0.2)
+    up = torch.full((300,), tiny, device="cuda")
+    for g in call(data, labels, dict(reduction="none"), up)[1]:
+        assert (g == 0).all()
