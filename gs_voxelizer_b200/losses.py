@@ -24,7 +24,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import cuda as _C
 from ._lib import CeOptions, check, i3, lib
@@ -355,6 +355,14 @@ class _Once(Function):
         raise RuntimeError("the class losses are differentiable once")
 
 
+def _recorded(*tensors):
+    """Whether autograd has to see the call: an input needs a gradient, or may
+    carry a tangent, which the function refuses (a dual tensor needs no gradient
+    and would lose its tangent in silence)."""
+    return forward_ad._current_level >= 0 or (
+        torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
+
+
 def _saved(t):
     """A saved tensor as the kernels take it: a hook may have brought it back
     with other strides, or (raw bytes) off the alignment of what it holds."""
@@ -440,7 +448,7 @@ def softmax_cross_entropy(
     if scores.shape[-1] < 1:
         raise ValueError("scores must have at least one class")
     scores = scores.contiguous()
-    if not (scores.requires_grad and torch.is_grad_enabled()):
+    if not _recorded(scores):
         return _softmax_ce(scores, labels, opt)[0]
     return _SoftmaxCe.apply(scores, labels, opt)
 
@@ -543,7 +551,6 @@ def linear_cross_entropy(
     if weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError("weight must have at least one class and one channel")
     features, weight = features.contiguous(), weight.contiguous()
-    if not ((features.requires_grad or weight.requires_grad)
-            and torch.is_grad_enabled()):
+    if not _recorded(features, weight):
         return _linear_ce(features, weight, labels, opt, False)[0]
     return _LinearCe.apply(features, weight, labels, opt)

@@ -143,3 +143,24 @@ def test_vanishing_upstream_fp16(D, tiny):
     up = torch.full((300,), tiny, device="cuda")
     for g in call(data, labels, dict(reduction="none"), up)[1]:
         assert (g == 0).all()
+
+
+@pytest.mark.parametrize("D", [0, 4, 64])
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_is_refused(D, leaf):
+    """A dual tensor's tangent is not dropped in silence."""
+    from torch.autograd import forward_ad
+    from gs_voxelizer_b200 import losses
+    fn = losses.linear_cross_entropy if D else losses.softmax_cross_entropy
+    data, labels = make(30, 12, D, F32, 55)
+    data = [t.requires_grad_(leaf) for t in data]
+    with forward_ad.dual_level():
+        for i in range(len(data)):
+            args = list(data)
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                fn(*args, labels)
+            with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+                fn(*args, labels)
+        plain = fn(*[t.detach() for t in data], labels)
+    assert torch.equal(plain, fn(*data, labels))
