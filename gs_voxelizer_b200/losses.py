@@ -355,19 +355,26 @@ class _Once(Function):
         raise RuntimeError("the class losses are differentiable once")
 
 
-def _recorded(*tensors):
+def _recorded(a, b):
     """Whether autograd has to see the call: an input needs a gradient, or may
     carry a tangent, which the function refuses (a dual tensor needs no gradient
     and would lose its tangent in silence)."""
     return forward_ad._current_level >= 0 or (
-        torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
+        (a.requires_grad or b.requires_grad) and torch.is_grad_enabled())
 
 
-def _saved(t):
-    """A saved tensor as the kernels take it: a hook may have brought it back
-    with other strides, or (raw bytes) off the alignment of what it holds."""
-    t = t.contiguous()
-    return t.clone() if t.dtype == torch.uint8 and t.data_ptr() & 15 else t
+def _as_kept(saved):
+    """Saved tensors as the kernels take them: a hook may have brought them back
+    with other strides, or the last one (raw bytes) off the alignment of what it
+    holds."""
+    for t in saved:
+        if not t.is_contiguous():
+            break
+    else:
+        if not saved[-1].data_ptr() & 15:
+            return saved
+    *rest, raw = (t.contiguous() for t in saved)
+    return (*rest, raw.clone() if raw.data_ptr() & 15 else raw)
 
 
 def _softmax_ce(scores, labels, opt):
@@ -402,7 +409,7 @@ class _SoftmaxCe(Function):
         saved = ctx.saved_tensors
         if len(saved) == 1:
             return torch.zeros_like(saved[0]), None, None
-        scores, labels, stats = map(_saved, saved)
+        scores, labels, stats = _as_kept(saved)
         dev, rows, V = scores.device, labels.numel(), scores.size(-1)
         grad_loss = grad_loss.contiguous()  # float32, as the loss is
         g = torch.empty_like(scores)
@@ -448,7 +455,7 @@ def softmax_cross_entropy(
     if scores.shape[-1] < 1:
         raise ValueError("scores must have at least one class")
     scores = scores.contiguous()
-    if not _recorded(scores):
+    if not _recorded(scores, scores):
         return _softmax_ce(scores, labels, opt)[0]
     return _SoftmaxCe.apply(scores, labels, opt)
 
@@ -490,7 +497,7 @@ class _LinearCe(Function):
         if len(saved) == 2:
             return (*(torch.zeros_like(t) if need else None for t, need in
                       zip(saved, (need_x, need_w))), None, None)
-        features, weight, labels, state = map(_saved, saved)
+        features, weight, labels, state = _as_kept(saved)
         dev = features.device
         rows, (V, D) = labels.numel(), weight.shape
         dtype = _CE_DTYPES[features.dtype]
