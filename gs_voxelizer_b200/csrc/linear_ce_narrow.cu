@@ -38,6 +38,10 @@ constexpr int chunk_of(int dp) { return 4096 / dp; }  // classes staged at once
 constexpr int kRows = 2;                              // rows a thread
 // classes a thread (dW): the registers hold 2 DP each
 constexpr int classes_of(int dp) { return dp == 4 ? 4 : 2; }
+// Rows that a thread of dW adds up before its sum joins the block's: a sum of
+// all of a block's rows, hundreds of thousands with many classes, was off by
+// 1e-3 where all were alike
+constexpr int kDwChain = 1024;
 // blocks an SM, as many as registers hold without spills
 constexpr int per_sm(int dp) { return dp <= 8 ? 3 : dp == 16 ? 2 : 1; }
 constexpr int width_of(int D) { return D <= 4 ? 4 : D <= 8 ? 8 : D <= 16 ? 16 : 32; }
@@ -395,7 +399,7 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int d = 0; d < DP / 2; ++d) w[c].v[d] = dw[c].v[d] = f2(0.f);
+        for (int d = 0; d < DP / 2; ++d) w[c].v[d] = f2(0.f);
         if (active && j0 + c * lanes < V)
             w[c] = table_pairs<DP, CAP>(load_row<T, DP, VEC>(weight, j0 + c * lanes, D));
     }
@@ -418,80 +422,95 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
     Ahead<DP, 1> next;
     read_ahead<T, DP, VEC, 1, true>(next, stager ? t0 : N, 0, N, D, features, labels, o.ignore,
                                     lse);
-    for (; t0 < N; t0 += stride) {
-        DwRow<DP> *rows = buffers + buffer * kDwRows;
-        buffer ^= 1;
-        if (stager) {
-            // an unlabelled row is all zeros
-            DwRow<DP> s{};
-            s.y = ce_label(next.label[0], o.ignore, V);
-            if (s.y != kCeIgnored) {
-                const RowGrad q = row_grad<CAP>(t0 + threadIdx.x, s.y, next.lse[0], o, per_row,
-                                                common, ev);
-                s.x = to_pairs<DP>(next.x[0]);
-                s.lse = q.lse;
-                s.kz = q.kz;
-                s.e = q.e;
-                s.hit = q.hit;
+    const int tiles = max(1, kDwChain * slices / kDwRows);
+    for (bool first = true; t0 < N; first = false) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int d = 0; d < DP / 2; ++d) dw[c].v[d] = f2(0.f);
+        const long long stop = min(N, t0 + tiles * stride);
+        for (; t0 < stop; t0 += stride) {
+            DwRow<DP> *rows = buffers + buffer * kDwRows;
+            buffer ^= 1;
+            if (stager) {
+                // an unlabelled row is all zeros
+                DwRow<DP> s{};
+                s.y = ce_label(next.label[0], o.ignore, V);
+                if (s.y != kCeIgnored) {
+                    const RowGrad q = row_grad<CAP>(t0 + threadIdx.x, s.y, next.lse[0], o, per_row,
+                                                    common, ev);
+                    s.x = to_pairs<DP>(next.x[0]);
+                    s.lse = q.lse;
+                    s.kz = q.kz;
+                    s.e = q.e;
+                    s.hit = q.hit;
+                }
+                rows[threadIdx.x] = s;
+                read_ahead<T, DP, VEC, 1, true>(next, t0 + stride, 0, N, D, features, labels,
+                                                o.ignore, lse);
             }
-            rows[threadIdx.x] = s;
-            read_ahead<T, DP, VEC, 1, true>(next, t0 + stride, 0, N, D, features, labels,
-                                            o.ignore, lse);
-        }
-        __syncthreads();
-        if (!active) continue;
-        auto add_rows = [&](auto pass_over) {
+            __syncthreads();
+            if (!active) continue;
+            auto add_rows = [&](auto pass_over) {
 #pragma unroll(DP == 8 || DP == 32 ? 2 : 1)
-            for (int i = slice; i < kDwRows; i += slices) {
-                const Pairs<DP> x = rows[i].x;
-                const float2 l = rows[i].lse;
-                const float kz = rows[i].kz;
-                const int y = rows[i].y;
-                if (decltype(pass_over)::value && y == kCeIgnored) continue;
-                float hit = kz, e = 0.f;
-                if (!plain) {
-                    hit = rows[i].hit;
-                    e = rows[i].e;
-                }
+                for (int i = slice; i < kDwRows; i += slices) {
+                    const Pairs<DP> x = rows[i].x;
+                    const float2 l = rows[i].lse;
+                    const float kz = rows[i].kz;
+                    const int y = rows[i].y;
+                    if (decltype(pass_over)::value && y == kCeIgnored) continue;
+                    float hit = kz, e = 0.f;
+                    if (!plain) {
+                        hit = rows[i].hit;
+                        e = rows[i].e;
+                    }
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    float slope = 1.f;
-                    const float p =
-                        prob<CAP, sizeof(T) == 2>(dot_pairs<DP>(x, w[c]), l, o.cap, slope);
-                    float d = fmaf(kz, p, -e);
-                    if (y == j0 + c * lanes) d -= hit;
-                    if (CAP) d *= slope;
+                    for (int c = 0; c < C; ++c) {
+                        float slope = 1.f;
+                        const float p =
+                            prob<CAP, sizeof(T) == 2>(dot_pairs<DP>(x, w[c]), l, o.cap, slope);
+                        float d = fmaf(kz, p, -e);
+                        if (y == j0 + c * lanes) d -= hit;
+                        if (CAP) d *= slope;
 #pragma unroll
-                    for (int k = 0; k < DP / 2; ++k)
-                        dw[c].v[k] = __ffma2_rn(f2(d), x.v[k], dw[c].v[k]);
+                        for (int k = 0; k < DP / 2; ++k)
+                            dw[c].v[k] = __ffma2_rn(f2(d), x.v[k], dw[c].v[k]);
+                    }
                 }
+            };
+            if (infinite)
+                add_rows(std::true_type{});
+            else
+                add_rows(std::false_type{});
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float out[DP];
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < DP / 2; ++d) {
+                out[2 * d] = dw[c].v[d].x;
+                out[2 * d + 1] = dw[c].v[d].y;
             }
-        };
-        if (infinite)
-            add_rows(std::true_type{});
-        else
-            add_rows(std::false_type{});
-    }
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        float out[DP];
-        __syncthreads();
+            for (int d = 0; d < DP; ++d) red[threadIdx.x * (DP + 1) + d] = out[d];
+            __syncthreads();
+            const int j = j0 + c * lanes;
+            if (slice == 0 && j < V) {
+                for (int s = 1; s < slices; ++s)
 #pragma unroll
-        for (int d = 0; d < DP / 2; ++d) {
-            out[2 * d] = dw[c].v[d].x;
-            out[2 * d + 1] = dw[c].v[d].y;
+                    for (int d = 0; d < DP; ++d)
+                        out[d] += red[(s * lanes + threadIdx.x) * (DP + 1) + d];
+                float *sum = acc + (long long)blockIdx.x * V * D;
+                if (!first) {
+                    const Row<DP> old = load_row<float, DP, false>(sum, j, D);
+#pragma unroll
+                    for (int d = 0; d < DP; ++d) out[d] += old.v[d];
+                }
+                store_row<float, DP, false>(sum, j, D, out);
+            }
         }
-#pragma unroll
-        for (int d = 0; d < DP; ++d) red[threadIdx.x * (DP + 1) + d] = out[d];
         __syncthreads();
-        const int j = j0 + c * lanes;
-        if (slice == 0 && j < V) {
-            for (int s = 1; s < slices; ++s)
-#pragma unroll
-                for (int d = 0; d < DP; ++d)
-                    out[d] += red[(s * lanes + threadIdx.x) * (DP + 1) + d];
-            store_row<float, DP, false>(acc + (long long)blockIdx.x * V * D, j, D, out);
-        }
     }
 }
 

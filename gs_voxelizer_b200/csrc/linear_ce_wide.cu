@@ -34,6 +34,8 @@ constexpr int kPitch = kDepth + 4;
 constexpr int kDwNT = 256, kDwWarps = kDwNT / 32;
 constexpr int kDwRows = 64;              // rows a tile of dW, eight a warp
 constexpr int kChunk = 128;              // channels of a dW block
+// rows that a warp of dW adds up before its sums join the block's
+constexpr int kDwChain = 1024;
 
 template <int VP>
 struct alignas(16) Stage {
@@ -359,62 +361,67 @@ wide_dw_kernel(long long N, int V, int D, const float *__restrict__ features,
     __shared__ Derivatives<VP> ds;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, words = (V + 3) / 4;
     const int c = blockIdx.y * kChunk + (VEC ? 4 * lane : lane);
-    float4 a[VP];
-#pragma unroll
-    for (int j = 0; j < VP; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     int b = 0;
-    for (long long r0 = (long long)blockIdx.x * kDwRows; r0 < N;
-         r0 += (long long)gridDim.x * kDwRows, b ^= 1) {
-        // eight rows of features a warp on their way with the derivatives
-        ds.load(b, p, labels, ignore, r0, N, words);
-        float4 x[kPer];
+    long long r0 = (long long)blockIdx.x * kDwRows;
+    for (bool first = true; r0 < N; first = false) {
+        float4 a[VP];
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const long long r = r0 + warp * kPer + k;
-            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < N && c < D) x[k] = load4<VEC>(features + r * D, c, D);
-        }
-        __syncthreads();
+        for (int j = 0; j < VP; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < kDwChain / kPer && r0 < N;
+             ++i, r0 += (long long)gridDim.x * kDwRows, b ^= 1) {
+            // eight rows of features a warp on their way with the derivatives
+            ds.load(b, p, labels, ignore, r0, N, words);
+            float4 x[kPer];
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int r = warp * kPer + k;
-            if (!ds.keep[b][r]) continue;  // the whole warp alike
+            for (int k = 0; k < kPer; ++k) {
+                const long long r = r0 + warp * kPer + k;
+                x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < N && c < D) x[k] = load4<VEC>(features + r * D, c, D);
+            }
+            __syncthreads();
 #pragma unroll
-            for (int j = 0; j < VP; j += 4) {
-                if (j >= V) break;
-                const float4 d = ds.p[b][r][j / 4];
-                const float dv[4] = {d.x, d.y, d.z, d.w};
+            for (int k = 0; k < kPer; ++k) {
+                const int r = warp * kPer + k;
+                if (!ds.keep[b][r]) continue;  // the whole warp alike
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    a[j + i].x = fmaf(dv[i], x[k].x, a[j + i].x);
-                    a[j + i].y = fmaf(dv[i], x[k].y, a[j + i].y);
-                    a[j + i].z = fmaf(dv[i], x[k].z, a[j + i].z);
-                    a[j + i].w = fmaf(dv[i], x[k].w, a[j + i].w);
+                for (int j = 0; j < VP; j += 4) {
+                    if (j >= V) break;
+                    const float4 d = ds.p[b][r][j / 4];
+                    const float dv[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        a[j + i].x = fmaf(dv[i], x[k].x, a[j + i].x);
+                        a[j + i].y = fmaf(dv[i], x[k].y, a[j + i].y);
+                        a[j + i].z = fmaf(dv[i], x[k].z, a[j + i].z);
+                        a[j + i].w = fmaf(dv[i], x[k].w, a[j + i].w);
+                    }
                 }
             }
         }
-    }
-    for (int k = 0; k < kDwWarps; ++k) {
-        if (warp == k) {
+        for (int k = 0; k < kDwWarps; ++k) {
+            if (warp == k) {
 #pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                float4 s = a[j];
-                if (k) {
-                    const float4 t = sum[j][lane];
-                    s = make_float4(s.x + t.x, s.y + t.y, s.z + t.z, s.w + t.w);
+                for (int j = 0; j < VP; ++j) {
+                    float4 s = a[j];
+                    if (k) {
+                        const float4 t = sum[j][lane];
+                        s = make_float4(s.x + t.x, s.y + t.y, s.z + t.z, s.w + t.w);
+                    }
+                    sum[j][lane] = s;
                 }
-                sum[j][lane] = s;
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < V * kChunk; i += kDwNT) {
+            const int j = i / kChunk, k = i % kChunk, d = blockIdx.y * kChunk + k;
+            // column k: lane and component
+            const int at = VEC ? k : k % 32 * 4 + k / 32;
+            if (d < D) {
+                float *to = acc + ((long long)blockIdx.x * V + j) * D + d;
+                const float v = reinterpret_cast<const float *>(&sum[j][0])[at];
+                *to = first ? v : *to + v;
             }
         }
-        __syncthreads();
-    }
-    for (int i = threadIdx.x; i < V * kChunk; i += kDwNT) {
-        const int j = i / kChunk, k = i % kChunk, d = blockIdx.y * kChunk + k;
-        // column k: lane and component
-        const int at = VEC ? k : k % 32 * 4 + k / 32;
-        if (d < D)
-            acc[((long long)blockIdx.x * V + j) * D + d] =
-                reinterpret_cast<const float *>(&sum[j][0])[at];
     }
 }
 

@@ -164,3 +164,28 @@ def test_forward_mode_is_refused(D, leaf):
                 fn(*args, labels)
         plain = fn(*[t.detach() for t in data], labels)
     assert torch.equal(plain, fn(*data, labels))
+
+
+@pytest.mark.parametrize("n,V,D,dtype", [
+    (1 << 20, 20000, 1, F32), (300007, 20000, 4, F32), (300007, 9000, 16, F32),
+    (1 << 20, 700, 4, F32), (1 << 20, 9, 4096, F32)])
+def test_table_gradient_of_many_equal_rows(n, V, D, dtype):
+    """Rows all alike: a class's gradient is n times one number, of which
+    every addition onto a long running sum is off the same way. The kernels
+    add 1024 rows at most before they begin a new sum, join at most a few
+    hundred of those (counted as 1024 too), and each addition is off by 2^-24
+    of the sum. The probabilities are off by 2^-15 (exponents below 32, a few
+    roundings of 2^-24 of them; scores of D products, (D + 8) 2^-24 of a sum
+    of magnitudes below 0.5 where D is large)."""
+    from gs_voxelizer_b200.losses import linear_cross_entropy
+    g = torch.Generator("cuda").manual_seed(56)
+    row = torch.rand(1, D, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(V, D, generator=g, device="cuda") / D).to(dtype).requires_grad_(True)
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")
+    loss = linear_cross_entropy(row.expand(n, D), w, labels, reduction="sum")
+    (got,) = torch.autograd.grad(loss, w)
+    p = torch.softmax(row.double() @ w.detach().double().t(), 1)[0]
+    p[0] -= 1.0
+    want = n * p[:, None] * row.double()
+    tol = (2048 * 2.0 ** -24 + 2.0 ** -15) * want.abs()
+    assert ((got.double() - want).abs() <= tol).all()
