@@ -13,8 +13,8 @@
 // needs atomics.
 //
 // What bounds it: issue and latency at the occupancy that the registers leave
-// (256^3 rows x 4 channels, 20 classes, float32: forward 180 us, dX 209 us,
-// dW 258 us; 0.6 instructions a clock and scheduler, 12 to 20 a score, the
+// (256^3 rows x 4 channels, 20 classes, float32: forward 190 us, dX 209 us,
+// dW 264 us; 0.6 instructions a clock and scheduler, 12 to 20 a score, the
 // exponentials alone would take 75 us each). One, two or four rows a thread,
 // three to five blocks an SM and pairs of rows instead of channels came to
 // 636 to 770 us for the three.
@@ -224,7 +224,7 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
                 continue;
             }
             float l = 0.f;
-            float2 lse = make_float2(m[k], __log2f(s[k]));
+            float2 lse = make_float2(m[k], ce_log2(s[k]));
             if (y[k] >= 0)
                 l = ce_row_loss(make_float2(CAP ? lse.x : lse.x * kCeLn2, lse.y), zy, sz[k], V,
                                 o);

@@ -222,7 +222,7 @@ staged_fwd_kernel(long long rows, int V, int passes, const T *__restrict__ score
             float l = 0.f;
             if (y >= 0) {
                 const float s = ce_to_float(p[y]);
-                l = ce_row_loss(make_float2(CeAcc::base(a.m), __log2f(a.s)),
+                l = ce_row_loss(make_float2(CeAcc::base(a.m), ce_log2(a.s)),
                                 CAP ? o.cap * ce_tanh<sizeof(T) == 2>(s, o.cap) : s, sz,
                                 V, o);
             } else if (y == kCeInvalid) {
@@ -290,12 +290,16 @@ staged_bwd_kernel(long long rows, int V, int passes, const T *__restrict__ score
         if (r + kPass < nr) y_next = labels[row0 + r + kPass];
         row.load(p, o.cap);
         const CeAcc a = row.reduce();
-        float2 lse = make_float2(CeAcc::base(a.m), __log2f(a.s));
-        if (y == kCeInvalid) lse.x = ce_nan();
-        const RowGrad q = row_grad(
-            lse, V, o.reduction == kCeNone ? grad_loss[row0 + r] : common, o);
+        // probabilities are exp(z - max) over their sum: no logarithm, unless
+        // the z-loss asks for the logsumexp itself
+        const float base = CeAcc::base(a.m);
+        float lse = 0.f;
+        if (o.zeta > 0.f) lse = ce_lse(make_float2(base, ce_log2(a.s)));
+        RowGrad q = row_grad(make_float2(lse, 0.f), V,
+                             o.reduction == kCeNone ? grad_loss[row0 + r] : common, o);
+        q.kz = y == kCeInvalid ? ce_nan() : __fdividef(q.kz, a.s);
         row.store(p, [&](int k, int j) {
-            float d = fmaf(q.kz, ce_prob(row.z[k], q.lse), -q.e);
+            float d = fmaf(q.kz, ex2((row.z[k] - base) * kLog2e), -q.e);
             if (j == y) d -= q.hit;
             if (CAP) d *= fmaf(-row.t[CAP ? k : 0], row.t[CAP ? k : 0], 1.f);
             return y == kCeIgnored ? 0.f : d;

@@ -2,6 +2,8 @@
 lowest table entries, infinite and vanishing upstream gradients, saved-tensor
 hooks, forward mode, long sums, and float32 results held to float32's own
 rounding (test_gpu_class_losses.py has the definition over all shapes)."""
+import math
+
 import pytest
 import torch
 
@@ -189,3 +191,45 @@ def test_table_gradient_of_many_equal_rows(n, V, D, dtype):
     want = n * p[:, None] * row.double()
     tol = (2048 * 2.0 ** -24 + 2.0 ** -15) * want.abs()
     assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("D", [0, 3, 4, 12, 40])
+def test_confident_rows_float32(D):
+    """Two classes, the label at score 0 and the other at -s: the loss is
+    log(1 + e^-s) and its error the rounding of that sum, 2^-24, but for what
+    e^-s < 0.0068 brings: (s 2^-20 + 2^-22) of it, below 2^-24 / 1.7, and the
+    logarithm's own rounding, 2^-22 of a loss below 0.0068."""
+    n = 4000
+    s = torch.linspace(5.0, 9.0, n, device="cuda")
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")
+    if D:
+        x = torch.zeros(n, D, device="cuda")
+        x[:, 0] = s
+        w = torch.zeros(2, D, device="cuda")
+        w[1, 0] = -1.0
+        data = (x, w)
+    else:
+        data = (torch.stack([torch.zeros_like(s), -s], 1),)
+    want = torch.log1p(torch.exp(-s.double()))
+    for needed in (False, True):
+        up = torch.ones(n, device="cuda") if needed else None
+        loss, _ = call(data, labels, dict(reduction="none"), up)
+        assert float((loss.double() - want).abs().max()) <= 1.7 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("D", [0, 4, 40])
+def test_equal_classes_float32(D):
+    """V equal scores: the sum is V exactly, and the loss its logarithm, off by
+    2^-22 of that of a number below 1.5, an addition and a product's rounding."""
+    for V in (*range(1, 70), 127, 129, 500, 777, 1000, 1024):
+        data = ((torch.zeros(9, D, device="cuda"), torch.zeros(V, D, device="cuda")) if D
+                else (torch.full((9, V), -7.25, device="cuda"),))
+        labels = torch.full((9,), V // 2, dtype=torch.int64, device="cuda")
+        loss, grads = call(data, labels, dict(reduction="sum"),
+                           torch.ones((), device="cuda"))
+        want = 9 * math.log(V)
+        assert abs(float(loss) - want) <= 9 * (0.41 * 2.0 ** -22 + 2.0 ** -23 * math.log(V))
+        if not D:
+            p = torch.full((9, V), 1.0 / V, dtype=torch.float64, device="cuda")
+            p[:, V // 2] -= 1.0
+            assert float((grads[0].double() - p).abs().max()) <= 2.0 ** -24 * (1 + 4.0 / V)
