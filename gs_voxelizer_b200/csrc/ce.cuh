@@ -112,6 +112,20 @@ struct CeAcc {
 
 __device__ __forceinline__ float ce_lse(float2 l) { return fmaf(l.y, kCeLn2, l.x); }
 
+// What the z-loss brings to a row's derivative; 0 where that is not finite.
+__device__ __forceinline__ float ce_z_factor(float2 lse, const CeOpt &o) {
+    const float f = 1.f + 2.f * o.zeta * fabsf(ce_lse(lse));
+    return isfinite(f) ? f : 0.f;
+}
+// out[0] = max(out[0], v) over a warp's values; the bits of non-negative floats
+// order as integers, and a maximum has no order
+__device__ __forceinline__ void ce_warp_max(float v, float *out) {
+#pragma unroll
+    for (int k = 16; k; k >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, k));
+    if ((threadIdx.x & 31) == 0 && v > 0.f)
+        atomicMax(reinterpret_cast<int *>(out), __float_as_int(v));
+}
+
 // probability of score z in a row of logsumexp l
 __device__ __forceinline__ float ce_prob(float z, float2 l) {
     return ex2(fmaf(z - l.x, kLog2e, -l.y));

@@ -14,6 +14,7 @@ struct FewArgs {
     CeOpt opt;
     float2 *lse;
     float *count;
+    float *zmax;  // largest factor of the z-loss, or null
 };
 
 size_t few_workspace_bytes(int N, int V);

@@ -485,6 +485,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // (the ratio is formed first: 2^14 over a vanishing gmax is infinite)
         float gmax = 1.f;
         if (PRODUCT == kCeProbs && g.grow && g.gmax && *g.gmax > 0.f) gmax = *g.gmax;
+        const float unit_scale = PRODUCT == kCeProbs ? g.p_scale / ce_z_scale(g.up) : 1.f;
         // a unit's row, read a unit ahead: units of few classes and channels
         // take no longer than these loads
         auto row_of = [&](int u) {
@@ -511,7 +512,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             float top = ce_neg_inf(), s = 0.f, sz = 0.f;
             float kz = 1.f, e = 0.f, hit = 0.f;
             if (PRODUCT == kCeProbs) {
-                const float f = g.p_scale * row.g;
+                const float f = unit_scale * row.g;
                 kz = (1.f + 2.f * o.zeta * ce_lse(lse)) * f;
                 e = o.eps / (float)g.V * f;
                 hit = (1.f - o.eps) * f;

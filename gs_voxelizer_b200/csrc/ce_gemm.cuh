@@ -30,12 +30,17 @@ struct CeUpstream {
     const float *gmax;   // or null
     float inv_p;         // 1 / p_scale
     int reduction;
+    const float *zmax = nullptr;  // largest factor of the z-loss, over which P is
 };
 
+__device__ __forceinline__ float ce_z_scale(const CeUpstream &u) {
+    return u.zmax ? fmaxf(*u.zmax, 1.f) : 1.f;
+}
+
 __device__ __forceinline__ float ce_grad_scale(const CeUpstream &u) {
-    if (u.reduction == kCeNone)
-        return (u.gmax && *u.gmax > 0.f ? *u.gmax : 1.f) * u.inv_p;
-    return (u.reduction == kCeMean ? u.g[0] / u.count[0] : u.g[0]) * u.inv_p;
+    const float inv = u.inv_p * ce_z_scale(u);
+    if (u.reduction == kCeNone) return (u.gmax && *u.gmax > 0.f ? *u.gmax : 1.f) * inv;
+    return (u.reduction == kCeMean ? u.g[0] / u.count[0] : u.g[0]) * inv;
 }
 
 struct CeGemm {
@@ -62,7 +67,7 @@ struct CeGemm {
     float2 *part;       // [2 * runs][rows] (maximum, sum)
     float *psum;        // [2 * runs][rows] plain sums (label smoothing) or null
     float *zt;          // [rows] score of the row's class
-    // kCeProbs: derivative * p_scale * (row's upstream gradient / gmax)
+    // kCeProbs: derivative * p_scale / z_scale * (row's upstream gradient / gmax)
     const float2 *lse;  // as X's rows
     void *p_out;        // P's storage (P describes it)
     float p_scale;

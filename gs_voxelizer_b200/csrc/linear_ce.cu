@@ -12,8 +12,8 @@
 //
 // Rounding P to 16 bits costs at most half a step (2^-8 of the value in bf16,
 // 2^-11 in fp16), no more than rounding the gradients themselves to the same
-// type. fp16 keeps P times a power of two (see p_scale_of) so that small
-// probabilities stay normal numbers. float32 inputs keep three bf16 planes of
+// type. fp16 keeps P times 2^14, over the largest factor that a z-loss brings to
+// a row, so that small probabilities stay normal numbers and none overflows. float32 inputs keep three bf16 planes of
 // every operand, which hold all 24 bits.
 //
 // Few channels, few classes of many float32 channels, and few rows have
@@ -96,6 +96,7 @@ index_kernel(long long n, long long padded, int V, const long long *__restrict__
     if (i == 0) {
         total[0] = (int)all;
         total[1] = 0;  // the merge's ticket
+        total[2] = 0;  // the z-loss's largest factor
     }
 }
 
@@ -196,7 +197,7 @@ merge_kernel(long long rows, int tiles, int V, bool packed, const float2 *__rest
              const int *__restrict__ lab, const long long *__restrict__ labels, CeOpt o,
              float *__restrict__ loss, float2 *__restrict__ lse_out,
              float *__restrict__ count, float2 *__restrict__ block_sums,
-             int *__restrict__ ticket) {
+             int *__restrict__ ticket, float *__restrict__ zmax) {
     constexpr int kRows = kMergeNT / SLICES;
     __shared__ float sm[SLICES][kRows], ss[SLICES][kRows], sz[SLICES][kRows];
     __shared__ float2 sh[kMergeNT / 32];
@@ -217,7 +218,7 @@ merge_kernel(long long rows, int tiles, int V, bool packed, const float2 *__rest
         sz[slice][lane] = a.sz;
         __syncthreads();
     }
-    float l = 0.f, c = 0.f;
+    float l = 0.f, c = 0.f, factor = 0.f;
     if (live && slice == 0) {
         for (int s = 1; s < SLICES; ++s)
             a.merge<LOG2>(sm[s][lane], ss[s][lane], sz[s][lane]);
@@ -230,8 +231,10 @@ merge_kernel(long long rows, int tiles, int V, bool packed, const float2 *__rest
             l = lse.x = ce_nan();
         c = y == kCeIgnored ? 0.f : 1.f;
         lse_out[r] = lse;
+        if (zmax) factor = ce_z_factor(lse, o);
         if (o.reduction == kCeNone) loss[idx ? idx[r] : r] = l;
     }
+    if (zmax) ce_warp_max(factor, zmax);
     const float2 t = ce_block_sum<kMergeNT>(l, c, sh);
     if (gridDim.x == 1) {
         if (threadIdx.x == 0) ce_finish(t.x, t.y, o.reduction, loss, count);
@@ -282,20 +285,20 @@ void launch_merge(long long rows, long long grid_rows, int parts, int V, bool pa
                   const float2 *part,
                   const float *psum, const float *zt, const int *total, const int *idx,
                   const int *lab, const long long *labels, const CeOpt &o, float *loss,
-                  float2 *lse, float *count, float2 *sums, int *ticket, cudaStream_t st) {
+                  float2 *lse, float *count, float2 *sums, int *ticket, float *zmax,
+                  cudaStream_t st) {
     const int per = merge_rows(parts);
     const unsigned blocks = (unsigned)((grid_rows + per - 1) / per);
     const auto kernel = per == kMergeNT ? merge_kernel<LOG2, 1> : merge_kernel<LOG2, 8>;
-    kernel<<<blocks, kMergeNT, 0, st>>>(rows, parts, V, packed, part, psum, zt, total, idx, lab, labels,
-                                        o, loss, lse, count, sums, ticket);
+    kernel<<<blocks, kMergeNT, 0, st>>>(rows, parts, V, packed, part, psum, zt, total, idx, lab,
+                                        labels, o, loss, lse, count, sums, ticket, zmax);
     count_launches(1);
 }
 
 // -------------------------------------------------------------- gradients
 
 // out[0] (zero before) = largest finite |g| of the labelled rows (an infinite
-// one is its own row's, and its factor is infinite over any other); the bits of
-// non-negative floats order as integers, and a maximum has no order
+// one is its own row's, and its factor is infinite over any other)
 __global__ void __launch_bounds__(256)
 max_abs_kernel(const float *__restrict__ g, const int *__restrict__ idx,
                const int *__restrict__ total, float *__restrict__ out) {
@@ -305,10 +308,7 @@ max_abs_kernel(const float *__restrict__ g, const int *__restrict__ idx,
         const float a = fabsf(g[idx[r]]);
         if (isfinite(a)) m = fmaxf(m, a);
     }
-#pragma unroll
-    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-    if ((threadIdx.x & 31) == 0 && m > 0.f)
-        atomicMax(reinterpret_cast<int *>(out), __float_as_int(m));
+    ce_warp_max(m, out);
 }
 
 // A gradient to be finished: dst[row of r] = scale * sum over splits of
@@ -459,7 +459,7 @@ struct Plan {
 
 // State (kept between the two directions): count (float, padded to 4 words),
 // lse [N] (two floats; of packed rows but on the narrow path), packed total
-// (int, padded to 4 words), idx [Np], lab [Np], block counts; then the packed
+// (int; then a ticket and the z-loss's largest factor, padded to 4 words), idx [Np], lab [Np], block counts; then the packed
 // features and the packed table where they are small: their kernels' launches
 // cost more than their memory, and the backward need not repeat them. On the
 // wide path the scores instead.
@@ -496,14 +496,12 @@ State state_of(void *p, long long N) {
     return s;
 }
 
-// |dloss / dscore| <= 1 + 2 zeta |lse|: the largest power of two, up to 2^14,
-// that keeps fp16 finite for |lse| <= 4096. The other types have the range
-// of float32.
-float p_scale_of(int type, const CeOpt &o) {
-    if (type != kCeF16) return 1.f;
-    float s = 16384.f;
-    while (s > 1.f / 1024.f && s * (1.f + 8192.f * o.zeta) > 65504.f) s *= 0.5f;
-    return s;
+// |dloss / dscore| <= 1 + 2 zeta |lse|. fp16 keeps it times 2^14, and with a
+// z-loss over the largest such factor of the labelled rows, which the forward
+// leaves in the state. The other types have the range of float32.
+float p_scale_of(int type) { return type == kCeF16 ? 16384.f : 1.f; }
+float *zmax_of(int type, const CeOpt &o, const State &s) {
+    return type == kCeF16 && o.zeta > 0.f ? reinterpret_cast<float *>(s.total + 2) : nullptr;
 }
 
 // Parts of the summed axis, at least 512 each. A product of `tiles` tiles takes
@@ -731,7 +729,7 @@ cudaError_t narrow_forward(const NarrowArgs &a, float *loss, unsigned char *ws,
         blocks = (a.N + merge_rows(p.splits) - 1) / merge_rows(p.splits);
         const auto merge = a.opt.cap > 0.f ? launch_merge<false> : launch_merge<true>;
         merge(a.N, a.N, p.splits, a.V, false, part, psum, zt, nullptr, nullptr, nullptr, a.labels,
-              a.opt, loss, a.lse, a.count, sums, nullptr, st);
+              a.opt, loss, a.lse, a.count, sums, nullptr, nullptr, st);
         GSV_CE_TRY(cudaGetLastError());
     }
     if (blocks > 1)
@@ -902,6 +900,7 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
                             ws, st);
     const Plan p = make_plan(N, V, D, type, weight, false, o);
     const bool direct = in_place(N, V, D, type, features);
+    float *zmax = zmax_of(type, o, s);
     if (!forward_only || (path == kTiles && !direct)) {
         const int nb = (int)((p.Np + kIdxNT - 1) / kIdxNT);
         if (nb > 1) {
@@ -914,7 +913,8 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         GSV_CE_TRY(cudaGetLastError());
     }
     if (path == kFew) {
-        const FewArgs a{(int)N, V, D, features, weight, labels, o, s.lse, s.count};
+        const FewArgs a{(int)N, V, D, features, weight, labels, o, s.lse, s.count,
+                        forward_only ? nullptr : zmax};
         return launch_few_forward(a, type, loss, ws, st);
     }
     // merged by packed rows, which leaves out those without a label
@@ -943,7 +943,7 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     launch_merge<false>(g.rows, N, 2 * p.runs, V, !direct, g.part, g.psum, g.zt,
                         indexed ? s.total : nullptr, indexed ? s.idx : nullptr,
                         indexed ? s.lab : nullptr, labels, o, loss, s.lse, s.count, sums,
-                        indexed ? s.total + 1 : nullptr, st);
+                        indexed ? s.total + 1 : nullptr, forward_only ? nullptr : zmax, st);
     GSV_CE_TRY(cudaGetLastError());
     if (mb > 1 && !indexed)
         GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));
@@ -988,10 +988,10 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
     CeGemm g = gemm_of(p, s, weight, ws, o);
     g.lse = s.lse;
     g.p_out = ws + p.p;
-    g.p_scale = p_scale_of(type, o);
+    g.p_scale = p_scale_of(type);
     g.grow = none ? grad_loss : nullptr;
     g.gmax = gmax;
-    g.up = {grad_loss, s.count, gmax, 1.f / g.p_scale, o.reduction};
+    g.up = {grad_loss, s.count, gmax, 1.f / g.p_scale, o.reduction, zmax_of(type, o, s)};
     float *dx = reinterpret_cast<float *>(ws + p.dx);
     float *dw = reinterpret_cast<float *>(ws + p.dw);
     g.acc_ld = up(D, 4);

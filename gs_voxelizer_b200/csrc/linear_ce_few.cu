@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(kMergeNT *kFewRows)
 few_merge_kernel(int N, int V, int parts, const float2 *__restrict__ part,
                  const float *__restrict__ psum, const float *__restrict__ zt,
                  const long long *__restrict__ labels, CeOpt o, float *__restrict__ loss,
-                 float2 *__restrict__ lse_out, float *__restrict__ count) {
+                 float2 *__restrict__ lse_out, float *__restrict__ count,
+                 float *__restrict__ zmax) {
     __shared__ float sh[kFewRows][kMergeNT / 32][3];
     __shared__ float s_loss[kFewRows], s_count[kFewRows];
     const int r = threadIdx.x / kMergeNT, t = threadIdx.x % kMergeNT;
@@ -155,6 +156,8 @@ few_merge_kernel(int N, int V, int parts, const float2 *__restrict__ part,
         int before = 0;
         for (int k = 0; k < r; ++k) before += labels[k] != o.ignore;
         if (y != kCeIgnored) lse_out[before] = lse;
+        if (zmax && y != kCeIgnored)
+            atomicMax(reinterpret_cast<int *>(zmax), __float_as_int(ce_z_factor(lse, o)));
         if (o.reduction == kCeNone) loss[r] = l;
         s_loss[r] = l;
         s_count[r] = y == kCeIgnored ? 0.f : 1.f;
@@ -205,7 +208,7 @@ cudaError_t few_forward(const FewArgs &a, float *loss, unsigned char *ws, cudaSt
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     few_merge_kernel<<<1, kMergeNT * a.N, 0, st>>>(a.N, a.V, blocks, part, psum, zt, a.labels,
-                                                   a.opt, loss, a.lse, a.count);
+                                                   a.opt, loss, a.lse, a.count, a.zmax);
     count_launches(2);
     return cudaGetLastError();
 }

@@ -233,3 +233,33 @@ def test_equal_classes_float32(D):
             p = torch.full((9, V), 1.0 / V, dtype=torch.float64, device="cuda")
             p[:, V // 2] -= 1.0
             assert float((grads[0].double() - p).abs().max()) <= 2.0 ** -24 * (1 + 4.0 / V)
+
+
+@pytest.mark.parametrize("size,zeta", [(8000.0, 1e-2), (30000.0, 1e-3), (60000.0, 1.0)])
+@pytest.mark.parametrize("n", [3, 100])
+def test_z_loss_of_large_scores_fp16(n, size, zeta):
+    """Scores in the tens of thousands: the z-loss's factor 1 + 2 zeta lse
+    takes no derivative out of fp16's range."""
+    g = torch.Generator("cuda").manual_seed(57)
+    D, V = 64, 300
+    x = (8.0 + 0.1 * torch.randn(n, D, generator=g, device="cuda")).half()
+    w = (size / (8.0 * D) + 0.3 * torch.randn(V, D, generator=g, device="cuda")).half()
+    labels = torch.randint(0, V, (n,), generator=g, device="cuda")
+    labels[1] = -100
+    up = torch.tensor(0.1 / (1.0 + 2.0 * zeta * size), device="cuda")
+    loss, grads = call((x, w), labels, dict(z_loss=zeta), up)
+    assert all(t.isfinite().all() for t in grads)
+    # A float32 score of this size is off by (D + 8) 2^-23 of it at most, too
+    # much for its probability, but a row's probabilities sum to 1: the sum of
+    # dW over the classes is the z-loss's factor alone. (Few rows: the backward
+    # forms the scores another way than the forward, and they sum to 1 within
+    # e^(both errors).)
+    es = 2 * (D + 8) * 2.0 ** -23 * size if n < 5 else 0.0
+    lse = torch.logsumexp(x.double() @ w.double().t(), 1)
+    keep = labels != -100
+    total = (2.0 * zeta * lse * float(up) / int(keep.sum()))[keep]
+    # dW summed over classes = sum over rows of the row's total times x; each
+    # of n V products is off by 2^-11 of P or of the result's rounding
+    want = (total[:, None] * x[keep].double()).sum(0)
+    size_of = ((total + 2 * float(up) / int(keep.sum()))[:, None] * x[keep].double()).sum(0)
+    assert ((grads[1].double().sum(0) - want).abs() <= (2.0 ** -9 + math.expm1(es)) * size_of).all()
