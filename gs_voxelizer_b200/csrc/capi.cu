@@ -1094,6 +1094,8 @@ int check_ce(const char *fn, int64_t rows, int32_t classes, int32_t channels, in
                     o->z_loss <= 1e30f,
                 GSV_ERR_INVALID_ARGUMENT,
                 "%s: softcap and z_loss must be finite and not negative", fn);
+    GSV_REQUIRE(o->softcap == 0.f || o->softcap >= 1e-30f, GSV_ERR_INVALID_ARGUMENT,
+                "%s: softcap must be 0 (none) or at least 1e-30", fn);
     GSV_REQUIRE(o->reduction >= GSV_REDUCE_NONE && o->reduction <= GSV_REDUCE_MEAN,
                 GSV_ERR_INVALID_ARGUMENT, "%s: unknown reduction %d", fn, o->reduction);
     return GSV_OK;

@@ -312,10 +312,15 @@ def _ce_args(named, labels, ignore_index, label_smoothing, softcap, z_loss,
                          f"{tuple(first.shape[:-1])}")
     if reduction not in _CE_REDUCTIONS:
         raise ValueError(f"unsupported reduction {reduction!r}")
-    if not 0.0 <= label_smoothing < 1.0:
+    # (the largest float32 below 1: what rounds to 1 is refused too)
+    if not 0.0 <= label_smoothing <= 1.0 - 2.0 ** -24:
         raise ValueError("label_smoothing must be in [0, 1)")
     if not (0.0 <= softcap <= 1e30 and 0.0 <= z_loss <= 1e30):
         raise ValueError("softcap and z_loss must be finite and >= 0")
+    if 0.0 < softcap < 1e-30:  # float32's 0 would be no cap
+        raise ValueError("softcap must be 0 (none) or at least 1e-30")
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index must be a 64-bit integer")
     opt = CeOptions(int(ignore_index), label_smoothing, softcap, z_loss,
                     _CE_REDUCTIONS[reduction])
     return labels.to(torch.int64).contiguous(), opt

@@ -536,8 +536,8 @@ enum gsv_reduction { GSV_REDUCE_NONE = 0, GSV_REDUCE_SUM = 1, GSV_REDUCE_MEAN = 
 typedef struct gsv_ce_options {
     int64_t ignore_index;
     float label_smoothing; /* 0 <= . < 1 */
-    float softcap;         /* >= 0; 0: no cap */
-    float z_loss;          /* >= 0 */
+    float softcap;         /* 0: no cap; else 1e-30 to 1e30 */
+    float z_loss;          /* 0 to 1e30 */
     int32_t reduction;     /* gsv_reduction */
 } gsv_ce_options;
 

@@ -66,3 +66,14 @@ def test_linear_entries_refuse_misaligned_pointers(dtype, size, sizes):
         ptr[name] += size_of // 2
         assert refused(call(lib.gsv_linear_ce_backward, sizes, ptr, dtype,
                             (1 << 40, None))), name
+
+
+@pytest.mark.parametrize("cap", [1e-31, 1e-40, 1e31, float("nan")])
+def test_caps_that_float32_cannot_divide_by(cap):
+    """1 / cap would be infinite, and a score of 0 NaN."""
+    p = ctypes.c_void_p(P)
+    opt = CeOptions(-100, 0.0, cap, 0.0, 2)
+    assert lib.gsv_softmax_ce_forward(7, 5, 0, p, p, opt, p, p, p, p, 1 << 20, None) == 1
+    assert b"softcap" in lib.gsv_last_error()
+    assert lib.gsv_linear_ce_forward(7, 5, 4, 0, p, p, p, opt, p, p, p, 1 << 40, None) == 1
+    assert lib.gsv_linear_ce_workspace_bytes(7, 5, 4, 0, opt, 0) == 0

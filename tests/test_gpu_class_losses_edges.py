@@ -263,3 +263,18 @@ def test_z_loss_of_large_scores_fp16(n, size, zeta):
     want = (total[:, None] * x[keep].double()).sum(0)
     size_of = ((total + 2 * float(up) / int(keep.sum()))[:, None] * x[keep].double()).sum(0)
     assert ((grads[1].double().sum(0) - want).abs() <= (2.0 ** -9 + math.expm1(es)) * size_of).all()
+
+
+def test_options_that_float32_and_int64_do_not_hold():
+    from gs_voxelizer_b200.losses import linear_cross_entropy, softmax_cross_entropy
+    (x, w), y = make(10, 7, 5, F32, 58)
+    for bad in (dict(softcap=1e-50), dict(softcap=1e-40), dict(softcap=1e-31),
+                dict(ignore_index=2 ** 63), dict(ignore_index=2 ** 64 - 100),
+                dict(ignore_index=-2 ** 63 - 1), dict(label_smoothing=1 - 1e-12)):
+        with pytest.raises(ValueError):
+            softmax_cross_entropy(x, y.clamp_max(4), **bad)
+        with pytest.raises(ValueError):
+            linear_cross_entropy(x, w, y, **bad)
+    for cap in (1e-30, 1e-6):
+        loss, _ = call((x,), y.clamp_max(4), dict(softcap=cap))
+        assert float(loss) == pytest.approx(1.6094379, abs=1e-5)  # log 5
