@@ -27,7 +27,6 @@ _I3 = ctypes.c_int32 * 3
 _F3 = ctypes.c_float * 3
 
 
-
 class CeOptions(ctypes.Structure):
     """gsv_ce_options of include/gsvox.h."""
     _fields_ = [("ignore_index", _I64), ("label_smoothing", ctypes.c_float),
@@ -120,6 +119,7 @@ SIGNATURES = {
         ctypes.c_int, [_I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P,
                        _P, _P]),
     "gsv_softmax_ce_workspace_bytes": (_SZ, [_I64, _I32]),
+    "gsv_softmax_ce_lse_bytes": (_SZ, [_I64, _I32]),
     "gsv_softmax_ce_forward": (
         ctypes.c_int, [_I64, _I32, _I32, _P, _P, _OPT, _P, _P, _P, _P, _SZ, _P]),
     "gsv_softmax_ce_backward": (

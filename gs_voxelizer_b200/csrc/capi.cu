@@ -142,8 +142,9 @@ cudaError_t launch_softmax_ce(bool fwd, int type, long long rows, int V, const v
                               float2 *lse, float *count, const float *grad_loss, void *grad,
                               void *ws, cudaStream_t st);
 size_t linear_ce_state_bytes(long long N, int V, int D, int type);
-size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
-                                 const CeOpt &o);
+size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, CeCall call, bool aligned_x,
+                                 bool aligned_w, const CeOpt &o);
+bool softmax_ce_keeps_lse(int V);
 cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
                                      const void *features, const void *weight,
                                      const long long *labels, const CeOpt &o, float *loss,
@@ -1126,14 +1127,19 @@ size_t gsv_softmax_ce_workspace_bytes(int64_t rows, int32_t classes) {
     return gsv::softmax_ce_workspace_bytes(rows, classes);
 }
 
+size_t gsv_softmax_ce_lse_bytes(int64_t rows, int32_t classes) {
+    if (rows < 1 || classes < 1 || !gsv::softmax_ce_keeps_lse(classes)) return 0;
+    return sizeof(float2) * (size_t)rows;
+}
+
 int gsv_softmax_ce_forward(int64_t rows, int32_t classes, int32_t dtype, const void *scores,
                            const int64_t *labels, const gsv_ce_options *options, float *loss,
                            float *lse, float *count, void *ws, size_t ws_bytes,
                            void *stream) {
     const char *fn = "gsv_softmax_ce_forward";
     if (const int st = check_ce(fn, rows, classes, 1, dtype, options)) return st;
-    GSV_REQUIRE(scores && labels && loss && lse && count, GSV_ERR_INVALID_ARGUMENT,
-                "%s: null pointer", fn);
+    GSV_REQUIRE(scores && labels && loss && (lse || !gsv::softmax_ce_keeps_lse(classes)) && count,
+                GSV_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
     const size_t need = gsv_softmax_ce_workspace_bytes(rows, classes);
     GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
                 "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
@@ -1152,7 +1158,8 @@ int gsv_softmax_ce_backward(int64_t rows, int32_t classes, int32_t dtype, const 
                             void *grad_scores, void *stream) {
     const char *fn = "gsv_softmax_ce_backward";
     if (const int st = check_ce(fn, rows, classes, 1, dtype, options)) return st;
-    GSV_REQUIRE(scores && labels && lse && count && grad_loss && grad_scores,
+    GSV_REQUIRE(scores && labels && (lse || !gsv::softmax_ce_keeps_lse(classes)) && count &&
+                    grad_loss && grad_scores,
                 GSV_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
     GSV_REQUIRE(aligned(ce_size(dtype), {scores, grad_scores}) && aligned(8, {labels, lse}) &&
                     aligned(4, {count, grad_loss}),
@@ -1175,11 +1182,15 @@ size_t gsv_linear_ce_state_bytes(int64_t rows, int32_t classes, int32_t channels
 
 size_t gsv_linear_ce_workspace_bytes(int64_t rows, int32_t classes, int32_t channels,
                                      int32_t dtype, const gsv_ce_options *options,
-                                     int32_t backward) {
+                                     int32_t call) {
     if (check_ce("gsv_linear_ce_workspace_bytes", rows, classes, channels, dtype, options))
         return 0;
-    return gsv::linear_ce_workspace_bytes(rows, classes, channels, dtype, backward != 0,
-                                          ce_opt(options));
+    const bool on_16 = (call & GSV_CE_ALIGNED) != 0;
+    return gsv::linear_ce_workspace_bytes(rows, classes, channels, dtype,
+                                          (call & GSV_CE_BACKWARD) ? gsv::kCeBackward
+                                          : (call & GSV_CE_STATE)  ? gsv::kCeForward
+                                                                   : gsv::kCeForwardOnly,
+                                          on_16, on_16, ce_opt(options));
 }
 
 int gsv_linear_ce_forward(int64_t rows, int32_t classes, int32_t channels, int32_t dtype,
@@ -1190,8 +1201,9 @@ int gsv_linear_ce_forward(int64_t rows, int32_t classes, int32_t channels, int32
     if (const int st = check_ce(fn, rows, classes, channels, dtype, options)) return st;
     GSV_REQUIRE(features && weight && labels && loss, GSV_ERR_INVALID_ARGUMENT,
                 "%s: null pointer", fn);
-    const size_t need =
-        gsv_linear_ce_workspace_bytes(rows, classes, channels, dtype, options, 0);
+    const size_t need = gsv::linear_ce_workspace_bytes(
+        rows, classes, channels, dtype, state ? gsv::kCeForward : gsv::kCeForwardOnly,
+        aligned(16, {features}), aligned(16, {weight}), ce_opt(options));
     GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
                 "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
     GSV_REQUIRE(aligned(256, {ws}) && aligned(16, {state}), GSV_ERR_INVALID_ARGUMENT,
@@ -1214,8 +1226,9 @@ int gsv_linear_ce_backward(int64_t rows, int32_t classes, int32_t channels, int3
     if (const int st = check_ce(fn, rows, classes, channels, dtype, options)) return st;
     GSV_REQUIRE(features && weight && labels && state && grad_loss, GSV_ERR_INVALID_ARGUMENT,
                 "%s: null pointer", fn);
-    const size_t need =
-        gsv_linear_ce_workspace_bytes(rows, classes, channels, dtype, options, 1);
+    const size_t need = gsv::linear_ce_workspace_bytes(
+        rows, classes, channels, dtype, gsv::kCeBackward, aligned(16, {features}),
+        aligned(16, {weight}), ce_opt(options));
     GSV_REQUIRE(ws && ws_bytes >= need, GSV_ERR_WORKSPACE_TOO_SMALL,
                 "%s: workspace of %zu bytes given, %zu needed", fn, ws_bytes, need);
     GSV_REQUIRE(aligned(256, {ws}) && aligned(16, {state}), GSV_ERR_INVALID_ARGUMENT,

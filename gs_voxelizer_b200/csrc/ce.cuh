@@ -18,6 +18,9 @@ namespace gsv {
 
 enum CeType { kCeF32 = 0, kCeBf16 = 1, kCeF16 = 2 };
 enum CeReduction { kCeNone = 0, kCeSum = 1, kCeMean = 2 };
+// Directions of the linear loss: a forward without a backward to follow, one
+// that leaves a state, the backward.
+enum CeCall { kCeForwardOnly, kCeForward, kCeBackward };
 
 // Options of a class loss, by value into the kernels.
 struct CeOpt {

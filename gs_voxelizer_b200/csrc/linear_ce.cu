@@ -1,7 +1,7 @@
 // Softmax cross entropy of a linear map: scores X W^T of N feature rows
 // against a table of V classes, without keeping the N x V scores.
 //
-// Forward: the labelled rows are packed into whole 128-row tiles (rows
+// Forward: the labelled rows are packed into whole 256-row tiles (rows
 // without a label cost nothing and cannot leak what they hold), the product
 // runs tile by tile and leaves one (maximum, sum) pair per row and class
 // tile, and a merge turns the pairs into lse and loss.
@@ -444,6 +444,8 @@ struct Plan {
     long long N, Np;      // rows, rows in whole tiles
     int V, D, type, planes;
     long long ld;         // of packed features / table
+    bool direct;          // the forward reads the rows in place
+    bool indexed;         // the labelled rows are listed
     bool pack_w;          // the table cannot be read in place
     bool keep_x, keep_w;  // packed in the state, not in the workspace
     int runs;             // runs of class tiles in the forward
@@ -458,11 +460,13 @@ struct Plan {
 };
 
 // State (kept between the two directions): count (float, padded to 4 words),
-// lse [N] (two floats; of packed rows but on the narrow path), packed total
-// (int; then a ticket and the z-loss's largest factor, padded to 4 words), idx [Np], lab [Np], block counts; then the packed
-// features and the packed table where they are small: their kernels' launches
-// cost more than their memory, and the backward need not repeat them. On the
-// wide path the scores instead.
+// lse [N] (two floats; of packed rows but on the narrow and wide paths); then,
+// where the labelled rows are listed, packed total (int; a ticket and the
+// z-loss's largest factor; padded to 4 words), idx [Np], lab [Np], block counts;
+// then the packed features and the packed table where they are small: their
+// kernels' launches cost more than their memory, and the backward need not
+// repeat them. On the wide path the scores instead. A forward without a state
+// has its first parts in the workspace.
 struct State {
     float *count;
     float2 *lse;
@@ -477,22 +481,25 @@ size_t packed_bytes(long long rows, int D, int type) {
 }
 bool kept(size_t bytes) { return bytes <= kKeepBytes; }
 
-long long state_words(long long N) {
-    const long long Np = up(N, kCeTileM);
-    return up(4 + up(2 * N, 4) + 4 + 2 * Np + up((N + kIdxNT - 1) / kIdxNT, 4), 64);
+long long state_words(long long N, bool indexed) {
+    const long long stats = 4 + up(2 * N, 4);
+    if (!indexed) return up(stats, 64);
+    return up(stats + 4 + 2 * up(N, kCeTileM) + up((N + kIdxNT - 1) / kIdxNT, 4), 64);
 }
 
-State state_of(void *p, long long N) {
+State state_of(void *p, long long N, bool indexed) {
     const long long Np = up(N, kCeTileM);
     float *f = static_cast<float *>(p);
-    State s;
+    State s{};
     s.count = f;
     s.lse = reinterpret_cast<float2 *>(f + 4);
-    s.total = reinterpret_cast<int *>(f + 4 + up(2 * N, 4));
-    s.idx = s.total + 4;
-    s.lab = s.idx + Np;
-    s.counts = s.lab + Np;
-    s.packed = reinterpret_cast<unsigned char *>(f + state_words(N));
+    if (indexed) {
+        s.total = reinterpret_cast<int *>(f + 4 + up(2 * N, 4));
+        s.idx = s.total + 4;
+        s.lab = s.idx + Np;
+        s.counts = s.lab + Np;
+    }
+    s.packed = reinterpret_cast<unsigned char *>(f + state_words(N, indexed));
     return s;
 }
 
@@ -525,7 +532,39 @@ int splits_for(long long tiles, long long depth, bool f32, long long elements) {
     return best;
 }
 
-Plan make_plan(long long N, int V, int D, int type, const void *weight, bool backward,
+// Which kernels serve a call. kNarrow (linear_ce_narrow.cu, the CUDA cores
+// without tiles): where it is the faster. Kernels' time of a training step,
+// narrow against tiles: 53000 rows x 203 classes, D = 16, 99 against 180 us of
+// float32, 90 against 98 of bf16; D = 32, 156 against 170 and 145 against 80;
+// 10^6 rows x 20 classes, D = 16, 148 against 1311 and 134 against 530, D = 32,
+// 356 and 299 against 530 of bf16; 1000 rows x 50000 classes, D = 16, 267
+// against 472 and 250 against 160, D = 32, 584 against 480 of float32.
+// kWide: few classes, many float32 channels (linear_ce_wide.cu). kFew
+// (linear_ce_few.cu): the forward alone; its backward takes tiles.
+enum Path { kNarrow, kWide, kFew, kTiles };
+Path path_of(long long N, int V, int D, int type) {
+    const int most = D <= 8 ? INT_MAX
+                     : D <= 16 ? (type == kCeF32 ? INT_MAX : 128)
+                     : D <= kNarrowD ? (type == kCeF32 ? 256 : 64)
+                                     : 0;
+    if (V <= most) return kNarrow;
+    if (type == kCeF32 && V <= kWideV && N >= kWideRows) return kWide;
+    return N <= (type == kCeF32 ? kFewRows : kFewRows / 2) ? kFew : kTiles;
+}
+
+// Rows that the forward's tiles read in place, 16 bits and aligned for TMA:
+// where packing them costs more than the products of unlabelled rows that it
+// saves. Packing moves 4 N D bytes, a share f of unlabelled rows takes
+// 2 f N V D operations: at 5 TB/s and 1.4 PFLOP/s they meet at f V = 570.
+// One tile of rows cannot become fewer.
+bool in_place(long long N, int V, int D, int type) {
+    return (N <= kCeTileM || V <= 1024) && type != kCeF32 && D % 8 == 0;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// aligned_x, aligned_w: the inputs are, for TMA
+Plan make_plan(long long N, int V, int D, int type, CeCall call, bool aligned_x, bool aligned_w,
                const CeOpt &o) {
     Plan p{};
     p.N = N;
@@ -535,9 +574,9 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     p.type = type;
     p.planes = type == kCeF32 ? 3 : 1;
     p.ld = up(D, 8);
-    // `weight` null: the workspace query, which allows for any alignment
-    p.pack_w = p.planes == 3 || D % 8 != 0 || weight == nullptr ||
-               (reinterpret_cast<uintptr_t>(weight) & 15) != 0;
+    p.pack_w = p.planes == 3 || D % 8 != 0 || !aligned_w;
+    p.direct = call != kCeBackward && aligned_x && in_place(N, V, D, type);
+    p.indexed = call != kCeForwardOnly || !p.direct;
     size_t at = 0;
     auto take = [&](size_t b) {
         const size_t o = at;
@@ -547,11 +586,11 @@ Plan make_plan(long long N, int V, int D, int type, const void *weight, bool bac
     p.sums = take(sizeof(float2) * (size_t)(N / 32 + 1));
     // packed operands: in the state where they are kept
     const size_t xb = packed_bytes(p.Np, D, type), wb = packed_bytes(V, D, type);
-    p.keep_x = kept(xb);
-    p.keep_w = kept(wb);
-    p.xp = p.keep_x ? 0 : take(xb);
+    p.keep_x = call != kCeForwardOnly && kept(xb);
+    p.keep_w = call != kCeForwardOnly && kept(wb);
+    p.xp = p.keep_x ? 0 : take(p.direct ? 0 : xb);
     p.wp = p.keep_w ? (p.keep_x ? align256(xb) : 0) : take(p.pack_w ? wb : 0);
-    if (!backward) {
+    if (call != kCeBackward) {
         p.runs = ce_runs(N, V, p.planes == 3);
         p.part = take(sizeof(float2) * 2 * (size_t)p.runs * p.Np);
         p.psum = take(o.eps > 0.f ? sizeof(float) * 2 * (size_t)p.runs * p.Np : 0);
@@ -806,44 +845,12 @@ cudaError_t wide_backward(const NarrowArgs &a, const float *z, const float *grad
                                 gw, st);
 }
 
-// Which kernels serve a call. kNarrow (linear_ce_narrow.cu, the CUDA cores
-// without tiles): where it is the faster. Kernels' time of a training step,
-// narrow against tiles: 53000 rows x 203 classes, D = 16, 99 against 180 us of
-// float32, 90 against 98 of bf16; D = 32, 156 against 170 and 145 against 80;
-// 10^6 rows x 20 classes, D = 16, 148 against 1311 and 134 against 530, D = 32,
-// 356 and 299 against 530 of bf16; 1000 rows x 50000 classes, D = 16, 267
-// against 472 and 250 against 160, D = 32, 584 against 480 of float32.
-// kWide: few classes, many float32 channels (linear_ce_wide.cu). kFew
-// (linear_ce_few.cu): the forward alone; its backward takes tiles.
-enum Path { kNarrow, kWide, kFew, kTiles };
-Path path_of(long long N, int V, int D, int type) {
-    const int most = D <= 8 ? INT_MAX
-                     : D <= 16 ? (type == kCeF32 ? INT_MAX : 128)
-                     : D <= kNarrowD ? (type == kCeF32 ? 256 : 64)
-                                     : 0;
-    if (V <= most) return kNarrow;
-    if (type == kCeF32 && V <= kWideV && N >= kWideRows) return kWide;
-    return N <= (type == kCeF32 ? kFewRows : kFewRows / 2) ? kFew : kTiles;
-}
-
-// Rows that the forward's tiles read in place, 16 bits and aligned for TMA:
-// where packing them costs more than the products of unlabelled rows that it
-// saves. Packing moves 4 N D bytes, a share f of unlabelled rows takes
-// 2 f N V D operations: at 5 TB/s and 1.4 PFLOP/s they meet at f V = 570.
-// One tile of rows cannot become fewer.
-bool in_place_sizes(long long N, int V, int D, int type) {
-    return (N <= kCeTileM || V <= 1024) && type != kCeF32 && D % 8 == 0;
-}
-bool in_place(long long N, int V, int D, int type, const void *features) {
-    return in_place_sizes(N, V, D, type) && (reinterpret_cast<uintptr_t>(features) & 15) == 0;
-}
-
 // What a forward with a state has packed and kept whatever its pointers were:
 // the backward's may be others (of the same contents), and what the forward
 // packed only for its pointers' alignment is packed again.
 bool x_is_kept(const Plan &p) {
     return path_of(p.N, p.V, p.D, p.type) == kTiles && p.keep_x &&
-           !in_place_sizes(p.N, p.V, p.D, p.type);
+           !in_place(p.N, p.V, p.D, p.type);
 }
 bool w_is_kept(const Plan &p) {
     return path_of(p.N, p.V, p.D, p.type) == kTiles && p.keep_w &&
@@ -853,8 +860,8 @@ bool w_is_kept(const Plan &p) {
 }  // namespace
 
 size_t linear_ce_state_bytes(long long N, int V, int D, int type) {
-    size_t b = (size_t)state_words(N) * 4;
     const Path path = path_of(N, V, D, type);
+    size_t b = 4 * (size_t)state_words(N, path == kTiles || path == kFew);
     if (path == kNarrow) return b;
     if (path == kWide) return b + wide_p_bytes(N, V);
     const size_t xb = packed_bytes(up(N, kCeTileM), D, type), wb = packed_bytes(V, D, type);
@@ -863,18 +870,21 @@ size_t linear_ce_state_bytes(long long N, int V, int D, int type) {
     return b;
 }
 
-size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, bool backward,
-                                 const CeOpt &o) {
-    // a forward without a state keeps its statistics (and, of tiles, the
-    // packed rows' index) here
-    const size_t own = backward ? 0 : align256(linear_ce_state_bytes(N, V, D, type));
+size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, CeCall call, bool aligned_x,
+                                 bool aligned_w, const CeOpt &o) {
+    const bool backward = call == kCeBackward;
     const Path path = path_of(N, V, D, type);
-    switch (backward && path == kFew ? kTiles : path) {
-        case kNarrow: return own + narrow_plan(N, V, D, backward, o).bytes;
-        case kWide: return own + wide_plan(N, V, D, backward).bytes;
-        case kFew: return own + few_workspace_bytes((int)N, V);
-        default: return own + make_plan(N, V, D, type, nullptr, backward, o).bytes;
-    }
+    const bool tiles = path == kTiles || (backward && path == kFew);
+    Plan p{};
+    if (tiles) p = make_plan(N, V, D, type, call, aligned_x, aligned_w, o);
+    // a forward without a state keeps its statistics (and, of tiles, the
+    // labelled rows' list) here
+    const size_t own =
+        call == kCeForwardOnly ? align256(4 * (size_t)state_words(N, p.indexed)) : 0;
+    if (tiles) return own + p.bytes;
+    return own + (path == kNarrow ? narrow_plan(N, V, D, backward, o).bytes
+                  : path == kWide ? wide_plan(N, V, D, backward).bytes
+                                  : few_workspace_bytes((int)N, V));
 }
 
 cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
@@ -882,10 +892,15 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
                                      const long long *labels, const CeOpt &o, float *loss,
                                      void *state, void *workspace, cudaStream_t st) {
     const bool forward_only = state == nullptr;
-    unsigned char *ws = static_cast<unsigned char *>(workspace);
-    const State s = state_of(forward_only ? ws : state, N);
-    ws += align256(linear_ce_state_bytes(N, V, D, type));
     const Path path = path_of(N, V, D, type);
+    Plan p{};
+    if (path == kTiles)
+        p = make_plan(N, V, D, type, forward_only ? kCeForwardOnly : kCeForward,
+                      aligned16(features), aligned16(weight), o);
+    const bool indexed = path == kTiles ? p.indexed : path == kFew && !forward_only;
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    const State s = state_of(forward_only ? ws : state, N, indexed);
+    if (forward_only) ws += align256(4 * (size_t)state_words(N, indexed));
     if (path == kNarrow) {
         const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
         switch (type) {
@@ -898,29 +913,27 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         return wide_forward({N, V, D, features, weight, labels, o, s.lse, s.count},
                             forward_only ? nullptr : reinterpret_cast<float *>(s.packed), loss,
                             ws, st);
-    const Plan p = make_plan(N, V, D, type, weight, false, o);
-    const bool direct = in_place(N, V, D, type, features);
-    float *zmax = zmax_of(type, o, s);
-    if (!forward_only || (path == kTiles && !direct)) {
-        const int nb = (int)((p.Np + kIdxNT - 1) / kIdxNT);
+    float *zmax = forward_only ? nullptr : zmax_of(type, o, s);
+    if (indexed) {
+        const long long Np = up(N, kCeTileM);
+        const int nb = (int)((Np + kIdxNT - 1) / kIdxNT);
         if (nb > 1) {
             count_labels_kernel<<<nb, kIdxNT, 0, st>>>(N, labels, o.ignore, s.counts);
             count_launches(1);
         }
-        index_kernel<<<nb, kIdxNT, 0, st>>>(N, p.Np, V, labels, o.ignore, s.counts, nb, s.total,
+        index_kernel<<<nb, kIdxNT, 0, st>>>(N, Np, V, labels, o.ignore, s.counts, nb, s.total,
                                             s.idx, s.lab);
         count_launches(1);
         GSV_CE_TRY(cudaGetLastError());
     }
     if (path == kFew) {
-        const FewArgs a{(int)N, V, D, features, weight, labels, o, s.lse, s.count,
-                        forward_only ? nullptr : zmax};
+        const FewArgs a{(int)N, V, D, features, weight, labels, o, s.lse, s.count, zmax};
         return launch_few_forward(a, type, loss, ws, st);
     }
     // merged by packed rows, which leaves out those without a label
-    if (o.reduction == kCeNone && !(direct && forward_only))
+    if (o.reduction == kCeNone && indexed)
         GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
-    if (!direct) GSV_CE_TRY(pack_any(p, true, features, s, x_of(p, s, ws), st));
+    if (!p.direct) GSV_CE_TRY(pack_any(p, true, features, s, x_of(p, s, ws), st));
     if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, w_of(p, s, ws), st));
     CeGemm g = gemm_of(p, s, weight, ws, o);
     g.product = kCeScores;
@@ -930,7 +943,7 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     g.part = reinterpret_cast<float2 *>(ws + p.part);
     g.psum = o.eps > 0.f ? reinterpret_cast<float *>(ws + p.psum) : nullptr;
     g.zt = reinterpret_cast<float *>(ws + p.zt);
-    if (direct) {
+    if (p.direct) {
         g.X = {features, N, D, D, 0};
         g.rows = N;
         g.count = g.lab = g.idx = nullptr;
@@ -939,11 +952,9 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     GSV_CE_TRY(launch_ce_gemm(g, st));
     const int per = merge_rows(2 * p.runs), mb = (int)((N + per - 1) / per);
     float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
-    const bool indexed = !forward_only || !direct;
-    launch_merge<false>(g.rows, N, 2 * p.runs, V, !direct, g.part, g.psum, g.zt,
-                        indexed ? s.total : nullptr, indexed ? s.idx : nullptr,
-                        indexed ? s.lab : nullptr, labels, o, loss, s.lse, s.count, sums,
-                        indexed ? s.total + 1 : nullptr, forward_only ? nullptr : zmax, st);
+    launch_merge<false>(g.rows, N, 2 * p.runs, V, !p.direct, g.part, g.psum, g.zt,
+                        s.total, s.idx, s.lab, labels, o, loss, s.lse, s.count, sums,
+                        indexed ? s.total + 1 : nullptr, zmax, st);
     GSV_CE_TRY(cudaGetLastError());
     if (mb > 1 && !indexed)
         GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));
@@ -956,9 +967,10 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
                                       const float *grad_loss, void *grad_features,
                                       void *grad_weight, void *workspace, cudaStream_t st) {
     if (!grad_features && !grad_weight) return cudaSuccess;
-    const State s = state_of(state, N);
+    const Path path = path_of(N, V, D, type);
+    const State s = state_of(state, N, path == kTiles || path == kFew);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
-    if (path_of(N, V, D, type) == kNarrow) {
+    if (path == kNarrow) {
         const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
 #define GSV_CE_T(T) narrow_backward<T>(a, grad_loss, grad_features, grad_weight, ws, st)
         switch (type) {
@@ -968,11 +980,12 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
         }
 #undef GSV_CE_T
     }
-    if (path_of(N, V, D, type) == kWide)
+    if (path == kWide)
         return wide_backward({N, V, D, features, weight, labels, o, s.lse, s.count},
                              reinterpret_cast<const float *>(s.packed), grad_loss, grad_features,
                              grad_weight, ws, st);
-    const Plan p = make_plan(N, V, D, type, weight, true, o);
+    const Plan p =
+        make_plan(N, V, D, type, kCeBackward, aligned16(features), aligned16(weight), o);
     float *gmax = type == kCeF16 ? reinterpret_cast<float *>(ws + p.gmax) : nullptr;
     const bool none = o.reduction == kCeNone;
     if (!x_is_kept(p)) GSV_CE_TRY(pack_any(p, true, features, s, x_of(p, s, ws), st));

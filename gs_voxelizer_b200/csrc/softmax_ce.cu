@@ -619,6 +619,8 @@ cudaError_t launch_ce_finish(const float2 *partials, int n, int reduction, float
     return cudaGetLastError();
 }
 
+bool softmax_ce_keeps_lse(int V) { return V > kStagedV; }
+
 size_t softmax_ce_workspace_bytes(long long rows, int V) {
     // with one pass a block, the most blocks there can be
     const long long r = V <= kStagedV ? kNT / lanes_of(V) : 1;

@@ -315,10 +315,10 @@ def _ce_args(named, labels, ignore_index, label_smoothing, softcap, z_loss,
     # (the largest float32 below 1: what rounds to 1 is refused too)
     if not 0.0 <= label_smoothing <= 1.0 - 2.0 ** -24:
         raise ValueError("label_smoothing must be in [0, 1)")
-    if not (0.0 <= softcap <= 1e30 and 0.0 <= z_loss <= 1e30):
-        raise ValueError("softcap and z_loss must be finite and >= 0")
-    if 0.0 < softcap < 1e-30:  # float32's 0 would be no cap
-        raise ValueError("softcap must be 0 (none) or at least 1e-30")
+    # (a softcap below float32's least number would be none)
+    if not ((softcap == 0.0 or 1e-30 <= softcap <= 1e30) and 0.0 <= z_loss <= 1e30):
+        raise ValueError("softcap and z_loss must be finite and >= 0, and a "
+                         "softcap at least 1e-30")
     if not -2 ** 63 <= ignore_index < 2 ** 63:
         raise ValueError("ignore_index must be a 64-bit integer")
     opt = CeOptions(int(ignore_index), label_smoothing, softcap, z_loss,
@@ -369,40 +369,36 @@ def _recorded(a, b):
 
 
 def _as_kept(saved):
-    """Saved tensors as the kernels take them: a hook may have brought them back
-    with other strides, or the last one (raw bytes) off the alignment of what it
-    holds."""
-    for t in saved:
-        if not t.is_contiguous():
-            break
-    else:
-        if not saved[-1].data_ptr() & 15:
-            return saved
+    """Saved tensors that a hook brought back with other strides, or the last
+    one (raw bytes) off the alignment of what it holds, as the kernels take
+    them."""
     *rest, raw = (t.contiguous() for t in saved)
     return (*rest, raw.clone() if raw.data_ptr() & 15 else raw)
 
 
 def _softmax_ce(scores, labels, opt):
-    """(loss, stats): per row (maximum, log2 of the sum), then the number of
-    labelled rows, then the call's workspace."""
+    """(loss, stats, where in stats the count is): per row of more than 1024
+    classes (maximum, log2 of the sum), then the number of labelled rows, then
+    the call's workspace."""
     dev, V, rows = scores.device, scores.size(-1), labels.numel()
     loss = _ce_loss_out(labels, opt, dev)
     if rows == 0:
-        return loss.zero_(), None
+        return loss.zero_(), None, 0
+    lse = lib.gsv_softmax_ce_lse_bytes(rows, V)
     nbytes = lib.gsv_softmax_ce_workspace_bytes(rows, V)
-    stats = torch.empty((8 * rows + 8 + nbytes,), dtype=torch.uint8, device=dev)
+    stats = torch.empty((lse + 8 + nbytes,), dtype=torch.uint8, device=dev)
     p = stats.data_ptr()
     _ce_call(lib.gsv_softmax_ce_forward, dev, rows, V, _CE_DTYPES[scores.dtype],
              scores.data_ptr(), labels.data_ptr(), opt, loss.data_ptr(), p,
-             p + 8 * rows, p + 8 * rows + 8, nbytes)
-    return loss, stats
+             p + lse, p + lse + 8, nbytes)
+    return loss, stats, lse
 
 
 class _SoftmaxCe(Function):
     @staticmethod
     def forward(ctx, scores, labels, opt):
         ctx.opt = opt
-        loss, stats = _softmax_ce(scores, labels, opt)
+        loss, stats, ctx.lse = _softmax_ce(scores, labels, opt)
         if stats is None:
             ctx.save_for_backward(scores)
         else:
@@ -414,14 +410,18 @@ class _SoftmaxCe(Function):
         saved = ctx.saved_tensors
         if len(saved) == 1:
             return torch.zeros_like(saved[0]), None, None
-        scores, labels, stats = _as_kept(saved)
+        scores, labels, stats = saved
+        if stats.data_ptr() & 15 or not (
+                scores.is_contiguous() and labels.is_contiguous()
+                and stats.is_contiguous()):
+            scores, labels, stats = _as_kept(saved)
         dev, rows, V = scores.device, labels.numel(), scores.size(-1)
         grad_loss = grad_loss.contiguous()  # float32, as the loss is
         g = torch.empty_like(scores)
         p = stats.data_ptr()
         _ce_call(lib.gsv_softmax_ce_backward, dev, rows, V,
                  _CE_DTYPES[scores.dtype], scores.data_ptr(), labels.data_ptr(),
-                 ctx.opt, p, p + 8 * rows, grad_loss.data_ptr(), g.data_ptr())
+                 ctx.opt, p, p + ctx.lse, grad_loss.data_ptr(), g.data_ptr())
         if torch.is_grad_enabled():
             g = _Once.apply(g, scores, grad_loss)
         return g, None, None
@@ -476,11 +476,13 @@ def _linear_ce(features, weight, labels, opt, with_state):
     if with_state:
         state = _C._workspace(
             lib.gsv_linear_ce_state_bytes(rows, V, D, dtype), dev)
+    x, w = features.data_ptr(), weight.data_ptr()
+    call = 2 * with_state | (0 if (x | w) & 15 else 4)  # gsv_ce_call
     ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
-        rows, V, D, dtype, opt, 0), dev)
-    _ce_call(lib.gsv_linear_ce_forward, dev, rows, V, D, dtype,
-             features.data_ptr(), weight.data_ptr(), labels.data_ptr(), opt,
-             loss.data_ptr(), _C._ptr(state), ws.data_ptr(), ws.numel())
+        rows, V, D, dtype, opt, call), dev)
+    _ce_call(lib.gsv_linear_ce_forward, dev, rows, V, D, dtype, x, w,
+             labels.data_ptr(), opt, loss.data_ptr(), _C._ptr(state),
+             ws.data_ptr(), ws.numel())
     return loss, state
 
 
@@ -502,19 +504,25 @@ class _LinearCe(Function):
         if len(saved) == 2:
             return (*(torch.zeros_like(t) if need else None for t, need in
                       zip(saved, (need_x, need_w))), None, None)
-        features, weight, labels, state = _as_kept(saved)
+        features, weight, labels, state = saved
+        if state.data_ptr() & 15 or not (
+                features.is_contiguous() and weight.is_contiguous()
+                and labels.is_contiguous() and state.is_contiguous()):
+            features, weight, labels, state = _as_kept(saved)
         dev = features.device
         rows, (V, D) = labels.numel(), weight.shape
         dtype = _CE_DTYPES[features.dtype]
         grad_loss = grad_loss.contiguous()  # float32, as the loss is
         gx = torch.empty_like(features) if need_x else None
         gw = torch.empty_like(weight) if need_w else None
+        x, w = features.data_ptr(), weight.data_ptr()
+        call = 1 if (x | w) & 15 else 1 | 4  # gsv_ce_call
         ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
-            rows, V, D, dtype, ctx.opt, 1), dev)
-        _ce_call(lib.gsv_linear_ce_backward, dev, rows, V, D, dtype,
-                 features.data_ptr(), weight.data_ptr(), labels.data_ptr(),
-                 ctx.opt, state.data_ptr(), grad_loss.data_ptr(), _C._ptr(gx),
-                 _C._ptr(gw), ws.data_ptr(), ws.numel())
+            rows, V, D, dtype, ctx.opt, call), dev)
+        _ce_call(lib.gsv_linear_ce_backward, dev, rows, V, D, dtype, x, w,
+                 labels.data_ptr(), ctx.opt, state.data_ptr(),
+                 grad_loss.data_ptr(), _C._ptr(gx), _C._ptr(gw), ws.data_ptr(),
+                 ws.numel())
         if torch.is_grad_enabled():
             gx, gw = (g if g is None else _Once.apply(g, features, weight, grad_loss)
                       for g in (gx, gw))

@@ -522,16 +522,25 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
  * 2^20.
  *
  * The forward leaves what the backward needs in `lse` / `count` (device
- * float32 [rows][2], 8-byte aligned, and [1]) or in `state` (gsv_linear_ce_state_bytes, 16-byte
- * aligned); the backward is called with the same sizes, contents and options
+ * gsv_softmax_ce_lse_bytes, 8-byte aligned, or null where those are 0; and
+ * float32 [1]) or in `state` (gsv_linear_ce_state_bytes, 16-byte aligned); the
+ * backward is called with the same sizes, contents and options
  * (the inputs may lie elsewhere by then).
  * A null state: no backward follows.
+ * gsv_linear_ce_workspace_bytes takes what the workspace is for, as bits
+ * (gsv_ce_call); without GSV_CE_STATE or GSV_CE_ALIGNED it is enough for either.
  * Workspaces are scratch of one call, 256-byte aligned (gsv_softmax_ce_forward:
  * 8-byte). Everything else is aligned to its elements; a pointer that is not is
  * refused. A null gradient output of gsv_linear_ce_backward is not computed.
  */
 enum gsv_dtype { GSV_F32 = 0, GSV_BF16 = 1, GSV_F16 = 2 };
 enum gsv_reduction { GSV_REDUCE_NONE = 0, GSV_REDUCE_SUM = 1, GSV_REDUCE_MEAN = 2 };
+
+enum gsv_ce_call {
+    GSV_CE_BACKWARD = 1, /* gsv_linear_ce_backward; else _forward            */
+    GSV_CE_STATE = 2,    /* the forward is given a state                     */
+    GSV_CE_ALIGNED = 4   /* features and weight are aligned to 16 bytes      */
+};
 
 typedef struct gsv_ce_options {
     int64_t ignore_index;
@@ -542,6 +551,7 @@ typedef struct gsv_ce_options {
 } gsv_ce_options;
 
 GSV_API size_t gsv_softmax_ce_workspace_bytes(int64_t rows, int32_t classes);
+GSV_API size_t gsv_softmax_ce_lse_bytes(int64_t rows, int32_t classes);
 GSV_API int gsv_softmax_ce_forward(int64_t rows, int32_t classes, int32_t dtype,
                                    const void *scores, const int64_t *labels,
                                    const gsv_ce_options *options, float *loss,
@@ -558,7 +568,7 @@ GSV_API size_t gsv_linear_ce_state_bytes(int64_t rows, int32_t classes,
 GSV_API size_t gsv_linear_ce_workspace_bytes(int64_t rows, int32_t classes,
                                              int32_t channels, int32_t dtype,
                                              const gsv_ce_options *options,
-                                             int32_t backward);
+                                             int32_t call);
 GSV_API int gsv_linear_ce_forward(int64_t rows, int32_t classes, int32_t channels,
                                   int32_t dtype, const void *features,
                                   const void *weight, const int64_t *labels,

@@ -278,3 +278,22 @@ def test_options_that_float32_and_int64_do_not_hold():
     for cap in (1e-30, 1e-6):
         loss, _ = call((x,), y.clamp_max(4), dict(softcap=cap))
         assert float(loss) == pytest.approx(1.6094379, abs=1e-5)  # log 5
+
+
+@pytest.mark.parametrize("V,D,most", [(4, 0, 1), (37, 0, 1), (20, 4, 9), (20, 24, 9)])
+def test_memory_between_forward_and_backward(V, D, most):
+    """Bytes a row that a forward holds for its backward, and that it takes
+    for itself."""
+    from gs_voxelizer_b200 import losses
+    fn = losses.linear_cross_entropy if D else losses.softmax_cross_entropy
+    n = 1 << 20
+    data, labels = make(n, V, D, F32, 59, garbage=False)
+    leaves = [t.requires_grad_(True) for t in data]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    loss = fn(*leaves, labels)
+    held = torch.cuda.memory_allocated() - before
+    peak = torch.cuda.max_memory_allocated() - before
+    assert held <= most * n and peak <= (most + 1) * n
+    del loss
