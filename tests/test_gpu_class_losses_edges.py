@@ -297,3 +297,97 @@ def test_memory_between_forward_and_backward(V, D, most):
     peak = torch.cuda.max_memory_allocated() - before
     assert held <= most * n and peak <= (most + 1) * n
     del loss
+
+
+@pytest.mark.parametrize("n,V,D,dtype", [
+    (300001, 20, 4, F32), (200003, 11, 24, F32), (150001, 9, 64, F32), (70001, 4097, 40, F32),
+    (9001, 20021, 40, F32), (70001, 4097, 40, F16), (9001, 20021, 264, F16)])
+def test_table_gradient_has_every_row(n, V, D, dtype):
+    """Features and (of classes that are no row's label) derivatives of one
+    sign: 256 rows left out anywhere are 256 / n of such a class's gradient.
+    The bound does not grow with n: the probability's error (two scores' and
+    the exponents', below 32, a few 2^-24 of them), 2048 additions (1024 onto
+    one sum, the joins; 512 of K in the tensor cores are 32, each of twice
+    that), and 16-bit roundings of P and of the result."""
+    from tests._class_ref import HALF_ULP, reference
+    g = torch.Generator("cuda").manual_seed(60)
+    x = (0.5 + torch.rand(n, D, generator=g, device="cuda")).to(dtype)
+    w = (torch.randn(V, D, generator=g, device="cuda") / D).to(dtype)
+    labels = torch.randint(0, V // 2, (n,), generator=g, device="cuda")
+    labels[torch.rand(n, generator=g, device="cuda") < 0.1] = -100
+    up = torch.tensor(16.0 if dtype == F16 else 1.0, device="cuda")
+    loss, grads = call((x, w), labels, dict(reduction="sum"), up)
+    ref = reference(x.double() @ w.double().t(), labels, reduction="sum", upstream=up)
+    es = (D + 8) * 2.0 ** -23 * float((x.double() @ w.double().abs().t()).max())
+    rel = 2 * es + 2.0 ** -17 + 2048 * 2.0 ** -24 + (
+        2 * HALF_ULP[dtype] if dtype == F16 else 0.0)
+    assert rel < 0.5 * 256 / n
+    want, size = ref["ds"].t() @ x.double(), ref["dabs"].t() @ x.double()
+    # half of fp16's least step, of the result and (times 2^-14) of n products
+    tiny = 2.0 ** -25 * (1 + float(up) * n * 2.0 ** -14 * 1.5) if dtype == F16 else 0.0
+    assert ((grads[1].double() - want).abs() <= rel * size + tiny).all()
+    want, size = ref["ds"] @ w.double(), ref["dabs"] @ w.double().abs()
+    tiny = 2.0 ** -25 * (1 + float(up) * 2.0 ** -14 * float(w.abs().double().sum(0).max())) \
+        if dtype == F16 else 0.0
+    assert ((grads[0].double() - want).abs() <= rel * size + tiny).all()
+    assert float(loss) == pytest.approx(float(ref["loss"]), rel=2.0 ** -17)
+
+
+def test_float32_products_keep_their_bits():
+    """Operands whose three bf16 parts are 1, 2^-9 and 2^-17, all of one sign:
+    a product without one of its small parts is off by 2^-18 at least, the
+    same way in every term. The bounds count the roundings that there are: the
+    tensor cores truncate each addition of 16 terms (2^-23 of the sum) in both
+    accumulators, and a few float32 operations join them."""
+    v = 1.0 + 2.0 ** -9 + 2.0 ** -17
+    n, V, D = 160, 20, 48
+    x = torch.full((n, D), v, device="cuda")
+    w = torch.zeros(V, D, device="cuda")
+    w[0] = v
+    labels = torch.ones(n, dtype=torch.int64, device="cuda")
+    up = torch.full((n,), v, device="cuda")
+    loss, (dx, dw) = call((x, w), labels, dict(reduction="none"), up)
+    parts = (1.0, 2.0 ** -9, 2.0 ** -17)
+    lost = min(parts[i] * parts[j] for i, j in ((0, 2), (2, 0), (1, 1))) / (v * v)
+    # the label scores 0 and class 0 has all the probability, so the loss is
+    # class 0's score; P of class 0 is the upstream gradient, P of the label
+    # minus it, on a table row of zeros
+    for got, want, steps in ((loss, D * v * v, D // 16), (dx, v * v, 2),
+                             (dw[0], n * v * v, n // 16)):
+        tol = (2 * steps + 8) * 2.0 ** -24
+        assert tol < lost / 2
+        assert float((got.double() / want - 1.0).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("n,V,D,dtype", [
+    (70001, 32771, 0, BF16), ((1 << 22) + 5, 517, 0, BF16), ((1 << 29) + 7, 4, 0, BF16),
+    ((1 << 28) + 3, 5, 9, BF16), ((1 << 25) + 3, 20, 72, BF16), ((1 << 25) + 3, 7, 72, F32)])
+def test_more_than_2_to_31_elements(n, V, D, dtype):
+    """The first and the last rows of inputs beyond 32-bit offsets."""
+    from gs_voxelizer_b200 import losses
+    from tests._class_ref import HALF_ULP, grad_error, loss_error, reference, score_error
+    from tests.test_gpu_class_losses import within
+    g = torch.Generator("cuda").manual_seed(61)
+    first = torch.empty(n, D or V, dtype=dtype, device="cuda").normal_(generator=g)
+    assert first.numel() > 2 ** 31
+    labels = torch.randint(0, V, (n,), generator=g, device="cuda")
+    labels[5::7] = -100
+    leaves = [first.requires_grad_(True)]
+    if D:
+        leaves.append(torch.randn(V, D, generator=g, device="cuda").to(dtype))
+    fn = losses.linear_cross_entropy if D else losses.softmax_cross_entropy
+    loss = fn(*leaves, labels, reduction="none")
+    (grad,) = torch.autograd.grad(loss, first, torch.ones_like(loss))
+    u = HALF_ULP[dtype]
+    for part in (slice(0, 300), slice(n - 300, n)):
+        x, y = first.detach()[part].double(), labels[part]
+        w = leaves[1].double() if D else None
+        s = x @ w.t() if D else x
+        es = score_error(float((x.abs() @ w.abs().t()).max()), D, 0.0) if D else 0.0
+        ref = reference(s, y, reduction="none", upstream=torch.ones(300, device="cuda"))
+        within(loss.detach()[part], ref["loss"], loss_error(ref, es, 0.0), "loss")
+        want, size = ref["ds"], ref["dabs"]
+        if D:
+            want, size = want @ w, size @ w.abs()
+        rel = grad_error(ref, es) + (u if D and dtype != F32 else 0.0) + 2.0 ** -18
+        within(grad[part], want, u * want.abs() + rel * size + 2.0 ** -100, "gradient")
