@@ -42,6 +42,41 @@ count_labels_kernel(long long n, const long long *__restrict__ labels, long long
     if (threadIdx.x == 0) counts[blockIdx.x] = c;
 }
 
+// Blocks' counts up to which each block of index_kernel adds up all of them; of
+// more it would read the square of their number (391 us for 256^3 rows, 203 with
+// a launch that adds them up first).
+constexpr int kScan = 64;
+
+// counts -> labelled rows before each block, and total[0] = all of them
+__global__ void __launch_bounds__(kIdxNT)
+scan_counts_kernel(int nblocks, int *__restrict__ counts, int *__restrict__ total) {
+    __shared__ int s_warp[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (nblocks + kIdxNT - 1) / kIdxNT;
+    const int b0 = min(nblocks, (int)threadIdx.x * per), b1 = min(nblocks, b0 + per);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += counts[b];
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) s_warp[warp] = upto;
+    __syncthreads();
+    int before = upto - mine, all = 0;
+    for (int w = 0; w < 32; ++w) {
+        if (w < warp) before += s_warp[w];
+        all += s_warp[w];
+    }
+    for (int b = b0; b < b1; ++b) {
+        const int c = counts[b];
+        counts[b] = before;
+        before += c;
+    }
+    if (threadIdx.x == 0) total[0] = all;
+}
+
 // idx / lab of the packed rows in their order; positions from the number of
 // labelled rows up to padded are kCeIgnored. total[0] = labelled rows.
 __global__ void __launch_bounds__(kIdxNT)
@@ -55,7 +90,7 @@ index_kernel(long long n, long long padded, int V, const long long *__restrict__
     const long long y = i < n ? labels[i] : ignore;
     const bool keep = i < n && y != ignore;
     long long before = 0, all = 0;
-    if (nblocks > 1) {
+    if (nblocks > 1 && nblocks <= kScan) {
         for (int b = threadIdx.x; b < nblocks; b += kIdxNT) {
             const int c = counts[b];
             all += c;
@@ -75,7 +110,10 @@ index_kernel(long long n, long long padded, int V, const long long *__restrict__
     if (lane == 0) s_warp[warp] = __popc(ballot);
     __syncthreads();
     before = all = 0;
-    if (nblocks > 1) {
+    if (nblocks > kScan) {
+        before = counts[blockIdx.x];
+        all = total[0];
+    } else if (nblocks > 1) {
         for (int w = 0; w < 32; ++w) {
             before += s_before[w];
             all += s_all[w];
@@ -94,7 +132,7 @@ index_kernel(long long n, long long padded, int V, const long long *__restrict__
     }
     if (i >= all && i < padded) lab[i] = kCeIgnored;
     if (i == 0) {
-        total[0] = (int)all;
+        if (nblocks <= kScan) total[0] = (int)all;
         total[1] = 0;  // the merge's ticket
         total[2] = 0;  // the z-loss's largest factor
     }
@@ -919,6 +957,10 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         const int nb = (int)((Np + kIdxNT - 1) / kIdxNT);
         if (nb > 1) {
             count_labels_kernel<<<nb, kIdxNT, 0, st>>>(N, labels, o.ignore, s.counts);
+            count_launches(1);
+        }
+        if (nb > kScan) {
+            scan_counts_kernel<<<1, kIdxNT, 0, st>>>(nb, s.counts, s.total);
             count_launches(1);
         }
         index_kernel<<<nb, kIdxNT, 0, st>>>(N, Np, V, labels, o.ignore, s.counts, nb, s.total,

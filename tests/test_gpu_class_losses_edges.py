@@ -391,3 +391,14 @@ def test_more_than_2_to_31_elements(n, V, D, dtype):
             want, size = want @ w, size @ w.abs()
         rel = grad_error(ref, es) + (u if D and dtype != F32 else 0.0) + 2.0 ** -18
         within(grad[part], want, u * want.abs() + rel * size + 2.0 ** -100, "gradient")
+
+
+@pytest.mark.parametrize("n", [1023, 1025, 65535, 65537, 66561, (1 << 20) + 300])
+@pytest.mark.parametrize("ignored", [0.0, 0.4, 0.9999])
+def test_labelled_rows_of_many_blocks(n, ignored):
+    data, labels = make(n, 20, 40, BF16, 62, ignored=ignored)
+    up = torch.ones(n, device="cuda")
+    for opt in (dict(reduction="none"), dict(reduction="mean")):
+        g = up if opt["reduction"] == "none" else up[0]
+        loss, grads = call(data, labels, opt, g)
+        check(data, labels, opt, g, loss, grads)
