@@ -92,13 +92,6 @@ __device__ __forceinline__ void store_row(T *p, long long r, int D, const float 
     }
 }
 
-template <int DP>
-__device__ __forceinline__ float dot(const Row<DP> &a, const Row<DP> &b) {
-    float s = 0.f;
-#pragma unroll
-    for (int d = 0; d < DP; ++d) s = fmaf(a.v[d], b.v[d], s);
-    return s;
-}
 struct Span {
     int v0, v1;
 };

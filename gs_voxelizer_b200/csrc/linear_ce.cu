@@ -12,7 +12,8 @@
 //
 // Rounding P to 16 bits costs at most half a step (2^-8 of the value in bf16,
 // 2^-11 in fp16), no more than rounding the gradients themselves to the same
-// type. fp16 keeps P times 2^14, over the largest factor that a z-loss brings to
+// type (against float64: 2.4e-3 of bf16 gradients where the products of an
+// unrounded P give 1.7e-3, 2.4e-4 of fp16 ones for 2.1e-4). fp16 keeps P times 2^14, over the largest factor that a z-loss brings to
 // a row, so that small probabilities stay normal numbers and none overflows. float32 inputs keep three bf16 planes of
 // every operand, which hold all 24 bits.
 //
@@ -572,11 +573,18 @@ int splits_for(long long tiles, long long depth, bool f32, long long elements) {
 
 // Which kernels serve a call. kNarrow (linear_ce_narrow.cu, the CUDA cores
 // without tiles): where it is the faster. Kernels' time of a training step,
-// narrow against tiles: 53000 rows x 203 classes, D = 16, 99 against 180 us of
-// float32, 90 against 98 of bf16; D = 32, 156 against 170 and 145 against 80;
-// 10^6 rows x 20 classes, D = 16, 148 against 1311 and 134 against 530, D = 32,
-// 356 and 299 against 530 of bf16; 1000 rows x 50000 classes, D = 16, 267
-// against 472 and 250 against 160, D = 32, 584 against 480 of float32.
+// narrow against tiles (us):
+//   rows x classes     D = 8 float32   bf16          D = 4 bf16
+//   1000 x 50000       165 : 419       161 : 168     110 : 186
+//   16384 x 20000      862 : 2467      839 : 778     500 : 789
+//   100000 x 2000      579 : 1464      562 : 553     339 : 554
+//   10^6 x 300                         842 : 1265    477 : 1187
+//   10^6 x 20                           89 : 514
+//                      D = 16 float32  bf16          D = 32 float32  bf16
+//   53000 x 203        99 : 180        90 : 98       156 : 170       145 : 80
+//   10^6 x 20          148 : 1311      134 : 530                     299 : 530
+//   1000 x 50000       267 : 472       250 : 160     584 : 480
+// (At D = 8 in 16 bits and thousands of classes the two are level.)
 // kWide: few classes, many float32 channels (linear_ce_wide.cu). kFew
 // (linear_ce_few.cu): the forward alone; its backward takes tiles.
 enum Path { kNarrow, kWide, kFew, kTiles };

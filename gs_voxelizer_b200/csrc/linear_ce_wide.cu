@@ -13,8 +13,10 @@
 // derivatives P from them, then dX with a lane's four columns of the table in
 // registers and whole rows written, and dW with V x 4 sums a lane. V
 // multiply-adds a channel against the 11 floats a clock and SM that HBM
-// delivers; it reaches 2.4 to 3 TB/s a pass, the loads in flight limit it. 603768 x
-// 9 x 440: 1242 us of kernels (scores formed again and dX written by their
+// delivers; it reaches 2.4 to 3 TB/s a pass, bound by the loads in flight that
+// this choice of stages leaves: 74 KB of them a block in the forward, 10 to 25 %
+// of the warps resident. (More and smaller stages were not tried.) 603768 x
+// 9 x 440: 1237 us of kernels (scores formed again and dX written by their
 // threads: 1518; a warp a row with sums by shuffles: 2437); 147949 x 6 x 1578:
 // 1063 (1906).
 #include <atomic>

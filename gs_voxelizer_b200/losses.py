@@ -450,10 +450,13 @@ def softmax_cross_entropy(
             a zero gradient whatever they hold; any other label outside
             [0, V) makes the row's loss and gradient NaN.
         ignore_index, label_smoothing, softcap, z_loss: see above.
-        reduction: "mean" over the labelled rows (0 if there is none), "sum"
-            or "none" (the losses in the shape of labels).
+        reduction: "mean" over the labelled rows of this call (0 if there is
+            none), "sum" or "none" (the losses in the shape of labels). Ranks
+            that each hold a slab of a volume take "sum" over the all-reduced
+            number of labelled voxels: a slab's mean is over its own.
     Returns:
-        float32 loss, differentiable once in scores (gradient in their type).
+        float32 loss, differentiable once in scores, in reverse mode (gradient
+        in their type).
     """
     labels, opt = _ce_args([("scores", scores)], labels, ignore_index,
                            label_smoothing, softcap, z_loss, reduction)
@@ -544,14 +547,18 @@ def linear_cross_entropy(
     embeddings, or the hidden states of a model against a vocabulary.
 
     The scores are products of the inputs summed in float32 and are not
-    rounded to the inputs' type. The forward keeps 16 bytes a row and, up to
-    16 MB each, its packed operands; the backward computes the scores again in
-    pieces, with a workspace of a few hundred MB beside packed copies of the
-    operands and float32 copies of what it accumulates over several pieces.
-    (Scores of at most 16 classes over more than 32 float32 channels, less than
-    half of the features' size, are kept instead, from 16384 rows on.) With
-    ``reduction="none"`` and no gradient it is minus the
-    log-probability of each row's label.
+    rounded to the inputs' type. The forward keeps 8 or 16 bytes a row and, up
+    to 16 MB each, its packed operands; the backward computes the scores again
+    in pieces, with a workspace of a few hundred MB beside packed copies of the
+    features (and of a table that cannot be read in place) and float32 copies
+    of what it accumulates over several pieces. (Scores of at most 16 classes
+    over more than 32 float32 channels, less than half of the features' size,
+    are kept instead, from 16384 rows on.) The derivatives in the scores are
+    rounded to a 16-bit type before its gradients are formed of them; in
+    float16 with ``reduction="none"`` relative to the largest row's upstream
+    gradient, below 2^-10 of which a row loses digits. With
+    ``reduction="none"`` and no gradient it is minus the log-probability of
+    each row's label.
 
     Args:
         features: [..., D] float32, bfloat16 or float16.
@@ -559,8 +566,8 @@ def linear_cross_entropy(
         labels, ignore_index, label_smoothing, softcap, z_loss, reduction: as
             for ``softmax_cross_entropy``.
     Returns:
-        float32 loss, differentiable once in features and weight (gradients
-        in their type).
+        float32 loss, differentiable once in features and weight, in reverse
+        mode (gradients in their type).
     """
     labels, opt = _ce_args([("features", features), ("weight", weight)], labels,
                            ignore_index, label_smoothing, softcap, z_loss,

@@ -517,8 +517,12 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
  * channels] are contiguous and of one type (gsv_dtype), labels int64 [rows],
  * loss float32 ([1], or [rows] with GSV_REDUCE_NONE), grad_loss float32 of
  * the same size. Arithmetic is float32 or wider; the products of 16-bit
- * types are exact and summed in float32, those of float32 are taken with all
- * their bits. 1 <= rows < 2^31 - 1024, 1 <= classes <= 2^24, 1 <= channels <=
+ * types are exact and summed in float32, and so are those of float32 but for
+ * what is below 2^-26 of each (six of nine products of 8-bit parts). The
+ * derivatives in the scores are rounded to the inputs' type before 16-bit
+ * gradients are formed of them; in float16 with GSV_REDUCE_NONE relative to the
+ * largest row's upstream gradient, below 2^-10 of which a row loses digits.
+ * 1 <= rows < 2^31 - 1024, 1 <= classes <= 2^24, 1 <= channels <=
  * 2^20.
  *
  * The forward leaves what the backward needs in `lse` / `count` (device
