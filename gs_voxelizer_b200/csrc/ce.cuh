@@ -153,6 +153,19 @@ template <> __device__ __forceinline__ __half ce_from_float(float v) {
     return __float2half_rn(v);
 }
 
+// A thread's sum of the losses of its rows, thousands in a large volume, and
+// what each addition has lost (exact while the sum is the larger one, as a sum
+// of losses is).
+struct CeSum {
+    float s = 0.f, lost = 0.f;
+    __device__ __forceinline__ void add(float v) {
+        const float t = s + v;
+        lost += v - (t - s);
+        s = t;
+    }
+    __device__ __forceinline__ float value() const { return isfinite(s) ? s + lost : s; }
+};
+
 // Sums (loss, labelled rows) over a block of NT threads; valid in thread 0.
 template <int NT>
 __device__ __forceinline__ float2 ce_block_sum(float loss, float cnt, float2 *sh) {

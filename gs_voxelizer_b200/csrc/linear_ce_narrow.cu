@@ -140,7 +140,8 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
         if (threadIdx.x == 0) s_wsum = wsum;
         __syncthreads();
     }
-    float lsum = 0.f, cnt = 0.f;
+    CeSum lsum;
+    float cnt = 0.f;
     bool staged = false;
     const long long stride = (long long)gridDim.x * kNT * R;
     long long t0 = (long long)blockIdx.x * kNT * R;
@@ -232,7 +233,7 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
                 l = lse.x = ce_nan();
             lse_out[r] = lse;
             if (o.reduction == kCeNone) loss[r] = l;
-            lsum += l;
+            lsum.add(l);
             cnt += y[k] == kCeIgnored ? 0.f : 1.f;
         }
         if (DP > 4)
@@ -240,7 +241,7 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
                                              o.ignore, nullptr);
     }
     if (gridDim.y > 1) return;
-    const float2 t = ce_block_sum<kNT>(lsum, cnt, sh);
+    const float2 t = ce_block_sum<kNT>(lsum.value(), cnt, sh);
     if (threadIdx.x == 0) {
         if (gridDim.x == 1)
             ce_finish(t.x, t.y, o.reduction, loss, count);

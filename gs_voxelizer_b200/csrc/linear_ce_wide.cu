@@ -173,7 +173,8 @@ wide_fwd_kernel(long long N, int V, int D, const float *__restrict__ features,
     extern __shared__ __align__(16) unsigned char wide_smem[];
     __shared__ float2 sh[kNT / 32];
     Stage<VP> *st = reinterpret_cast<Stage<VP> *>(wide_smem);
-    float lsum = 0.f, cnt = 0.f;
+    CeSum lsum;
+    float cnt = 0.f;
     for (long long r0 = (long long)blockIdx.x * kRows; r0 < N;
          r0 += (long long)gridDim.x * kRows) {
         float z[kR][VP];
@@ -213,11 +214,11 @@ wide_fwd_kernel(long long N, int V, int D, const float *__restrict__ features,
                         to[j / 4] = make_float4(z[k][j], z[k][j + 1], z[k][j + 2], z[k][j + 3]);
             }
             if (o.reduction == kCeNone) loss[r] = l;
-            lsum += l;
+            lsum.add(l);
             cnt += y == kCeIgnored ? 0.f : 1.f;
         }
     }
-    const float2 s = ce_block_sum<kNT>(lsum, cnt, sh);
+    const float2 s = ce_block_sum<kNT>(lsum.value(), cnt, sh);
     if (threadIdx.x == 0) {
         if (gridDim.x == 1)
             ce_finish(s.x, s.y, o.reduction, loss, count);

@@ -402,3 +402,28 @@ def test_labelled_rows_of_many_blocks(n, ignored):
         g = up if opt["reduction"] == "none" else up[0]
         loss, grads = call(data, labels, opt, g)
         check(data, labels, opt, g, loss, grads)
+
+
+@pytest.mark.parametrize("n,V,D", [(1 << 27, 2, 1), (1 << 26, 5, 4), (1 << 25, 3, 12),
+                                   (1 << 25, 7, 33), (1 << 25, 7, 0), (1 << 22, 20, 40)])
+def test_loss_of_many_equal_rows(n, V, D):
+    """A sum of equal losses is off by a row's own error (below 2^-21 of a loss
+    near 1: exponents below 8 and a sum's rounding), a block's 8 joins of 2^-24
+    each and the last rounding, however many rows there are."""
+    from gs_voxelizer_b200 import losses
+    g = torch.Generator("cuda").manual_seed(63)
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")
+    row = torch.rand(1, D or V, generator=g, device="cuda")
+    if D:
+        w = torch.rand(V, D, generator=g, device="cuda") / D
+        one = losses.linear_cross_entropy(row, w, labels[:1])
+        s = row.double() @ w.double().t()
+        loss = losses.linear_cross_entropy(row.expand(n, D), w, labels, reduction="sum")
+    else:
+        one = losses.softmax_cross_entropy(row, labels[:1])
+        s = row.double()
+        loss = losses.softmax_cross_entropy(row.expand(n, V), labels, reduction="sum")
+    want = torch.logsumexp(s, 1)[0] - s[0, 0]
+    assert 0.25 < float(want) < 4
+    assert abs(float(one) / float(want) - 1) < 2.0 ** -19
+    assert abs(float(loss) / (n * float(want)) - 1) < 2.0 ** -19
