@@ -1,6 +1,7 @@
 // extern "C" entry points declared in include/gsvox.h: argument checks,
 // workspace layout and dispatch to the kernels. No device allocation happens
 // here; errors are returned as status codes with a per-thread message.
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
@@ -1186,11 +1187,14 @@ size_t gsv_linear_ce_workspace_bytes(int64_t rows, int32_t classes, int32_t chan
     if (check_ce("gsv_linear_ce_workspace_bytes", rows, classes, channels, dtype, options))
         return 0;
     const bool on_16 = (call & GSV_CE_ALIGNED) != 0;
-    return gsv::linear_ce_workspace_bytes(rows, classes, channels, dtype,
-                                          (call & GSV_CE_BACKWARD) ? gsv::kCeBackward
-                                          : (call & GSV_CE_STATE)  ? gsv::kCeForward
-                                                                   : gsv::kCeForwardOnly,
-                                          on_16, on_16, ce_opt(options));
+    auto bytes = [&](gsv::CeCall c) {
+        return gsv::linear_ce_workspace_bytes(rows, classes, channels, dtype, c, on_16, on_16,
+                                              ce_opt(options));
+    };
+    if (call & GSV_CE_BACKWARD) return bytes(gsv::kCeBackward);
+    if (call & GSV_CE_STATE) return bytes(gsv::kCeForward);
+    if (call & GSV_CE_NO_STATE) return bytes(gsv::kCeForwardOnly);
+    return std::max(bytes(gsv::kCeForward), bytes(gsv::kCeForwardOnly));
 }
 
 int gsv_linear_ce_forward(int64_t rows, int32_t classes, int32_t channels, int32_t dtype,

@@ -1,4 +1,4 @@
-// Linear class loss of a few rows (linear_ce_few.cu).
+// Linear class loss of a few rows, without a gradient (linear_ce_few.cu).
 #pragma once
 
 #include "ce.cuh"
@@ -12,9 +12,7 @@ struct FewArgs {
     const void *features, *weight;
     const long long *labels;
     CeOpt opt;
-    float2 *lse;
     float *count;
-    float *zmax;  // largest factor of the z-loss, or null
 };
 
 size_t few_workspace_bytes(int N, int V);

@@ -589,16 +589,20 @@ int splits_for(long long tiles, long long depth, bool f32, long long elements) {
 //   1000 x 50000       267 : 472       250 : 160     584 : 480
 // (At D = 8 in 16 bits and thousands of classes the two are level.)
 // kWide: few classes, many float32 channels (linear_ce_wide.cu). kFew
-// (linear_ce_few.cu): the forward alone; its backward takes tiles.
+// (linear_ce_few.cu): a forward without a backward to follow. Where one follows,
+// both directions take tiles: 1 - p of a confident row keeps its digits only if
+// its logsumexp comes from the very scores that the backward forms (0.2 % off
+// where p = 1 - 1e-5; with sums in another order, the whole of it).
 enum Path { kNarrow, kWide, kFew, kTiles };
-Path path_of(long long N, int V, int D, int type) {
+Path path_of(long long N, int V, int D, int type, CeCall call) {
     const int most = D <= 8 ? INT_MAX
                      : D <= 16 ? (type == kCeF32 ? INT_MAX : 128)
                      : D <= kNarrowD ? (type == kCeF32 ? 256 : 64)
                                      : 0;
     if (V <= most) return kNarrow;
     if (type == kCeF32 && V <= kWideV && N >= kWideRows) return kWide;
-    return N <= (type == kCeF32 ? kFewRows : kFewRows / 2) ? kFew : kTiles;
+    const int few = type == kCeF32 ? kFewRows : kFewRows / 2;
+    return call == kCeForwardOnly && N <= few ? kFew : kTiles;
 }
 
 // Rows that the forward's tiles read in place, 16 bits and aligned for TMA:
@@ -897,20 +901,14 @@ cudaError_t wide_backward(const NarrowArgs &a, const float *z, const float *grad
 // What a forward with a state has packed and kept whatever its pointers were:
 // the backward's may be others (of the same contents), and what the forward
 // packed only for its pointers' alignment is packed again.
-bool x_is_kept(const Plan &p) {
-    return path_of(p.N, p.V, p.D, p.type) == kTiles && p.keep_x &&
-           !in_place(p.N, p.V, p.D, p.type);
-}
-bool w_is_kept(const Plan &p) {
-    return path_of(p.N, p.V, p.D, p.type) == kTiles && p.keep_w &&
-           (p.planes == 3 || p.D % 8 != 0);
-}
+bool x_is_kept(const Plan &p) { return p.keep_x && !in_place(p.N, p.V, p.D, p.type); }
+bool w_is_kept(const Plan &p) { return p.keep_w && (p.planes == 3 || p.D % 8 != 0); }
 
 }  // namespace
 
 size_t linear_ce_state_bytes(long long N, int V, int D, int type) {
-    const Path path = path_of(N, V, D, type);
-    size_t b = 4 * (size_t)state_words(N, path == kTiles || path == kFew);
+    const Path path = path_of(N, V, D, type, kCeForward);
+    size_t b = 4 * (size_t)state_words(N, path == kTiles);
     if (path == kNarrow) return b;
     if (path == kWide) return b + wide_p_bytes(N, V);
     const size_t xb = packed_bytes(up(N, kCeTileM), D, type), wb = packed_bytes(V, D, type);
@@ -922,15 +920,14 @@ size_t linear_ce_state_bytes(long long N, int V, int D, int type) {
 size_t linear_ce_workspace_bytes(long long N, int V, int D, int type, CeCall call, bool aligned_x,
                                  bool aligned_w, const CeOpt &o) {
     const bool backward = call == kCeBackward;
-    const Path path = path_of(N, V, D, type);
-    const bool tiles = path == kTiles || (backward && path == kFew);
+    const Path path = path_of(N, V, D, type, call);
     Plan p{};
-    if (tiles) p = make_plan(N, V, D, type, call, aligned_x, aligned_w, o);
+    if (path == kTiles) p = make_plan(N, V, D, type, call, aligned_x, aligned_w, o);
     // a forward without a state keeps its statistics (and, of tiles, the
     // labelled rows' list) here
     const size_t own =
         call == kCeForwardOnly ? align256(4 * (size_t)state_words(N, p.indexed)) : 0;
-    if (tiles) return own + p.bytes;
+    if (path == kTiles) return own + p.bytes;
     return own + (path == kNarrow ? narrow_plan(N, V, D, backward, o).bytes
                   : path == kWide ? wide_plan(N, V, D, backward).bytes
                                   : few_workspace_bytes((int)N, V));
@@ -941,15 +938,14 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
                                      const long long *labels, const CeOpt &o, float *loss,
                                      void *state, void *workspace, cudaStream_t st) {
     const bool forward_only = state == nullptr;
-    const Path path = path_of(N, V, D, type);
+    const CeCall call = forward_only ? kCeForwardOnly : kCeForward;
+    const Path path = path_of(N, V, D, type, call);
     Plan p{};
     if (path == kTiles)
-        p = make_plan(N, V, D, type, forward_only ? kCeForwardOnly : kCeForward,
-                      aligned16(features), aligned16(weight), o);
-    const bool indexed = path == kTiles ? p.indexed : path == kFew && !forward_only;
+        p = make_plan(N, V, D, type, call, aligned16(features), aligned16(weight), o);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
-    const State s = state_of(forward_only ? ws : state, N, indexed);
-    if (forward_only) ws += align256(4 * (size_t)state_words(N, indexed));
+    const State s = state_of(forward_only ? ws : state, N, p.indexed);
+    if (forward_only) ws += align256(4 * (size_t)state_words(N, p.indexed));
     if (path == kNarrow) {
         const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};
         switch (type) {
@@ -962,10 +958,12 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
         return wide_forward({N, V, D, features, weight, labels, o, s.lse, s.count},
                             forward_only ? nullptr : reinterpret_cast<float *>(s.packed), loss,
                             ws, st);
+    if (path == kFew)
+        return launch_few_forward({(int)N, V, D, features, weight, labels, o, s.count},
+                                  type, loss, ws, st);
     float *zmax = forward_only ? nullptr : zmax_of(type, o, s);
-    if (indexed) {
-        const long long Np = up(N, kCeTileM);
-        const int nb = (int)((Np + kIdxNT - 1) / kIdxNT);
+    if (p.indexed) {
+        const int nb = (int)((p.Np + kIdxNT - 1) / kIdxNT);
         if (nb > 1) {
             count_labels_kernel<<<nb, kIdxNT, 0, st>>>(N, labels, o.ignore, s.counts);
             count_launches(1);
@@ -974,17 +972,13 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
             scan_counts_kernel<<<1, kIdxNT, 0, st>>>(nb, s.counts, s.total);
             count_launches(1);
         }
-        index_kernel<<<nb, kIdxNT, 0, st>>>(N, Np, V, labels, o.ignore, s.counts, nb, s.total,
+        index_kernel<<<nb, kIdxNT, 0, st>>>(N, p.Np, V, labels, o.ignore, s.counts, nb, s.total,
                                             s.idx, s.lab);
         count_launches(1);
         GSV_CE_TRY(cudaGetLastError());
     }
-    if (path == kFew) {
-        const FewArgs a{(int)N, V, D, features, weight, labels, o, s.lse, s.count, zmax};
-        return launch_few_forward(a, type, loss, ws, st);
-    }
     // merged by packed rows, which leaves out those without a label
-    if (o.reduction == kCeNone && indexed)
+    if (o.reduction == kCeNone && p.indexed)
         GSV_CE_TRY(cudaMemsetAsync(loss, 0, sizeof(float) * (size_t)N, st));
     if (!p.direct) GSV_CE_TRY(pack_any(p, true, features, s, x_of(p, s, ws), st));
     if (p.pack_w) GSV_CE_TRY(pack_any(p, false, weight, s, w_of(p, s, ws), st));
@@ -1007,9 +1001,9 @@ cudaError_t launch_linear_ce_forward(long long N, int V, int D, int type,
     float2 *sums = reinterpret_cast<float2 *>(ws + p.sums);
     launch_merge<false>(g.rows, N, 2 * p.runs, V, !p.direct, g.part, g.psum, g.zt,
                         s.total, s.idx, s.lab, labels, o, loss, s.lse, s.count, sums,
-                        indexed ? s.total + 1 : nullptr, zmax, st);
+                        p.indexed ? s.total + 1 : nullptr, zmax, st);
     GSV_CE_TRY(cudaGetLastError());
-    if (mb > 1 && !indexed)
+    if (mb > 1 && !p.indexed)
         GSV_CE_TRY(launch_ce_finish(sums, mb, o.reduction, loss, s.count, st));
     return cudaSuccess;
 }
@@ -1020,8 +1014,8 @@ cudaError_t launch_linear_ce_backward(long long N, int V, int D, int type,
                                       const float *grad_loss, void *grad_features,
                                       void *grad_weight, void *workspace, cudaStream_t st) {
     if (!grad_features && !grad_weight) return cudaSuccess;
-    const Path path = path_of(N, V, D, type);
-    const State s = state_of(state, N, path == kTiles || path == kFew);
+    const Path path = path_of(N, V, D, type, kCeBackward);
+    const State s = state_of(state, N, path == kTiles);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     if (path == kNarrow) {
         const NarrowArgs a{N, V, D, features, weight, labels, o, s.lse, s.count};

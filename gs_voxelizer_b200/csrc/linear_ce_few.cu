@@ -1,5 +1,5 @@
-// Linear class loss of at most four rows, forward: scoring one token, or the
-// few that are decoded together.
+// Linear class loss of at most four rows, without a gradient: scoring one token,
+// or the few that are decoded together.
 //
 // The table is read once and nothing else counts: 2 V D bytes (16 bits)
 // against V D multiply-adds a row. A tile of the tensor cores would be 256
@@ -117,13 +117,12 @@ few_fwd_kernel(int N, int V, int D, const T *__restrict__ features, const T *__r
     psum[blockIdx.x * N + r] = t.sz;
 }
 
-// All parts of all rows, 128 threads a row -> lse, loss, count.
+// All parts of all rows, 128 threads a row -> loss, count.
 __global__ void __launch_bounds__(kMergeNT *kFewRows)
 few_merge_kernel(int N, int V, int parts, const float2 *__restrict__ part,
                  const float *__restrict__ psum, const float *__restrict__ zt,
                  const long long *__restrict__ labels, CeOpt o, float *__restrict__ loss,
-                 float2 *__restrict__ lse_out, float *__restrict__ count,
-                 float *__restrict__ zmax) {
+                 float *__restrict__ count) {
     __shared__ float sh[kFewRows][kMergeNT / 32][3];
     __shared__ float s_loss[kFewRows], s_count[kFewRows];
     const int r = threadIdx.x / kMergeNT, t = threadIdx.x % kMergeNT;
@@ -146,18 +145,11 @@ few_merge_kernel(int N, int V, int parts, const float2 *__restrict__ part,
     if (t == 0) {
         for (int k = 1; k < kMergeNT / 32; ++k) a.merge(sh[r][k][0], sh[r][k][1], sh[r][k][2]);
         const int y = ce_label(labels[r], o.ignore, V);
-        float2 lse = a.lse();
         float l = 0.f;
         if (y >= 0)
-            l = ce_row_loss(lse, zt[r], a.sz, V, o);
+            l = ce_row_loss(a.lse(), zt[r], a.sz, V, o);
         else if (y == kCeInvalid)
-            l = lse.x = ce_nan();
-        // lse goes by the labelled rows alone, as the backward's rows do
-        int before = 0;
-        for (int k = 0; k < r; ++k) before += labels[k] != o.ignore;
-        if (y != kCeIgnored) lse_out[before] = lse;
-        if (zmax && y != kCeIgnored)
-            atomicMax(reinterpret_cast<int *>(zmax), __float_as_int(ce_z_factor(lse, o)));
+            l = ce_nan();
         if (o.reduction == kCeNone) loss[r] = l;
         s_loss[r] = l;
         s_count[r] = y == kCeIgnored ? 0.f : 1.f;
@@ -208,7 +200,7 @@ cudaError_t few_forward(const FewArgs &a, float *loss, unsigned char *ws, cudaSt
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     few_merge_kernel<<<1, kMergeNT * a.N, 0, st>>>(a.N, a.V, blocks, part, psum, zt, a.labels,
-                                                   a.opt, loss, a.lse, a.count, a.zmax);
+                                                   a.opt, loss, a.count);
     count_launches(2);
     return cudaGetLastError();
 }

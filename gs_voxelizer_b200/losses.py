@@ -480,7 +480,7 @@ def _linear_ce(features, weight, labels, opt, with_state):
         state = _C._workspace(
             lib.gsv_linear_ce_state_bytes(rows, V, D, dtype), dev)
     x, w = features.data_ptr(), weight.data_ptr()
-    call = 2 * with_state | (0 if (x | w) & 15 else 4)  # gsv_ce_call
+    call = (2 if with_state else 8) | (0 if (x | w) & 15 else 4)  # gsv_ce_call
     ws = _C._workspace(lib.gsv_linear_ce_workspace_bytes(
         rows, V, D, dtype, opt, call), dev)
     _ce_call(lib.gsv_linear_ce_forward, dev, rows, V, D, dtype, x, w,

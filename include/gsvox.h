@@ -532,7 +532,8 @@ GSV_API int gsv_halo_accumulate(int32_t num_gaussians, int32_t channels,
  * (the inputs may lie elsewhere by then).
  * A null state: no backward follows.
  * gsv_linear_ce_workspace_bytes takes what the workspace is for, as bits
- * (gsv_ce_call); without GSV_CE_STATE or GSV_CE_ALIGNED it is enough for either.
+ * (gsv_ce_call); a forward's without GSV_CE_STATE or GSV_CE_NO_STATE is enough
+ * for either, and without GSV_CE_ALIGNED it is enough for any alignment.
  * Workspaces are scratch of one call, 256-byte aligned (gsv_softmax_ce_forward:
  * 8-byte). Everything else is aligned to its elements; a pointer that is not is
  * refused. A null gradient output of gsv_linear_ce_backward is not computed.
@@ -543,7 +544,8 @@ enum gsv_reduction { GSV_REDUCE_NONE = 0, GSV_REDUCE_SUM = 1, GSV_REDUCE_MEAN = 
 enum gsv_ce_call {
     GSV_CE_BACKWARD = 1, /* gsv_linear_ce_backward; else _forward            */
     GSV_CE_STATE = 2,    /* the forward is given a state                     */
-    GSV_CE_ALIGNED = 4   /* features and weight are aligned to 16 bytes      */
+    GSV_CE_ALIGNED = 4,  /* features and weight are aligned to 16 bytes      */
+    GSV_CE_NO_STATE = 8  /* the forward is given a null state                */
 };
 
 typedef struct gsv_ce_options {

@@ -79,7 +79,7 @@ def test_caps_that_float32_cannot_divide_by(cap):
     assert lib.gsv_linear_ce_workspace_bytes(7, 5, 4, 0, opt, 0) == 0
 
 
-BACKWARD, STATE, ALIGNED = 1, 2, 4
+BACKWARD, STATE, ALIGNED, NO_STATE = 1, 2, 4, 8
 
 
 def test_memory_of_the_linear_loss():
@@ -91,23 +91,23 @@ def test_memory_of_the_linear_loss():
     n = 256 ** 3
     assert 8 * n <= lib.gsv_linear_ce_state_bytes(n, 20, 4, 0) < 8 * n + 4096
     assert ws(n, 20, 4, 0, STATE) < n
-    assert 8 * n <= ws(n, 20, 4, 0, 0) < 9 * n
+    assert 8 * n <= ws(n, 20, 4, 0, NO_STATE) < 9 * n
     # scores of few classes are the state's alone
     n = 1 << 23
     assert lib.gsv_linear_ce_state_bytes(n, 16, 64, 0) < (8 + 4 * 16) * n + 4096
-    assert ws(n, 16, 64, 0, 0) < 9 * n and ws(n, 16, 64, 0, STATE) < n
+    assert ws(n, 16, 64, 0, NO_STATE) < 9 * n and ws(n, 16, 64, 0, STATE) < n
     # a table of 1 GB that is read in place, rows too large to be kept
     n, V, D = 8192, 131072, 4096
     assert ws(n, V, D, 1, STATE | ALIGNED) < 2 * n * D + (32 << 20)
     assert ws(n, V, D, 1, BACKWARD | ALIGNED) < 2 * n * D + 4 * n * D + (600 << 20)
     # rows that are read in place
-    assert ws(256 ** 3, 20, 64, 1, ALIGNED) < 64 * 256 ** 3
+    assert ws(256 ** 3, 20, 64, 1, ALIGNED | NO_STATE) < 64 * 256 ** 3
     # a few rows, loss alone: no packed operands
-    assert ws(4, 32768, 2048, 1, ALIGNED) < 1 << 17
+    assert ws(4, 32768, 2048, 1, ALIGNED | NO_STATE) < 1 << 17
     # without the bits it is enough for either
     for sizes in ((700, 500, 64, 1), (3, 500, 64, 1), (20000, 9, 64, 0), (70000, 20, 4, 0),
                   (100000, 2000, 72, 2), (300, 2000, 264, 2), (300, 2000, 33, 0)):
-        for call in (STATE, ALIGNED, STATE | ALIGNED):
+        for call in (STATE, NO_STATE, ALIGNED, STATE | ALIGNED, NO_STATE | ALIGNED):
             assert 0 < ws(*sizes, call) <= ws(*sizes, 0)
         assert 0 < ws(*sizes, BACKWARD | ALIGNED) <= ws(*sizes, BACKWARD)
 
