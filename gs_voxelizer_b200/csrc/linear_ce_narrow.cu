@@ -143,6 +143,7 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
     CeSum lsum;
     float cnt = 0.f;
     bool staged = false;
+    const bool whole = gridDim.y == 1 && V <= kChunk;  // the table is staged, and stays
     const long long stride = (long long)gridDim.x * kNT * R;
     long long t0 = (long long)blockIdx.x * kNT * R;
     Ahead<DP, R> next;
@@ -214,9 +215,12 @@ narrow_fwd_kernel(long long N, int V, int D, const T *__restrict__ features,
             if (smooth && !CAP) sz[k] = dot_pairs<DP>(x[k], to_pairs<DP>(s_wsum));
             float zy = 0.f;
             if (y[k] >= 0) {
-                zy = dot_pairs<DP>(x[k],
-                                   to_pairs<DP>(load_row<T, DP, VEC>(weight, y[k], D)));
-                if (CAP) zy = o.cap * ce_tanh<sizeof(T) == 2>(zy, o.cap);
+                // the same products as among all classes: where the label's
+                // score is the maximum, their difference is 0
+                zy = dot_pairs<DP>(x[k], whole ? sw[y[k]]
+                                               : table_pairs<DP, CAP>(load_row<T, DP, VEC>(
+                                                     weight, y[k], D)));
+                zy = CAP ? o.cap * ce_tanh<sizeof(T) == 2>(zy, o.cap) : zy * kCeLn2;
             }
             if (gridDim.y > 1) {
                 part[blockIdx.y * N + r] = make_float2(m[k], s[k]);

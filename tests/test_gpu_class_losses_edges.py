@@ -455,3 +455,37 @@ def test_gradient_of_confident_rows(V, D, size, n, dtype):
     es = 64 * 2.0 ** -24 * float((x.double().abs() * w[labels].double().abs()).max())
     tol = 2.0 ** -20 / rest + 4 * es + 4 * HALF_ULP[dtype] + 2.0 ** -18
     assert ((dx.double() - want).norm(dim=1) <= tol * want.norm(dim=1)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,D", [(1000, 20, 4), (40, 900, 4), (1000, 37, 8), (300, 60, 12),
+                                   (300, 40, 24), (300, 700, 40), (16500, 9, 40), (3, 700, 64),
+                                   (300, 50, 0), (20, 3000, 0)])
+def test_loss_of_confident_rows(n, V, D, dtype):
+    """A row whose label scores hundreds and far above the rest: the loss is
+    nearly 0 and keeps float32's absolute error at 1 (2^-22), not at the
+    score's size, as the label's score and the maximum are the same number; and
+    of the rest's probability the scores' own error."""
+    g = torch.Generator("cuda").manual_seed(65)
+    labels = torch.randint(0, V, (n,), generator=g, device="cuda")
+    if D:
+        w = torch.randn(V, D, generator=g, device="cuda")
+        w = (w / w.norm(dim=1, keepdim=True)).to(dtype)
+        x = (300.0 * w[labels].float() + torch.randn(n, D, generator=g, device="cuda")).to(dtype)
+        data = (x, w)
+        z = x.double() @ w.double().t()
+        es = (D + 8) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()).amax(1)
+    else:
+        s = torch.randn(n, V, generator=g, device="cuda")
+        s[torch.arange(n, device="cuda"), labels] = 300.0
+        data = (s.to(dtype),)
+        z, es = data[0].double(), torch.zeros(n, dtype=torch.float64, device="cuda")
+    rows = torch.arange(n, device="cuda")
+    others = (z - z[rows, labels][:, None]).index_put((rows, labels), torch.tensor(
+        float("-inf"), dtype=torch.float64, device="cuda"))
+    want = torch.log1p(others.exp().sum(1))
+    for up in (None, torch.ones(n, device="cuda")):
+        loss, _ = call(data, labels, dict(reduction="none"), up)
+        tol = 2.0 ** -22 + (4 * es + 2.0 ** -18) * want
+        assert ((loss.double() - want).abs() <= tol).all()
+        assert (loss >= 0).all()
