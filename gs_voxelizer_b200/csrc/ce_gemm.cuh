@@ -30,11 +30,16 @@ struct CeUpstream {
     const float *gmax;   // or null
     float inv_p;         // 1 / p_scale
     int reduction;
-    const float *zmax = nullptr;  // largest factor of the z-loss, over which P is
+    const float *zmax = nullptr;  // largest factor of the z-loss
 };
 
+// The power of two from the largest factor of the z-loss on (up to 2^127), over
+// which P is kept: another factor would round derivatives near 1 and 1/2, the
+// most frequent ones, more coarsely (2.6e-4 of the gradients for 2.4e-4).
 __device__ __forceinline__ float ce_z_scale(const CeUpstream &u) {
-    return u.zmax ? fmaxf(*u.zmax, 1.f) : 1.f;
+    if (!u.zmax) return 1.f;
+    const int up = (__float_as_int(fmaxf(*u.zmax, 1.f)) + 0x7fffff) & 0x7f800000;
+    return __int_as_float(min(up, 0x7f000000));
 }
 
 __device__ __forceinline__ float ce_grad_scale(const CeUpstream &u) {
