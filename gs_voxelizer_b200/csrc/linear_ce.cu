@@ -13,10 +13,10 @@
 // Rounding P to 16 bits costs at most half a step (2^-8 of the value in bf16,
 // 2^-11 in fp16), no more than rounding the gradients themselves to the same
 // type (against float64: 2.4e-3 of bf16 gradients where the products of an
-// unrounded P give 1.7e-3, 2.4e-4 of fp16 ones for 2.1e-4). fp16 keeps P times 2^14, over the largest factor that a z-loss brings to
-// a row (as a power of two), so that small probabilities stay normal numbers and
-// none overflows. float32 inputs keep three bf16 planes of
-// every operand, which hold all 24 bits.
+// unrounded P give 1.7e-3, 2.4e-4 of fp16 ones for 2.1e-4). fp16 keeps P times
+// 2^14, over the largest factor that a z-loss brings to a row (as a power of
+// two), so that small probabilities stay normal numbers and none overflows.
+// float32 inputs keep three bf16 planes of every operand, which hold all 24 bits.
 //
 // Few channels, few classes of many float32 channels, and few rows have
 // kernels of their own (see path_of).
