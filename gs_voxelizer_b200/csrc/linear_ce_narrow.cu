@@ -13,8 +13,8 @@
 // needs atomics.
 //
 // What bounds it: issue and latency at the occupancy that the registers leave
-// (256^3 rows x 4 channels, 20 classes, float32: forward 190 us, dX 209 us,
-// dW 264 us; 0.6 instructions a clock and scheduler, 12 to 20 a score, the
+// (256^3 rows x 4 channels, 20 classes, float32: forward 193 us, dX 209 us,
+// dW 258 us; 0.6 instructions a clock and scheduler, 12 to 20 a score, the
 // exponentials alone would take 75 us each). One, two or four rows a thread,
 // three to five blocks an SM and pairs of rows instead of channels came to
 // 636 to 770 us for the three.
@@ -38,9 +38,10 @@ constexpr int chunk_of(int dp) { return 4096 / dp; }  // classes staged at once
 constexpr int kRows = 2;                              // rows a thread
 // classes a thread (dW): the registers hold 2 DP each
 constexpr int classes_of(int dp) { return dp == 4 ? 4 : 2; }
-// Rows that a thread of dW adds up before its sum joins the block's: a sum of
-// all of a block's rows, hundreds of thousands with many classes, was off by
-// 1e-3 where all were alike
+// Rows that a thread of dW adds up in a launch, after which its sum joins the
+// block's so far: a sum of all of a block's rows, hundreds of thousands with
+// many classes, was off by 1e-3 where all were alike. (Joined within the kernel,
+// a loop around the tiles, 256^3 x 20 x 4 took 264 to 284 us for 258.)
 constexpr int kDwChain = 1024;
 // blocks an SM, as many as registers hold without spills
 constexpr int per_sm(int dp) { return dp <= 8 ? 3 : dp == 16 ? 2 : 1; }
@@ -60,15 +61,18 @@ __device__ __forceinline__ Pairs<DP> to_pairs(const Row<DP> &r) {
 }
 
 // A row of the table times unit<CAP>(). What was finite stays so: rows at the
-// type's lowest value mask classes, and 0 times infinity would be NaN.
-template <int DP, bool CAP>
+// type's lowest value mask classes, and 0 times infinity would be NaN. For dW
+// (FINITE) infinities become the largest numbers: rows without a label are
+// staged as zeros, and of the others a probability is 0 either way (but against
+// features below 2^-100, which add nothing).
+template <int DP, bool CAP, bool FINITE = false>
 __device__ __forceinline__ Pairs<DP> table_pairs(Row<DP> r) {
-    if (!CAP) {
+    if (!CAP || FINITE) {
 #pragma unroll
         for (int d = 0; d < DP; ++d) {
             const float v = r.v[d];
-            r.v[d] = isinf(v) ? v : fminf(fmaxf(v * unit<CAP>(), -FLT_MAX), FLT_MAX);
-            if (isnan(v)) r.v[d] = v;  // (the bounds above would replace it)
+            if (isnan(v) || (!FINITE && isinf(v))) continue;
+            r.v[d] = fminf(fmaxf(v * unit<CAP>(), -FLT_MAX), FLT_MAX);
         }
     }
     return to_pairs<DP>(r);
@@ -381,14 +385,16 @@ struct alignas(16) DwRow {
     float e, hit, unused[2];
 };
 
-// acc[blockIdx.x][V][D]: the block's rows' part of its classes' gradients.
+// acc[blockIdx.x][V][D] (+)= the part of its classes' gradients of the block's
+// rows among [row0, N).
 // Threads: `lanes` groups of classes (j, j + lanes, ...) x (kNT / lanes)
 // slices of the staged rows.
 template <typename T, int DP, bool CAP, bool VEC>
 __global__ void __launch_bounds__(kNT, per_sm(DP))
-narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ features,
+narrow_dw_kernel(long long row0, long long N, int V, int D, int lanes,
+                 const T *__restrict__ features,
                  const T *__restrict__ weight, const long long *__restrict__ labels, CeOpt o,
-                 const float2 *__restrict__ lse, CeUpstream u, float *__restrict__ acc) {
+                 const float2 *__restrict__ lse, CeUpstream u, float *__restrict__ acc, bool add) {
     constexpr int C = classes_of(DP), kDwRows = dw_rows_of(DP);
     constexpr size_t kRowBytes = sizeof(DwRow<DP>) * kDwRows * 2;
     constexpr size_t kRedBytes = sizeof(float) * kNT * (DP + 1);
@@ -404,118 +410,94 @@ narrow_dw_kernel(long long N, int V, int D, int lanes, const T *__restrict__ fea
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int d = 0; d < DP / 2; ++d) w[c].v[d] = f2(0.f);
+        for (int d = 0; d < DP / 2; ++d) w[c].v[d] = dw[c].v[d] = f2(0.f);
         if (active && j0 + c * lanes < V)
-            w[c] = table_pairs<DP, CAP>(load_row<T, DP, VEC>(weight, j0 + c * lanes, D));
+            w[c] = table_pairs<DP, CAP, true>(
+                load_row<T, DP, VEC>(weight, j0 + c * lanes, D));
     }
-    // The zeros of a row without a label are NaN times an infinite entry. Only
-    // then are such rows passed over: the branch in the loop costs 6 to 12 %.
-    bool infinite = false;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int d = 0; d < DP / 2; ++d)
-            infinite = infinite || !isfinite(w[c].v[d].x) || !isfinite(w[c].v[d].y);
-    infinite = __syncthreads_or(infinite);
     const bool plain = o.eps == 0.f && o.zeta == 0.f;
     const float common = common_grad(u), ev = o.eps / (float)V;
     const float *per_row = u.reduction == kCeNone ? u.g : nullptr;
     const long long stride = (long long)gridDim.x * kDwRows;
-    long long t0 = (long long)blockIdx.x * kDwRows;
+    long long t0 = row0 + (long long)blockIdx.x * kDwRows;
     int buffer = 0;
     const bool stager = threadIdx.x < kDwRows;
     Ahead<DP, 1> next;
     read_ahead<T, DP, VEC, 1, true>(next, stager ? t0 : N, 0, N, D, features, labels, o.ignore,
                                     lse);
-    const int tiles = max(1, kDwChain * slices / kDwRows);
-    for (bool first = true; t0 < N; first = false) {
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int d = 0; d < DP / 2; ++d) dw[c].v[d] = f2(0.f);
-        const long long stop = min(N, t0 + tiles * stride);
-        for (; t0 < stop; t0 += stride) {
-            DwRow<DP> *rows = buffers + buffer * kDwRows;
-            buffer ^= 1;
-            if (stager) {
-                // an unlabelled row is all zeros
-                DwRow<DP> s{};
-                s.y = ce_label(next.label[0], o.ignore, V);
-                if (s.y != kCeIgnored) {
-                    const RowGrad q = row_grad<CAP>(t0 + threadIdx.x, s.y, next.lse[0], o, per_row,
-                                                    common, ev);
-                    s.x = to_pairs<DP>(next.x[0]);
-                    s.lse = q.lse;
-                    s.kz = q.kz;
-                    s.e = q.e;
-                    s.hit = q.hit;
-                }
-                rows[threadIdx.x] = s;
-                read_ahead<T, DP, VEC, 1, true>(next, t0 + stride, 0, N, D, features, labels,
-                                                o.ignore, lse);
+    for (; t0 < N; t0 += stride) {
+        DwRow<DP> *rows = buffers + buffer * kDwRows;
+        buffer ^= 1;
+        if (stager) {
+            // an unlabelled row is all zeros
+            DwRow<DP> s{};
+            s.y = ce_label(next.label[0], o.ignore, V);
+            if (s.y != kCeIgnored) {
+                const RowGrad q = row_grad<CAP>(t0 + threadIdx.x, s.y, next.lse[0], o, per_row,
+                                                common, ev);
+                s.x = to_pairs<DP>(next.x[0]);
+                s.lse = q.lse;
+                s.kz = q.kz;
+                s.e = q.e;
+                s.hit = q.hit;
             }
-            __syncthreads();
-            if (!active) continue;
-            auto add_rows = [&](auto pass_over) {
-#pragma unroll(DP == 8 || DP == 32 ? 2 : 1)
-                for (int i = slice; i < kDwRows; i += slices) {
-                    const Pairs<DP> x = rows[i].x;
-                    const float2 l = rows[i].lse;
-                    const float kz = rows[i].kz;
-                    const int y = rows[i].y;
-                    if (decltype(pass_over)::value && y == kCeIgnored) continue;
-                    float hit = kz, e = 0.f;
-                    if (!plain) {
-                        hit = rows[i].hit;
-                        e = rows[i].e;
-                    }
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        float slope = 1.f;
-                        const float p =
-                            prob<CAP, sizeof(T) == 2>(dot_pairs<DP>(x, w[c]), l, o.cap, slope);
-                        float d = fmaf(kz, p, -e);
-                        if (y == j0 + c * lanes) d -= hit;
-                        if (CAP) d *= slope;
-#pragma unroll
-                        for (int k = 0; k < DP / 2; ++k)
-                            dw[c].v[k] = __ffma2_rn(f2(d), x.v[k], dw[c].v[k]);
-                    }
-                }
-            };
-            if (infinite)
-                add_rows(std::true_type{});
-            else
-                add_rows(std::false_type{});
-        }
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float out[DP];
-            __syncthreads();
-#pragma unroll
-            for (int d = 0; d < DP / 2; ++d) {
-                out[2 * d] = dw[c].v[d].x;
-                out[2 * d + 1] = dw[c].v[d].y;
-            }
-#pragma unroll
-            for (int d = 0; d < DP; ++d) red[threadIdx.x * (DP + 1) + d] = out[d];
-            __syncthreads();
-            const int j = j0 + c * lanes;
-            if (slice == 0 && j < V) {
-                for (int s = 1; s < slices; ++s)
-#pragma unroll
-                    for (int d = 0; d < DP; ++d)
-                        out[d] += red[(s * lanes + threadIdx.x) * (DP + 1) + d];
-                float *sum = acc + (long long)blockIdx.x * V * D;
-                if (!first) {
-                    const Row<DP> old = load_row<float, DP, false>(sum, j, D);
-#pragma unroll
-                    for (int d = 0; d < DP; ++d) out[d] += old.v[d];
-                }
-                store_row<float, DP, false>(sum, j, D, out);
-            }
+            rows[threadIdx.x] = s;
+            read_ahead<T, DP, VEC, 1, true>(next, t0 + stride, 0, N, D, features, labels,
+                                            o.ignore, lse);
         }
         __syncthreads();
+        if (!active) continue;
+#pragma unroll(DP == 8 || DP == 32 ? 2 : 1)
+        for (int i = slice; i < kDwRows; i += slices) {
+            const Pairs<DP> x = rows[i].x;
+            const float2 l = rows[i].lse;
+            const float kz = rows[i].kz;
+            const int y = rows[i].y;
+            float hit = kz, e = 0.f;
+            if (!plain) {
+                hit = rows[i].hit;
+                e = rows[i].e;
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float slope = 1.f;
+                const float p =
+                    prob<CAP, sizeof(T) == 2>(dot_pairs<DP>(x, w[c]), l, o.cap, slope);
+                float d = fmaf(kz, p, -e);
+                if (y == j0 + c * lanes) d -= hit;
+                if (CAP) d *= slope;
+#pragma unroll
+                for (int k = 0; k < DP / 2; ++k)
+                    dw[c].v[k] = __ffma2_rn(f2(d), x.v[k], dw[c].v[k]);
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        float out[DP];
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DP / 2; ++d) {
+            out[2 * d] = dw[c].v[d].x;
+            out[2 * d + 1] = dw[c].v[d].y;
+        }
+#pragma unroll
+        for (int d = 0; d < DP; ++d) red[threadIdx.x * (DP + 1) + d] = out[d];
+        __syncthreads();
+        const int j = j0 + c * lanes;
+        if (slice == 0 && j < V) {
+            for (int s = 1; s < slices; ++s)
+#pragma unroll
+                for (int d = 0; d < DP; ++d)
+                    out[d] += red[(s * lanes + threadIdx.x) * (DP + 1) + d];
+            float *sum = acc + (long long)blockIdx.x * V * D;
+            if (add) {
+                const Row<DP> old = load_row<float, DP, false>(sum, j, D);
+#pragma unroll
+                for (int d = 0; d < DP; ++d) out[d] += old.v[d];
+            }
+            store_row<float, DP, false>(sum, j, D, out);
+        }
     }
 }
 
@@ -596,11 +578,15 @@ cudaError_t launch_narrow_dw(const NarrowArgs &a, const CeUpstream &u, float *ac
     return by_form(a.D, a.opt.cap > 0.f, a.wide_rows(sizeof(T), nullptr),
                    [&](auto dp, auto cap, auto vec) {
         const NarrowShape s = narrow_shape(a.N, a.V, a.D);
-        narrow_dw_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value>
-            <<<dim3(s.dw_blocks, s.dw_chunks), kNT, 0, st>>>(
-                a.N, a.V, a.D, s.dw_lanes, static_cast<const T *>(a.features),
-                static_cast<const T *>(a.weight), a.labels, a.opt, a.lse, u, acc);
-        count_launches(1);
+        const long long rows = (long long)s.dw_blocks * (kNT / s.dw_lanes) * kDwChain;
+        for (long long row0 = 0; row0 < a.N; row0 += rows) {
+            narrow_dw_kernel<T, decltype(dp)::value, decltype(cap)::value, decltype(vec)::value>
+                <<<dim3(s.dw_blocks, s.dw_chunks), kNT, 0, st>>>(
+                    row0, std::min(a.N, row0 + rows), a.V, a.D, s.dw_lanes,
+                    static_cast<const T *>(a.features), static_cast<const T *>(a.weight),
+                    a.labels, a.opt, a.lse, u, acc, row0 > 0);
+            count_launches(1);
+        }
         return cudaGetLastError();
     });
 }
