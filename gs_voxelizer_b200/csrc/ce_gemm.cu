@@ -482,9 +482,14 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                               (reinterpret_cast<uintptr_t>(g.dst) & 15) == 0);
             if (g.dst) scale = ce_grad_scale(g.up);
         }
-        // (the ratio is formed first: 2^14 over a vanishing gmax is infinite)
-        float gmax = 1.f;
-        if (PRODUCT == kCeProbs && g.grow && g.gmax && *g.gmax > 0.f) gmax = *g.gmax;
+        // A row's upstream gradient over gmax: by a power of two, so that neither
+        // a vanishing nor a huge gmax has an infinite or vanishing reciprocal.
+        float g_power = 1.f, g_inv = 1.f;
+        if (PRODUCT == kCeProbs && g.grow && g.gmax && *g.gmax > 0.f) {
+            const float top = *g.gmax;
+            g_power = top < 0x1p-64f ? 0x1p64f : top > 0x1p64f ? 0x1p-64f : 1.f;
+            g_inv = 1.f / (top * g_power);
+        }
         const float unit_scale = PRODUCT == kCeProbs ? g.p_scale / ce_z_scale(g.up) : 1.f;
         // a unit's row, read a unit ahead: units of few classes and channels
         // take no longer than these loads
@@ -497,7 +502,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             x.y = g.lab ? g.lab[g.row0 + r] : ce_label(g.labels[g.row0 + r], o.ignore, g.V);
             if (PRODUCT == kCeProbs) {
                 x.lse = g.lse[g.row0 + r];
-                if (g.grow) x.g = g.grow[g.idx[g.row0 + r]] / gmax;
+                if (g.grow) x.g = g.grow[g.idx[g.row0 + r]];
             }
             return x;
         };
@@ -512,7 +517,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             float top = ce_neg_inf(), s = 0.f, sz = 0.f;
             float kz = 1.f, e = 0.f, hit = 0.f;
             if (PRODUCT == kCeProbs) {
-                const float f = unit_scale * row.g;
+                const float f = unit_scale * (row.g * g_power * g_inv);
                 kz = (1.f + 2.f * o.zeta * ce_lse(lse)) * f;
                 e = o.eps / (float)g.V * f;
                 hit = (1.f - o.eps) * f;
