@@ -61,9 +61,8 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
         if verbose:
             print(" ".join(cmd))
         jobs.append((name, cmd))
-    # side by side, the largest sources first: 70 s on 8 cores, where one after
-    # another takes 226 s of the compiler's time
-    jobs.sort(key=lambda job: -(SRC / job[0]).stat().st_size)
+    # side by side, those of the most kernels first
+    jobs.sort(key=lambda job: (job[0] not in PRECISE, -(SRC / job[0]).stat().st_size))
     with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
         results = list(pool.map(
             lambda job: subprocess.run(job[1], capture_output=True, text=True), jobs))
